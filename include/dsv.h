@@ -437,6 +437,126 @@ int dsv_bundle_order(const dsv_tensor* parent, int64_t bundle_size,
                      int64_t num_bundles, int64_t max_bundles, dsv_tensor* perm,
                      dsv_tensor* bundle_of, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Verification of drafted tokens from given random numbers                   */
+/* ------------------------------------------------------------------------- */
+
+/* Workspace for dsv_spec_accept with T trees of M nodes over vocab V (0 on
+ * invalid sizes). */
+size_t dsv_spec_workspace_bytes(int64_t T, int64_t M, int64_t V);
+
+/*
+ * Rejection sampling of drafted trees (chains among them): the outputs are
+ * those of the walk of verify_new (draft/tree_verification.py:100-182), the
+ * rule keeps the target's distribution, which the reference has no mode for.
+ * From the root, the children x_1, x_2, .. of the current node (index order)
+ * are tested in turn.  p and q are the target's and the draft's rows of the
+ * current node, w_0 = p, S_0 = 1, c_0 = 0; child j is accepted iff
+ *     uniform[j] * S_{j-1} * q(x_j) < w_{j-1}(x_j),
+ * and becomes the current node; after a rejection c_j = c_{j-1} + S_{j-1},
+ * w_j = max(p - c_j q, 0), S_j = sum w_j.  Without draft_probs the children
+ * are given tokens: q is one at the child's token, so child j is accepted iff
+ * uniform[j] * R < p(x_j), R = 1 - the sum of p over the rejected siblings'
+ * tokens (each token once; a repeated rejected token is rejected), and w is p
+ * without those tokens.  Where no child is accepted, the next token is the
+ * first v with sum_{v' <= v} w > uniform[root] * sum w; if w is zero
+ * everywhere, it is drawn from p so, and it is 0 if p is.
+ * Rows are taken as they are (not normalised again); negative, infinite and
+ * NaN entries count as 0; numbers outside [0, 1) are clamped into it (NaN to
+ * 0).  All sums are in 64 bits and in a fixed order.
+ *   target      [T, M, V] bf16|f16|f32: the target's probabilities after
+ *               every node, innermost stride 1
+ *   draft       [T, M] int64 tokens (node 0 = root; tokens outside [0, V)
+ *               have probability 0)
+ *   parent      [T, M-1] int64, the reference's convention (dsv_tree_accept)
+ *   uniform     [T, M] f32: number 0 draws the next token, number i tests
+ *               node i
+ *   draft_probs optional [T, M, V], dtype of target: row i is the
+ *               distribution that the children of node i were drawn from,
+ *               independently (ndim 0: the children are given tokens)
+ *   out_path, out_tokens [T, M], out_info [T, 4] int64: as dsv_tree_accept
+ *               ({last node, accept length, next token, path length})
+ * 1 <= M <= 1024, 1 <= T <= 2^20, V < 2^31.
+ */
+int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft,
+                    const dsv_tensor* parent, const dsv_tensor* uniform,
+                    const dsv_tensor* draft_probs, dsv_tensor* out_path,
+                    dsv_tensor* out_tokens, dsv_tensor* out_info,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Pages: fork, extend, free, compact                                         */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Page bookkeeping on the device, in place of the host's in
+ * core/kv_cache/paged_kv.py:81-166 and :364-402.  Shared by the four calls:
+ *   kv_pages    [L, 2, P, Hk, page, D] bf16|f16|f32, rows of D contiguous and
+ *               16-byte aligned multiples of 16 bytes
+ *   page_table  [B, n_logical] int32, innermost stride 1: physical page of
+ *               each sequence's logical page, -1 for none
+ *   refcount    [P] int32, contiguous: table entries that name the page,
+ *               0 = free
+ *   seqlens     [B] int32|int64, contiguous: tokens of each sequence
+ *   page_size   a power of two;  B <= 2^17, P < 2^31
+ * Pages are taken lowest first, for requests in ascending order, so results
+ * are reproducible.  fork and extend either do all that is asked or change
+ * nothing; info [3] int32 receives {pages taken, pages lacking, requests
+ * refused}.
+ */
+/* Workspace of the page calls for P pages, B sequences and n pairs (0 on
+ * invalid sizes). */
+size_t dsv_pages_workspace_bytes(int64_t P, int64_t B, int64_t n);
+
+/*
+ * Sequence children[i] becomes a continuation of parents[i]: whole pages are
+ * shared, a partly filled last page is copied into a page of the child's own
+ * (every layer, K and V, the whole page).  Refused: indices out of range,
+ * parent == child, a child that is not empty (seqlens != 0), is named twice or
+ * is a parent of the same call, a parent longer than its table row.
+ *   parents, children  [n] int32|int64
+ */
+int dsv_pages_fork(const dsv_tensor* kv_pages, const dsv_tensor* page_table,
+                   const dsv_tensor* refcount, const dsv_tensor* seqlens,
+                   const dsv_tensor* parents, const dsv_tensor* children,
+                   dsv_tensor* info, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/*
+ * Sequences grow to new_lens [B] int32|int64 tokens (shorter or equal ones
+ * stay as they are): table entries up to the last page of the new length
+ * receive free pages, seqlens the new length.  Refused: new lengths beyond the
+ * table row, negative seqlens.  The new tokens' contents are the caller's.
+ */
+int dsv_pages_extend(const dsv_tensor* page_table, const dsv_tensor* refcount,
+                     const dsv_tensor* seqlens, const dsv_tensor* new_lens,
+                     int64_t page_size, dsv_tensor* info, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * Pages are given back (their entries become -1, counts fall; 0 = free).
+ * window == 0: every page of the sequences, whose lengths become 0.
+ * window > 0: the pages that no later token sees through a sliding window of
+ * that many tokens with `sinks` first tokens that stay visible
+ * (dsv_window_attention): those that start at or behind token `sinks` and end
+ * before token seqlens - window + 2; lengths stay.
+ *   seqs [n] int32|int64: entries out of range are skipped, a sequence named
+ *   twice is freed once
+ */
+int dsv_pages_free(const dsv_tensor* page_table, const dsv_tensor* refcount,
+                   const dsv_tensor* seqlens, const dsv_tensor* seqs,
+                   int64_t page_size, int64_t window, int64_t sinks,
+                   void* stream);
+
+/*
+ * The n pages in use move to places [0, n): those at or behind n, in order,
+ * into the free ones below n.  Contents, counts and table entries follow.
+ * info receives {pages in use, pages moved, 0}.  (seqlens do not change.)
+ */
+int dsv_pages_compact(const dsv_tensor* kv_pages, const dsv_tensor* page_table,
+                      const dsv_tensor* refcount, dsv_tensor* info,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1481,3 +1481,377 @@ int dsv_lmhead_accept(int mode, const dsv_tensor* hidden, const dsv_tensor* weig
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Verification of drafted tokens from given random numbers
+// ---------------------------------------------------------------------------
+
+namespace {
+
+struct SpecPlan {
+  int64_t nsub = 0;
+  size_t state_bytes = 0, rej_bytes = 0, total = 0;
+};
+
+bool spec_plan(int64_t T, int64_t M, int64_t V, SpecPlan& p) {
+  if (M < 1 || M > dsv::kSpecMaxM || T < 1 || T > (1 << 20) || V < 1 || V > 0x7fffffff) return false;
+  p.nsub = (V + dsv::kSpecSub - 1) / dsv::kSpecSub;
+  p.state_bytes = align_up((size_t)T * sizeof(dsv::SpecState), 256);
+  p.rej_bytes = align_up((size_t)T * M * sizeof(int32_t), 256);
+  p.total = p.state_bytes + p.rej_bytes + align_up((size_t)T * p.nsub * sizeof(double), 256);
+  return true;
+}
+
+int check_workspace(size_t need, void* ws, size_t ws_bytes) {
+  if (ws == nullptr || ws_bytes < need)
+    return fail(DSV_ERR_WORKSPACE, "workspace of %zu bytes required (got %zu)", need, ws == nullptr ? 0 : ws_bytes);
+  if ((reinterpret_cast<uintptr_t>(ws) & 255) != 0) return fail(DSV_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  return DSV_OK;
+}
+
+// Byte ranges that share an address.
+bool overlap(const Extent& x, const Extent& y) { return x.lo < y.hi && y.lo < x.hi; }
+
+}  // namespace
+
+extern "C" {
+
+size_t dsv_spec_workspace_bytes(int64_t T, int64_t M, int64_t V) {
+  SpecPlan p;
+  return spec_plan(T, M, V, p) ? p.total : 0;
+}
+
+int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft, const dsv_tensor* parent,
+                    const dsv_tensor* uniform, const dsv_tensor* draft_probs, dsv_tensor* out_path,
+                    dsv_tensor* out_tokens, dsv_tensor* out_info, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  int rc;
+  if ((rc = check_nd(target, "target", 3)) != DSV_OK) return rc;
+  if (target->dtype != DSV_BF16 && target->dtype != DSV_F16 && target->dtype != DSV_F32)
+    return fail(DSV_ERR_INVALID, "target must be bf16, f16 or f32 (got %s)", dt_name(target->dtype));
+  const int64_t T = target->shape[0], M = target->shape[1], V = target->shape[2];
+  if (target->stride[2] != 1) return fail(DSV_ERR_INVALID, "target: vocab stride must be 1");
+  SpecPlan p;
+  if (!spec_plan(T, M, V, p))
+    return fail(DSV_ERR_UNSUPPORTED, "sizes out of range: %lld trees (1..2^20) of %lld nodes (1..%d) over %lld tokens (1..2^31 - 1)",
+                (long long)T, (long long)M, dsv::kSpecMaxM, (long long)V);
+  if ((rc = check_nd(draft, "draft", 2)) != DSV_OK) return rc;
+  if (draft->dtype != DSV_I64 || draft->shape[0] != T || draft->shape[1] != M)
+    return fail(DSV_ERR_INVALID, "draft must be int64 [T, M]");
+  // A root-only tree has an empty parent tensor, possibly without storage.
+  if (M > 1 && (rc = check_nd(parent, "parent", 2)) != DSV_OK) return rc;
+  if (parent == nullptr || parent->ndim != 2 || parent->dtype != DSV_I64 || parent->shape[0] != T ||
+      parent->shape[1] != M - 1)
+    return fail(DSV_ERR_INVALID, "parent must be int64 [T, M-1]");
+  if ((rc = check_nd(uniform, "uniform", 2)) != DSV_OK) return rc;
+  if (uniform->dtype != DSV_F32 || uniform->shape[0] != T || uniform->shape[1] != M)
+    return fail(DSV_ERR_INVALID, "uniform must be float32 [T, M]");
+  if (present(draft_probs)) {
+    if ((rc = check_nd(draft_probs, "draft_probs", 3)) != DSV_OK) return rc;
+    if (draft_probs->dtype != target->dtype || draft_probs->shape[0] != T || draft_probs->shape[1] != M ||
+        draft_probs->shape[2] != V || draft_probs->stride[2] != 1)
+      return fail(DSV_ERR_INVALID, "draft_probs must have target's dtype and shape [T, M, V], vocab stride 1");
+  }
+  struct Out { dsv_tensor* t; const char* name; int64_t cols; };
+  const Out outs[3] = {{out_path, "out_path", M}, {out_tokens, "out_tokens", M}, {out_info, "out_info", 4}};
+  const Extent ins[5] = {extent_of("target", target), extent_of("draft", draft),
+                         M > 1 ? extent_of("parent", parent) : Extent{"parent", 0, 0},
+                         extent_of("uniform", uniform), extent_of("draft_probs", draft_probs)};
+  for (const Out& o : outs) {
+    if ((rc = check_nd(o.t, o.name, 2)) != DSV_OK) return rc;
+    if (o.t->dtype != DSV_I64 || o.t->shape[0] != T || o.t->shape[1] != o.cols || o.t->stride[1] != 1)
+      return fail(DSV_ERR_INVALID, "%s must be int64 [T, %lld] with innermost stride 1", o.name, (long long)o.cols);
+    if (T > 1 && o.t->stride[0] < o.cols) return fail(DSV_ERR_INVALID, "%s: rows overlap", o.name);
+    // Every workgroup of a tree reads the inputs while the first one writes.
+    for (const Extent& in : ins)
+      if (overlap(extent_of(o.name, o.t), in)) return fail(DSV_ERR_INVALID, "%s overlaps %s", o.name, in.name);
+  }
+  if (overlap(extent_of("", out_path), extent_of("", out_tokens)) || overlap(extent_of("", out_path), extent_of("", out_info)) ||
+      overlap(extent_of("", out_tokens), extent_of("", out_info)))
+    return fail(DSV_ERR_INVALID, "outputs overlap each other");
+  if ((rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+
+  dsv::SpecArgs a{};
+  a.dtype = target->dtype;
+  a.T = (int)T;
+  a.M = (int)M;
+  a.V = V;
+  a.target = target->data;
+  a.t_st = target->stride[0];
+  a.t_sm = target->stride[1];
+  if (present(draft_probs)) {
+    a.dprobs = draft_probs->data;
+    a.q_st = draft_probs->stride[0];
+    a.q_sm = draft_probs->stride[1];
+  }
+  a.draft = static_cast<const int64_t*>(draft->data);
+  a.d_st = draft->stride[0];
+  a.d_sm = draft->stride[1];
+  a.parent = static_cast<const int64_t*>(parent->data);
+  a.p_st = parent->stride[0];
+  a.p_sm = parent->stride[1];
+  a.uniform = static_cast<const float*>(uniform->data);
+  a.u_st = uniform->stride[0];
+  a.u_sm = uniform->stride[1];
+  a.out_path = static_cast<int64_t*>(out_path->data);
+  a.op_st = out_path->stride[0];
+  a.out_tok = static_cast<int64_t*>(out_tokens->data);
+  a.ot_st = out_tokens->stride[0];
+  a.out_info = static_cast<int64_t*>(out_info->data);
+  a.oi_st = out_info->stride[0];
+  char* w = static_cast<char*>(workspace);
+  a.state = reinterpret_cast<dsv::SpecState*>(w);
+  a.rej = reinterpret_cast<int32_t*>(w + p.state_bytes);
+  a.part = reinterpret_cast<double*>(w + p.state_bytes + p.rej_bytes);
+  a.nsub = p.nsub;
+  // Workgroups per tree: enough to fill the GPU, at most one per sub-block
+  // (each walks the tree itself).
+  const int64_t fill = std::max<int64_t>(1, (int64_t)device_cus() * 4 / T);
+  a.nwg = (int)std::min(p.nsub, fill);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_spec(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "speculative acceptance launch");
+  return DSV_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Pages
+// ---------------------------------------------------------------------------
+
+namespace {
+
+struct PagesPlan {
+  size_t list_bytes = 0, off_bytes = 0, total = 0;
+};
+
+bool pages_plan(int64_t P, int64_t B, int64_t n, PagesPlan& p) {
+  if (P < 0 || P > 0x7fffffff || B < 0 || B > dsv::kPageMaxSeqs || n < 0 || n > dsv::kPageMaxSeqs) return false;
+  // Page lists: fork 3 n (source, destination, free pages), extend P, compact
+  // P / 2 + P / 2 + P; behind them extend's offsets and the state words.
+  p.list_bytes = align_up((size_t)std::max<int64_t>(2 * P + 2, 3 * n) * sizeof(int32_t), 256);
+  p.off_bytes = align_up((size_t)B * sizeof(int64_t), 256);
+  p.total = p.list_bytes + p.off_bytes + 256;
+  return true;
+}
+
+int check_book(const dsv_tensor* table, const dsv_tensor* ref, const dsv_tensor* lens, int64_t page_size,
+               dsv::PageBook& b) {
+  int rc;
+  if ((rc = check_nd(table, "page_table", 2)) != DSV_OK) return rc;
+  if (table->dtype != DSV_I32 || table->stride[1] != 1)
+    return fail(DSV_ERR_INVALID, "page_table must be int32 [B, n_logical] with innermost stride 1");
+  if (table->shape[0] > 1 && table->stride[0] < table->shape[1])
+    return fail(DSV_ERR_INVALID, "page_table rows overlap");
+  if ((rc = check_nd(ref, "refcount", 1)) != DSV_OK) return rc;
+  if (ref->dtype != DSV_I32 || (ref->shape[0] > 1 && ref->stride[0] != 1))
+    return fail(DSV_ERR_INVALID, "refcount must be contiguous int32 [P]");
+  const int sh = log2_exact(page_size);
+  if (sh < 0) return fail(DSV_ERR_UNSUPPORTED, "page_size %lld must be a power of two", (long long)page_size);
+  b.table = static_cast<int32_t*>(table->data);
+  b.t_sb = table->stride[0];
+  b.B = table->shape[0];
+  b.n_log = table->shape[1];
+  b.ref = static_cast<int32_t*>(ref->data);
+  b.P = ref->shape[0];
+  b.ps_shift = sh;
+  if (b.B > dsv::kPageMaxSeqs) return fail(DSV_ERR_UNSUPPORTED, "more than %d sequences", dsv::kPageMaxSeqs);
+  if (b.P > 0x7fffffff) return fail(DSV_ERR_UNSUPPORTED, "more than 2^31 - 1 pages");
+  if (b.n_log > ((int64_t)1 << 40) >> sh) return fail(DSV_ERR_UNSUPPORTED, "page_table rows beyond 2^40 tokens");
+  if (overlap(extent_of("", table), extent_of("", ref))) return fail(DSV_ERR_INVALID, "page_table overlaps refcount");
+  if (lens != nullptr) {
+    if ((rc = check_nd(lens, "seqlens", 1)) != DSV_OK) return rc;
+    if ((lens->dtype != DSV_I32 && lens->dtype != DSV_I64) || lens->shape[0] != b.B ||
+        (b.B > 1 && lens->stride[0] != 1))
+      return fail(DSV_ERR_INVALID, "seqlens must be contiguous int32 or int64 [B]");
+    if (lens->dtype == DSV_I32 && b.n_log > 0x7fffffff >> sh)
+      return fail(DSV_ERR_UNSUPPORTED, "table rows beyond 2^31 tokens need int64 seqlens");
+    if (overlap(extent_of("", lens), extent_of("", table)) || overlap(extent_of("", lens), extent_of("", ref)))
+      return fail(DSV_ERR_INVALID, "seqlens overlaps page_table or refcount");
+    b.lens = lens->data;
+    b.lens_i64 = lens->dtype == DSV_I64;
+  }
+  return DSV_OK;
+}
+
+// An index argument: [n] int32|int64 that no output overlaps.
+int check_index(const dsv_tensor* t, const char* name, int64_t n, const dsv_tensor* const* outs, int n_outs,
+                dsv::PageIndex& x) {
+  int rc;
+  // (An empty list may come without storage; nothing reads it.)
+  if ((t == nullptr || t->ndim != 1 || t->shape[0] != 0) && (rc = check_nd(t, name, 1)) != DSV_OK) return rc;
+  if (t->dtype != DSV_I32 && t->dtype != DSV_I64) return fail(DSV_ERR_INVALID, "%s must be int32 or int64", name);
+  if (t->shape[0] != n) return fail(DSV_ERR_INVALID, "%s must have %lld entries", name, (long long)n);
+  for (int i = 0; i < n_outs; ++i)
+    if (outs[i] != nullptr && overlap(extent_of("", t), extent_of("", outs[i])))
+      return fail(DSV_ERR_INVALID, "%s overlaps a tensor that the call writes", name);
+  x.p = t->data;
+  x.is64 = t->dtype == DSV_I64;
+  x.stride = t->stride[0];
+  return DSV_OK;
+}
+
+int check_info(const dsv_tensor* info, const dsv_tensor* const* others, int n) {
+  int rc;
+  if ((rc = check_nd(info, "info", 1)) != DSV_OK) return rc;
+  if (info->dtype != DSV_I32 || info->shape[0] != 3 || info->stride[0] != 1)
+    return fail(DSV_ERR_INVALID, "info must be contiguous int32 [3]");
+  for (int i = 0; i < n; ++i)
+    if (others[i] != nullptr && overlap(extent_of("", info), extent_of("", others[i])))
+      return fail(DSV_ERR_INVALID, "info overlaps another argument");
+  return DSV_OK;
+}
+
+int check_page_data(const dsv_tensor* kv, int64_t P, dsv::PageData& d) {
+  int rc;
+  if ((rc = check_nd(kv, "kv_pages", 6)) != DSV_OK) return rc;
+  if ((rc = check_vec16(kv, "kv_pages")) != DSV_OK) return rc;
+  if (kv->shape[1] != 2) return fail(DSV_ERR_INVALID, "kv_pages dim 1 must be 2 (K, V)");
+  if (kv->shape[2] != P)
+    return fail(DSV_ERR_INVALID, "kv_pages holds %lld pages, refcount %lld", (long long)kv->shape[2], (long long)P);
+  const int es = elem_size(kv->dtype);
+  if ((kv->shape[5] * es) % 16 != 0) return fail(DSV_ERR_UNSUPPORTED, "token rows must be a multiple of 16 bytes");
+  if (kv->shape[0] > (1 << 20)) return fail(DSV_ERR_UNSUPPORTED, "more than 2^20 layers");
+  if (kv->shape[3] * kv->shape[4] * (kv->shape[5] * es / 16) > ((int64_t)1 << 26))
+    return fail(DSV_ERR_UNSUPPORTED, "a page of one layer beyond 1 GiB");
+  // Pages that share bytes would be copied into each other: strides from the
+  // smallest up must each step over what lies below.
+  int order[6];
+  int nd = 0;
+  for (int i = 0; i < 6; ++i)
+    if (kv->shape[i] > 1) order[nd++] = i;
+  std::sort(order, order + nd, [&](int x, int y) { return kv->stride[x] < kv->stride[y]; });
+  int64_t extent = 1;
+  for (int i = 0; i < nd; ++i) {
+    const int x = order[i];
+    if (kv->stride[x] < extent) return fail(DSV_ERR_INVALID, "kv_pages overlaps itself (stride[%d])", x);
+    extent = kv->stride[x] * (kv->shape[x] - 1) + extent;
+  }
+  d.kv = static_cast<char*>(kv->data);
+  d.s_l = kv->stride[0] * es;
+  d.s_h = kv->stride[1] * es;
+  d.s_p = kv->stride[2] * es;
+  d.s_1 = kv->stride[3] * es;
+  d.s_2 = kv->stride[4] * es;
+  d.n_l = (int)kv->shape[0];
+  d.n1 = (int)kv->shape[3];
+  d.n2 = (int)kv->shape[4];
+  d.row16 = (int)(kv->shape[5] * es / 16);
+  d.contiguous = (d.n2 <= 1 || kv->stride[4] == kv->shape[5]) && (d.n1 <= 1 || kv->stride[3] == kv->shape[4] * kv->shape[5]);
+  return DSV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dsv_pages_workspace_bytes(int64_t P, int64_t B, int64_t n) {
+  PagesPlan p;
+  return pages_plan(P, B, n, p) ? p.total : 0;
+}
+
+int dsv_pages_fork(const dsv_tensor* kv_pages, const dsv_tensor* page_table, const dsv_tensor* refcount,
+                   const dsv_tensor* seqlens, const dsv_tensor* parents, const dsv_tensor* children, dsv_tensor* info,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  dsv::ForkArgs a{};
+  if (kv_pages == nullptr || kv_pages->ndim != 6) return fail(DSV_ERR_INVALID, "kv_pages must be [L, 2, P, Hk, page, D]");
+  if ((rc = check_nd(seqlens, "seqlens", 1)) != DSV_OK) return rc;
+  if ((rc = check_book(page_table, refcount, seqlens, kv_pages->shape[4], a.book)) != DSV_OK) return rc;
+  if ((rc = check_page_data(kv_pages, a.book.P, a.data)) != DSV_OK) return rc;
+  const dsv_tensor* written[5] = {kv_pages, page_table, refcount, seqlens, info};
+  for (int i = 1; i < 4; ++i)
+    if (overlap(extent_of("", kv_pages), extent_of("", written[i])))
+      return fail(DSV_ERR_INVALID, "kv_pages overlaps the bookkeeping");
+  if ((rc = check_info(info, written, 4)) != DSV_OK) return rc;
+  if (parents == nullptr || parents->ndim != 1) return fail(DSV_ERR_INVALID, "parents must be a 1-d tensor");
+  a.n = parents->shape[0];
+  if ((rc = check_index(parents, "parents", a.n, written, 5, a.parents)) != DSV_OK) return rc;
+  if ((rc = check_index(children, "children", a.n, written, 5, a.children)) != DSV_OK) return rc;
+  PagesPlan p;
+  if (!pages_plan(a.book.P, a.book.B, a.n, p)) return fail(DSV_ERR_UNSUPPORTED, "more than %d pairs", dsv::kPageMaxSeqs);
+  if ((rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+  char* w = static_cast<char*>(workspace);
+  a.info = static_cast<int32_t*>(info->data);
+  a.src = reinterpret_cast<int32_t*>(w);
+  a.dst = a.src + a.n;
+  a.state = reinterpret_cast<int32_t*>(w + p.list_bytes + p.off_bytes);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_fork(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "page fork launch");
+  return DSV_OK;
+}
+
+int dsv_pages_extend(const dsv_tensor* page_table, const dsv_tensor* refcount, const dsv_tensor* seqlens,
+                     const dsv_tensor* new_lens, int64_t page_size, dsv_tensor* info, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int rc;
+  dsv::ExtendArgs a{};
+  if ((rc = check_nd(seqlens, "seqlens", 1)) != DSV_OK) return rc;
+  if ((rc = check_book(page_table, refcount, seqlens, page_size, a.book)) != DSV_OK) return rc;
+  const dsv_tensor* written[4] = {page_table, refcount, seqlens, info};
+  if ((rc = check_info(info, written, 3)) != DSV_OK) return rc;
+  if ((rc = check_index(new_lens, "new_lens", a.book.B, written, 4, a.newlens)) != DSV_OK) return rc;
+  PagesPlan p;
+  if (!pages_plan(a.book.P, a.book.B, 0, p)) return fail(DSV_ERR_UNSUPPORTED, "sizes out of range");
+  if ((rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+  char* w = static_cast<char*>(workspace);
+  a.info = static_cast<int32_t*>(info->data);
+  a.list = reinterpret_cast<int32_t*>(w);
+  a.off = reinterpret_cast<int64_t*>(w + p.list_bytes);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_extend(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "page extend launch");
+  return DSV_OK;
+}
+
+int dsv_pages_free(const dsv_tensor* page_table, const dsv_tensor* refcount, const dsv_tensor* seqlens,
+                   const dsv_tensor* seqs, int64_t page_size, int64_t window, int64_t sinks, void* stream) {
+  int rc;
+  dsv::FreeArgs a{};
+  if ((rc = check_nd(seqlens, "seqlens", 1)) != DSV_OK) return rc;
+  if ((rc = check_book(page_table, refcount, seqlens, page_size, a.book)) != DSV_OK) return rc;
+  if (window < 0 || sinks < 0) return fail(DSV_ERR_INVALID, "window and sinks must be >= 0");
+  if (window == 0 && sinks != 0) return fail(DSV_ERR_INVALID, "sinks without a window: every page is freed");
+  const dsv_tensor* written[3] = {page_table, refcount, seqlens};
+  if (seqs == nullptr || seqs->ndim != 1) return fail(DSV_ERR_INVALID, "seqs must be a 1-d tensor");
+  a.n = seqs->shape[0];
+  if (a.n > ((int64_t)1 << 22)) return fail(DSV_ERR_UNSUPPORTED, "more than 2^22 sequences named");
+  if ((rc = check_index(seqs, "seqs", a.n, written, 3, a.seqs)) != DSV_OK) return rc;
+  a.window = std::min<int64_t>(window, (int64_t)1 << 41);
+  a.sinks = std::min<int64_t>(sinks, (int64_t)1 << 41);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_free(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "page free launch");
+  return DSV_OK;
+}
+
+int dsv_pages_compact(const dsv_tensor* kv_pages, const dsv_tensor* page_table, const dsv_tensor* refcount,
+                      dsv_tensor* info, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  dsv::CompactArgs a{};
+  if (kv_pages == nullptr || kv_pages->ndim != 6) return fail(DSV_ERR_INVALID, "kv_pages must be [L, 2, P, Hk, page, D]");
+  if ((rc = check_book(page_table, refcount, nullptr, kv_pages->shape[4], a.book)) != DSV_OK) return rc;
+  if ((rc = check_page_data(kv_pages, a.book.P, a.data)) != DSV_OK) return rc;
+  const dsv_tensor* written[3] = {kv_pages, page_table, refcount};
+  for (int i = 1; i < 3; ++i)
+    if (overlap(extent_of("", kv_pages), extent_of("", written[i])))
+      return fail(DSV_ERR_INVALID, "kv_pages overlaps the bookkeeping");
+  if ((rc = check_info(info, written, 3)) != DSV_OK) return rc;
+  PagesPlan p;
+  if (!pages_plan(a.book.P, a.book.B, 0, p)) return fail(DSV_ERR_UNSUPPORTED, "sizes out of range");
+  if ((rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+  char* w = static_cast<char*>(workspace);
+  a.info = static_cast<int32_t*>(info->data);
+  a.to = reinterpret_cast<int32_t*>(w);
+  a.src = a.to + a.book.P;
+  a.dst = a.src + (a.book.P + 1) / 2;
+  a.state = reinterpret_cast<int32_t*>(w + p.list_bytes + p.off_bytes);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_compact(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "page compact launch");
+  return DSV_OK;
+}
+
+}  // extern "C"

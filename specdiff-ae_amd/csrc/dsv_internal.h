@@ -205,6 +205,86 @@ struct BundleArgs {
   int32_t* bundle_of;                      // optional [B, M] bundle of each node (-1: none)
 };
 
+// Arguments of the verification of drafted tokens from given random numbers.
+constexpr int kSpecMaxM = 1024;            // tree nodes
+constexpr int kSpecThreads = 256;
+constexpr int kSpecSub = 4096;             // vocabulary entries per partial sum
+struct SpecState {
+  double c;                                // share of the draft's row taken from the last node's
+  int32_t node, len, nrej, pad;            // last node, path length, rejected tokens listed in rej
+};
+struct SpecArgs {
+  int dtype;                               // dsv_dtype of target and dprobs
+  int T, M;
+  int64_t V;
+  const void* target; int64_t t_st, t_sm;  // [T, M, V] target probabilities (vocab stride 1)
+  const void* dprobs; int64_t q_st, q_sm;  // optional [T, M, V] draft probabilities
+  const int64_t* draft; int64_t d_st, d_sm;
+  const int64_t* parent; int64_t p_st, p_sm;
+  const float* uniform; int64_t u_st, u_sm;  // [T, M]: node 0's for the draw, the others' for their tests
+  int64_t* out_path; int64_t op_st;
+  int64_t* out_tok; int64_t ot_st;
+  int64_t* out_info; int64_t oi_st;
+  SpecState* state;                        // [T]
+  int32_t* rej;                            // [T, M]
+  double* part;                            // [T, nsub]
+  int64_t nsub;                            // sub-blocks of a row
+  int nwg;                                 // workgroups per tree
+};
+
+// Arguments of the page operations.  The bookkeeping of a pool lives on the
+// device: page_table [B, n_log] (-1: no page), refcount [P] (0: free) and
+// seqlens [B] (tokens).
+constexpr int kPlanThreads = 1024;         // the planning kernels' one workgroup
+constexpr int kPageMaxSeqs = 1 << 17;      // sequences (two LDS bitmaps)
+struct PageBook {
+  int32_t* table; int64_t t_sb;            // page_table and its row stride
+  int32_t* ref;
+  void* lens; int lens_i64;
+  int64_t B, n_log, P;
+  int ps_shift;
+};
+struct PageIndex {
+  const void* p; int is64; int64_t stride;
+};
+// Page contents: kv_pages [L, 2, P, Hk, page, D] as slabs (layer, half) of
+// pages of n1 x n2 rows of row16 16-byte chunks (strides in bytes).
+struct PageData {
+  char* kv;
+  int64_t s_l, s_h, s_p, s_1, s_2;
+  int n_l;                                 // layers
+  int n1, n2, row16;
+  int contiguous;                          // a page is one run of n1 * n2 * row16 chunks
+};
+struct ForkArgs {
+  PageBook book;
+  PageData data;
+  PageIndex parents, children; int64_t n;
+  int32_t* info;                           // [3]
+  int32_t* src; int32_t* dst;              // [n] page pairs (dst -1: none)
+  int32_t* state;                          // [1]: pairs to carry out (n or 0)
+};
+struct ExtendArgs {
+  PageBook book;
+  PageIndex newlens;
+  int32_t* info;
+  int32_t* list;                           // [P] pages taken
+  int64_t* off;                            // [B] a sequence's first place in list
+};
+struct FreeArgs {
+  PageBook book;
+  PageIndex seqs; int64_t n;
+  int64_t window, sinks;                   // window 0: every page
+};
+struct CompactArgs {
+  PageBook book;                           // (lens unused)
+  PageData data;
+  int32_t* info;
+  int32_t* src; int32_t* dst;              // [P / 2] page pairs
+  int32_t* to;                             // [P] new place of a page at or behind the pages in use
+  int32_t* state;                          // [2]: pages in use, pairs
+};
+
 // Arguments of the lm_head fused with the acceptance statistics.
 constexpr int kLmKS = 4;                   // 16-element MFMA sub-steps per step
 constexpr int kLmVocab = 256;              // vocabulary rows per workgroup
@@ -256,6 +336,11 @@ hipError_t launch_accept_from_parts(const AcceptArgs& a, const float4* part, con
 hipError_t launch_commit(const CommitArgs& a, hipStream_t s);
 hipError_t launch_append(const AppendArgs& a, hipStream_t s);
 hipError_t launch_bundle_order(const BundleArgs& a, hipStream_t s);
+hipError_t launch_spec(const SpecArgs& a, hipStream_t s);
+hipError_t launch_fork(const ForkArgs& a, hipStream_t s);
+hipError_t launch_extend(const ExtendArgs& a, hipStream_t s);
+hipError_t launch_free(const FreeArgs& a, hipStream_t s);
+hipError_t launch_compact(const CompactArgs& a, hipStream_t s);
 // Vocabulary ranges of the acceptance statistics: sets a.chunk and a.nchunk
 // from the logits layout, T, M, V and the GPU's CU count.
 void accept_chunking(AcceptArgs& a, int cus);

@@ -1,0 +1,473 @@
+// dsv_pages.hip — page operations of a paged KV cache on gfx950: fork, extend,
+// free and compact, on device tables and reference counts.
+//
+// Bookkeeping.  A pool of P pages is shared by B sequences: page_table
+// [B, n_log] names each sequence's pages (-1: none), refcount [P] counts the
+// tables' entries (0: free), seqlens [B] holds the tokens.  Every operation
+// reads and writes these on the device, so a serving loop needs no host round
+// trip.  Pages are taken in ascending order, for the requests in ascending
+// order: results do not depend on which thread comes first (reference counts
+// change by integer atomics, whose order does not matter).
+//
+// Split.  fork and compact are two launches: a plan by one workgroup (who gets
+// which page: prefix sums over the counts, 4 bytes a page), then the copies by
+// the whole chip.  extend is the plan alone, free one launch over the entries.
+// The plan is latency, a few passes of 64 KiB; the copies are bound by HBM:
+// each page is read and written once, in 16-byte pieces, eight in flight per
+// thread.
+//
+// Reference: core/kv_cache/paged_kv.py:81-166 (allocation, sharing with copy
+// on write, release) and :364-402 (defragmentation) keep this on the host.
+
+#include "dsv_internal.h"
+
+namespace dsv {
+
+namespace {
+
+constexpr int kPT = kPlanThreads;
+constexpr int kPW = kPT / 64;       // waves of the planning workgroup
+constexpr int kScanK = 16;          // entries per thread and scan step
+constexpr int kScanStep = kPT * kScanK;
+
+__device__ __forceinline__ int64_t get(const PageIndex& x, int64_t i) {
+  return x.is64 ? reinterpret_cast<const int64_t*>(x.p)[i * x.stride]
+                : (int64_t) reinterpret_cast<const int32_t*>(x.p)[i * x.stride];
+}
+__device__ __forceinline__ int64_t seqlen(const PageBook& b, int64_t i) {
+  return b.lens_i64 ? reinterpret_cast<const int64_t*>(b.lens)[i] : (int64_t) reinterpret_cast<const int32_t*>(b.lens)[i];
+}
+__device__ __forceinline__ void set_seqlen(const PageBook& b, int64_t i, int64_t n) {
+  if (b.lens_i64)
+    reinterpret_cast<int64_t*>(b.lens)[i] = n;
+  else
+    reinterpret_cast<int32_t*>(b.lens)[i] = (int32_t)n;
+}
+
+// Exclusive scan of one value per thread over the planning workgroup.
+__device__ __forceinline__ int64_t scan1(int64_t x, int64_t* scratch, int64_t& total) {
+  int64_t inc = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(inc, o);
+    if ((int)(threadIdx.x & 63) >= o) inc += y;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = inc;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kPW; ++i) {
+    if (i == (int)(threadIdx.x >> 6)) before = total;
+    total += scratch[i];
+  }
+  return before + inc - x;
+}
+
+// Visits the entries of [lo, hi) that satisfy pred in ascending order: each
+// calls emit(index, rank), rank counted from 0; stops after the step in which
+// `limit` were found.  Returns how many were found (more than limit possible).
+// Entry lo + step * kScanStep + k * kPT + tid belongs to thread tid, so loads
+// are whole lines; a step is one round of 16 loads in flight.
+template <typename Pred, typename Emit>
+__device__ int64_t scan_entries(int64_t lo, int64_t hi, int64_t limit, int32_t* cnt, Pred pred, Emit emit) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t found = 0;
+  for (int64_t s0 = lo; s0 < hi && found < limit; s0 += kScanStep) {
+    uint32_t bits = 0;
+    bool f[kScanK];
+#pragma unroll
+    for (int k = 0; k < kScanK; ++k) {
+      const int64_t i = s0 + k * kPT + threadIdx.x;
+      f[k] = i < hi && pred(i);
+    }
+    uint64_t mask[kScanK];
+#pragma unroll
+    for (int k = 0; k < kScanK; ++k) {
+      mask[k] = __ballot(f[k]);
+      bits |= (f[k] ? 1u : 0u) << k;
+    }
+    __syncthreads();  // the previous step's counts have been read
+    if (lane == 0) {
+#pragma unroll
+      for (int k = 0; k < kScanK; ++k) cnt[k * kPW + wave] = __builtin_popcountll(mask[k]);
+    }
+    __syncthreads();
+    // Exclusive scan of the kScanK * kPW counts by wave 0, four a lane.
+    static_assert(kScanK * kPW == 256, "four counts a lane");
+    if (wave == 0) {
+      int v[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = cnt[lane * 4 + e];
+        sum += v[e];
+      }
+      int inc = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(inc, o);
+        if (lane >= o) inc += y;
+      }
+      int run = inc - sum;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        cnt[lane * 4 + e] = run;
+        run += v[e];
+      }
+      if (lane == 63) cnt[256] = inc;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kScanK; ++k)
+      if ((bits >> k) & 1u)
+        emit(s0 + k * kPT + threadIdx.x,
+             found + cnt[k * kPW + wave] + __builtin_popcountll(mask[k] & ((1ull << lane) - 1ull)));
+    found += cnt[256];
+  }
+  return found;
+}
+
+// ---- copies ---------------------------------------------------------------
+
+constexpr int kCopyT = 256;
+constexpr int kCopyN = 8;                          // 16-byte chunks per thread and piece
+constexpr int kCopyPiece = kCopyT * kCopyN;        // chunks of a piece
+
+// Copies page src[i] to dst[i] of every slab for the pairs [0, n), the pieces
+// shared out over the workgroups [wg, wg + step, ..).  Pairs with dst < 0 are
+// skipped.
+template <bool CONTIG>
+__device__ __forceinline__ void copy_pages(const PageData& d, const int32_t* src, const int32_t* dst, int64_t n,
+                                           int64_t wg, int64_t step) {
+  const int chunks = d.n1 * d.n2 * d.row16;
+  const int pieces = (chunks + kCopyPiece - 1) / kCopyPiece;
+  const int64_t slabs = 2 * (int64_t)d.n_l;
+  const int64_t items = n * slabs * pieces;
+  for (int64_t it = wg; it < items; it += step) {
+    const int piece = (int)(it % pieces);
+    const int64_t r = it / pieces;
+    const int64_t slab = r % slabs, i = r / slabs;
+    const int32_t to = dst[i], from = src[i];
+    if (to < 0) continue;
+    char* base = d.kv + (slab >> 1) * d.s_l + (slab & 1) * d.s_h;
+    const char* s = base + from * d.s_p;
+    char* t = base + to * d.s_p;
+    u32x4 x[kCopyN];
+    int64_t off[kCopyN];
+#pragma unroll
+    for (int k = 0; k < kCopyN; ++k) {
+      const int c = piece * kCopyPiece + k * kCopyT + (int)threadIdx.x;
+      if (CONTIG) {
+        off[k] = (int64_t)c * 16;
+      } else {
+        const int row = c / d.row16;
+        off[k] = (int64_t)(row / d.n2) * d.s_1 + (int64_t)(row % d.n2) * d.s_2 + (int64_t)(c - row * d.row16) * 16;
+      }
+      if (c < chunks) x[k] = *reinterpret_cast<const u32x4*>(s + off[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kCopyN; ++k)
+      if (piece * kCopyPiece + k * kCopyT + (int)threadIdx.x < chunks) *reinterpret_cast<u32x4*>(t + off[k]) = x[k];
+  }
+}
+
+// ---- fork -------------------------------------------------------------------
+
+// Checks the pairs, finds the pages for the copies of partly filled last
+// pages and, if all is well, takes them; otherwise nothing changes.
+__global__ void __launch_bounds__(kPT) fork_plan_kernel(const ForkArgs a) {
+  __shared__ uint32_t is_child[kPageMaxSeqs / 32], is_parent[kPageMaxSeqs / 32];
+  __shared__ int64_t scratch[kPW];
+  __shared__ int32_t cnt[257];
+  __shared__ int32_t bad;
+  const PageBook& b = a.book;
+  const int64_t ps = 1ll << b.ps_shift;
+  for (int64_t i = threadIdx.x; i < (b.B + 31) / 32; i += kPT) is_child[i] = is_parent[i] = 0;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < a.n; i += kPT) {
+    const int64_t p = get(a.parents, i), c = get(a.children, i);
+    bool ok = p >= 0 && p < b.B && c >= 0 && c < b.B && p != c;
+    if (ok) {
+      const int64_t len = seqlen(b, p);
+      ok = len >= 0 && len <= b.n_log * ps && seqlen(b, c) == 0;
+      ok = (atomicOr(&is_child[c >> 5], 1u << (c & 31)) >> (c & 31) & 1u) == 0 && ok;
+      atomicOr(&is_parent[p >> 5], 1u << (p & 31));
+    }
+    if (!ok) atomicAdd(&bad, 1);
+  }
+  __syncthreads();
+  // A child that is also a parent of this call: its state would depend on the order.
+  for (int64_t i = threadIdx.x; i < a.n; i += kPT) {
+    const int64_t c = get(a.children, i);
+    if (c >= 0 && c < b.B && (is_parent[c >> 5] >> (c & 31) & 1u)) atomicAdd(&bad, 1);
+  }
+  __syncthreads();
+  const int refused = bad;
+  // The pairs with a partly filled last page, in order: src, and in dst the rank.
+  int64_t want = 0;
+  if (refused == 0) {
+    for (int64_t i0 = 0; i0 < a.n; i0 += kPT) {
+      const int64_t i = i0 + threadIdx.x;
+      int32_t page = -1;
+      if (i < a.n) {
+        const int64_t p = get(a.parents, i), len = seqlen(b, p);
+        if ((len & (ps - 1)) != 0) {
+          page = b.table[p * b.t_sb + (len >> b.ps_shift)];
+          if (page < 0 || page >= b.P) page = -1;
+        }
+      }
+      int64_t total;
+      const int64_t rank = want + scan1(page >= 0 ? 1 : 0, scratch, total);
+      if (i < a.n) {
+        a.src[i] = page;
+        a.dst[i] = page >= 0 ? (int32_t)rank : -1;
+      }
+      want += total;
+    }
+  }
+  // list[rank] = page, kept behind the pairs.
+  int32_t* list = a.dst + a.n;
+  const int64_t found = scan_entries(
+      0, b.P, want, cnt, [&](int64_t i) { return b.ref[i] == 0; },
+      [&](int64_t i, int64_t r) {
+        if (r < want) list[r] = (int32_t)i;
+      });
+  const bool go = refused == 0 && found >= want;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.state[0] = go ? (int32_t)a.n : 0;
+    a.info[0] = go ? (int32_t)want : 0;
+    a.info[1] = go ? 0 : (int32_t)(want > found ? want - found : 0);
+    a.info[2] = refused;
+  }
+  if (!go) return;
+  for (int64_t i = threadIdx.x; i < a.n; i += kPT) {
+    if (a.dst[i] >= 0) {
+      const int32_t page = list[a.dst[i]];
+      a.dst[i] = page;
+      b.ref[page] = 1;
+    }
+    set_seqlen(b, get(a.children, i), seqlen(b, get(a.parents, i)));
+  }
+}
+
+template <bool CONTIG>
+__global__ void __launch_bounds__(kCopyT) fork_kernel(const ForkArgs a, int64_t rows_wg) {
+  const int64_t n = a.state[0];
+  const PageBook& b = a.book;
+  if (blockIdx.x < rows_wg) {
+    // The children's table rows and the shared pages' counts.
+    const int64_t ps = 1ll << b.ps_shift;
+    for (int64_t x = (int64_t)blockIdx.x * kCopyT + threadIdx.x; x < n * b.n_log; x += rows_wg * kCopyT) {
+      const int64_t i = x / b.n_log, j = x - i * b.n_log;
+      const int64_t p = get(a.parents, i), len = seqlen(b, p);
+      int32_t page = j * ps < len ? b.table[p * b.t_sb + j] : -1;
+      if ((j + 1) * ps <= len) {
+        if (page >= 0 && page < b.P) atomicAdd(&b.ref[page], 1);
+      } else if (page >= 0 && a.dst[i] >= 0) {
+        page = a.dst[i];
+      }
+      b.table[get(a.children, i) * b.t_sb + j] = page;
+    }
+    return;
+  }
+  copy_pages<CONTIG>(a.data, a.src, a.dst, n, blockIdx.x - rows_wg, gridDim.x - rows_wg);
+}
+
+// ---- extend ----------------------------------------------------------------
+
+__global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
+  __shared__ int64_t scratch[kPW];
+  __shared__ int32_t cnt[257];
+  __shared__ int32_t bad;
+  const PageBook& b = a.book;
+  const int64_t ps = 1ll << b.ps_shift;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  auto pages_of = [&](int64_t n) { return (n >> b.ps_shift) + ((n & (ps - 1)) != 0 ? 1 : 0); };
+  int64_t want = 0;
+  for (int64_t i0 = 0; i0 < b.B; i0 += kPT) {
+    const int64_t i = i0 + threadIdx.x;
+    int64_t need = 0;
+    if (i < b.B) {
+      const int64_t len = seqlen(b, i), n = get(a.newlens, i);
+      if (n > len) {
+        if (len < 0 || n > b.n_log * ps)
+          atomicAdd(&bad, 1);
+        else
+          need = pages_of(n) - pages_of(len);
+      }
+    }
+    int64_t total;
+    const int64_t at = want + scan1(need, scratch, total);
+    if (i < b.B) a.off[i] = at;
+    want += total;
+  }
+  __syncthreads();
+  const int refused = bad;
+  const int64_t limit = refused == 0 ? want : 0;
+  const int64_t found = scan_entries(
+      0, b.P, limit, cnt, [&](int64_t i) { return b.ref[i] == 0; },
+      [&](int64_t i, int64_t r) {
+        if (r < limit) a.list[r] = (int32_t)i;
+      });
+  const bool go = refused == 0 && found >= want;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.info[0] = go ? (int32_t)want : 0;
+    a.info[1] = refused == 0 && want > found ? (int32_t)(want - found) : 0;
+    a.info[2] = refused;
+  }
+  if (!go) return;
+  // A wave per sequence: its entries from its place in the list.
+  for (int64_t i = threadIdx.x >> 6; i < b.B; i += kPW) {
+    const int64_t len = seqlen(b, i), n = get(a.newlens, i);
+    if (n <= len) continue;
+    const int64_t have = pages_of(len), need = pages_of(n) - have, at = a.off[i];
+    for (int64_t j = threadIdx.x & 63; j < need; j += 64) {
+      const int32_t page = a.list[at + j];
+      b.table[i * b.t_sb + have + j] = page;
+      b.ref[page] = 1;
+    }
+    if ((threadIdx.x & 63) == 0) set_seqlen(b, i, n);
+  }
+}
+
+// ---- free -------------------------------------------------------------------
+
+__global__ void __launch_bounds__(256) free_kernel(const FreeArgs a) {
+  const PageBook& b = a.book;
+  const int64_t ps = 1ll << b.ps_shift;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < a.n * b.n_log; x += (int64_t)gridDim.x * 256) {
+    const int64_t i = x / b.n_log, j = x - i * b.n_log;
+    const int64_t s = get(a.seqs, i);
+    if (s < 0 || s >= b.B) continue;
+    // Behind the window: every token of the page lies after the sinks and is
+    // out of sight of the next token, at position len, which sees n > len - window.
+    const bool gone = a.window == 0 || (j * ps >= a.sinks && (j + 1) * ps <= seqlen(b, s) - a.window + 1);
+    if (gone) {
+      // A sequence named twice gives its pages back once.
+      const int32_t page = atomicExch(&b.table[s * b.t_sb + j], -1);
+      if (page >= 0 && page < b.P && atomicSub(&b.ref[page], 1) <= 0) atomicAdd(&b.ref[page], 1);
+    }
+    if (a.window == 0 && j == 0) set_seqlen(b, s, 0);
+  }
+}
+
+// ---- compact ----------------------------------------------------------------
+
+// The pages in use at or behind n = their number move, in order, into the
+// free pages below n.
+__global__ void __launch_bounds__(kPT) compact_plan_kernel(const CompactArgs a) {
+  __shared__ int64_t scratch[kPW];
+  __shared__ int32_t cnt[257];
+  const PageBook& b = a.book;
+  int64_t mine = 0;
+  for (int64_t i0 = 0; i0 < b.P; i0 += kScanStep) {
+    int32_t v[kScanK];
+#pragma unroll
+    for (int k = 0; k < kScanK; ++k) {
+      const int64_t i = i0 + k * kPT + threadIdx.x;
+      v[k] = i < b.P ? b.ref[i] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kScanK; ++k) mine += v[k] > 0 ? 1 : 0;
+  }
+  int64_t n;
+  scan1(mine, scratch, n);
+  const int64_t holes = scan_entries(
+      0, n, b.P, cnt, [&](int64_t i) { return b.ref[i] <= 0; }, [&](int64_t i, int64_t r) { a.dst[r] = (int32_t)i; });
+  const int64_t moved = scan_entries(
+      n, b.P, b.P, cnt,
+      [&](int64_t i) {
+        a.to[i] = (int32_t)i;
+        return b.ref[i] > 0;
+      },
+      [&](int64_t i, int64_t r) { a.src[r] = (int32_t)i; });
+  (void)holes;  // equal: n pages are in use, those below n and the moved ones
+  __syncthreads();
+  for (int64_t r = threadIdx.x; r < moved; r += kPT) {
+    const int32_t s = a.src[r], d = a.dst[r];
+    a.to[s] = d;
+    b.ref[d] = b.ref[s];
+    b.ref[s] = 0;
+  }
+  if (threadIdx.x == 0) {
+    a.state[0] = (int32_t)n;
+    a.state[1] = (int32_t)moved;
+    a.info[0] = (int32_t)n;
+    a.info[1] = (int32_t)moved;
+    a.info[2] = 0;
+  }
+}
+
+template <bool CONTIG>
+__global__ void __launch_bounds__(kCopyT) compact_kernel(const CompactArgs a, int64_t rows_wg) {
+  const PageBook& b = a.book;
+  if (blockIdx.x < rows_wg) {
+    const int64_t n = a.state[0];
+    for (int64_t x = (int64_t)blockIdx.x * kCopyT + threadIdx.x; x < b.B * b.n_log; x += rows_wg * kCopyT) {
+      const int64_t i = x / b.n_log, j = x - i * b.n_log;
+      int32_t* e = &b.table[i * b.t_sb + j];
+      const int32_t page = *e;
+      if (page >= n && page < b.P) *e = a.to[page];
+    }
+    return;
+  }
+  copy_pages<CONTIG>(a.data, a.src, a.dst, a.state[1], blockIdx.x - rows_wg, gridDim.x - rows_wg);
+}
+
+// Workgroups for the table's entries and for the copies (at most pairs pairs).
+int64_t entry_wgs(int64_t entries) {
+  const int64_t n = (entries + kCopyT - 1) / kCopyT;
+  return n < 1 ? 1 : (n > 256 ? 256 : n);
+}
+int64_t copy_wgs(const PageData& d, int64_t pairs) {
+  const int64_t pieces = ((int64_t)d.n1 * d.n2 * d.row16 + kCopyPiece - 1) / kCopyPiece;
+  const int64_t n = pairs * 2 * d.n_l * pieces;
+  return n > 2048 ? 2048 : n;
+}
+
+}  // namespace
+
+hipError_t launch_fork(const ForkArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPT), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = entry_wgs(a.n * a.book.n_log);
+  const dim3 grid((unsigned)(rows + copy_wgs(a.data, a.n)));
+  if (a.data.contiguous)
+    hipLaunchKernelGGL(fork_kernel<true>, grid, dim3(kCopyT), 0, s, a, rows);
+  else
+    hipLaunchKernelGGL(fork_kernel<false>, grid, dim3(kCopyT), 0, s, a, rows);
+  return hipGetLastError();
+}
+
+hipError_t launch_extend(const ExtendArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(extend_kernel, dim3(1), dim3(kPT), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_free(const FreeArgs& a, hipStream_t s) {
+  const int64_t n = (a.n * a.book.n_log + 255) / 256;
+  if (n <= 0) return hipSuccess;
+  hipLaunchKernelGGL(free_kernel, dim3((unsigned)(n > 2048 ? 2048 : n)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_compact(const CompactArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPT), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = entry_wgs(a.book.B * a.book.n_log);
+  const dim3 grid((unsigned)(rows + copy_wgs(a.data, a.book.P / 2)));
+  if (a.data.contiguous)
+    hipLaunchKernelGGL(compact_kernel<true>, grid, dim3(kCopyT), 0, s, a, rows);
+  else
+    hipLaunchKernelGGL(compact_kernel<false>, grid, dim3(kCopyT), 0, s, a, rows);
+  return hipGetLastError();
+}
+
+}  // namespace dsv

@@ -10,6 +10,7 @@ tensors that are not on a GPU, a RuntimeError is raised.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -81,6 +82,13 @@ SIGNATURES = {
     "dsv_lmhead_accept_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "dsv_lmhead_accept": (ctypes.c_int, [ctypes.c_int, _P, _P, _P, _P, _P, _I64, ctypes.c_float, ctypes.c_float,
                                          ctypes.c_float, _P, _P, _P, _P, _P, _V, ctypes.c_size_t, _V]),
+    "dsv_spec_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "dsv_spec_accept": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _V, _SZ, _V]),
+    "dsv_pages_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "dsv_pages_fork": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _V, _SZ, _V]),
+    "dsv_pages_extend": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _V, _SZ, _V]),
+    "dsv_pages_free": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _V]),
+    "dsv_pages_compact": (ctypes.c_int, [_P, _P, _P, _P, _V, _SZ, _V]),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -163,6 +171,11 @@ def require_gpu(*tensors: Optional[torch.Tensor]) -> torch.device:
 
 def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to ``device`` (a no-op where it is current)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -34,7 +34,7 @@ import torch
 from .. import _ext
 from ..core.bundle_scheduler import BundleScheduler
 
-__all__ = ["tree_accept", "evaluate_tree", "kv_commit", "verify", "verify_new", "prepare_logits_processor",
+__all__ = ["tree_accept", "speculative_accept", "evaluate_tree", "kv_commit", "verify", "verify_new", "prepare_logits_processor",
            "SamplingParams"]
 
 
@@ -149,6 +149,67 @@ def tree_accept(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Tensor,
     if return_next:
         out["next"] = nxt
     return out
+
+
+def speculative_accept(target_probs: torch.Tensor, draft: torch.Tensor, parent: torch.Tensor, uniform: torch.Tensor,
+                       draft_probs: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
+    """Rejection-sampling acceptance of T drafted trees or chains from given random numbers.
+
+    The accepted path and its next token are distributed as if the target had
+    sampled every token itself.  From the root, the children of the current
+    node are tested in index order; child ``x`` is accepted iff
+    ``u * S * q(x) < w(x)``, where ``w`` starts as the target's row ``p`` and
+    ``S`` as 1, and after a rejection ``w`` becomes the positive part of
+    ``w - S * q`` and ``S`` its sum.  Where no child is accepted the next token
+    is drawn from ``w`` by its cumulative sum.  Without ``draft_probs`` the
+    children are given tokens (``q`` one at the child's token): accepted with
+    the target's probability of the token among those not yet rejected.
+
+    Args:
+        target_probs: [T, M, V] (or [M, V]) bf16/f16/f32, the target's
+            probabilities after every node (after any temperature, top-p or
+            top-k of the caller's).
+        draft: [T, M] int64 drafted tokens (node 0 = root).
+        parent: [T, M-1] int64, as :func:`tree_accept`; a chain is
+            ``torch.arange(-1, M - 2)``.
+        uniform: [T, M] float32 numbers in [0, 1): number 0 draws the next
+            token, number i tests node i.
+        draft_probs: optional, shape and dtype of ``target_probs``: row i is
+            the distribution that the children of node i were drawn from.
+
+    Returns:
+        dict of device tensors: ``path`` [T, M], ``tokens`` [T, M] and ``info``
+        [T, 4] = (last node, accept length, next token, path length), as
+        :func:`tree_accept` returns them (``kv_commit`` takes them).
+    """
+    if target_probs.dim() == 2:
+        target_probs = target_probs.unsqueeze(0)
+        draft_probs = draft_probs.unsqueeze(0) if draft_probs is not None and draft_probs.dim() == 2 else draft_probs
+    if draft.dim() == 1:
+        draft = draft.unsqueeze(0)
+    if parent.dim() == 1:
+        parent = parent.unsqueeze(0)
+    if uniform.dim() == 1:
+        uniform = uniform.unsqueeze(0)
+    dev = _ext.require_gpu(target_probs, draft, parent, uniform, draft_probs)
+    if target_probs.dim() != 3:
+        raise ValueError(f"target_probs must be [T, M, V] (got {tuple(target_probs.shape)})")
+    T, M, V = target_probs.shape
+    if draft.dtype != torch.int64:
+        draft = draft.to(torch.int64)
+    if parent.dtype != torch.int64:
+        parent = parent.to(torch.int64)
+    lib = _ext.load()
+    with _ext.on_device(dev):
+        path = torch.empty((T, M), dtype=torch.int64, device=dev)
+        tokens = torch.empty((T, M), dtype=torch.int64, device=dev)
+        info = torch.empty((T, 4), dtype=torch.int64, device=dev)
+        ws = _ext.workspace(lib.dsv_spec_workspace_bytes(T, M, V), dev)
+        rc = lib.dsv_spec_accept(_ext.desc(target_probs), _ext.desc(draft), _ext.desc(parent), _ext.desc(uniform),
+                                 _ext.desc(draft_probs), _ext.desc(path), _ext.desc(tokens), _ext.desc(info),
+                                 ws.data_ptr(), ws.numel(), _ext.stream_of(dev))
+    _ext.check(rc, "speculative_accept")
+    return {"path": path, "tokens": tokens, "info": info}
 
 
 def lmhead_tree_accept(hidden: torch.Tensor, weight: torch.Tensor, draft: torch.Tensor, parent: torch.Tensor,
