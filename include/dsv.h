@@ -244,6 +244,52 @@ int dsv_tree_verify_noalloc(const dsv_tensor* q, const dsv_tensor* k,
                             const dsv_tensor* row_perm, dsv_tensor* out,
                             dsv_tensor* lse, void* stream);
 
+/*
+ * Workspace of dsv_window_attention for queries [B, M, H, D] of dtype
+ * (dsv_dtype) over a cache of n_keys keys with Hk heads.  0 on invalid
+ * arguments and on sizes that the call refuses (those of
+ * dsv_attn_workspace_bytes).
+ */
+size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk,
+                                  int64_t D, int dtype, int64_t n_keys,
+                                  int64_t window, int64_t sinks, int has_tree);
+
+/*
+ * Attention through a sliding window with a few first tokens that stay
+ * visible: flash_attn_with_kvcache (runtime/attention_compat.py:103-132) with
+ * window, sinks, a page table and an optional tree of new tokens, for models
+ * with windowed layers and for caches that keep first and recent tokens
+ * (draft/draft_network.py:1250-1331).
+ * The M queries of sequence b are the last M of its len_b tokens, n0 = len_b -
+ * M.  Query m has position p = n0 + m and its past is the keys n <= p.  With
+ * parent it is node m of a tree whose keys follow the prefix: p = n0 + its
+ * depth, and its past is every key n < n0, its ancestors' and its own.  Of its
+ * past it sees the keys at positions > p - window or < sinks (key n0 + j of a
+ * tree stands at position n0 + the depth of j).
+ *   q            [B, M, H, D] bf16|f16|f32
+ *   k, v         dense caches [B, N, Hk, D], or page-pool halves
+ *                [P, Hk, page, D] with page_table [n_pages] or [B, n_pages]
+ *                int32|int64 (page a power of two; entries that no query needs
+ *                may be anything, -1 among them; others are clamped to [0, P))
+ *   cache_seqlens optional [B] int32|int64: len_b, the new tokens included,
+ *                clamped to [0, n_keys]; ndim 0: n_keys for every sequence
+ *   n_keys       < 0 (or beyond the cache): all that the cache holds
+ *   window >= 1; sinks >= 0
+ *   parent       optional [M] or [B, M] int32|int64 (as dsv_tree_verify),
+ *                M <= 1024; ndim 0: causal
+ *   out          [B, M, H, D] bf16|f16|f32;  lse optional [B, H, M] f32
+ * A query that sees no key gets out = 0 and lse = -inf; that holds for those
+ * before the first token (len_b < M) and, with a tree, for every query of a
+ * sequence with len_b < M.  Keys and values that a query does not see never
+ * affect it, whatever they hold.  out and lse may not overlap an input.
+ */
+int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k,
+                         const dsv_tensor* v, const dsv_tensor* page_table,
+                         const dsv_tensor* cache_seqlens, int64_t n_keys,
+                         int64_t window, int64_t sinks, const dsv_tensor* parent,
+                         dsv_tensor* out, dsv_tensor* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------- */
 /* Acceptance (kernel 4)                                                      */
 /* ------------------------------------------------------------------------- */

@@ -6,6 +6,7 @@
 #include "dsv_attn_geo.h"
 #include "dsv_check.h"
 #include "dsv_internal.h"
+#include "dsv_window.h"
 
 #include <algorithm>
 #include <cmath>
@@ -1851,6 +1852,213 @@ int dsv_pages_compact(const dsv_tensor* kv_pages, const dsv_tensor* page_table, 
   if (g_dry_run) return DSV_OK;
   const hipError_t e = dsv::launch_compact(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "page compact launch");
+  return DSV_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Windowed attention
+// ---------------------------------------------------------------------------
+
+namespace {
+
+struct WinPlan {
+  int G = 0, R = 0, MW = 0, rpb = 0, n_rb = 0, splits = 1;
+  size_t opart_bytes = 0, ml_bytes = 0, depth_bytes = 0, total = 0;
+  const char* err = nullptr;
+};
+
+bool win_args_ok(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys, int64_t window,
+                 int64_t sinks) {
+  return B >= 1 && M >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && (D == 64 || D == 128) && dtype >= DSV_BF16 &&
+         dtype <= DSV_F32 && n_keys >= 0 && window >= 1 && sinks >= 0;
+}
+
+WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys, int64_t window,
+                 int64_t sinks, bool tree) {
+  WinPlan p;
+  const bool in_range = B <= (1 << 20) && M <= (1 << 24) && H <= (1 << 16) && n_keys <= ((int64_t)1 << 35);
+  const int64_t R = in_range ? (H / Hk) * M : 0;
+  if (!in_range || R > ((int64_t)1 << 24) || B * Hk * R > ((int64_t)1 << 30)) {
+    p.err = "sizes beyond the windowed attention's range (batch <= 2^20, heads <= 65536, keys <= 2^35, query heads / "
+            "key heads x rows <= 2^24, batch x query heads x rows <= 2^30)";
+    return p;
+  }
+  p.G = (int)(H / Hk);
+  p.R = (int)R;
+  p.MW = tree ? (int)((M + 63) / 64) : 0;
+  p.rpb = dtype == DSV_F32 || R <= 16 ? 16 : 32;
+  p.n_rb = (int)((R + p.rpb - 1) / p.rpb);
+  // Splits over the keys: four waves per workgroup and at least one tile per
+  // wave, until there are four workgroups per CU.
+  const int64_t units = B * Hk * p.n_rb;
+  const int64_t span = tree ? M : std::min<int64_t>(M, p.rpb / p.G + 2);
+  const int64_t reach = std::min(n_keys, window + span) / 32 + 2 + std::min(n_keys, sinks) / 32;
+  const int64_t want = std::max<int64_t>(1, (int64_t)device_cus() * 4 / units);
+  p.splits = (int)std::max<int64_t>(1, std::min(want, reach / 4));
+  const size_t rows = p.splits > 1 ? (size_t)B * Hk * p.splits * R : 0;
+  p.opart_bytes = align_up(rows * D * sizeof(float), 256);
+  p.ml_bytes = align_up(rows * sizeof(float2), 256);
+  p.depth_bytes = tree ? align_up((size_t)B * M * sizeof(int32_t), 256) : 0;
+  p.total = p.opart_bytes + p.ml_bytes + p.depth_bytes + (tree ? align_up((size_t)B * M * p.MW * 8, 256) : 0);
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys,
+                                  int64_t window, int64_t sinks, int has_tree) {
+  if (!win_args_ok(B, M, H, Hk, D, dtype, n_keys, window, sinks) || (has_tree && M > dsv::kTreeMaxM)) return 0;
+  const WinPlan p = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0);
+  return p.err != nullptr ? 0 : std::max<size_t>(p.total, 256);
+}
+
+int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_tensor* v, const dsv_tensor* page_table,
+                         const dsv_tensor* cache_seqlens, int64_t n_keys, int64_t window, int64_t sinks,
+                         const dsv_tensor* parent, dsv_tensor* out, dsv_tensor* lse, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_q_out(q, out)) != DSV_OK) return rc;
+  const int64_t B = q->shape[0], M = q->shape[1], H = q->shape[2], D = q->shape[3];
+  if (B < 1 || M < 1 || H < 1) return fail(DSV_ERR_INVALID, "q must hold at least one query");
+  if (window < 1) return fail(DSV_ERR_INVALID, "window must be at least 1 (got %lld)", (long long)window);
+  if (sinks < 0) return fail(DSV_ERR_INVALID, "sinks must be >= 0");
+  dsv::WinArgs a{};
+  int64_t Hk = 0, cap = 0;
+  if (present(page_table)) {
+    if ((rc = check_nd(k, "k_pages", 4)) != DSV_OK) return rc;
+    if ((rc = check_nd(v, "v_pages", 4)) != DSV_OK) return rc;
+    if ((rc = check_vec16(k, "k_pages")) != DSV_OK) return rc;
+    if ((rc = check_vec16(v, "v_pages")) != DSV_OK) return rc;
+    for (int i = 0; i < 4; ++i)
+      if (k->shape[i] != v->shape[i]) return fail(DSV_ERR_INVALID, "k_pages and v_pages shapes differ");
+    if (k->dtype != q->dtype || v->dtype != q->dtype) return fail(DSV_ERR_INVALID, "q and pages must share a dtype");
+    if (k->shape[3] != D) return fail(DSV_ERR_INVALID, "page head_dim differs from q");
+    if (k->shape[0] < 1 || k->shape[0] > 0x7fffffff) return fail(DSV_ERR_INVALID, "the pool must hold 1 to 2^31 - 1 pages");
+    const int sh = log2_exact(k->shape[2]);
+    if (sh < 0) return fail(DSV_ERR_UNSUPPORTED, "page_size %lld must be a power of two", (long long)k->shape[2]);
+    if ((rc = check_nd(page_table, "page_table", page_table->ndim)) != DSV_OK) return rc;
+    if (page_table->ndim != 1 && page_table->ndim != 2) return fail(DSV_ERR_INVALID, "page_table must be 1-d or 2-d");
+    if (page_table->dtype != DSV_I32 && page_table->dtype != DSV_I64)
+      return fail(DSV_ERR_INVALID, "page_table must be int32 or int64");
+    if (page_table->ndim == 2 && page_table->shape[0] != B && page_table->shape[0] != 1)
+      return fail(DSV_ERR_INVALID, "page_table batch must be 1 or B");
+    const int64_t npt = page_table->shape[page_table->ndim - 1];
+    if (npt > 1 && page_table->stride[page_table->ndim - 1] != 1)
+      return fail(DSV_ERR_INVALID, "page_table innermost stride must be 1");
+    Hk = k->shape[1];
+    a.k_sp = k->stride[0];
+    a.k_sh = k->stride[1];
+    a.k_st = k->stride[2];
+    a.v_sp = v->stride[0];
+    a.v_sh = v->stride[1];
+    a.v_st = v->stride[2];
+    a.pt = page_table->data;
+    a.pt_i64 = page_table->dtype == DSV_I64;
+    a.ps_shift = sh;
+    a.pt_sb = (page_table->ndim == 2 && page_table->shape[0] > 1) ? page_table->stride[0] : 0;
+    a.n_phys = k->shape[0];
+    cap = npt > ((int64_t)1 << 40) >> sh ? (int64_t)1 << 40 : npt << sh;
+  } else {
+    if ((rc = check_kv_dense(k, v, q, "k_cache", "v_cache")) != DSV_OK) return rc;
+    Hk = k->shape[2];
+    a.k_sb = B > 1 ? k->stride[0] : 0;
+    a.k_st = k->stride[1];
+    a.k_sh = k->stride[2];
+    a.v_sb = B > 1 ? v->stride[0] : 0;
+    a.v_st = v->stride[1];
+    a.v_sh = v->stride[2];
+    cap = k->shape[1];
+  }
+  if (Hk < 1 || H % Hk != 0)
+    return fail(DSV_ERR_INVALID, "query heads (%lld) must be a multiple of key heads (%lld)", (long long)H, (long long)Hk);
+  const int64_t n = n_keys < 0 || n_keys > cap ? cap : n_keys;
+  if (present(cache_seqlens)) {
+    if ((rc = check_nd(cache_seqlens, "cache_seqlens", 1)) != DSV_OK) return rc;
+    if ((cache_seqlens->dtype != DSV_I32 && cache_seqlens->dtype != DSV_I64) || cache_seqlens->shape[0] != B ||
+        (B > 1 && cache_seqlens->stride[0] != 1))
+      return fail(DSV_ERR_INVALID, "cache_seqlens must be a contiguous int32 or int64 [B] tensor");
+    a.seqlens = cache_seqlens->data;
+    a.seqlens_i64 = cache_seqlens->dtype == DSV_I64;
+  }
+  dsv::WinTree tree{};
+  if (present(parent)) {
+    if (parent->ndim != 1 && parent->ndim != 2) return fail(DSV_ERR_INVALID, "parent must be [M] or [B, M]");
+    if ((rc = check_nd(parent, "parent", parent->ndim)) != DSV_OK) return rc;
+    if (parent->dtype != DSV_I32 && parent->dtype != DSV_I64) return fail(DSV_ERR_INVALID, "parent must be int32 or int64");
+    if (parent->shape[parent->ndim - 1] != M) return fail(DSV_ERR_INVALID, "parent must have M entries per tree");
+    if (parent->ndim == 2 && parent->shape[0] != B && parent->shape[0] != 1)
+      return fail(DSV_ERR_INVALID, "parent batch must be 1 or B");
+    if (M > dsv::kTreeMaxM) return fail(DSV_ERR_UNSUPPORTED, "trees larger than %d nodes are not supported", dsv::kTreeMaxM);
+    tree.parent = parent->data;
+    tree.i64 = parent->dtype == DSV_I64;
+    tree.sb = (parent->ndim == 2 && parent->shape[0] > 1) ? parent->stride[0] : 0;
+    tree.sm = parent->stride[parent->ndim - 1];
+  }
+  if (present(lse)) {
+    if ((rc = check_nd(lse, "lse", 3)) != DSV_OK) return rc;
+    if (lse->dtype != DSV_F32 || lse->shape[0] != B || lse->shape[1] != H || lse->shape[2] != M)
+      return fail(DSV_ERR_INVALID, "lse must be float32 [B, H, M]");
+    a.lse = static_cast<float*>(lse->data);
+    a.l_sb = lse->stride[0];
+    a.l_sh = lse->stride[1];
+    a.l_sm = lse->stride[2];
+  }
+  // Rows are written while others' inputs are still read.
+  const Extent ins[6] = {extent_of("q", q), extent_of("k", k), extent_of("v", v), extent_of("page_table", page_table),
+                         extent_of("cache_seqlens", cache_seqlens), extent_of("parent", parent)};
+  for (const Extent& in : ins)
+    if (overlap(extent_of("out", out), in) || overlap(extent_of("lse", lse), in))
+      return fail(DSV_ERR_INVALID, "out or lse overlaps %s", in.name);
+  if (overlap(extent_of("out", out), extent_of("lse", lse))) return fail(DSV_ERR_INVALID, "out overlaps lse");
+
+  // (Positions, window and sinks fit well inside 64 bits then.)
+  const int64_t W = std::min<int64_t>(window, (int64_t)1 << 41), S = std::min<int64_t>(sinks, (int64_t)1 << 41);
+  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, tree.parent != nullptr);
+  if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
+  if ((rc = check_workspace(std::max<size_t>(p.total, 256), workspace, workspace_bytes)) != DSV_OK) return rc;
+  a.dtype = q->dtype;
+  a.q = static_cast<const uint16_t*>(q->data);
+  a.q_sb = q->stride[0];
+  a.q_sm = q->stride[1];
+  a.q_sh = q->stride[2];
+  a.k = static_cast<const uint16_t*>(k->data);
+  a.v = static_cast<const uint16_t*>(v->data);
+  a.n_keys = n;
+  a.B = (int)B;
+  a.M = (int)M;
+  a.H = (int)H;
+  a.Hk = (int)Hk;
+  a.G = p.G;
+  a.R = p.R;
+  a.W = W;
+  a.S = S;
+  a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
+  a.rows_per_block = p.rpb;
+  a.n_rb = p.n_rb;
+  a.splits = p.splits;
+  char* w = static_cast<char*>(workspace);
+  a.opart = reinterpret_cast<float*>(w);
+  a.ml = reinterpret_cast<float2*>(w + p.opart_bytes);
+  if (tree.parent != nullptr) {
+    a.depth = reinterpret_cast<const int32_t*>(w + p.opart_bytes + p.ml_bytes);
+    a.bits = reinterpret_cast<const uint64_t*>(w + p.opart_bytes + p.ml_bytes + p.depth_bytes);
+    a.MW = p.MW;
+  }
+  a.out = out->data;
+  a.out_dtype = out->dtype;
+  a.o_sb = out->stride[0];
+  a.o_sm = out->stride[1];
+  a.o_sh = out->stride[2];
+  const int per16 = 16 / elem_size(out->dtype);
+  a.out_vec = (reinterpret_cast<uintptr_t>(out->data) & 15) == 0 && (B == 1 || a.o_sb % per16 == 0) &&
+              (M == 1 || a.o_sm % per16 == 0) && (H == 1 || a.o_sh % per16 == 0);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_window(a, tree, (int)D, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "windowed attention launch");
   return DSV_OK;
 }
 

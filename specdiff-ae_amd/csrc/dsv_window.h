@@ -1,0 +1,87 @@
+// dsv_window.h — launch arguments and key geometry of the windowed attention
+// (dsv_window.hip), shared by the kernels, the host's plan and the CPU tests'
+// emulation of it.
+#pragma once
+
+#include <stdint.h>
+
+#include "dsv_attn_geo.h"
+#include "dsv_internal.h"
+
+namespace dsv {
+
+struct WinArgs {
+  int dtype;                               // dsv_dtype of q, k, v
+  const uint16_t* q;                       // (element strides; fp32 data too)
+  int64_t q_sb, q_sm, q_sh;
+  const uint16_t* k; int64_t k_sb, k_sp, k_sh, k_st;
+  const uint16_t* v; int64_t v_sb, v_sp, v_sh, v_st;
+  const void* pt; int pt_i64, ps_shift;    // page table (nullptr: dense)
+  int64_t pt_sb, n_phys;
+  const void* seqlens; int seqlens_i64;    // optional [B]
+  int64_t n_keys;                          // keys of the cache (lengths are clamped to it)
+  int B, M, H, Hk, G, R;                   // R = G * M rows per KV head, row m * G + g
+  int64_t W, S;                            // window (>= 1) and sinks
+  float scale_log2;                        // log2(e) / sqrt(D)
+  const int32_t* depth;                    // tree: [B, M] depths
+  const uint64_t* bits; int MW;            // tree: [B, M, MW] visible ancestors
+  int rows_per_block, n_rb, splits;
+  float* opart;                            // [B, Hk, splits, R, D] (splits > 1), relative to the maximum
+  float2* ml;                              // [B, Hk, splits, R] (maximum in log2 units, sum)
+  void* out; int out_dtype, out_vec;       // out_vec: rows take 16-byte stores
+  int64_t o_sb, o_sm, o_sh;
+  float* lse; int64_t l_sb, l_sm, l_sh;
+};
+
+struct WinTree {
+  const void* parent;                      // nullptr: causal
+  int i64;
+  int64_t sb, sm;
+};
+
+// Bits [0, x) of a 32-bit word, x clamped to [0, 32].
+DSV_HD uint32_t win_below(int64_t x) { return x <= 0 ? 0u : (x >= 32 ? ~0u : (1u << (int)x) - 1u); }
+
+// The keys of a block of rows: [0, sink) and [lo, hi), as nt tiles of 32: nst
+// tiles from key 0, the others from lo_al (a multiple of 32).  Where the two
+// meet, nst is 0 and lo_al is 0.
+struct WinKeys {
+  int64_t lo, hi, sink, lo_al;
+  int nst, nt;
+  DSV_HD int64_t base(int t) const { return t < nst ? 32ll * t : lo_al + 32ll * (t - nst); }
+  // Does any row of the block see key n?
+  DSV_HD bool has(int64_t n) const { return n < sink || (n >= lo && n < hi); }
+  DSV_HD bool whole(int64_t kb) const { return kb + 32 <= sink || (kb >= lo && kb + 32 <= hi); }
+  // Is every key of the tile seen by every row between positions pmin and pmax?
+  DSV_HD bool seen_by_all(int64_t kb, int64_t pmin, int64_t pmax, int64_t W, int64_t S, int64_t n0, bool tree) const {
+    return (tree ? kb + 32 <= n0 : kb + 31 <= pmin) && (kb > pmax - W || kb + 32 <= S);
+  }
+};
+
+// The keys of rows [r0, r0 + nrows) of a sequence whose new tokens start at n0.
+DSV_HD WinKeys win_keys(int M, int G, int R, int64_t W, int64_t S, bool tree, int64_t n0, int r0, int nrows) {
+  WinKeys k;
+  const int rl = (r0 + nrows < R ? r0 + nrows : R) - 1;
+  // Positions of the first and last row; a tree's rows lie anywhere from n0 on.
+  const int64_t pmin = tree ? n0 : n0 + r0 / G, pmax = tree ? n0 + M - 1 : n0 + rl / G;
+  k.hi = pmax + 1 > 0 ? pmax + 1 : 0;
+  if (tree && n0 < 0) k.hi = 0;
+  k.lo = pmin - W + 1;
+  if (k.lo < 0) k.lo = 0;
+  if (k.lo > k.hi) k.lo = k.hi;
+  k.sink = S < k.hi ? S : k.hi;
+  const int64_t sink_al = (k.sink + 31) & ~31ll;
+  k.lo_al = k.lo & ~31ll;
+  if (k.lo_al <= sink_al) {
+    k.nst = 0;
+    if (k.sink > 0) k.lo_al = 0;
+  } else {
+    k.nst = (int)(sink_al >> 5);
+  }
+  k.nt = k.nst + (k.hi > k.lo_al ? (int)((k.hi - k.lo_al + 31) >> 5) : 0);
+  return k;
+}
+
+hipError_t launch_window(const WinArgs& a, const WinTree& tree, int D, hipStream_t s);
+
+}  // namespace dsv

@@ -1,0 +1,720 @@
+// dsv_window.hip — attention through a sliding window with a few first tokens
+// that stay visible (sinks), over a dense or paged cache, on gfx950.
+//
+// Mathematics.  The M new tokens of a sequence of len tokens sit at the end of
+// its cache, n0 = len - M.  Row m has position p = n0 + m (causal), or n0 +
+// its depth in the drafted tree, and sees key n of its past at position pos(n)
+// iff pos(n) > p - W or pos(n) < S; the past is n <= p, or, with a tree, every
+// n < n0 and the row's ancestors and itself.  out = sum softmax(q.k / sqrt D)
+// v, lse = ln sum exp; a row without a key writes zeros and -inf.
+//
+// The G query heads of a KV head and neighbouring rows see nearly the same
+// keys, so rows are packed row-major over (m, g), r = m * G + g: a workgroup's
+// rows read each key once.  A workgroup's keys are the sinks' tiles followed by
+// the tiles from its first row's window to its last row's position (32 keys a
+// tile); what lies between is never read.  Only tiles at either border or in
+// the tree are masked: one keep word of 32 bits per row, from comparisons of
+// positions, so a mask costs no memory.
+//
+// Scores, sums and running maxima are fp32 (log2 domain); the probabilities
+// are rounded to the inputs' 16-bit type for the second matrix product (off by
+// half a step of values at most one, the inputs' own rounding); their sum
+// takes them unrounded.  Partial outputs of splits are fp32.
+//
+// Values of keys that a row does not see never reach it, whatever they hold: a
+// masked score is replaced, rows of V outside the workgroup's keys are
+// replaced by zeros, and a tile whose V holds infinities or NaN while some row
+// of the wave drops some of its keys takes a slow path that adds those entries
+// row by row (0 * inf would be NaN in the matrix product).
+//
+// win_rows_kernel (this file's simplest; few rows: single tokens, short
+// chunks): bound by reading K and V.  Four waves share a workgroup's tiles, each
+// with a softmax of its own, merged in LDS at the end, so no barrier stands in
+// the loop.  A tile goes memory -> registers in whole rows (16 bytes a lane,
+// the next tile in flight while this one is used) -> the wave's own LDS -> MFMA
+// operands: K rows by ds_read_b128, V transposed by ds_read_b64_tr_b16.  Splits
+// over the keys fill the GPU when there are few rows; win_merge_kernel joins
+// them.
+//
+// Reference context: runtime/attention_compat.py:103-132 (the cache call whose
+// layouts are kept), runtime/cache_state.py:52-66 (the tree behind the prefix),
+// draft/draft_network.py:1250-1331 (a working cache of first and recent
+// tokens).
+
+#include "dsv_internal.h"
+#include "dsv_window.h"
+
+namespace dsv {
+
+namespace {
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLn2 = 0.69314718055994530942f;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mfma16<BF16>(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mfma16<F16>(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<BF16>(float lo, float hi) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  bf2 r = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, r);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<F16>(float lo, float hi) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  h2 r = {(_Float16)lo, (_Float16)hi};
+  return __builtin_bit_cast(uint32_t, r);
+}
+template <typename T>
+__device__ __forceinline__ float unpack1(uint16_t x);
+template <>
+__device__ __forceinline__ float unpack1<BF16>(uint16_t x) {
+  return __uint_as_float((uint32_t)x << 16);
+}
+template <>
+__device__ __forceinline__ float unpack1<F16>(uint16_t x) {
+  return (float)__builtin_bit_cast(_Float16, x);
+}
+// Nonzero where a half of x is infinite or NaN (bits 15 and 31).
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x);
+template <>
+__device__ __forceinline__ uint32_t nonfinite2<BF16>(uint32_t x) {
+  return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+template <>
+__device__ __forceinline__ uint32_t nonfinite2<F16>(uint32_t x) {
+  return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+
+// Over the four lanes of a row (lane ^ 16, lane ^ 32).
+__device__ __forceinline__ float row_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Lanes of a wave read LDS that other lanes of it wrote (LDS operations of a
+// wave execute in order; this keeps the compiler from moving them).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// One query row as a lane sees it.
+struct Row {
+  int m, g;
+  int64_t pos;
+};
+__device__ __forceinline__ Row row_of(const WinArgs& a, int b, int r, int64_t n0) {
+  Row w;
+  w.m = r / a.G;
+  w.g = r - w.m * a.G;
+  w.pos = n0 + (a.depth != nullptr ? a.depth[(int64_t)b * a.M + w.m] : w.m);
+  return w;
+}
+
+// The keep word of a row for the tile at key kb: bit i = key kb + i is seen.
+__device__ __forceinline__ uint32_t keep_word(const WinArgs& a, int b, const Row& w, int64_t kb, int64_t n0) {
+  const uint32_t win = ~win_below(w.pos - a.W + 1 - kb) | win_below(a.S - kb);
+  if (a.bits == nullptr) return win & win_below(w.pos + 1 - kb);
+  uint32_t keep = win & win_below(n0 - kb);
+  if (kb + 32 > n0) {
+    // Tree keys: bits [kb - n0, kb - n0 + 32) of the row's set.
+    const uint64_t* t = a.bits + ((int64_t)b * a.M + w.m) * a.MW;
+    const int64_t at = kb - n0;
+    uint64_t x = 0;
+    if (at < 0) {
+      x = t[0] << (int)-at;
+    } else if ((at >> 6) < a.MW) {
+      const int i = (int)(at >> 6), sh = (int)(at & 63);
+      x = t[i] >> sh;
+      if (sh > 32 && i + 1 < a.MW) x |= t[i + 1] << (64 - sh);
+    }
+    keep |= (uint32_t)x;
+  }
+  return keep;
+}
+
+// Element offset of key n of the K or V half, for its physical page.
+__device__ __forceinline__ int64_t key_off(const WinArgs& a, int64_t sp, int64_t st, int64_t n, int32_t page) {
+  return a.pt != nullptr ? page * sp + (n & ((1ll << a.ps_shift) - 1)) * st : n * st;
+}
+__device__ __forceinline__ int32_t page_of(const WinArgs& a, int b, int64_t n) {
+  const int64_t i = (int64_t)b * a.pt_sb + (n >> a.ps_shift);
+  int64_t p = a.pt_i64 ? reinterpret_cast<const int64_t*>(a.pt)[i] : (int64_t) reinterpret_cast<const int32_t*>(a.pt)[i];
+  p = p < 0 ? 0 : (p >= a.n_phys ? a.n_phys - 1 : p);
+  return (int32_t)p;
+}
+
+__device__ __forceinline__ int64_t len_of(const WinArgs& a, int b) {
+  int64_t n = a.n_keys;
+  if (a.seqlens != nullptr) {
+    const int64_t x = a.seqlens_i64 ? reinterpret_cast<const int64_t*>(a.seqlens)[b]
+                                    : (int64_t) reinterpret_cast<const int32_t*>(a.seqlens)[b];
+    n = x < 0 ? 0 : (x < n ? x : n);
+  }
+  return n;
+}
+
+// Writes N consecutive output elements.
+template <int N>
+__device__ __forceinline__ void store_out(const WinArgs& a, int64_t off, const float (&x)[N]) {
+  static_assert(N == 4 || N == 8, "");
+  if (a.out_dtype == 2) {
+    float* o = reinterpret_cast<float*>(a.out) + off;
+    if (a.out_vec) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<f32x4*>(o + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = x[i];
+    }
+    return;
+  }
+  uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + off;
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i)
+    w[i] = a.out_dtype == 0 ? pack2<BF16>(x[2 * i], x[2 * i + 1]) : pack2<F16>(x[2 * i], x[2 * i + 1]);
+  if (a.out_vec) {
+    if constexpr (N == 8)
+      *reinterpret_cast<u32x4*>(o) = u32x4{w[0], w[1], w[2], w[3]};
+    else
+      *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+
+// ---- the tree's visibility ---------------------------------------------------
+// Depth and the visible ancestor-or-self set of every node, once per call: a
+// walk up the parents of at most M steps (a parent < 0, >= M or equal to the
+// node ends it, as in the tree split of dsv_attn.hip).
+__global__ void __launch_bounds__(256) win_tree_kernel(const WinArgs a, const void* parent, int p_i64, int64_t p_sb,
+                                                       int64_t p_sm, int32_t* depth, uint64_t* bits) {
+  __shared__ int32_t par[kTreeMaxM];
+  const int b = blockIdx.x, M = a.M;
+  for (int i = threadIdx.x; i < M; i += 256) {
+    const int64_t o = b * p_sb + (int64_t)i * p_sm;
+    const int64_t x = p_i64 ? reinterpret_cast<const int64_t*>(parent)[o] : (int64_t) reinterpret_cast<const int32_t*>(parent)[o];
+    par[i] = x < 0 || x >= M || x == i ? -1 : (int32_t)x;
+  }
+  __syncthreads();
+  const int64_t n0 = len_of(a, b) - M;
+  for (int i = threadIdx.x; i < M; i += 256) {
+    int d = 0;
+    for (int x = par[i]; x >= 0 && d < M; x = par[x]) ++d;
+    depth[(int64_t)b * M + i] = d;
+    uint64_t* t = bits + ((int64_t)b * M + i) * a.MW;
+    for (int w = 0; w < a.MW; ++w) t[w] = 0;
+    // Ancestor at h hops: position n0 + d - h against the row's n0 + d.
+    for (int x = i, h = 0; x >= 0 && h <= d; x = par[x], ++h)
+      if (h < a.W || n0 + d - h < a.S) t[x >> 6] |= 1ull << (x & 63);
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
+  constexpr int NW = 4;
+  constexpr int CH = D / 8;           // 16-byte chunks per key
+  constexpr int KPI = 64 / CH;        // keys per load instruction
+  constexpr int NL = 32 / KPI;        // load instructions per tile and half
+  constexpr int KS = D / 32;          // k-steps of Q.K^T
+  constexpr int DT = D / 16;          // d tiles of P.V
+  // Row strides of the LDS images: K rows shift by 4 banks a key (b128 reads
+  // of 16 keys), V rows by 8 (transposed reads of 16 keys x 32 bytes): free of
+  // bank conflicts.  K, then V, then the wave's partial output use one region.
+  constexpr int KST = 2 * D + 16, VST = 2 * D + 32, OST = (D + 4) * 4;
+  constexpr int REGION = 32 * VST;
+  static_assert(16 * OST <= REGION && 32 * KST <= REGION, "one region per wave");
+  __shared__ __attribute__((aligned(16))) uint8_t smem[NW * REGION];
+  __shared__ float sm_m[NW][16], sm_l[NW][16];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  uint8_t* mine = smem + wave * REGION;
+
+  int w = blockIdx.x;
+  const int split = w % a.splits;
+  w /= a.splits;
+  const int rb = w % a.n_rb;
+  w /= a.n_rb;
+  const int kvh = w % a.Hk, b = w / a.Hk;
+  const int64_t n0 = len_of(a, b) - a.M;
+  const int r0 = rb * 16 * NR;
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, r0, 16 * NR);
+  const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
+  int t = (int)((int64_t)kl.nt * split / a.splits) + wave;
+
+  // This lane's rows: Q fragments (B operand): row lr, elements 32 ks + 8 lg ..
+  Row row[NR];
+  u32x4 qf[NR][KS];
+  int64_t pmin = INT64_MAX, pmax = INT64_MIN;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int r = min(r0 + 16 * i + lr, a.R - 1);
+    row[i] = row_of(a, b, r, n0);
+    const uint16_t* q = a.q + b * a.q_sb + (int64_t)row[i].m * a.q_sm + (int64_t)(kvh * a.G + row[i].g) * a.q_sh + 8 * lg;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[i][ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks);
+    pmin = min(pmin, row[i].pos);
+    pmax = max(pmax, row[i].pos);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    pmin = min(pmin, (int64_t)__shfl_xor((long long)pmin, o));
+    pmax = max(pmax, (int64_t)__shfl_xor((long long)pmax, o));
+  }
+
+  float mx[NR], ls[NR];
+  f32x4 acc[NR][DT];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    mx[i] = kNegInf;
+    ls[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{};
+  }
+
+  const uint16_t* kbase = a.k + b * a.k_sb + kvh * a.k_sh + (lane % CH) * 8;
+  const uint16_t* vbase = a.v + b * a.v_sb + kvh * a.v_sh + (lane % CH) * 8;
+  // Lane l holds the page of key l (mod 32) of a tile, read a tile ahead.
+  auto tile_pages = [&](int tt) -> int32_t {
+    if (a.pt == nullptr || tt >= t_end) return 0;
+    return page_of(a, b, min(kl.base(tt) + (lane & 31), kl.hi - 1));
+  };
+  u32x4 kr[NL], vr[NL];
+  auto load_tile = [&](int tt, int32_t pg) {
+    const int64_t kb = kl.base(tt);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = j * KPI + lane / CH;
+      // Keys behind the last one read the last one (inside the tensor).
+      const int64_t n = min(kb + i, kl.hi - 1);
+      const int32_t page = a.pt != nullptr ? __shfl(pg, i) : 0;
+      kr[j] = *reinterpret_cast<const u32x4*>(kbase + key_off(a, a.k_sp, a.k_st, n, page));
+      vr[j] = *reinterpret_cast<const u32x4*>(vbase + key_off(a, a.v_sp, a.v_st, n, page));
+    }
+  };
+
+  int32_t pg = tile_pages(t);
+  if (t < t_end) load_tile(t, pg);
+  pg = tile_pages(t + NW);
+  for (; t < t_end; t += NW) {
+    const int64_t kb = kl.base(t);
+    // ---- S^T = K . Q^T
+#pragma unroll
+    for (int j = 0; j < NL; ++j)
+      *reinterpret_cast<u32x4*>(mine + (j * KPI + lane / CH) * KST + (lane % CH) * 16) = kr[j];
+    wave_lds_fence();
+    f32x4 s[NR][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) s[i][h] = f32x4{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(mine + (16 * h + lr) * KST + (4 * ks + lg) * 16);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) s[i][h] = mfma16<T>(kf, qf[i][ks], s[i][h]);
+      }
+    }
+    wave_lds_fence();
+    // ---- V into LDS; rows that no row of the workgroup sees become zeros.
+    const bool edge = !kl.whole(kb);
+    uint32_t odd = 0;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = j * KPI + lane / CH;
+      if (edge && !kl.has(kb + i)) vr[j] = u32x4{0, 0, 0, 0};
+      odd |= nonfinite2<T>(vr[j][0]) | nonfinite2<T>(vr[j][1]) | nonfinite2<T>(vr[j][2]) | nonfinite2<T>(vr[j][3]);
+      *reinterpret_cast<u32x4*>(mine + i * VST + (lane % CH) * 16) = vr[j];
+    }
+    wave_lds_fence();
+    // ---- the next tile's loads
+    if (t + NW < t_end) load_tile(t + NW, pg);
+    pg = tile_pages(t + 2 * NW);
+    // ---- mask and softmax
+    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
+    uint32_t keep[NR];
+    u32x4 pf[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      keep[i] = ~0u;
+      if (masked) {
+        keep[i] = keep_word(a, b, row[i], kb, n0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!((keep[i] >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[i][e >> 2][e & 3] = kNegInf;
+      }
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s[i][e >> 2][e & 3];
+      float mt = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
+      const float mn = fmaxf(mx[i], row_max(mt) * a.scale_log2);
+      if (__ballot(mn > mx[i]) != 0ull) {
+        const float al = mx[i] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mx[i] - mn);
+        ls[i] *= al;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[i][d] *= al;
+        mx[i] = mn;
+      }
+      const float ms = mx[i] == kNegInf ? 0.f : mx[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -ms));
+        ls[i] += x[e];
+      }
+      pf[i] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
+    }
+    // ---- O^T += V^T . P^T; element e of lane group lg is key 16 (e / 4) + 4 lg + e % 4.
+    if (masked && __ballot(odd != 0) != 0ull) {
+      // Infinite or NaN entries of V: added to the rows that see them, and out of the product.
+      for (int n = 0; n < 32; ++n) {
+        uint16_t* v = reinterpret_cast<uint16_t*>(mine + n * VST);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = unpack1<T>(v[16 * d + 4 * lg + e]);
+            const bool bad = !(x - x == 0.f);
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+              if (bad && ((keep[i] >> n) & 1u)) acc[i][d][e] += x;
+          }
+        wave_lds_fence();
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = unpack1<T>(v[16 * d + 4 * lg + e]);
+            if (lr == 0 && !(x - x == 0.f)) v[16 * d + 4 * lg + e] = 0;
+          }
+      }
+      wave_lds_fence();
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const uint8_t* p = mine + (4 * lg + (lr >> 2)) * VST + (16 * d + 4 * (lr & 3)) * 2;
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * VST)));
+      const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+      for (int i = 0; i < NR; ++i) acc[i][d] = mfma16<T>(vf, pf[i], acc[i][d]);
+    }
+    wave_lds_fence();
+  }
+
+  // ---- the four waves' rows joined, 16 at a time
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const float lt = row_sum(ls[i]);
+    if (lg == 0) {
+      sm_m[wave][lr] = mx[i];
+      sm_l[wave][lr] = lt;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(mine + lr * OST + (16 * d + 4 * lg) * 4) = acc[i][d];
+    __syncthreads();
+    constexpr int N = D / 16;  // elements per thread
+    const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * N;
+    float m = sm_m[0][rr];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) m = fmaxf(m, sm_m[x][rr]);
+    const float ms = m == kNegInf ? 0.f : m;
+    float l = 0.f, o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      if (sm_l[x][rr] == 0.f) continue;  // a wave without a key of this row
+      const float f = __builtin_amdgcn_exp2f(sm_m[x][rr] - ms);
+      l += sm_l[x][rr] * f;
+      const f32x4* p = reinterpret_cast<const f32x4*>(smem + x * REGION + rr * OST + d0 * 4);
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] += p[e / 4][e % 4] * f;
+    }
+    const int r = r0 + 16 * i + rr;
+    if (r < a.R) {
+      if (a.splits == 1) {
+        const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] *= inv;
+        store_out<N>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
+        if (d0 == 0 && a.lse != nullptr)
+          a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+      } else {
+        const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
+#pragma unroll
+        for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(a.opart + pr * D + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+        if (d0 == 0) a.ml[pr] = make_float2(m, l);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- fp32 ------------------------------------------------------------------------
+// The same walk over tiles with v_mfma_f32_16x16x4_f32, 16 rows and 32 keys a
+// step.  K's operand takes a lane's 16 bytes as four k-steps (the order of the
+// head dimension in the product is free as long as Q's agrees), V's operand is a
+// row-major element, so nothing passes through LDS but the join of the waves.
+template <int D>
+__global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
+  constexpr int NW = 4;
+  constexpr int KC = D / 16;          // 16-byte chunks per lane and key
+  constexpr int DT = D / 16;
+  constexpr int OST = D + 4;
+  __shared__ __attribute__((aligned(16))) float smem[NW][16 * OST];
+  __shared__ float sm_m[NW][16], sm_l[NW][16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  int w = blockIdx.x;
+  const int split = w % a.splits;
+  w /= a.splits;
+  const int rb = w % a.n_rb;
+  w /= a.n_rb;
+  const int kvh = w % a.Hk, b = w / a.Hk;
+  const int64_t n0 = len_of(a, b) - a.M;
+  const int r0 = rb * 16;
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, r0, 16);
+  const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
+  const float* kbase = reinterpret_cast<const float*>(a.k) + b * a.k_sb + kvh * a.k_sh;
+  const float* vbase = reinterpret_cast<const float*>(a.v) + b * a.v_sb + kvh * a.v_sh;
+
+  const Row row = row_of(a, b, min(r0 + lr, a.R - 1), n0);
+  f32x4 qf[KC];
+  const float* q = reinterpret_cast<const float*>(a.q) + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh;
+#pragma unroll
+  for (int c = 0; c < KC; ++c) qf[c] = *reinterpret_cast<const f32x4*>(q + 16 * c + 4 * lg);
+  int64_t pmin = row.pos, pmax = row.pos;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    pmin = min(pmin, (int64_t)__shfl_xor((long long)pmin, o));
+    pmax = max(pmax, (int64_t)__shfl_xor((long long)pmax, o));
+  }
+  float mx = kNegInf, ls = 0.f;
+  f32x4 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
+
+  for (int t = (int)((int64_t)kl.nt * split / a.splits) + wave; t < t_end; t += NW) {
+    const int64_t kb = kl.base(t);
+    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
+    const uint32_t keep = masked ? keep_word(a, b, row, kb, n0) : ~0u;
+    f32x4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t n = min(kb + 16 * h + lr, kl.hi - 1);
+      const float* k = kbase + key_off(a, a.k_sp, a.k_st, n, a.pt != nullptr ? page_of(a, b, n) : 0) + 4 * lg;
+      f32x4 kf[KC];
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kf[c] = *reinterpret_cast<const f32x4*>(k + 16 * c);
+      s[h] = f32x4{};
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][e], qf[c][e], s[h], 0, 0, 0);
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = s[e >> 2][e & 3];
+      if (masked && !((keep >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) x[e] = kNegInf;
+    }
+    float mt = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
+    const float mn = fmaxf(mx, row_max(mt) * a.scale_log2);
+    if (__ballot(mn > mx) != 0ull) {
+      const float al = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+      ls *= al;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] *= al;
+      mx = mn;
+    }
+    const float ms = mx == kNegInf ? 0.f : mx;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -ms));
+      ls += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t n = min(kb + 16 * (e >> 2) + 4 * lg + (e & 3), kl.hi - 1);
+      const float* v = vbase + key_off(a, a.v_sp, a.v_st, n, a.pt != nullptr ? page_of(a, b, n) : 0) + lr;
+      const bool has = kl.has(kb + 16 * (e >> 2) + 4 * lg + (e & 3));
+      float vf[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vf[d] = v[16 * d];
+      bool odd = false;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        if (masked && !has) vf[d] = 0.f;
+        odd |= !(vf[d] - vf[d] == 0.f);
+      }
+      if (masked && __ballot(odd) != 0ull) {
+        // Infinite or NaN entries: added to the rows that see them, and out of
+        // the product.  Lane group y holds key 4 y + e % 4; this lane's
+        // accumulators are d = 16 d + 4 lg + z of row lr.
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const float o = __shfl(vf[d], 16 * y + 4 * lg + z);
+              if (!(o - o == 0.f) && ((keep >> (16 * (e >> 2) + 4 * y + (e & 3))) & 1u)) acc[d][z] += o;
+            }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vf[d] = vf[d] - vf[d] == 0.f ? vf[d] : 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[d], x[e], acc[d], 0, 0, 0);
+    }
+  }
+
+  const float lt = row_sum(ls);
+  if (lg == 0) {
+    sm_m[wave][lr] = mx;
+    sm_l[wave][lr] = lt;
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&smem[wave][lr * OST + 16 * d + 4 * lg]) = acc[d];
+  __syncthreads();
+  constexpr int N = D / 16;
+  const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * N;
+  float m = sm_m[0][rr];
+#pragma unroll
+  for (int y = 1; y < NW; ++y) m = fmaxf(m, sm_m[y][rr]);
+  const float ms = m == kNegInf ? 0.f : m;
+  float l = 0.f, o[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int y = 0; y < NW; ++y) {
+    if (sm_l[y][rr] == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(sm_m[y][rr] - ms);
+    l += sm_l[y][rr] * f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] += smem[y][rr * OST + d0 + e] * f;
+  }
+  const int r = r0 + rr;
+  if (r >= a.R) return;
+  if (a.splits == 1) {
+    const int mm = r / a.G, hh = kvh * a.G + r - mm * a.G;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] *= inv;
+    store_out<N>(a, b * a.o_sb + mm * a.o_sm + hh * a.o_sh + d0, o);
+    if (d0 == 0 && a.lse != nullptr)
+      a.lse[b * a.l_sb + mm * a.l_sm + hh * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+  } else {
+    const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
+#pragma unroll
+    for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(a.opart + pr * D + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+    if (d0 == 0) a.ml[pr] = make_float2(m, l);
+  }
+}
+
+// ---- the splits joined -------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
+  constexpr int TPR = D / 4;  // threads per row, four elements each
+  const int64_t x = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int d0 = (threadIdx.x % TPR) * 4;
+  if (x >= (int64_t)a.B * a.Hk * a.R) return;
+  const int64_t bh = x / a.R;
+  const int r = (int)(x - bh * a.R);
+  const int b = (int)(bh / a.Hk), kvh = (int)(bh % a.Hk);
+  float m = kNegInf, l = 0.f;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t pr = (bh * a.splits + s) * a.R + r;
+    const float2 ml = a.ml[pr];
+    const f32x4 p = *reinterpret_cast<const f32x4*>(a.opart + pr * D + d0);
+    if (ml.y == 0.f) continue;
+    const float mn = fmaxf(m, ml.x);
+    const float f0 = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
+    m = mn;
+    l = l * f0 + ml.y * f1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + p[e] * f1;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
+  store_out<4>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
+  if (d0 == 0 && a.lse != nullptr)
+    a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+}
+
+template <typename T, int D>
+hipError_t launch_rows(const WinArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits));
+  if (a.rows_per_block == 16)
+    hipLaunchKernelGGL((win_rows_kernel<T, D, 1>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((win_rows_kernel<T, D, 2>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_d(const WinArgs& a, hipStream_t s) {
+  hipError_t e;
+  if (a.dtype == 2) {
+    hipLaunchKernelGGL(win_rows_f32_kernel<D>, dim3((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), dim3(256), 0, s, a);
+    e = hipGetLastError();
+  } else {
+    e = a.dtype == 0 ? launch_rows<BF16, D>(a, s) : launch_rows<F16, D>(a, s);
+  }
+  if (e != hipSuccess || a.splits == 1) return e;
+  const int64_t rows = (int64_t)a.B * a.Hk * a.R;
+  const int per = 256 / (D / 4);
+  hipLaunchKernelGGL(win_merge_kernel<D>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_window(const WinArgs& a, const WinTree& tree, int D, hipStream_t s) {
+  if (tree.parent != nullptr) {
+    hipLaunchKernelGGL(win_tree_kernel, dim3((unsigned)a.B), dim3(256), 0, s, a, tree.parent, tree.i64, tree.sb, tree.sm,
+                       const_cast<int32_t*>(a.depth), const_cast<uint64_t*>(a.bits));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return D == 64 ? launch_d<64>(a, s) : launch_d<128>(a, s);
+}
+
+}  // namespace dsv

@@ -82,6 +82,8 @@ SIGNATURES = {
     "dsv_lmhead_accept_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "dsv_lmhead_accept": (ctypes.c_int, [ctypes.c_int, _P, _P, _P, _P, _P, _I64, ctypes.c_float, ctypes.c_float,
                                          ctypes.c_float, _P, _P, _P, _P, _P, _V, ctypes.c_size_t, _V]),
+    "dsv_window_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, ctypes.c_int, _I64, _I64, _I64, ctypes.c_int]),
+    "dsv_window_attention": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _V, _SZ, _V]),
     "dsv_spec_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "dsv_spec_accept": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _V, _SZ, _V]),
     "dsv_pages_workspace_bytes": (_SZ, [_I64, _I64, _I64]),

@@ -1,0 +1,107 @@
+"""Refusals and key geometry of the windowed attention (CPU only: nothing is launched)."""
+
+import numpy as np
+import pytest
+import torch
+
+from diffspec_mi355x import _ext
+from diffspec_mi355x.runtime.window_attention import window_attn_with_kvcache
+from oracle import window as oracle
+
+INVALID, UNSUPPORTED, WORKSPACE = -1, -2, -3
+WS = torch.empty(1 << 24, dtype=torch.uint8)
+
+
+@pytest.fixture()
+def dry(dsv_lib):
+    dsv_lib.dsv_set_dry_run(1)
+    yield dsv_lib
+    dsv_lib.dsv_set_dry_run(0)
+
+
+def call(lib, B=2, M=3, H=4, Hk=2, D=64, N=40, window=9, sinks=2, n_keys=-1, nbytes=1 << 23, ws=None, **kw):
+    t = dict(q=torch.zeros(B, M, H, D), k=torch.zeros(B, N, Hk, D), v=torch.zeros(B, N, Hk, D), table=None, lens=None,
+             parent=None, out=torch.zeros(B, M, H, D), lse=torch.zeros(B, H, M))
+    t.update(kw)
+    d = {x: _ext.desc(y) for x, y in t.items()}
+    ptr = (WS.data_ptr() + 255) // 256 * 256 if ws is None else ws
+    return lib.dsv_window_attention(d["q"], d["k"], d["v"], d["table"], d["lens"], n_keys, window, sinks, d["parent"],
+                                    d["out"], d["lse"], ptr, nbytes, None)
+
+
+def test_accepts_and_refuses(dry):
+    f, i32 = torch.zeros, lambda *s: torch.zeros(s, dtype=torch.int32)
+    paged = dict(k=f(7, 2, 8, 64), v=f(7, 2, 8, 64), table=i32(2, 5))
+    assert call(dry) == 0
+    assert call(dry, lse=None) == 0
+    assert call(dry, n_keys=10 ** 12, window=1 << 62, sinks=1 << 62) == 0
+    assert call(dry, **paged) == 0
+    assert call(dry, **{**paged, "table": torch.zeros(5, dtype=torch.int64)}) == 0
+    assert call(dry, parent=i32(3), lens=i32(2)) == 0
+    assert call(dry, parent=i32(2, 3).long(), lens=i32(2).long()) == 0
+    assert call(dry, out=torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16)) == 0
+    for bad in [dict(window=0), dict(window=-4), dict(sinks=-1), dict(Hk=3), dict(k=f(2, 40, 2, 128)), dict(v=f(2, 41, 2, 64)),
+                dict(k=f(2, 40, 2, 64).bfloat16()), dict(q=f(2, 3, 64)), dict(out=f(2, 3, 4, 32)), dict(lse=f(2, 3, 4)),
+                dict(lse=f(2, 4, 3).double().to(torch.int64)), dict(lens=i32(3)), dict(lens=f(2)), dict(lens=i32(4)[::2]),
+                dict(parent=i32(4)), dict(parent=i32(3, 3)), dict(parent=f(3)), dict(table=i32(2, 5)),
+                {**paged, "table": i32(3, 5)}, {**paged, "table": f(2, 5)}, {**paged, "table": i32(5, 2).t()},
+                dict(q=f(2, 3, 4, 65)[..., 1:]), dict(q=f(2 * 3 * 4 * 64 + 1)[1:].view(2, 3, 4, 64)),
+                {**paged, "k": f(6, 2, 8, 64)}]:
+        assert call(dry, **bad) == INVALID, bad.keys()
+    assert call(dry, D=96) == UNSUPPORTED
+    assert call(dry, **{**paged, "k": f(7, 2, 6, 64), "v": f(7, 2, 6, 64)}) == UNSUPPORTED
+    big = torch.zeros(1, 1, 1, 64)
+    assert call(dry, B=1, M=1025, parent=i32(1025)) == UNSUPPORTED
+    assert call(dry, B=1, M=(1 << 24) + 1, H=1, Hk=1, q=big.expand(1, (1 << 24) + 1, 1, 64),
+                out=big.clone().expand(1, (1 << 24) + 1, 1, 64), lse=None) == UNSUPPORTED
+    assert call(dry, ws=0) == WORKSPACE
+    assert call(dry, nbytes=0) == WORKSPACE
+    assert call(dry, ws=(WS.data_ptr() + 255) // 256 * 256 + 64) == WORKSPACE
+    q = f(2, 3, 4, 64)
+    assert call(dry, q=q, out=q) == INVALID
+    assert call(dry, lse=q.view(-1)[:24].view(2, 4, 3), q=q) == INVALID
+
+
+def test_workspace_sizes(dsv_lib):
+    n = dsv_lib.dsv_window_workspace_bytes
+    assert n(1, 1, 32, 8, 128, _ext.DSV_BF16, 5000, 1024, 4, 0) > 0
+    for bad in [(0, 1, 4, 2, 64, 0, 10, 4, 0, 0), (1, 0, 4, 2, 64, 0, 10, 4, 0, 0), (1, 1, 4, 3, 64, 0, 10, 4, 0, 0),
+                (1, 1, 4, 2, 80, 0, 10, 4, 0, 0), (1, 1, 4, 2, 64, 3, 10, 4, 0, 0), (1, 1, 4, 2, 64, 0, -1, 4, 0, 0),
+                (1, 1, 4, 2, 64, 0, 10, 0, 0, 0), (1, 1, 4, 2, 64, 0, 10, 4, -1, 0), (1, 1025, 4, 2, 64, 0, 10, 4, 0, 1),
+                ((1 << 20) + 1, 1, 4, 2, 64, 0, 10, 4, 0, 0)]:
+        assert n(*bad) == 0, bad
+
+
+def test_python_refusals(dsv_lib):
+    q, k = torch.zeros(1, 2, 4, 64), torch.zeros(1, 9, 2, 64)
+    with pytest.raises(RuntimeError):
+        window_attn_with_kvcache(q, k, k, 4)
+
+
+def test_oracle_against_a_dense_mask():
+    """The oracle's visible keys against the definition as one mask."""
+    rng = np.random.default_rng(0)
+    for _ in range(200):
+        M, n = int(rng.integers(1, 9)), int(rng.integers(0, 30))
+        W, S = int(rng.integers(1, 12)), int(rng.integers(0, 8))
+        got = oracle.visible(M, n, W, S)
+        for m in range(M):
+            p = n - M + m
+            assert got[m].tolist() == [j for j in range(n) if j <= p and (j > p - W or j < S)]
+        par = [-1] + [int(rng.integers(-1, i)) for i in range(1, M)]
+        got = oracle.visible(M, n, W, S, par)
+        depth = [0] * M
+        for i in range(1, M):
+            depth[i] = 0 if par[i] < 0 else depth[par[i]] + 1
+        anc = np.eye(M, dtype=bool)
+        for i in range(1, M):
+            if par[i] >= 0:
+                anc[i] |= anc[par[i]]
+        n0 = n - M
+        for m in range(M):
+            want = []
+            for j in range(n) if n0 >= 0 else []:
+                pos = j if j < n0 else n0 + depth[j - n0]
+                if (j < n0 or anc[m, j - n0]) and (pos > n0 + depth[m] - W or pos < S):
+                    want.append(j)
+            assert got[m].tolist() == want
