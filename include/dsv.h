@@ -247,8 +247,8 @@ int dsv_tree_verify_noalloc(const dsv_tensor* q, const dsv_tensor* k,
 /*
  * Workspace of dsv_window_attention for queries [B, M, H, D] of dtype
  * (dsv_dtype) over a cache of n_keys keys with Hk heads.  0 on invalid
- * arguments and on sizes that the call refuses (those of
- * dsv_attn_workspace_bytes).
+ * arguments and on sizes that the call refuses: batch > 2^20, query heads >
+ * 65536, keys > 2^30, H / Hk * M > 2^24, B * H * M > 2^30 (DSV_ERR_UNSUPPORTED).
  */
 size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk,
                                   int64_t D, int dtype, int64_t n_keys,

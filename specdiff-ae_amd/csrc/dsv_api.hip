@@ -1876,26 +1876,27 @@ bool win_args_ok(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
 }
 
 WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys, int64_t window,
-                 int64_t sinks, bool tree) {
+                 int64_t sinks, bool tree, bool small_pages) {
   WinPlan p;
-  const bool in_range = B <= (1 << 20) && M <= (1 << 24) && H <= (1 << 16) && n_keys <= ((int64_t)1 << 35);
+  const bool in_range = B <= (1 << 20) && M <= (1 << 24) && H <= (1 << 16) && n_keys <= dsv::kWinMaxKeys;
   const int64_t R = in_range ? (H / Hk) * M : 0;
   if (!in_range || R > ((int64_t)1 << 24) || B * Hk * R > ((int64_t)1 << 30)) {
-    p.err = "sizes beyond the windowed attention's range (batch <= 2^20, heads <= 65536, keys <= 2^35, query heads / "
+    p.err = "sizes beyond the windowed attention's range (batch <= 2^20, heads <= 65536, keys <= 2^30, query heads / "
             "key heads x rows <= 2^24, batch x query heads x rows <= 2^30)";
     return p;
   }
   p.G = (int)(H / Hk);
   p.R = (int)R;
   p.MW = tree ? (int)((M + 63) / 64) : 0;
-  p.rpb = dtype == DSV_F32 || R <= 16 ? 16 : 32;
+  const bool tile = dtype != DSV_F32 && R > 64 && !small_pages;
+  p.rpb = tile ? 256 : dtype == DSV_F32 || R <= 16 ? 16 : 32;
   p.n_rb = (int)((R + p.rpb - 1) / p.rpb);
   // Splits over the keys: four waves per workgroup and at least one tile per
   // wave, until there are four workgroups per CU.
   const int64_t units = B * Hk * p.n_rb;
   const int64_t span = tree ? M : std::min<int64_t>(M, p.rpb / p.G + 2);
   const int64_t reach = std::min(n_keys, window + span) / 32 + 2 + std::min(n_keys, sinks) / 32;
-  const int64_t want = std::max<int64_t>(1, (int64_t)device_cus() * 4 / units);
+  const int64_t want = std::max<int64_t>(1, (int64_t)device_cus() * (tile ? 1 : 4) / units);
   p.splits = (int)std::max<int64_t>(1, std::min(want, reach / 4));
   const size_t rows = p.splits > 1 ? (size_t)B * Hk * p.splits * R : 0;
   p.opart_bytes = align_up(rows * D * sizeof(float), 256);
@@ -1912,7 +1913,7 @@ extern "C" {
 size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys,
                                   int64_t window, int64_t sinks, int has_tree) {
   if (!win_args_ok(B, M, H, Hk, D, dtype, n_keys, window, sinks) || (has_tree && M > dsv::kTreeMaxM)) return 0;
-  const WinPlan p = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0);
+  const WinPlan p = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0, false);
   return p.err != nullptr ? 0 : std::max<size_t>(p.total, 256);
 }
 
@@ -2015,9 +2016,9 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
       return fail(DSV_ERR_INVALID, "out or lse overlaps %s", in.name);
   if (overlap(extent_of("out", out), extent_of("lse", lse))) return fail(DSV_ERR_INVALID, "out overlaps lse");
 
-  // (Positions, window and sinks fit well inside 64 bits then.)
-  const int64_t W = std::min<int64_t>(window, (int64_t)1 << 41), S = std::min<int64_t>(sinks, (int64_t)1 << 41);
-  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, tree.parent != nullptr);
+  // (Beyond every key, either means all of them.)
+  const int64_t W = std::min<int64_t>(window, dsv::kWinMaxKeys), S = std::min<int64_t>(sinks, dsv::kWinMaxKeys);
+  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, tree.parent != nullptr, present(page_table) && k->shape[2] < 8);
   if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
   if ((rc = check_workspace(std::max<size_t>(p.total, 256), workspace, workspace_bytes)) != DSV_OK) return rc;
   a.dtype = q->dtype;
@@ -2034,8 +2035,8 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   a.Hk = (int)Hk;
   a.G = p.G;
   a.R = p.R;
-  a.W = W;
-  a.S = S;
+  a.W = (int)W;
+  a.S = (int)S;
   a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
   a.rows_per_block = p.rpb;
   a.n_rb = p.n_rb;

@@ -21,7 +21,7 @@ struct WinArgs {
   const void* seqlens; int seqlens_i64;    // optional [B]
   int64_t n_keys;                          // keys of the cache (lengths are clamped to it)
   int B, M, H, Hk, G, R;                   // R = G * M rows per KV head, row m * G + g
-  int64_t W, S;                            // window (>= 1) and sinks
+  int W, S;                                // window (>= 1) and sinks, at most kWinMaxKeys
   float scale_log2;                        // log2(e) / sqrt(D)
   const int32_t* depth;                    // tree: [B, M] depths
   const uint64_t* bits; int MW;            // tree: [B, M, MW] visible ancestors
@@ -39,49 +39,61 @@ struct WinTree {
   int64_t sb, sm;
 };
 
+// Keys of a sequence at most: token numbers, positions and their differences
+// are 32-bit (byte offsets are not).
+constexpr int64_t kWinMaxKeys = (int64_t)1 << 30;
+
 // Bits [0, x) of a 32-bit word, x clamped to [0, 32].
-DSV_HD uint32_t win_below(int64_t x) { return x <= 0 ? 0u : (x >= 32 ? ~0u : (1u << (int)x) - 1u); }
+DSV_HD uint32_t win_below(int x) { return x <= 0 ? 0u : (x >= 32 ? ~0u : (1u << x) - 1u); }
 
 // The keys of a block of rows: [0, sink) and [lo, hi), as nt tiles of 32: nst
 // tiles from key 0, the others from lo_al (a multiple of 32).  Where the two
 // meet, nst is 0 and lo_al is 0.
 struct WinKeys {
-  int64_t lo, hi, sink, lo_al;
+  int lo, hi, sink, lo_al;
   int nst, nt;
-  DSV_HD int64_t base(int t) const { return t < nst ? 32ll * t : lo_al + 32ll * (t - nst); }
+  DSV_HD int base(int t) const { return t < nst ? 32 * t : lo_al + 32 * (t - nst); }
   // Does any row of the block see key n?
-  DSV_HD bool has(int64_t n) const { return n < sink || (n >= lo && n < hi); }
-  DSV_HD bool whole(int64_t kb) const { return kb + 32 <= sink || (kb >= lo && kb + 32 <= hi); }
+  DSV_HD bool has(int n) const { return n < sink || (n >= lo && n < hi); }
+  DSV_HD bool whole(int kb) const { return kb + 32 <= sink || (kb >= lo && kb + 32 <= hi); }
+  // Key n, or where no row sees it one that some row does: what is read in its
+  // place (its own page may be gone).
+  DSV_HD int read(int n) const {
+    if (n < sink) return n;
+    n = n > lo ? n : lo;
+    return n < hi ? n : hi - 1;
+  }
   // Is every key of the tile seen by every row between positions pmin and pmax?
-  DSV_HD bool seen_by_all(int64_t kb, int64_t pmin, int64_t pmax, int64_t W, int64_t S, int64_t n0, bool tree) const {
+  DSV_HD bool seen_by_all(int kb, int pmin, int pmax, int W, int S, int n0, bool tree) const {
     return (tree ? kb + 32 <= n0 : kb + 31 <= pmin) && (kb > pmax - W || kb + 32 <= S);
   }
 };
 
 // The keys of rows [r0, r0 + nrows) of a sequence whose new tokens start at n0.
-DSV_HD WinKeys win_keys(int M, int G, int R, int64_t W, int64_t S, bool tree, int64_t n0, int r0, int nrows) {
+DSV_HD WinKeys win_keys(int M, int G, int R, int W, int S, bool tree, int n0, int r0, int nrows) {
   WinKeys k;
   const int rl = (r0 + nrows < R ? r0 + nrows : R) - 1;
   // Positions of the first and last row; a tree's rows lie anywhere from n0 on.
-  const int64_t pmin = tree ? n0 : n0 + r0 / G, pmax = tree ? n0 + M - 1 : n0 + rl / G;
+  const int pmin = tree ? n0 : n0 + r0 / G, pmax = tree ? n0 + M - 1 : n0 + rl / G;
   k.hi = pmax + 1 > 0 ? pmax + 1 : 0;
   if (tree && n0 < 0) k.hi = 0;
   k.lo = pmin - W + 1;
   if (k.lo < 0) k.lo = 0;
   if (k.lo > k.hi) k.lo = k.hi;
   k.sink = S < k.hi ? S : k.hi;
-  const int64_t sink_al = (k.sink + 31) & ~31ll;
-  k.lo_al = k.lo & ~31ll;
-  if (k.lo_al <= sink_al) {
-    k.nst = 0;
-    if (k.sink > 0) k.lo_al = 0;
-  } else {
-    k.nst = (int)(sink_al >> 5);
-  }
-  k.nt = k.nst + (k.hi > k.lo_al ? (int)((k.hi - k.lo_al + 31) >> 5) : 0);
+  const int sink_al = (k.sink + 31) & ~31;
+  k.lo_al = k.lo & ~31;
+  k.nst = 0;
+  if (k.lo_al > sink_al)
+    k.nst = sink_al >> 5;
+  else if (k.sink > 0)
+    k.lo_al = 0;
+  k.nt = k.nst + (k.hi > k.lo_al ? (k.hi - k.lo_al + 31) >> 5 : 0);
   return k;
 }
 
+// The kernel for many rows (rows_per_block 256, 16-bit, pages of at least 8 keys).
+hipError_t launch_window_tile(const WinArgs& a, int D, hipStream_t s);
 hipError_t launch_window(const WinArgs& a, const WinTree& tree, int D, hipStream_t s);
 
 }  // namespace dsv

@@ -42,17 +42,11 @@
 // tokens).
 
 #include "dsv_internal.h"
-#include "dsv_window.h"
+#include "dsv_window_dev.h"
 
 namespace dsv {
 
 namespace {
-
-constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kLn2 = 0.69314718055994530942f;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
@@ -63,42 +57,6 @@ __device__ __forceinline__ f32x4 mfma16<BF16>(u32x4 a, u32x4 b, f32x4 c) {
 template <>
 __device__ __forceinline__ f32x4 mfma16<F16>(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<BF16>(float lo, float hi) {
-  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-  bf2 r = {(__bf16)lo, (__bf16)hi};
-  return __builtin_bit_cast(uint32_t, r);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<F16>(float lo, float hi) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  h2 r = {(_Float16)lo, (_Float16)hi};
-  return __builtin_bit_cast(uint32_t, r);
-}
-template <typename T>
-__device__ __forceinline__ float unpack1(uint16_t x);
-template <>
-__device__ __forceinline__ float unpack1<BF16>(uint16_t x) {
-  return __uint_as_float((uint32_t)x << 16);
-}
-template <>
-__device__ __forceinline__ float unpack1<F16>(uint16_t x) {
-  return (float)__builtin_bit_cast(_Float16, x);
-}
-// Nonzero where a half of x is infinite or NaN (bits 15 and 31).
-template <typename T>
-__device__ __forceinline__ uint32_t nonfinite2(uint32_t x);
-template <>
-__device__ __forceinline__ uint32_t nonfinite2<BF16>(uint32_t x) {
-  return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-}
-template <>
-__device__ __forceinline__ uint32_t nonfinite2<F16>(uint32_t x) {
-  return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
 // Over the four lanes of a row (lane ^ 16, lane ^ 32).
@@ -115,101 +73,6 @@ __device__ __forceinline__ float row_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Lanes of a wave read LDS that other lanes of it wrote (LDS operations of a
-// wave execute in order; this keeps the compiler from moving them).
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// One query row as a lane sees it.
-struct Row {
-  int m, g;
-  int64_t pos;
-};
-__device__ __forceinline__ Row row_of(const WinArgs& a, int b, int r, int64_t n0) {
-  Row w;
-  w.m = r / a.G;
-  w.g = r - w.m * a.G;
-  w.pos = n0 + (a.depth != nullptr ? a.depth[(int64_t)b * a.M + w.m] : w.m);
-  return w;
-}
-
-// The keep word of a row for the tile at key kb: bit i = key kb + i is seen.
-__device__ __forceinline__ uint32_t keep_word(const WinArgs& a, int b, const Row& w, int64_t kb, int64_t n0) {
-  const uint32_t win = ~win_below(w.pos - a.W + 1 - kb) | win_below(a.S - kb);
-  if (a.bits == nullptr) return win & win_below(w.pos + 1 - kb);
-  uint32_t keep = win & win_below(n0 - kb);
-  if (kb + 32 > n0) {
-    // Tree keys: bits [kb - n0, kb - n0 + 32) of the row's set.
-    const uint64_t* t = a.bits + ((int64_t)b * a.M + w.m) * a.MW;
-    const int64_t at = kb - n0;
-    uint64_t x = 0;
-    if (at < 0) {
-      x = t[0] << (int)-at;
-    } else if ((at >> 6) < a.MW) {
-      const int i = (int)(at >> 6), sh = (int)(at & 63);
-      x = t[i] >> sh;
-      if (sh > 32 && i + 1 < a.MW) x |= t[i + 1] << (64 - sh);
-    }
-    keep |= (uint32_t)x;
-  }
-  return keep;
-}
-
-// Element offset of key n of the K or V half, for its physical page.
-__device__ __forceinline__ int64_t key_off(const WinArgs& a, int64_t sp, int64_t st, int64_t n, int32_t page) {
-  return a.pt != nullptr ? page * sp + (n & ((1ll << a.ps_shift) - 1)) * st : n * st;
-}
-__device__ __forceinline__ int32_t page_of(const WinArgs& a, int b, int64_t n) {
-  const int64_t i = (int64_t)b * a.pt_sb + (n >> a.ps_shift);
-  int64_t p = a.pt_i64 ? reinterpret_cast<const int64_t*>(a.pt)[i] : (int64_t) reinterpret_cast<const int32_t*>(a.pt)[i];
-  p = p < 0 ? 0 : (p >= a.n_phys ? a.n_phys - 1 : p);
-  return (int32_t)p;
-}
-
-__device__ __forceinline__ int64_t len_of(const WinArgs& a, int b) {
-  int64_t n = a.n_keys;
-  if (a.seqlens != nullptr) {
-    const int64_t x = a.seqlens_i64 ? reinterpret_cast<const int64_t*>(a.seqlens)[b]
-                                    : (int64_t) reinterpret_cast<const int32_t*>(a.seqlens)[b];
-    n = x < 0 ? 0 : (x < n ? x : n);
-  }
-  return n;
-}
-
-// Writes N consecutive output elements.
-template <int N>
-__device__ __forceinline__ void store_out(const WinArgs& a, int64_t off, const float (&x)[N]) {
-  static_assert(N == 4 || N == 8, "");
-  if (a.out_dtype == 2) {
-    float* o = reinterpret_cast<float*>(a.out) + off;
-    if (a.out_vec) {
-#pragma unroll
-      for (int i = 0; i < N; i += 4) *reinterpret_cast<f32x4*>(o + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = x[i];
-    }
-    return;
-  }
-  uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + off;
-  uint32_t w[N / 2];
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i)
-    w[i] = a.out_dtype == 0 ? pack2<BF16>(x[2 * i], x[2 * i + 1]) : pack2<F16>(x[2 * i], x[2 * i + 1]);
-  if (a.out_vec) {
-    if constexpr (N == 8)
-      *reinterpret_cast<u32x4*>(o) = u32x4{w[0], w[1], w[2], w[3]};
-    else
-      *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-  }
-}
-
 // ---- the tree's visibility ---------------------------------------------------
 // Depth and the visible ancestor-or-self set of every node, once per call: a
 // walk up the parents of at most M steps (a parent < 0, >= M or equal to the
@@ -224,7 +87,7 @@ __global__ void __launch_bounds__(256) win_tree_kernel(const WinArgs a, const vo
     par[i] = x < 0 || x >= M || x == i ? -1 : (int32_t)x;
   }
   __syncthreads();
-  const int64_t n0 = len_of(a, b) - M;
+  const int n0 = len_of(a, b) - M;
   for (int i = threadIdx.x; i < M; i += 256) {
     int d = 0;
     for (int x = par[i]; x >= 0 && d < M; x = par[x]) ++d;
@@ -266,7 +129,7 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
   const int rb = w % a.n_rb;
   w /= a.n_rb;
   const int kvh = w % a.Hk, b = w / a.Hk;
-  const int64_t n0 = len_of(a, b) - a.M;
+  const int n0 = len_of(a, b) - a.M;
   const int r0 = rb * 16 * NR;
   const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, r0, 16 * NR);
   const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
@@ -275,7 +138,7 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
   // This lane's rows: Q fragments (B operand): row lr, elements 32 ks + 8 lg ..
   Row row[NR];
   u32x4 qf[NR][KS];
-  int64_t pmin = INT64_MAX, pmax = INT64_MIN;
+  int pmin = 0x7fffffff, pmax = -0x7fffffff;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int r = min(r0 + 16 * i + lr, a.R - 1);
@@ -288,8 +151,8 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
   }
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
-    pmin = min(pmin, (int64_t)__shfl_xor((long long)pmin, o));
-    pmax = max(pmax, (int64_t)__shfl_xor((long long)pmax, o));
+    pmin = min(pmin, __shfl_xor(pmin, o));
+    pmax = max(pmax, __shfl_xor(pmax, o));
   }
 
   float mx[NR], ls[NR];
@@ -307,16 +170,15 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
   // Lane l holds the page of key l (mod 32) of a tile, read a tile ahead.
   auto tile_pages = [&](int tt) -> int32_t {
     if (a.pt == nullptr || tt >= t_end) return 0;
-    return page_of(a, b, min(kl.base(tt) + (lane & 31), kl.hi - 1));
+    return page_of(a, b, kl.read(kl.base(tt) + (lane & 31)));
   };
   u32x4 kr[NL], vr[NL];
   auto load_tile = [&](int tt, int32_t pg) {
-    const int64_t kb = kl.base(tt);
+    const int kb = kl.base(tt);
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int i = j * KPI + lane / CH;
-      // Keys behind the last one read the last one (inside the tensor).
-      const int64_t n = min(kb + i, kl.hi - 1);
+      const int n = kl.read(kb + i);
       const int32_t page = a.pt != nullptr ? __shfl(pg, i) : 0;
       kr[j] = *reinterpret_cast<const u32x4*>(kbase + key_off(a, a.k_sp, a.k_st, n, page));
       vr[j] = *reinterpret_cast<const u32x4*>(vbase + key_off(a, a.v_sp, a.v_st, n, page));
@@ -327,7 +189,7 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
   if (t < t_end) load_tile(t, pg);
   pg = tile_pages(t + NW);
   for (; t < t_end; t += NW) {
-    const int64_t kb = kl.base(t);
+    const int kb = kl.base(t);
     // ---- S^T = K . Q^T
 #pragma unroll
     for (int j = 0; j < NL; ++j)
@@ -504,7 +366,7 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
   const int rb = w % a.n_rb;
   w /= a.n_rb;
   const int kvh = w % a.Hk, b = w / a.Hk;
-  const int64_t n0 = len_of(a, b) - a.M;
+  const int n0 = len_of(a, b) - a.M;
   const int r0 = rb * 16;
   const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, r0, 16);
   const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
@@ -516,11 +378,11 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
   const float* q = reinterpret_cast<const float*>(a.q) + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh;
 #pragma unroll
   for (int c = 0; c < KC; ++c) qf[c] = *reinterpret_cast<const f32x4*>(q + 16 * c + 4 * lg);
-  int64_t pmin = row.pos, pmax = row.pos;
+  int pmin = row.pos, pmax = row.pos;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
-    pmin = min(pmin, (int64_t)__shfl_xor((long long)pmin, o));
-    pmax = max(pmax, (int64_t)__shfl_xor((long long)pmax, o));
+    pmin = min(pmin, __shfl_xor(pmin, o));
+    pmax = max(pmax, __shfl_xor(pmax, o));
   }
   float mx = kNegInf, ls = 0.f;
   f32x4 acc[DT];
@@ -528,13 +390,13 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
 
   for (int t = (int)((int64_t)kl.nt * split / a.splits) + wave; t < t_end; t += NW) {
-    const int64_t kb = kl.base(t);
+    const int kb = kl.base(t);
     const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
     const uint32_t keep = masked ? keep_word(a, b, row, kb, n0) : ~0u;
     f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int64_t n = min(kb + 16 * h + lr, kl.hi - 1);
+      const int n = kl.read(kb + 16 * h + lr);
       const float* k = kbase + key_off(a, a.k_sp, a.k_st, n, a.pt != nullptr ? page_of(a, b, n) : 0) + 4 * lg;
       f32x4 kf[KC];
 #pragma unroll
@@ -570,7 +432,7 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int64_t n = min(kb + 16 * (e >> 2) + 4 * lg + (e & 3), kl.hi - 1);
+      const int n = kl.read(kb + 16 * (e >> 2) + 4 * lg + (e & 3));
       const float* v = vbase + key_off(a, a.v_sp, a.v_st, n, a.pt != nullptr ? page_of(a, b, n) : 0) + lr;
       const bool has = kl.has(kb + 16 * (e >> 2) + 4 * lg + (e & 3));
       float vf[DT];
@@ -695,6 +557,8 @@ hipError_t launch_d(const WinArgs& a, hipStream_t s) {
   if (a.dtype == 2) {
     hipLaunchKernelGGL(win_rows_f32_kernel<D>, dim3((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), dim3(256), 0, s, a);
     e = hipGetLastError();
+  } else if (a.rows_per_block == 256) {
+    e = launch_window_tile(a, D, s);
   } else {
     e = a.dtype == 0 ? launch_rows<BF16, D>(a, s) : launch_rows<F16, D>(a, s);
   }

@@ -1,0 +1,505 @@
+// dsv_window_tile.hip — windowed attention for many rows (chunks of prompts,
+// trees): the matrix-bound side of dsv_window.hip, whose mathematics and row
+// packing it shares.
+//
+// A workgroup of 8 waves owns 256 rows of a KV head (256 / G positions, so the
+// keys outside a row's window are few), each wave 32.  K and V tiles of 32 keys
+// go HBM -> LDS by LDS-DMA into a ring of four tiles, and every tile feeds all
+// 256 rows.  The schedule is that of dsv_attn.hip: waves 0-3 issue the K half of
+// the DMA and waves 4-7 the V half, and on each SIMD one wave runs its softmax on
+// the VALU while the other's MFMAs run.  Differences: the tiles are the sinks'
+// and the window's (tile t -> key by WinKeys::base), rows and masks are the
+// window's, addresses are 64-bit per lane, so a cache of any size and stride
+// takes the one path, and pages of at least one DMA instruction's keys are
+// resolved from a register window of 64 tiles.
+
+#include "dsv_attn_geo.h"
+#include "dsv_dma.h"
+#include "dsv_window_dev.h"
+
+namespace dsv {
+
+namespace {
+
+// The running maximum used for the exponentials may lag the true one by this
+// much (log2 units), and, on unmasked tiles, a lane's probabilities may sum up to
+// 2^kSumTau before the tile is redone: every probability then stays below what
+// its 16-bit type holds (f16: 65504).
+constexpr float kRescaleTau = 8.0f;
+template <typename T>
+constexpr float kSumBound = 65536.f;
+template <>
+constexpr float kSumBound<F16> = 32768.f;
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
+template <>
+__device__ __forceinline__ f32x16 mfma32<BF16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 mfma32<F16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float xor32_max(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor32_sum(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// A lane's 16 scores (NaN-propagating).
+__device__ __forceinline__ float max16(const f32x16& s) {
+  float m = __builtin_elementwise_maximum(s[0], s[1]);
+#pragma unroll
+  for (int v = 2; v < 16; ++v) m = __builtin_elementwise_maximum(m, s[v]);
+  return m;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// LDS-DMA of 16 bytes per lane from a per-lane address; lane l lands at
+// lds + 16 l.
+__device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
+}
+
+template <int N>
+struct IC {
+  static constexpr int value = N;
+};
+
+// A wave's 32 rows once more, from memory and without matrix products, where V
+// holds infinities or NaN in keys that some of the rows do not see: in the
+// product 0 * inf would reach those rows.  A lane takes a key of 64 for the
+// scores and D / 64 columns for the sums.
+template <typename T, int D>
+__device__ __forceinline__ void exact_rows(const WinArgs& a, int b, int kvh, int split, const WinKeys& kl, int n0, int t0, int t1,
+                                        int row0) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const uint16_t* kbase = a.k + b * a.k_sb + kvh * a.k_sh;
+  const uint16_t* vbase = a.v + b * a.v_sb + kvh * a.v_sh;
+  for (int r = row0; r < row0 + 32 && r < a.R; ++r) {
+    const Row row = row_of(a, b, r, n0);
+    const int h = kvh * a.G + row.g;
+    const uint16_t* q = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)h * a.q_sh;
+    float m = kNegInf, l = 0.f, o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0.f;
+    for (int t = t0; t < t1; t += 2) {
+      const int tt = t + (lane >> 5), i = lane & 31;
+      const int kb = kl.base(min(tt, t1 - 1));
+      const bool seen = tt < t1 && ((keep_word(a, b, row, kb, n0) >> i) & 1u);
+      const int n = kl.read(kb + i);
+      const int32_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
+      const uint16_t* k = kbase + key_off(a, a.k_sp, a.k_st, n, page);
+      const int64_t vo = key_off(a, a.v_sp, a.v_st, n, page);
+      float s = kNegInf;
+      if (seen) {
+        s = 0.f;
+        for (int d = 0; d < D; ++d) s = fmaf(unpack1<T>(q[d]), unpack1<T>(k[d]), s);
+      }
+      float mt = s;
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) mt = fmaxf(mt, __shfl_xor(mt, x));
+      const float mn = fmaxf(m, mt * a.scale_log2), ms = mn == kNegInf ? 0.f : mn;
+      const float al = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, a.scale_log2, -ms)) : 0.f;
+      float ps = p;
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) ps += __shfl_xor(ps, x);
+      l = l * al + ps;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] *= al;
+      for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
+        const int src = __builtin_ctzll(left);
+        const float pn = __shfl(p, src);
+        const uint16_t* v = vbase + (int64_t)__shfl((long long)vo, src) + lane * N;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = fmaf(pn, unpack1<T>(v[e]), o[e]);
+      }
+    }
+    if (a.splits > 1) {
+      const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
+#pragma unroll
+      for (int e = 0; e < N; ++e) a.opart[pr * D + lane * N + e] = o[e];
+      if (lane == 0) a.ml[pr] = make_float2(m, l);
+      continue;
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const int64_t off = b * a.o_sb + (int64_t)row.m * a.o_sm + (int64_t)h * a.o_sh + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = o[e] * inv;
+      if (a.out_dtype == 2)
+        reinterpret_cast<float*>(a.out)[off + e] = x;
+      else
+        reinterpret_cast<uint16_t*>(a.out)[off + e] = (uint16_t)(a.out_dtype == 0 ? pack2<BF16>(x, x) : pack2<F16>(x, x));
+    }
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[b * a.l_sb + (int64_t)row.m * a.l_sm + (int64_t)h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+  }
+}
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
+  using G = Geo<D>;
+  constexpr int NW = 8;
+  constexpr int KS = D / 16;
+  constexpr int DT = D / 32;
+  constexpr int CH = G::CH;
+  constexpr int IPW = 2 * G::NINS / NW;  // DMA instructions per wave and tile
+  static_assert(IPW * NW == 2 * G::NINS && G::NINS % IPW == 0, "K and V DMA halves map to wave halves");
+  static_assert(G::STAGES == 4 && NW * 32 * D * 2 <= G::RING, "");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[G::RING];
+
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, lj = lane & 31, lg = lane >> 5;
+
+  // Dispatch ids go round-robin over the 8 XCDs: give each a contiguous eighth,
+  // so that the row blocks that share keys share an L2.
+  const int nblk = gridDim.x;
+  int w = (nblk & 7) == 0 ? (int)(blockIdx.x & 7) * (nblk >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+  const int rb = w % a.n_rb;
+  w /= a.n_rb;
+  const int split = w % a.splits;
+  w /= a.splits;
+  const int kvh = w % a.Hk, b = w / a.Hk;
+
+  const bool tree = a.bits != nullptr;
+  const int n0 = uniform(len_of(a, b) - a.M);
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, tree, n0, rb * 256, 256);
+  const int t_lo = (int)((int64_t)kl.nt * split / a.splits);
+  const int ntiles = (int)((int64_t)kl.nt * (split + 1) / a.splits) - t_lo;
+
+  // ---- this wave's rows: Q fragments (B operand of S^T = K . Q^T) ------------
+  const int row0 = rb * 256 + wid * 32;
+  const bool wave_active = row0 < a.R;
+  const int r_me = row0 + lj;
+  const bool rvalid = r_me < a.R;
+  const Row row = row_of(a, b, min(r_me, a.R - 1), n0);
+  u32x4 qf[KS];
+  {
+    const uint16_t* qp = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh + lg * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + ks * 16);
+  }
+  int pmin = row.pos, pmax = row.pos;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    pmin = min(pmin, __shfl_xor(pmin, o));
+    pmax = max(pmax, __shfl_xor(pmax, o));
+  }
+  pmin = uniform(pmin);
+  pmax = uniform(pmax);
+
+  // ---- DMA of one tile into its ring stage --------------------------------------
+  // Instruction x of this wave covers keys [j*KPI, (j+1)*KPI) of the tile's K
+  // (waves 0-3) or V half; lane p fills key j*KPI + p/CH, slot p%CH, which holds
+  // global chunk slot ^ swizzle(key).
+  const bool v_wave = wid >= NW / 2;
+  const int kii = lane / CH, slot = lane % CH;
+  const int64_t st2 = 2 * (v_wave ? a.v_st : a.k_st), sp2 = 2 * (v_wave ? a.v_sp : a.k_sp);
+  const char* hbase = reinterpret_cast<const char*>(v_wave ? a.v + b * a.v_sb + kvh * a.v_sh : a.k + b * a.k_sb + kvh * a.k_sh);
+  const char* lbase[IPW];  // + chunk
+  int jx[IPW];
+#pragma unroll
+  for (int x = 0; x < IPW; ++x) {
+    bool is_v;
+    dma_ins<D>(wid * IPW + x, is_v, jx[x]);
+    const int key_t = jx[x] * G::KPI + kii;
+    lbase[x] = hbase + (v_wave ? v_slot(CH, key_t, slot) : k_slot(CH, key_t, slot)) * 16;
+  }
+  const int psm = (1 << a.ps_shift) - 1;
+  const int64_t lane_off = kii * st2;
+  // Paged: lane l holds the page of instruction x's keys in tile pgw_t0 + l.
+  int32_t pgw[IPW];
+  int pgw_t0 = -64;
+#pragma unroll
+  for (int x = 0; x < IPW; ++x) pgw[x] = 0;
+  auto fill_pgw = [&](int t0) {
+    pgw_t0 = t0;
+#pragma unroll
+    for (int x = 0; x < IPW; ++x)
+      pgw[x] = page_of(a, b, kl.read(kl.base(t_lo + min(t0 + lane, ntiles - 1)) + jx[x] * G::KPI));
+  };
+  auto issue_tile = [&](auto stage_c, int t) {
+    constexpr int stage = decltype(stage_c)::value;
+    // (Windows start at multiples of 64: only stage 0 starts one.)
+    if (PAGED && stage == 0 && t - pgw_t0 >= 64) fill_pgw(t);
+    const int kb = kl.base(t_lo + t);
+    const bool whole = kl.whole(kb);
+#pragma unroll
+    for (int x = 0; x < IPW; ++x) {
+      const uint32_t dst = lds_addr(smem + (stage * 2 + (v_wave ? 1 : 0)) * G::TILE + jx[x] * 1024);
+      const int nb = kb + jx[x] * G::KPI;
+      // The lane's key; at a border one that some row sees (an instruction's keys
+      // share a page: those at its ends may have to be read through their own).
+      int64_t off = lane_off;
+      if (PAGED) {
+        const int32_t page = __builtin_amdgcn_readlane(pgw[x], t - pgw_t0);
+        off += page * sp2 + (nb & psm) * st2;
+      } else {
+        off += nb * st2;
+      }
+      if (!whole) {
+        const int n = kl.read(nb + kii);
+        off = key_off(a, sp2, st2, n, PAGED ? page_of(a, b, n) : 0);
+      }
+      dma_lane(dst, lbase[x] + off);
+    }
+  };
+
+  f32x16 acc[DT];
+  float mx = kNegInf, lsum = 0.f;
+  uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+
+  // Per-lane LDS offsets of the operand reads within a tile (as dsv_attn.hip).
+  uint32_t koff[KS], voff[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = lj * (2 * D) + k_slot(CH, lj, 2 * ks + lg) * 16;
+  {
+    const int bl = lane >> 4, bi = lane & 15;
+    const int vkey = 4 * (bl >> 1) + (bi >> 2);
+    const int vcol = 16 * (bl & 1) + 4 * (bi & 3);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int col = dt * 32 + vcol;
+      voff[dt] = vkey * (2 * D) + v_slot(CH, vkey, col >> 3) * 16 + (col & 7) * 2;
+    }
+  }
+
+  auto sync = [&](auto stage3_c, int k) {
+    if (k + 2 < ntiles)
+      wait_vmcnt<IPW>();
+    else
+      wait_vmcnt<0>();
+    barrier_lds();
+    if (k + 3 < ntiles) issue_tile(stage3_c, k + 3);
+  };
+
+  f32x16 s_cur = f32x16{};
+  auto read_k = [&](auto stage_c, u32x4 (&kf)[KS]) {
+    constexpr int stage = decltype(stage_c)::value;
+    const uint8_t* kt = smem + stage * 2 * G::TILE;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const u32x4*>(kt + koff[ks]);
+  };
+  auto read_vh = [&](auto stage_c, int hh, u32x4 (&vf)[2][DT]) {
+    constexpr int stage = decltype(stage_c)::value;
+    const uint8_t* vt = smem + (stage * 2 + 1) * G::TILE;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const uint8_t* p = vt + voff[dt] + hh * 16 * (2 * D);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * (2 * D)));
+      const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+      vf[hh][dt] = u32x4{l2[0], l2[1], h2[0], h2[1]};
+    }
+  };
+
+  const float scale_log2 = a.scale_log2;
+
+  auto step = [&](auto stage_c, int k) {
+    constexpr int S = decltype(stage_c)::value;
+    if (!v_wave && k > 0) sync(IC<(S + 3) & 3>{}, k);
+    u32x4 kf[KS], vf[2][DT];
+    u32x4 pk[2];
+    if (wave_active) {
+      read_k(IC<(S + 1) & 3>{}, kf);
+      const int kb = kl.base(t_lo + k);
+      const bool drops = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, tree);
+      uint32_t keep = ~0u;
+      if (drops) {
+        keep = keep_word(a, b, row, kb, n0);
+        // Bit v of a lane <-> key 8 * (v / 4) + 4 * lg + v % 4.
+        const uint32_t vb = keep >> (4 * lg);
+        const uint32_t kv = (vb & 0xFu) | ((vb >> 4) & 0xF0u) | ((vb >> 8) & 0xF00u) | ((vb >> 12) & 0xF000u);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s_cur[v] = ((kv >> v) & 1u) ? s_cur[v] : kNegInf;
+      }
+      auto rescale = [&]() {
+        const float mt = xor32_max(max16(s_cur)) * scale_log2;
+        if (__ballot(mt > mx + kRescaleTau) != 0ull) {
+          const float mn = __builtin_elementwise_maximum(mx, mt);
+          const float al = (mn == mx) ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
+          mx = mn;
+          lsum *= al;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
+        }
+      };
+      if (drops || __ballot(mx == kNegInf) != 0ull) rescale();
+      auto exps = [&](bool with_v) {
+        const float ms = (mx == kNegInf) ? 0.f : mx;
+        float ts = 0.f;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          if (with_v) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_vh(IC<S>{}, hh, vf);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          uint32_t w4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s_cur[hh * 8 + 2 * e], scale_log2, -ms));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s_cur[hh * 8 + 2 * e + 1], scale_log2, -ms));
+            w4[e] = pack2<T>(p0, p1);
+            ts += p0 + p1;
+          }
+          pk[hh] = u32x4{w4[0], w4[1], w4[2], w4[3]};
+        }
+        return ts;
+      };
+      float ts = exps(true);
+      if (!drops && __ballot(!(ts <= kSumBound<T>)) != 0ull) {
+        rescale();
+        ts = exps(false);
+      }
+      lsum += ts;
+      if (drops) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= nonfinite2<T>(vf[hh][dt][e]);
+      }
+    }
+    if (v_wave) sync(IC<(S + 3) & 3>{}, k);
+    if (wave_active) {
+      f32x16 sn = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) sn = mfma32<T>(kf[ks], qf[ks], sn);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<T>(vf[hh][dt], pk[hh], acc[dt]);
+      s_cur = sn;
+    }
+  };
+
+  // ---- prologue: K(0..2) and V(0..1) issued, barrier 0, S(0) ---------------------
+  if (ntiles > 0) issue_tile(IC<0>{}, 0);
+  if (ntiles > 1) issue_tile(IC<1>{}, 1);
+  if (ntiles > 2 && !v_wave) issue_tile(IC<2>{}, 2);
+  // The Q fragments and the score scale are complete before the loop: waits
+  // placed at a first use inside it would wait for the DMA in flight there.
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks]));
+  asm volatile("" ::"s"(scale_log2));
+  if (ntiles > 0) {
+    if (v_wave ? ntiles > 1 : ntiles > 2)
+      wait_vmcnt<IPW>();
+    else
+      wait_vmcnt<0>();
+    barrier_lds();
+    if (v_wave) {
+      if (ntiles > 2) issue_tile(IC<2>{}, 2);
+    } else {
+      if (ntiles > 3) issue_tile(IC<3>{}, 3);
+    }
+    if (wave_active) {
+      u32x4 kf[KS];
+      read_k(IC<0>{}, kf);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s_cur = mfma32<T>(kf[ks], qf[ks], s_cur);
+    }
+  }
+  for (int t0 = 0; t0 < ntiles; t0 += 4) {
+    step(IC<0>{}, t0);
+    if (t0 + 1 < ntiles) step(IC<1>{}, t0 + 1);
+    if (t0 + 2 < ntiles) step(IC<2>{}, t0 + 2);
+    if (t0 + 3 < ntiles) step(IC<3>{}, t0 + 3);
+  }
+  // K waves meet the last barrier (V waves met it after the softmax of the last tile).
+  if (ntiles > 0 && !v_wave) {
+    wait_vmcnt<0>();
+    barrier_lds();
+  }
+
+  // ---- epilogue -------------------------------------------------------------------
+  __syncthreads();
+  if (!wave_active) return;
+  if (__ballot(odd != 0) != 0ull) {
+    exact_rows<T, D>(a, b, kvh, split, kl, n0, t_lo, t_lo + ntiles, row0);
+    return;
+  }
+  const float ltot = xor32_sum(lsum);
+  const int h = kvh * a.G + row.g;
+  // Accumulator value v of d tile dt holds d = 32*dt + 8*(v/4) + 4*lg + v%4.
+  if (a.splits > 1) {
+    const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r_me;
+    if (!rvalid) return;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<f32x4*>(a.opart + pr * D + 32 * dt + 8 * q4 + 4 * lg) =
+            f32x4{acc[dt][4 * q4], acc[dt][4 * q4 + 1], acc[dt][4 * q4 + 2], acc[dt][4 * q4 + 3]};
+    if (lg == 0) a.ml[pr] = make_float2(mx, ltot);
+    return;
+  }
+  const float inv = ltot > 0.f ? 1.f / ltot : (ltot == 0.f ? 0.f : ltot);
+  const int64_t off = b * a.o_sb + (int64_t)row.m * a.o_sm + (int64_t)h * a.o_sh;
+  if (rvalid && lg == 0 && a.lse != nullptr)
+    a.lse[b * a.l_sb + (int64_t)row.m * a.l_sm + (int64_t)h * a.l_sh] = ltot == 0.f ? kNegInf : (mx + __log2f(ltot)) * kLn2;
+  if (a.out_dtype == 2 || !a.out_vec) {
+    if (!rvalid) return;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float x[4] = {acc[dt][4 * q4] * inv, acc[dt][4 * q4 + 1] * inv, acc[dt][4 * q4 + 2] * inv, acc[dt][4 * q4 + 3] * inv};
+        store_out<4>(a, off + 32 * dt + 8 * q4 + 4 * lg, x);
+      }
+    return;
+  }
+  // Rows through the ring, so that a store instruction writes whole rows.
+  constexpr int CHR = D / 8;
+  uint8_t* stage = smem + wid * (32 * D * 2);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const float x0 = acc[dt][4 * q4] * inv, x1 = acc[dt][4 * q4 + 1] * inv, x2 = acc[dt][4 * q4 + 2] * inv, x3 = acc[dt][4 * q4 + 3] * inv;
+      const u32x2 val = a.out_dtype == 0 ? u32x2{pack2<BF16>(x0, x1), pack2<BF16>(x2, x3)} : u32x2{pack2<F16>(x0, x1), pack2<F16>(x2, x3)};
+      const int c = 4 * dt + q4;
+      *reinterpret_cast<u32x2*>(stage + lj * (2 * D) + ((c ^ (lj % CHR)) * 16) + 8 * lg) = val;
+    }
+  wave_lds_fence();
+#pragma unroll
+  for (int k = 0; k < CHR / 2; ++k) {
+    const int f = k * 64 + lane, r = f / CHR, i = f % CHR;
+    const u32x4 chunk = *reinterpret_cast<const u32x4*>(stage + r * (2 * D) + ((i ^ (r % CHR)) * 16));
+    const int64_t o = __shfl((long long)off, r);
+    if (row0 + r < a.R) *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.out) + o + i * 8) = chunk;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_t(const WinArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits));
+  if (a.pt != nullptr)
+    hipLaunchKernelGGL((win_tile_kernel<T, D, true>), grid, dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((win_tile_kernel<T, D, false>), grid, dim3(512), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_window_tile(const WinArgs& a, int D, hipStream_t s) {
+  if (a.dtype == 0) return D == 64 ? launch_t<BF16, 64>(a, s) : launch_t<BF16, 128>(a, s);
+  return D == 64 ? launch_t<F16, 64>(a, s) : launch_t<F16, 128>(a, s);
+}
+
+}  // namespace dsv
