@@ -16,6 +16,7 @@ struct WinArgs {
   int64_t q_sb, q_sm, q_sh;
   const uint16_t* k; int64_t k_sb, k_sp, k_sh, k_st;
   const uint16_t* v; int64_t v_sb, v_sp, v_sh, v_st;
+  int64_t k_bytes, v_bytes;                // spans of the views
   const void* pt; int pt_i64, ps_shift;    // page table (nullptr: dense)
   int64_t pt_sb, n_phys;
   const void* seqlens; int seqlens_i64;    // optional [B]

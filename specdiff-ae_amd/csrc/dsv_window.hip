@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
     for (int i = 0; i < NR; ++i) {
       keep[i] = ~0u;
       if (masked) {
-        keep[i] = keep_word(a, b, row[i], kb, n0);
+        keep[i] = keep_word(a, b, row[i].m, row[i].pos, kb, n0);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (!((keep[i] >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[i][e >> 2][e & 3] = kNegInf;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
   for (int t = (int)((int64_t)kl.nt * split / a.splits) + wave; t < t_end; t += NW) {
     const int kb = kl.base(t);
     const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
-    const uint32_t keep = masked ? keep_word(a, b, row, kb, n0) : ~0u;
+    const uint32_t keep = masked ? keep_word(a, b, row.m, row.pos, kb, n0) : ~0u;
     f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {

@@ -68,13 +68,13 @@ __device__ __forceinline__ Row row_of(const WinArgs& a, int b, int r, int n0) {
 }
 
 // The keep word of a row for the tile at key kb: bit i = key kb + i is seen.
-__device__ __forceinline__ uint32_t keep_word(const WinArgs& a, int b, const Row& w, int kb, int n0) {
-  const uint32_t win = ~win_below(w.pos - a.W + 1 - kb) | win_below(a.S - kb);
-  if (a.bits == nullptr) return win & win_below(w.pos + 1 - kb);
+__device__ __forceinline__ uint32_t keep_word(const WinArgs& a, int b, int m, int pos, int kb, int n0) {
+  const uint32_t win = ~win_below(pos - a.W + 1 - kb) | win_below(a.S - kb);
+  if (a.bits == nullptr) return win & win_below(pos + 1 - kb);
   uint32_t keep = win & win_below(n0 - kb);
   if (kb + 32 > n0) {
     // Tree keys: bits [kb - n0, kb - n0 + 32) of the row's set.
-    const uint64_t* t = a.bits + ((int64_t)b * a.M + w.m) * a.MW;
+    const uint64_t* t = a.bits + ((int64_t)b * a.M + m) * a.MW;
     const int at = kb - n0;
     uint64_t x = 0;
     if (at < 0) {

@@ -58,13 +58,29 @@ __device__ __forceinline__ float max16(const f32x16& s) {
   return m;
 }
 
+// x, computed again at every use: what is derived from it is not held in
+// registers across the loop.
+__device__ __forceinline__ int again(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// LDS-DMA of 16 bytes per lane from a per-lane address; lane l lands at
-// lds + 16 l.
+// LDS-DMA of 16 bytes per lane; lane l lands at lds + 16 l.  From a per-lane
+// address, or from a uniform base plus a 32-bit lane offset through a buffer
+// resource whose range ends with the tensor.
 __device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
+}
+
+// The kernel's arguments, loaded again where they are needed: what the epilogue
+// reads does not stay in registers through the loop.
+__device__ __forceinline__ const WinArgs& args_again() {
+  typedef const WinArgs __attribute__((address_space(4))) * Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const WinArgs*)p;
 }
 
 template <int N>
@@ -77,8 +93,10 @@ struct IC {
 // product 0 * inf would reach those rows.  A lane takes a key of 64 for the
 // scores and D / 64 columns for the sums.
 template <typename T, int D>
-__device__ __forceinline__ void exact_rows(const WinArgs& a, int b, int kvh, int split, const WinKeys& kl, int n0, int t0, int t1,
-                                        int row0) {
+__device__ __noinline__ void exact_rows(const WinArgs* ap, int b, int kvh, int split, int rb, int t0, int t1, int row0) {
+  const WinArgs& a = *ap;
+  const int n0 = len_of(a, b) - a.M;
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, rb * 256, 256);
   constexpr int N = D / 64;
   const int lane = threadIdx.x & 63;
   const uint16_t* kbase = a.k + b * a.k_sb + kvh * a.k_sh;
@@ -93,7 +111,7 @@ __device__ __forceinline__ void exact_rows(const WinArgs& a, int b, int kvh, int
     for (int t = t0; t < t1; t += 2) {
       const int tt = t + (lane >> 5), i = lane & 31;
       const int kb = kl.base(min(tt, t1 - 1));
-      const bool seen = tt < t1 && ((keep_word(a, b, row, kb, n0) >> i) & 1u);
+      const bool seen = tt < t1 && ((keep_word(a, b, row.m, row.pos, kb, n0) >> i) & 1u);
       const int n = kl.read(kb + i);
       const int32_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
       const uint16_t* k = kbase + key_off(a, a.k_sp, a.k_st, n, page);
@@ -181,15 +199,16 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   const int row0 = rb * 256 + wid * 32;
   const bool wave_active = row0 < a.R;
   const int r_me = row0 + lj;
-  const bool rvalid = r_me < a.R;
-  const Row row = row_of(a, b, min(r_me, a.R - 1), n0);
   u32x4 qf[KS];
+  int pos;
   {
+    const Row row = row_of(a, b, min(r_me, a.R - 1), n0);
+    pos = row.pos;
     const uint16_t* qp = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh + lg * 8;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + ks * 16);
   }
-  int pmin = row.pos, pmax = row.pos;
+  int pmin = pos, pmax = pos;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     pmin = min(pmin, __shfl_xor(pmin, o));
@@ -203,20 +222,25 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   // (waves 0-3) or V half; lane p fills key j*KPI + p/CH, slot p%CH, which holds
   // global chunk slot ^ swizzle(key).
   const bool v_wave = wid >= NW / 2;
-  const int kii = lane / CH, slot = lane % CH;
   const int64_t st2 = 2 * (v_wave ? a.v_st : a.k_st), sp2 = 2 * (v_wave ? a.v_sp : a.k_sp);
-  const char* hbase = reinterpret_cast<const char*>(v_wave ? a.v + b * a.v_sb + kvh * a.v_sh : a.k + b * a.k_sb + kvh * a.k_sh);
-  const char* lbase[IPW];  // + chunk
+  const char* hbase = reinterpret_cast<const char*>(v_wave ? a.v : a.k);
+  const int64_t wg_off = 2 * (v_wave ? b * a.v_sb + kvh * a.v_sh : b * a.k_sb + kvh * a.k_sh);
+  const int64_t span = v_wave ? a.v_bytes : a.k_bytes;
+  const uint32_t half = lds_addr(smem) + (uint32_t)uniform(v_wave ? G::TILE : 0);
+  uint32_t lane_off[IPW];
   int jx[IPW];
+  auto chunk_of = [&](int x, int l) {
+    const int key_t = jx[x] * G::KPI + l / CH;
+    return v_wave ? v_slot(CH, key_t, l % CH) : k_slot(CH, key_t, l % CH);
+  };
 #pragma unroll
   for (int x = 0; x < IPW; ++x) {
     bool is_v;
     dma_ins<D>(wid * IPW + x, is_v, jx[x]);
-    const int key_t = jx[x] * G::KPI + kii;
-    lbase[x] = hbase + (v_wave ? v_slot(CH, key_t, slot) : k_slot(CH, key_t, slot)) * 16;
+    jx[x] = uniform(jx[x]);
+    lane_off[x] = (uint32_t)(lane / CH * st2) + (uint32_t)(chunk_of(x, lane) * 16);
   }
   const int psm = (1 << a.ps_shift) - 1;
-  const int64_t lane_off = kii * st2;
   // Paged: lane l holds the page of instruction x's keys in tile pgw_t0 + l.
   int32_t pgw[IPW];
   int pgw_t0 = -64;
@@ -226,7 +250,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     pgw_t0 = t0;
 #pragma unroll
     for (int x = 0; x < IPW; ++x)
-      pgw[x] = page_of(a, b, kl.read(kl.base(t_lo + min(t0 + lane, ntiles - 1)) + jx[x] * G::KPI));
+      pgw[x] = page_of(a, b, kl.read(kl.base(t_lo + min(t0 + again(lane), ntiles - 1)) + jx[x] * G::KPI));
   };
   auto issue_tile = [&](auto stage_c, int t) {
     constexpr int stage = decltype(stage_c)::value;
@@ -236,22 +260,21 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     const bool whole = kl.whole(kb);
 #pragma unroll
     for (int x = 0; x < IPW; ++x) {
-      const uint32_t dst = lds_addr(smem + (stage * 2 + (v_wave ? 1 : 0)) * G::TILE + jx[x] * 1024);
+      const uint32_t dst = half + (uint32_t)(stage * 2 * G::TILE + jx[x] * 1024);
       const int nb = kb + jx[x] * G::KPI;
-      // The lane's key; at a border one that some row sees (an instruction's keys
-      // share a page: those at its ends may have to be read through their own).
-      int64_t off = lane_off;
-      if (PAGED) {
-        const int32_t page = __builtin_amdgcn_readlane(pgw[x], t - pgw_t0);
-        off += page * sp2 + (nb & psm) * st2;
+      if (whole) {
+        int64_t off = wg_off;
+        if (PAGED)
+          off += __builtin_amdgcn_readlane(pgw[x], t - pgw_t0) * sp2 + (nb & psm) * st2;
+        else
+          off += nb * st2;
+        dma_rs<false>(dst, make_rsrc(hbase + off, rsrc_range(span, off / 2)), lane_off[x]);
       } else {
-        off += nb * st2;
+        // At a border: a key that some row sees, through its own page.
+        const int l = again(lane);
+        const int n = kl.read(nb + l / CH);
+        dma_lane(dst, hbase + wg_off + key_off(a, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
       }
-      if (!whole) {
-        const int n = kl.read(nb + kii);
-        off = key_off(a, sp2, st2, n, PAGED ? page_of(a, b, n) : 0);
-      }
-      dma_lane(dst, lbase[x] + off);
     }
   };
 
@@ -261,19 +284,17 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
 
-  // Per-lane LDS offsets of the operand reads within a tile (as dsv_attn.hip).
-  uint32_t koff[KS], voff[DT];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) koff[ks] = lj * (2 * D) + k_slot(CH, lj, 2 * ks + lg) * 16;
+  // Per-lane LDS offsets of the operand reads within a tile: K's of k-step ks is
+  // kofs ^ (ks << 5) and V's of d tile dt is vofs ^ (dt << 6) (the swizzles are
+  // XORs of whole chunks), one register each instead of one per step: 12 XORs a
+  // tile, where the registers would spill.
+  uint32_t kofs, vofs;
   {
     const int bl = lane >> 4, bi = lane & 15;
     const int vkey = 4 * (bl >> 1) + (bi >> 2);
     const int vcol = 16 * (bl & 1) + 4 * (bi & 3);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int col = dt * 32 + vcol;
-      voff[dt] = vkey * (2 * D) + v_slot(CH, vkey, col >> 3) * 16 + (col & 7) * 2;
-    }
+    kofs = lj * (2 * D) + k_slot(CH, lj, lg) * 16;
+    vofs = vkey * (2 * D) + v_slot(CH, vkey, vcol >> 3) * 16 + (vcol & 7) * 2;
   }
 
   auto sync = [&](auto stage3_c, int k) {
@@ -289,15 +310,17 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   auto read_k = [&](auto stage_c, u32x4 (&kf)[KS]) {
     constexpr int stage = decltype(stage_c)::value;
     const uint8_t* kt = smem + stage * 2 * G::TILE;
+    const uint32_t o = (uint32_t)again((int)kofs);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const u32x4*>(kt + koff[ks]);
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const u32x4*>(kt + (o ^ (ks << 5)));
   };
   auto read_vh = [&](auto stage_c, int hh, u32x4 (&vf)[2][DT]) {
     constexpr int stage = decltype(stage_c)::value;
     const uint8_t* vt = smem + (stage * 2 + 1) * G::TILE;
+    const uint32_t o = (uint32_t)again((int)vofs);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const uint8_t* p = vt + voff[dt] + hh * 16 * (2 * D);
+      const uint8_t* p = vt + (o ^ (dt << 6)) + hh * 16 * (2 * D);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * (2 * D)));
       const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
@@ -312,15 +335,15 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     if (!v_wave && k > 0) sync(IC<(S + 3) & 3>{}, k);
     u32x4 kf[KS], vf[2][DT];
     u32x4 pk[2];
-    if (wave_active) {
+    {
       read_k(IC<(S + 1) & 3>{}, kf);
       const int kb = kl.base(t_lo + k);
       const bool drops = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, tree);
       uint32_t keep = ~0u;
       if (drops) {
-        keep = keep_word(a, b, row, kb, n0);
+        keep = keep_word(a, b, tree ? min(row0 + (again(lane) & 31), a.R - 1) / a.G : 0, again(pos), kb, n0);
         // Bit v of a lane <-> key 8 * (v / 4) + 4 * lg + v % 4.
-        const uint32_t vb = keep >> (4 * lg);
+        const uint32_t vb = keep >> (again(lane) >> 5 << 2);
         const uint32_t kv = (vb & 0xFu) | ((vb >> 4) & 0xF0u) | ((vb >> 8) & 0xF00u) | ((vb >> 12) & 0xF000u);
 #pragma unroll
         for (int v = 0; v < 16; ++v) s_cur[v] = ((kv >> v) & 1u) ? s_cur[v] : kNegInf;
@@ -375,7 +398,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       }
     }
     if (v_wave) sync(IC<(S + 3) & 3>{}, k);
-    if (wave_active) {
+    {
       f32x16 sn = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sn = mfma32<T>(kf[ks], qf[ks], sn);
@@ -414,11 +437,22 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       for (int ks = 0; ks < KS; ++ks) s_cur = mfma32<T>(kf[ks], qf[ks], s_cur);
     }
   }
-  for (int t0 = 0; t0 < ntiles; t0 += 4) {
-    step(IC<0>{}, t0);
-    if (t0 + 1 < ntiles) step(IC<1>{}, t0 + 1);
-    if (t0 + 2 < ntiles) step(IC<2>{}, t0 + 2);
-    if (t0 + 3 < ntiles) step(IC<3>{}, t0 + 3);
+  if (wave_active) {
+    for (int t0 = 0; t0 < ntiles; t0 += 4) {
+      step(IC<0>{}, t0);
+      if (t0 + 1 < ntiles) step(IC<1>{}, t0 + 1);
+      if (t0 + 2 < ntiles) step(IC<2>{}, t0 + 2);
+      if (t0 + 3 < ntiles) step(IC<3>{}, t0 + 3);
+    }
+  } else {
+    // A wave without rows does its share of the DMA and meets the barriers.  (A
+    // loop of its own: tests inside the other one cost 20 registers.)
+    for (int t0 = 0; t0 < ntiles; t0 += 4) {
+      if (v_wave || t0 > 0) sync(IC<3>{}, t0);
+      if (t0 + 1 < ntiles) sync(IC<0>{}, t0 + 1);
+      if (t0 + 2 < ntiles) sync(IC<1>{}, t0 + 2);
+      if (t0 + 3 < ntiles) sync(IC<2>{}, t0 + 3);
+    }
   }
   // K waves meet the last barrier (V waves met it after the softmax of the last tile).
   if (ntiles > 0 && !v_wave) {
@@ -429,37 +463,45 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   // ---- epilogue -------------------------------------------------------------------
   __syncthreads();
   if (!wave_active) return;
+  const WinArgs& z = args_again();
+  // (Derived again, so that the loop keeps one register for all of them.)
+  int tid_ep = threadIdx.x;
+  asm volatile("" : "+v"(tid_ep));
+  const int le = tid_ep & 63, lje = le & 31, lge = le >> 5;
+  const int r_ep = row0 + lje;
+  const bool rvalid = r_ep < z.R;
   if (__ballot(odd != 0) != 0ull) {
-    exact_rows<T, D>(a, b, kvh, split, kl, n0, t_lo, t_lo + ntiles, row0);
+    exact_rows<T, D>(&z, b, kvh, split, rb, t_lo, t_lo + ntiles, row0);
     return;
   }
   const float ltot = xor32_sum(lsum);
-  const int h = kvh * a.G + row.g;
-  // Accumulator value v of d tile dt holds d = 32*dt + 8*(v/4) + 4*lg + v%4.
-  if (a.splits > 1) {
-    const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r_me;
+  const Row row = row_of(z, b, min(r_ep, z.R - 1), n0);
+  const int h = kvh * z.G + row.g;
+  // Accumulator value v of d tile dt holds d = 32*dt + 8*(v/4) + 4*lge + v%4.
+  if (z.splits > 1) {
+    const int64_t pr = ((int64_t)(b * z.Hk + kvh) * z.splits + split) * z.R + r_ep;
     if (!rvalid) return;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<f32x4*>(a.opart + pr * D + 32 * dt + 8 * q4 + 4 * lg) =
+        *reinterpret_cast<f32x4*>(z.opart + pr * D + 32 * dt + 8 * q4 + 4 * lge) =
             f32x4{acc[dt][4 * q4], acc[dt][4 * q4 + 1], acc[dt][4 * q4 + 2], acc[dt][4 * q4 + 3]};
-    if (lg == 0) a.ml[pr] = make_float2(mx, ltot);
+    if (lge == 0) z.ml[pr] = make_float2(mx, ltot);
     return;
   }
   const float inv = ltot > 0.f ? 1.f / ltot : (ltot == 0.f ? 0.f : ltot);
-  const int64_t off = b * a.o_sb + (int64_t)row.m * a.o_sm + (int64_t)h * a.o_sh;
-  if (rvalid && lg == 0 && a.lse != nullptr)
-    a.lse[b * a.l_sb + (int64_t)row.m * a.l_sm + (int64_t)h * a.l_sh] = ltot == 0.f ? kNegInf : (mx + __log2f(ltot)) * kLn2;
-  if (a.out_dtype == 2 || !a.out_vec) {
+  const int64_t off = b * z.o_sb + (int64_t)row.m * z.o_sm + (int64_t)h * z.o_sh;
+  if (rvalid && lge == 0 && z.lse != nullptr)
+    z.lse[b * z.l_sb + (int64_t)row.m * z.l_sm + (int64_t)h * z.l_sh] = ltot == 0.f ? kNegInf : (mx + __log2f(ltot)) * kLn2;
+  if (z.out_dtype == 2 || !z.out_vec) {
     if (!rvalid) return;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const float x[4] = {acc[dt][4 * q4] * inv, acc[dt][4 * q4 + 1] * inv, acc[dt][4 * q4 + 2] * inv, acc[dt][4 * q4 + 3] * inv};
-        store_out<4>(a, off + 32 * dt + 8 * q4 + 4 * lg, x);
+        store_out<4>(a, off + 32 * dt + 8 * q4 + 4 * lge, x);
       }
     return;
   }
@@ -471,17 +513,17 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
       const float x0 = acc[dt][4 * q4] * inv, x1 = acc[dt][4 * q4 + 1] * inv, x2 = acc[dt][4 * q4 + 2] * inv, x3 = acc[dt][4 * q4 + 3] * inv;
-      const u32x2 val = a.out_dtype == 0 ? u32x2{pack2<BF16>(x0, x1), pack2<BF16>(x2, x3)} : u32x2{pack2<F16>(x0, x1), pack2<F16>(x2, x3)};
+      const u32x2 val = z.out_dtype == 0 ? u32x2{pack2<BF16>(x0, x1), pack2<BF16>(x2, x3)} : u32x2{pack2<F16>(x0, x1), pack2<F16>(x2, x3)};
       const int c = 4 * dt + q4;
-      *reinterpret_cast<u32x2*>(stage + lj * (2 * D) + ((c ^ (lj % CHR)) * 16) + 8 * lg) = val;
+      *reinterpret_cast<u32x2*>(stage + lje * (2 * D) + ((c ^ (lje % CHR)) * 16) + 8 * lge) = val;
     }
   wave_lds_fence();
 #pragma unroll
   for (int k = 0; k < CHR / 2; ++k) {
-    const int f = k * 64 + lane, r = f / CHR, i = f % CHR;
+    const int f = k * 64 + le, r = f / CHR, i = f % CHR;
     const u32x4 chunk = *reinterpret_cast<const u32x4*>(stage + r * (2 * D) + ((i ^ (r % CHR)) * 16));
     const int64_t o = __shfl((long long)off, r);
-    if (row0 + r < a.R) *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.out) + o + i * 8) = chunk;
+    if (row0 + r < z.R) *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(z.out) + o + i * 8) = chunk;
   }
 }
 
