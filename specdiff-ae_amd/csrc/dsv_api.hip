@@ -1490,16 +1490,24 @@ int dsv_lmhead_accept(int mode, const dsv_tensor* hidden, const dsv_tensor* weig
 namespace {
 
 struct SpecPlan {
-  int64_t nsub = 0;
+  int nwg = 1, step = 0, step1 = 0;
   size_t state_bytes = 0, rej_bytes = 0, total = 0;
 };
 
+// Workgroups per tree: one per CU in all, at most so many that each wave has a
+// segment of the row.
 bool spec_plan(int64_t T, int64_t M, int64_t V, SpecPlan& p) {
   if (M < 1 || M > dsv::kSpecMaxM || T < 1 || T > (1 << 20) || V < 1 || V > 0x7fffffff) return false;
-  p.nsub = (V + dsv::kSpecSub - 1) / dsv::kSpecSub;
-  p.state_bytes = align_up((size_t)T * sizeof(dsv::SpecState), 256);
-  p.rej_bytes = align_up((size_t)T * M * sizeof(int32_t), 256);
-  p.total = p.state_bytes + p.rej_bytes + align_up((size_t)T * p.nsub * sizeof(double), 256);
+  const int64_t waves = dsv::kSpecThreads / 64, nseg = (V + dsv::kSpecSeg - 1) / dsv::kSpecSeg;
+  const int64_t most = std::min<int64_t>((nseg + waves - 1) / waves, dsv::kSpecSlots / waves);
+  p.nwg = (int)std::max<int64_t>(1, std::min(most, (int64_t)device_cus() / T));
+  p.step = (int)((nseg + waves * p.nwg - 1) / (waves * p.nwg));
+  p.step1 = (int)((nseg + waves - 1) / waves);
+  if (p.nwg > 1) {
+    p.state_bytes = align_up((size_t)T * sizeof(dsv::SpecState), 256);
+    p.rej_bytes = align_up((size_t)T * M * sizeof(int32_t), 256);
+    p.total = p.state_bytes + p.rej_bytes + align_up((size_t)T * p.nwg * waves * sizeof(double), 256);
+  }
   return true;
 }
 
@@ -1519,7 +1527,7 @@ extern "C" {
 
 size_t dsv_spec_workspace_bytes(int64_t T, int64_t M, int64_t V) {
   SpecPlan p;
-  return spec_plan(T, M, V, p) ? p.total : 0;
+  return spec_plan(T, M, V, p) ? std::max<size_t>(p.total, 256) : 0;
 }
 
 int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft, const dsv_tensor* parent,
@@ -1563,14 +1571,14 @@ int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft, const dsv
     if (o.t->dtype != DSV_I64 || o.t->shape[0] != T || o.t->shape[1] != o.cols || o.t->stride[1] != 1)
       return fail(DSV_ERR_INVALID, "%s must be int64 [T, %lld] with innermost stride 1", o.name, (long long)o.cols);
     if (T > 1 && o.t->stride[0] < o.cols) return fail(DSV_ERR_INVALID, "%s: rows overlap", o.name);
-    // Every workgroup of a tree reads the inputs while the first one writes.
+    // A tree's outputs are written while others' inputs are still read.
     for (const Extent& in : ins)
       if (overlap(extent_of(o.name, o.t), in)) return fail(DSV_ERR_INVALID, "%s overlaps %s", o.name, in.name);
   }
   if (overlap(extent_of("", out_path), extent_of("", out_tokens)) || overlap(extent_of("", out_path), extent_of("", out_info)) ||
       overlap(extent_of("", out_tokens), extent_of("", out_info)))
     return fail(DSV_ERR_INVALID, "outputs overlap each other");
-  if ((rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+  if (p.total > 0 && (rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
 
   dsv::SpecArgs a{};
   a.dtype = target->dtype;
@@ -1600,15 +1608,15 @@ int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft, const dsv
   a.ot_st = out_tokens->stride[0];
   a.out_info = static_cast<int64_t*>(out_info->data);
   a.oi_st = out_info->stride[0];
-  char* w = static_cast<char*>(workspace);
-  a.state = reinterpret_cast<dsv::SpecState*>(w);
-  a.rej = reinterpret_cast<int32_t*>(w + p.state_bytes);
-  a.part = reinterpret_cast<double*>(w + p.state_bytes + p.rej_bytes);
-  a.nsub = p.nsub;
-  // Workgroups per tree: enough to fill the GPU, at most one per sub-block
-  // (each walks the tree itself).
-  const int64_t fill = std::max<int64_t>(1, (int64_t)device_cus() * 4 / T);
-  a.nwg = (int)std::min(p.nsub, fill);
+  a.nwg = p.nwg;
+  a.step = p.step;
+  a.step1 = p.step1;
+  if (p.total > 0) {
+    char* w = static_cast<char*>(workspace);
+    a.state = reinterpret_cast<dsv::SpecState*>(w);
+    a.rej = reinterpret_cast<int32_t*>(w + p.state_bytes);
+    a.part = reinterpret_cast<double*>(w + p.state_bytes + p.rej_bytes);
+  }
   if (g_dry_run) return DSV_OK;
   const hipError_t e = dsv::launch_spec(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "speculative acceptance launch");

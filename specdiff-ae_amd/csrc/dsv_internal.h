@@ -207,11 +207,12 @@ struct BundleArgs {
 
 // Arguments of the verification of drafted tokens from given random numbers.
 constexpr int kSpecMaxM = 1024;            // tree nodes
-constexpr int kSpecThreads = 256;
-constexpr int kSpecSub = 4096;             // vocabulary entries per partial sum
+constexpr int kSpecThreads = 1024;
+constexpr int kSpecSeg = 512;              // vocabulary entries a wave sums at a time
+constexpr int kSpecSlots = 4096;           // sums of a row at most (16 per workgroup)
 struct SpecState {
   double c;                                // share of the draft's row taken from the last node's
-  int32_t node, len, nrej, pad;            // last node, path length, rejected tokens listed in rej
+  int32_t node, nrej;                      // last node, rejected tokens listed in rej
 };
 struct SpecArgs {
   int dtype;                               // dsv_dtype of target and dprobs
@@ -225,11 +226,11 @@ struct SpecArgs {
   int64_t* out_path; int64_t op_st;
   int64_t* out_tok; int64_t ot_st;
   int64_t* out_info; int64_t oi_st;
-  SpecState* state;                        // [T]
-  int32_t* rej;                            // [T, M]
-  double* part;                            // [T, nsub]
-  int64_t nsub;                            // sub-blocks of a row
   int nwg;                                 // workgroups per tree
+  int step, step1;                         // segments per slot: of 16 nwg slots, of 16
+  SpecState* state;                        // nwg > 1: [T]
+  int32_t* rej;                            // [T, M]
+  double* part;                            // [T, 16 nwg]
 };
 
 // Arguments of the page operations.  The bookkeeping of a pool lives on the

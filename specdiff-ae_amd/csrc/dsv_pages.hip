@@ -29,6 +29,7 @@ constexpr int kPT = kPlanThreads;
 constexpr int kPW = kPT / 64;       // waves of the planning workgroup
 constexpr int kScanK = 16;          // entries per thread and scan step
 constexpr int kScanStep = kPT * kScanK;
+constexpr int kFewPages = 8;        // pages that one thread hands to a sequence
 
 __device__ __forceinline__ int64_t get(const PageIndex& x, int64_t i) {
   return x.is64 ? reinterpret_cast<const int64_t*>(x.p)[i * x.stride]
@@ -321,16 +322,38 @@ __global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
     a.info[2] = refused;
   }
   if (!go) return;
-  // A wave per sequence: its entries from its place in the list.
-  for (int64_t i = threadIdx.x >> 6; i < b.B; i += kPW) {
+  // A thread per sequence for a few pages, then a wave per sequence for many.
+  __shared__ int32_t many;
+  if (threadIdx.x == 0) many = 0;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < b.B; i += kPT) {
     const int64_t len = seqlen(b, i), n = get(a.newlens, i);
     if (n <= len) continue;
+    const int64_t have = pages_of(len), need = pages_of(n) - have, at = a.off[i];
+    if (need > kFewPages) {
+      many = 1;
+      continue;
+    }
+    for (int j = 0; j < (int)need; ++j) {
+      const int32_t page = a.list[at + j];
+      b.table[i * b.t_sb + have + j] = page;
+      b.ref[page] = 1;
+    }
+    set_seqlen(b, i, n);
+  }
+  __syncthreads();
+  if (many == 0) return;
+  for (int64_t i = threadIdx.x >> 6; i < b.B; i += kPW) {
+    const int64_t len = seqlen(b, i), n = get(a.newlens, i);
+    if (n <= len) continue;  // (those done above among them)
     const int64_t have = pages_of(len), need = pages_of(n) - have, at = a.off[i];
     for (int64_t j = threadIdx.x & 63; j < need; j += 64) {
       const int32_t page = a.list[at + j];
       b.table[i * b.t_sb + have + j] = page;
       b.ref[page] = 1;
     }
+    // Every lane has read the length before it changes.
+    __builtin_amdgcn_wave_barrier();
     if ((threadIdx.x & 63) == 0) set_seqlen(b, i, n);
   }
 }

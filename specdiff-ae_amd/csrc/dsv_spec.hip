@@ -20,12 +20,15 @@
 // fixed order, so a call gives the same result every time.
 //
 // Layout.  The acceptance tests read two scalars a node; all M nodes' are
-// gathered at once and the walk runs in LDS.  The last row's sweep is the only
-// large read: it is cut into sub-blocks of kSpecSub entries that the
-// workgroups of a tree share out, each walking the tree by itself (the walk
-// needs no other workgroup, so no launch or wait stands between it and the
-// sweep).  A second launch, one workgroup a tree, finds the sub-block and the
-// token.  The memory traffic is the last row of p (and q).
+// gathered at once and wave 0 walks in LDS.  The last row's sweep is the large
+// read.  One CU takes in about 45 GB/s (a row pair of 128256 fp32 entries: 23
+// us), so with few trees a row is shared out over several workgroups of 16
+// waves, each walking the tree by itself (no wait stands between the walk and
+// the sweep), and a second launch, one workgroup a tree, draws from their sums;
+// with a tree per CU the one workgroup draws as well.  64 chains of 5 over 128256
+// fp32 entries: one workgroup each 33 us, four each 20.  A wave sums a
+// contiguous slot of the row, 8 entries a lane at a time with the next ones in
+// flight.
 //
 // Reference context: draft/tree_verification.py:100-182 (the walk whose
 // outputs are kept alike: path, tokens, winner, accept length, next token).
@@ -37,8 +40,8 @@ namespace dsv {
 namespace {
 
 constexpr int kT = kSpecThreads;
-constexpr int kPer = kSpecSub / kT;  // entries per thread and sub-block
-
+constexpr int kW = kT / 64;
+constexpr int kPer = kSpecSeg / 64;  // entries per lane and round of a sweep
 template <typename E>
 struct Load;
 template <>
@@ -63,116 +66,273 @@ __device__ __forceinline__ double unit(float u) {
   return u >= 0.f ? (double)(u < hi ? u : hi) : 0.0;
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+// x of the lane that DPP control CTRL names, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+// Inclusive scan over a wave: shifts by 1, 2, 4, 8 inside the rows of 16, then
+// the last lanes of rows 0 and 2, then of row 1, handed on.  (Through LDS
+// permutes the six steps took 10 times as long, and a draw has four scans in a
+// row.)
+__device__ __forceinline__ double wave_scan(double x) {
+  x += dpp<0x111, 0xf>(x);
+  x += dpp<0x112, 0xf>(x);
+  x += dpp<0x114, 0xf>(x);
+  x += dpp<0x118, 0xf>(x);
+  x += dpp<0x142, 0xa>(x);
+  x += dpp<0x143, 0xc>(x);
   return x;
 }
-
-// The sum of x over the workgroup, in every thread (scratch: one per wave).
-__device__ __forceinline__ double block_sum(double x, double* scratch) {
-  x = wave_sum(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
-  __syncthreads();
-  double s = scratch[0];
-#pragma unroll
-  for (int i = 1; i < kT / 64; ++i) s += scratch[i];
-  return s;
+__device__ __forceinline__ double last_lane(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-// The inclusive scan of x over the workgroup's threads, and its total.
+// The inclusive scan of x over the workgroup's NW waves, and its total.
+template <int NW>
 __device__ __forceinline__ double block_scan(double x, double* scratch, double& total) {
-  double inc = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(inc, o);
-    if ((int)(threadIdx.x & 63) >= o) inc += y;
-  }
+  const double inc = wave_scan(x), all = last_lane(inc);
+  const int wave = threadIdx.x >> 6;
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = inc;
+  if ((threadIdx.x & 63) == 0) scratch[wave] = all;
   __syncthreads();
   total = 0.0;
   double before = 0.0;
 #pragma unroll
-  for (int i = 0; i < kT / 64; ++i) {
-    if (i == (int)(threadIdx.x >> 6)) before = total;
+  for (int i = 0; i < NW; ++i) {
+    if (i == wave) before = total;
     total += scratch[i];
   }
   return before + inc;
 }
 
-// kPer consecutive-by-vector entries of a row's sub-block: entry e of thread
-// tid is v0 + (e / VE) * kT * VE + tid * VE + e % VE (VE entries per 16-byte
-// load; rows need no alignment).  Entries past the row read as 0.
+// What the remaining weights of a row are: max(p - c q, 0), or p without the
+// rejected tokens.
 template <typename E>
-struct Vec {
-  static constexpr int VE = 16 / (int)sizeof(E);
-  static constexpr int NV = kPer / VE;
-  typedef E vec __attribute__((ext_vector_type(VE), aligned(sizeof(E))));
-  static __device__ __forceinline__ int64_t index(int64_t v0, int e) {
-    return v0 + (int64_t)(e / VE) * (kT * VE) + threadIdx.x * VE + e % VE;
-  }
-  static __device__ __forceinline__ void load(const E* row, int64_t v0, int64_t V, float (&x)[kPer]) {
-    if (v0 + kSpecSub <= V) {
-      vec t[NV];
-#pragma unroll
-      for (int k = 0; k < NV; ++k) t[k] = *reinterpret_cast<const vec*>(row + index(v0, k * VE));
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) x[e] = prob((float)t[e / VE][e % VE]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int64_t v = index(v0, e);
-        x[e] = v < V ? prob(Load<E>::at(row + v)) : 0.f;
-      }
-    }
-  }
+struct Rows {
+  const E* p;
+  const E* q;
+  double c;
+  const int32_t* rej;
+  int nrej;
+  int64_t V;
 };
 
-// Weights of a sub-block's entries of this thread: max(p - c q, 0), or p
-// without the dropped tokens (bits of the sub-block).
-template <typename E, bool Q>
-__device__ __forceinline__ void weights(const E* p, const E* q, double c, const uint32_t* drop, int64_t v0, int64_t V,
-                                        double (&w)[kPer]) {
-  float x[kPer];
-  if constexpr (Q) {
-    float y[kPer];
-    Vec<E>::load(p, v0, V, x);
-    if (c != 0.0) {
-      Vec<E>::load(q, v0, V, y);
+// N entries that a lane holds of 64 N consecutive ones that its wave covers from
+// v0 on.  ROWS: 16-byte loads side by side over the lanes (whole lines; the order
+// of a sum is free), else N consecutive entries per lane (the draw walks them in
+// the vocabulary's order).  Rows need no alignment; entries past V are 0.
+template <typename E, int N, bool ROWS>
+struct Piece {
+  static constexpr int VE = 16 / (int)sizeof(E) < N ? 16 / (int)sizeof(E) : N;
+  static constexpr int NV = N / VE;
+  typedef E vec __attribute__((ext_vector_type(VE), aligned(sizeof(E))));
+  vec x[NV];
+  static __device__ __forceinline__ int index(int e) {
+    const int lane = threadIdx.x & 63;
+    return ROWS ? (e / VE) * (64 * VE) + lane * VE + e % VE : lane * N + e;
+  }
+  __device__ __forceinline__ void load(const E* row, int64_t v0, int64_t V) {
+    if (v0 + 64 * N <= V) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) x[k] = *reinterpret_cast<const vec*>(row + v0 + index(k * VE));
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) y[e] = 0.f;
+      for (int e = 0; e < N; ++e) x[e / VE][e % VE] = v0 + index(e) < V ? row[v0 + index(e)] : (E)0.f;
     }
+  }
+  __device__ __forceinline__ float at(int e) const { return (float)x[e / VE][e % VE]; }
+};
+
+// Weights of this lane's entries of the wave's piece at v0.  CHECK: infinite
+// entries count as 0; without it they are assumed absent (negative ones and NaN
+// are 0 either way: one maximum).
+template <typename E, bool Q, bool CHECK, int N, bool ROWS>
+__device__ __forceinline__ void weights(const Rows<E>& r, const Piece<E, N, ROWS>& p, const Piece<E, N, ROWS>& q, int64_t v0,
+                                        double (&w)[N]) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const double d = (double)x[e] - c * (double)y[e];
-      w[e] = d > 0.0 ? d : 0.0;
-    }
-  } else {
-    Vec<E>::load(p, v0, V, x);
+  for (int e = 0; e < N; ++e) {
+    w[e] = (double)(CHECK ? prob(p.at(e)) : fmaxf(p.at(e), 0.f));
+    if constexpr (Q) w[e] = fmax(fma(-r.c, (double)(CHECK ? prob(q.at(e)) : fmaxf(q.at(e), 0.f)), w[e]), 0.0);
+  }
+  if constexpr (!Q) {
+    // The rejected tokens among the wave's entries, found 64 at a time.
+    const int lane = threadIdx.x & 63;
+    for (int i = 0; i < r.nrej; i += 64) {
+      const int64_t d = i + lane < r.nrej ? (int64_t)r.rej[i + lane] - v0 : -1;
+      for (uint64_t in = __ballot(d >= 0 && d < 64 * N); in != 0; in &= in - 1) {
+        const int at = __shfl((int)d, __builtin_ctzll(in));
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      w[e] = (double)x[e];
-      if (drop != nullptr) {
-        const int i = (int)(Vec<E>::index(v0, e) - v0);
-        if ((drop[i >> 5] >> (i & 31)) & 1u) w[e] = 0.0;
+        for (int e = 0; e < N; ++e)
+          if (Piece<E, N, ROWS>::index(e) == at) w[e] = 0.0;
       }
     }
   }
 }
 
-// Bits of the rejected tokens inside a sub-block (every thread calls it).
-__device__ __forceinline__ void mark_dropped(uint32_t* drop, const int32_t* rej, int nrej, int64_t v0) {
+// The sums of the workgroup's 16 slots (step segments each, from slot first on)
+// into LDS, their total in every thread, in a fixed order.  Bound by its VALU operations where few trees share the GPU (a CU
+// issues one per SIMD and 4 cycles, 64-bit ones slower): the check for infinite
+// entries is one maximum over all of them, and the sweep runs again with the
+// full check only if there is one.
+template <typename E, bool Q, bool CHECK, int NW>
+__device__ __forceinline__ double sweep_as(const Rows<E>& r, int first, int step, double* sums) {
+  const int lane = threadIdx.x & 63;
+  typedef Piece<E, kPer, true> Pc;
   __syncthreads();
-  for (int i = threadIdx.x; i < kSpecSub / 32; i += kT) drop[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < nrej; i += kT) {
-    const int64_t d = (int64_t)rej[i] - v0;
-    if (d >= 0 && d < kSpecSub) atomicOr(&drop[d >> 5], 1u << (d & 31));
+  for (int slot = threadIdx.x >> 6; slot < kW; slot += NW) {
+    const int64_t w0 = ((int64_t)first + slot) * step * kSpecSeg, w1 = min(w0 + (int64_t)step * kSpecSeg, r.V);
+    double s0 = 0.0, s1 = 0.0;
+    float mx = 0.f;
+    Pc p, q, pn, qn;
+    auto fetch = [&](int64_t v, Pc& x, Pc& y) {
+      x.load(r.p, v, r.V);
+      if (Q && r.c != 0.0) y.load(r.q, v, r.V);
+    };
+#pragma unroll
+    for (int k = 0; k < Pc::NV; ++k) p.x[k] = pn.x[k] = q.x[k] = qn.x[k] = (E)0.f;
+    if (w0 < w1) fetch(w0, p, q);
+    for (int64_t v = w0; v < w1; v += kSpecSeg) {
+      if (v + kSpecSeg < w1) fetch(v + kSpecSeg, pn, qn);
+      double w[kPer];
+      weights<E, Q, CHECK, kPer, true>(r, p, q, v, w);
+      if constexpr (!CHECK) {
+#pragma unroll
+        for (int e = 0; e < kPer; e += Q ? 1 : 2) mx = fmaxf(fmaxf(mx, p.at(e)), Q ? q.at(e) : p.at(e + 1));
+      }
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        s0 += w[e];
+        s1 += w[e + 1];
+      }
+      p = pn;
+      q = qn;
+    }
+    const double s = last_lane(wave_scan(s0 + s1));
+    const bool inf = __ballot(mx == __builtin_huge_valf()) != 0ull;
+    if (lane == 0) sums[slot] = inf ? __builtin_huge_val() : s;  // (marked by an infinite sum)
   }
   __syncthreads();
+  double total = 0.0;
+#pragma unroll
+  for (int i = 0; i < kW; ++i) total += sums[i];
+  return total;
+}
+
+template <typename E, bool Q, int NW>
+__device__ __forceinline__ double sweep(const Rows<E>& r, int first, int step, double* sums) {
+  const double s = sweep_as<E, Q, false, NW>(r, first, step, sums);
+  return s < __builtin_huge_val() ? s : sweep_as<E, Q, true, NW>(r, first, step, sums);
+}
+
+// The next token from the remaining weights, whose nslot sums of step segments
+// are in LDS: the first v whose cumulative weight exceeds u W, W the total (the
+// last one with a weight if rounding left none).  Where nothing is left of the
+// weights (the target never exceeds the draft's share, or all of it was
+// rejected) it is drawn from the target's own row, and it is 0 if that has no
+// weight either.  NW waves.
+template <typename E, bool Q, int NW>
+__device__ __forceinline__ int64_t next_token(Rows<E> r, int nslot, int step, int step1, double u, double* sums,
+                                              double* scratch, int32_t* found, double* base_s) {
+  constexpr int N = 8, NT = NW * 64;  // entries per thread and round
+  double W, run;
+  int per;
+  for (int again = 0;; ++again) {
+    per = (nslot + NT - 1) / NT;
+    double mine = 0.0;
+    for (int k = 0; k < per; ++k) {
+      const int i = threadIdx.x * per + k;
+      mine += i < nslot ? sums[i] : 0.0;
+    }
+    run = block_scan<NW>(mine, scratch, W) - mine;
+    if (W > 0.0) break;
+    if (again != 0) return 0;
+    r.c = 0.0;
+    r.nrej = 0;
+    nslot = kW;
+    step = step1;
+    sweep<E, Q, NW>(r, 0, step, sums);
+  }
+  const double tau = u * W;
+  if (threadIdx.x == 0) {
+    found[0] = 0x7fffffff;
+    found[1] = -1;
+  }
+  __syncthreads();
+  // The slot: the first whose end passes tau, else the last with a weight.
+  int hit = 0x7fffffff, last = -1;
+  double hit_at = 0.0, last_at = 0.0;
+  for (int k = 0; k < per; ++k) {
+    const int i = threadIdx.x * per + k;
+    const double own = i < nslot ? sums[i] : 0.0;
+    if (own > 0.0) {
+      last = i;
+      last_at = run;
+      if (run + own > tau && hit == 0x7fffffff) {
+        hit = i;
+        hit_at = run;
+      }
+    }
+    run += own;
+  }
+  if (hit != 0x7fffffff) atomicMin(&found[0], hit);
+  if (last >= 0) atomicMax(&found[1], last);
+  __syncthreads();
+  const int slot = found[0] != 0x7fffffff ? found[0] : found[1];
+  if (slot == hit)
+    *base_s = hit_at;
+  else if (slot == last)
+    *base_s = last_at;
+  __syncthreads();
+  double base = *base_s;
+  int64_t tok = 0;
+  const int64_t v1 = (int64_t)(slot + 1) * step * kSpecSeg;
+  for (int64_t v0 = (int64_t)slot * step * kSpecSeg; v0 < v1 && v0 < r.V; v0 += (int64_t)NT * N) {
+    const int64_t v = v0 + (int64_t)threadIdx.x * N, vw = v0 + (int64_t)(threadIdx.x & ~63) * N;
+    typedef Piece<E, N, false> Pc;
+    Pc p, q;
+#pragma unroll
+    for (int k = 0; k < Pc::NV; ++k) q.x[k] = (E)0.f;
+    p.load(r.p, vw, r.V);
+    if (Q && r.c != 0.0) q.load(r.q, vw, r.V);
+    double w[N], mine = 0.0, total;
+    weights<E, Q, true, N, false>(r, p, q, vw, w);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (v + e >= v1) w[e] = 0.0;  // the next slot's
+      mine += w[e];
+    }
+    double cum = base + (block_scan<NW>(mine, scratch, total) - mine);
+    if (threadIdx.x == 0) {
+      found[0] = 0x7fffffff;
+      found[1] = -1;
+    }
+    __syncthreads();
+    hit = 0x7fffffff;
+    last = -1;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      cum += w[e];
+      if (w[e] > 0.0) {
+        last = threadIdx.x * N + e;
+        if (cum > tau && hit == 0x7fffffff) hit = last;
+      }
+    }
+    if (hit != 0x7fffffff) atomicMin(&found[0], hit);
+    if (last >= 0) atomicMax(&found[1], last);
+    __syncthreads();
+    if (found[0] != 0x7fffffff) return v0 + found[0];
+    if (found[1] >= 0) tok = v0 + found[1];
+    base += total;
+    __syncthreads();
+  }
+  return tok;
 }
 
 struct Walk {
@@ -185,14 +345,14 @@ struct Walk {
 };
 
 template <typename E, bool Q>
-__global__ void __launch_bounds__(kT) spec_walk_kernel(const SpecArgs a) {
+__global__ void __launch_bounds__(kT) spec_kernel(const SpecArgs a) {
   const int t = blockIdx.x / a.nwg, wg = blockIdx.x % a.nwg, M = a.M;
   const int64_t V = a.V;
   __shared__ int32_t par[kSpecMaxM], tok[kSpecMaxM], rej[kSpecMaxM];
   __shared__ float px[kSpecMaxM], qx[kSpecMaxM], un[kSpecMaxM];
   __shared__ int16_t path[kSpecMaxM];
-  __shared__ uint32_t drop[kSpecSub / 32];
-  __shared__ double scratch[kT / 64];
+  __shared__ double sums[kW], scratch[kW], base_s;
+  __shared__ int32_t found[2];
   __shared__ Walk wk;
   const E* P = reinterpret_cast<const E*>(a.target) + (int64_t)t * a.t_st;
   const E* Dp = Q ? reinterpret_cast<const E*>(a.dprobs) + (int64_t)t * a.q_st : nullptr;
@@ -284,195 +444,66 @@ __global__ void __launch_bounds__(kT) spec_walk_kernel(const SpecArgs a) {
     __syncthreads();
     if (!Q || wk.sweep == 0) break;
     if constexpr (Q) {
-      const E* p = P + (int64_t)wk.node * a.t_sm;
-      const E* q = Dp + (int64_t)wk.node * a.q_sm;
-      const double c = wk.c;
-      double s = 0.0;
-      for (int64_t v0 = 0; v0 < V; v0 += kSpecSub) {
-        double w[kPer];
-        weights<E, Q>(p, q, c, nullptr, v0, V, w);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) s += w[e];
-      }
-      s = block_sum(s, scratch);
+      const Rows<E> r{P + (int64_t)wk.node * a.t_sm, Dp + (int64_t)wk.node * a.q_sm, wk.c, rej, 0, V};
+      const double s = sweep<E, Q, kW>(r, 0, a.step1, sums);
       if (threadIdx.x == 0) wk.mass = s;
       __syncthreads();
     }
   }
 
-  const int node = wk.node, len = wk.len, nrej = wk.nrej;
-  const double c = wk.c;
+  const int node = wk.node, len = wk.len, nrej = Q ? 0 : wk.nrej;
+  int64_t* info = a.out_info + (int64_t)t * a.oi_st;
   if (wg == 0) {
     for (int i = threadIdx.x; i < M; i += kT) {
       const int id = i < len ? path[i] : -1;
       a.out_path[(int64_t)t * a.op_st + i] = id;
       a.out_tok[(int64_t)t * a.ot_st + i] = id >= 0 ? a.draft[(int64_t)t * a.d_st + (int64_t)id * a.d_sm] : -1;
     }
-    int32_t* rj = a.rej + (int64_t)t * M;
-    if constexpr (!Q)
-      for (int i = threadIdx.x; i < nrej; i += kT) rj[i] = rej[i];
     if (threadIdx.x == 0) {
-      a.state[t] = SpecState{c, node, len, nrej, 0};
-      int64_t* info = a.out_info + (int64_t)t * a.oi_st;
       info[0] = node;
       info[1] = len - 1;
       info[3] = len;
     }
   }
-
-  // The last row's weights, one sum per sub-block.
-  const E* p = P + (int64_t)node * a.t_sm;
-  const E* q = Q ? Dp + (int64_t)node * a.q_sm : nullptr;
-  for (int64_t j = wg; j < a.nsub; j += a.nwg) {
-    const int64_t v0 = j * kSpecSub;
-    if (!Q && nrej > 0) mark_dropped(drop, rej, nrej, v0);
-    double w[kPer], s = 0.0;
-    weights<E, Q>(p, q, c, !Q && nrej > 0 ? drop : nullptr, v0, V, w);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) s += w[e];
-    s = block_sum(s, scratch);
-    if (threadIdx.x == 0) a.part[(int64_t)t * a.nsub + j] = s;
+  // The last node's remaining weights.
+  Rows<E> r{P + (int64_t)node * a.t_sm, Q ? Dp + (int64_t)node * a.q_sm : nullptr, wk.c, rej, nrej, V};
+  sweep<E, Q, kW>(r, wg * kW, a.step, sums);
+  if (a.nwg == 1) {
+    const int64_t tok = next_token<E, Q, kW>(r, kW, a.step, a.step1, unit(un[0]), sums, scratch, found, &base_s);
+    if (threadIdx.x == 0) info[2] = tok;
+    return;
+  }
+  if (threadIdx.x < kW) a.part[((int64_t)t * a.nwg + wg) * kW + threadIdx.x] = sums[threadIdx.x];
+  if (wg == 0) {
+    if (threadIdx.x == 0) a.state[t] = SpecState{wk.c, node, nrej};
+    for (int i = threadIdx.x; i < nrej; i += kT) a.rej[(int64_t)t * M + i] = rej[i];
   }
 }
 
-// The first entry of sub-block v0 whose cumulative weight exceeds tau, in
-// the order of the vocabulary; the last entry with a weight if rounding left
-// none; -1 if no entry has one.
-template <typename E>
-__device__ int64_t pick(const double (&w)[kPer], int64_t v0, double tau, double* scratch, int32_t* found) {
-  using L = Vec<E>;
-  // Vector k of every thread covers VE consecutive entries; the vectors of the
-  // workgroup follow one another, then k + 1.
-  double run = 0.0;
-  if (threadIdx.x == 0) {
-    found[0] = 0x7fffffff;
-    found[1] = -1;
-  }
-  __syncthreads();
-  int last = -1, hit = 0x7fffffff;
-#pragma unroll
-  for (int k = 0; k < L::NV; ++k) {
-    double mine = 0.0;
-#pragma unroll
-    for (int e = 0; e < L::VE; ++e) mine += w[k * L::VE + e];
-    double all = 0.0;
-    const double inc = block_scan(mine, scratch, all);
-    double cum = run + (inc - mine);
-    run += all;
-#pragma unroll
-    for (int e = 0; e < L::VE; ++e) {
-      const int i = (int)(L::index(v0, k * L::VE + e) - v0);
-      cum += w[k * L::VE + e];
-      if (w[k * L::VE + e] > 0.0) {
-        last = i;
-        if (cum > tau && hit == 0x7fffffff) hit = i;
-      }
-    }
-  }
-  atomicMin(&found[0], hit);
-  atomicMax(&found[1], last);
-  __syncthreads();
-  const int h = found[0] != 0x7fffffff ? found[0] : found[1];
-  return h < 0 ? -1 : v0 + h;
-}
-
+// The draw from the sums that a tree's workgroups left.
+constexpr int kDW = 4;  // waves
 template <typename E, bool Q>
-__global__ void __launch_bounds__(kT) spec_pick_kernel(const SpecArgs a) {
-  const int t = blockIdx.x;
-  const int64_t V = a.V;
-  __shared__ uint32_t drop[kSpecSub / 32];
-  __shared__ double scratch[kT / 64];
+__global__ void __launch_bounds__(kDW * 64) spec_draw_kernel(const SpecArgs a) {
+  const int t = blockIdx.x, nslot = a.nwg * kW;
+  __shared__ double sums[kSpecSlots], scratch[kDW], base_s;
   __shared__ int32_t found[2];
-  __shared__ int64_t sel;
-  __shared__ double base_s;
+  for (int i = threadIdx.x; i < nslot; i += kDW * 64) sums[i] = a.part[(int64_t)t * nslot + i];
   const SpecState st = a.state[t];
-  const E* p = reinterpret_cast<const E*>(a.target) + (int64_t)t * a.t_st + (int64_t)st.node * a.t_sm;
-  const E* q = Q ? reinterpret_cast<const E*>(a.dprobs) + (int64_t)t * a.q_st + (int64_t)st.node * a.q_sm : nullptr;
-  const int32_t* rej = a.rej + (int64_t)t * a.M;
-  double* part = a.part + (int64_t)t * a.nsub;
   const double u = unit(a.uniform[(int64_t)t * a.u_st]);
-  double c = st.c;
-  int nrej = Q ? 0 : st.nrej;
-
-  // Thread i owns sub-blocks [i * nper, (i + 1) * nper): its sum, the
-  // cumulative sum up to its end and the total.
-  const int64_t nper = (a.nsub + kT - 1) / kT;
-  double own = 0.0, inc = 0.0;
-  auto total = [&]() {
-    own = 0.0;
-    for (int64_t j = 0; j < nper; ++j) {
-      const int64_t x = threadIdx.x * nper + j;
-      if (x < a.nsub) own += part[x];
-    }
-    double w = 0.0;
-    inc = block_scan(own, scratch, w);
-    return w;
-  };
-  double W = total();
-  if (!(W > 0.0)) {
-    // Nothing is left of the row (the target never exceeds the draft's share,
-    // or all of it was rejected): the target's own row is drawn from.
-    c = 0.0;
-    nrej = 0;
-    for (int64_t j = 0; j < a.nsub; ++j) {
-      double w[kPer], s = 0.0;
-      weights<E, Q>(p, q, c, nullptr, j * kSpecSub, V, w);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) s += w[e];
-      s = block_sum(s, scratch);
-      if (threadIdx.x == 0) part[j] = s;
-    }
-    __syncthreads();
-    W = total();
-  }
-  const double tau = u * W;
-  // The first owner whose end passes tau (the last one with a weight if
-  // rounding left none), then its sub-block.
-  if (threadIdx.x == 0) {
-    found[0] = kT;
-    found[1] = -1;
-    sel = -1;
-  }
+  const Rows<E> r{reinterpret_cast<const E*>(a.target) + (int64_t)t * a.t_st + (int64_t)st.node * a.t_sm,
+                  Q ? reinterpret_cast<const E*>(a.dprobs) + (int64_t)t * a.q_st + (int64_t)st.node * a.q_sm : nullptr,
+                  st.c, a.rej + (int64_t)t * a.M, st.nrej, a.V};
   __syncthreads();
-  if (own > 0.0) {
-    if (inc > tau) atomicMin(&found[0], (int)threadIdx.x);
-    atomicMax(&found[1], (int)threadIdx.x);
-  }
-  __syncthreads();
-  if ((int)threadIdx.x == (found[0] < kT ? found[0] : found[1])) {
-    double r = inc - own;
-    for (int64_t j = 0; j < nper; ++j) {
-      const int64_t x = threadIdx.x * nper + j;
-      if (x >= a.nsub) break;
-      const double s = part[x];
-      if (s > 0.0) {
-        sel = x;
-        base_s = r;
-        if (r + s > tau) break;
-      }
-      r += s;
-    }
-  }
-  __syncthreads();
-  int64_t tok = 0;  // a row without a positive entry draws token 0
-  if (sel >= 0) {
-    const int64_t v0 = sel * kSpecSub;
-    if (nrej > 0) mark_dropped(drop, rej, nrej, v0);
-    double w[kPer];
-    weights<E, Q>(p, q, c, nrej > 0 ? drop : nullptr, v0, V, w);
-    const int64_t r = pick<E>(w, v0, tau - base_s, scratch, found);
-    if (r >= 0) tok = r;
-  }
+  const int64_t tok = next_token<E, Q, kDW>(r, nslot, a.step, a.step1, u, sums, scratch, found, &base_s);
   if (threadIdx.x == 0) a.out_info[(int64_t)t * a.oi_st + 2] = tok;
 }
 
 template <typename E, bool Q>
 hipError_t launch_q(const SpecArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.nwg * a.T));
-  hipLaunchKernelGGL((spec_walk_kernel<E, Q>), grid, dim3(kT), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((spec_pick_kernel<E, Q>), dim3((unsigned)a.T), dim3(kT), 0, s, a);
+  hipLaunchKernelGGL((spec_kernel<E, Q>), dim3((unsigned)(a.T * a.nwg)), dim3(kT), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.nwg == 1) return e;
+  hipLaunchKernelGGL((spec_draw_kernel<E, Q>), dim3((unsigned)a.T), dim3(kDW * 64), 0, s, a);
   return hipGetLastError();
 }
 

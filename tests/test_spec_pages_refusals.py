@@ -54,9 +54,9 @@ def test_spec_accepts_and_refuses(dry):
         assert spec(dry, **bad) == INVALID, bad.keys()
     big = torch.zeros(2, 1, 10).expand(2, 1025, 10)
     assert spec(dry, target=big) == UNSUPPORTED
-    assert spec(dry, ws=0) == WORKSPACE
-    assert spec(dry, nbytes=8) == WORKSPACE
-    assert spec(dry, ws=ws_ptr() + 16) == WORKSPACE
+    assert spec(dry, V=50000, ws=0) == WORKSPACE       # (rows shared out over workgroups)
+    assert spec(dry, V=50000, nbytes=8) == WORKSPACE
+    assert spec(dry, V=50000, ws=ws_ptr() + 16) == WORKSPACE
     assert dry.dsv_spec_workspace_bytes(1, 1025, 10) == 0
     assert dry.dsv_spec_workspace_bytes(1, 4, 1 << 31) == 0
     assert dry.dsv_spec_workspace_bytes((1 << 20) + 1, 4, 10) == 0
