@@ -1899,13 +1899,14 @@ WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
   const bool tile = dtype != DSV_F32 && R > 64 && !small_pages;
   p.rpb = tile ? 256 : dtype == DSV_F32 || R <= 16 ? 16 : 32;
   p.n_rb = (int)((R + p.rpb - 1) / p.rpb);
-  // Splits over the keys: four waves per workgroup and at least one tile per
-  // wave, until there are four workgroups per CU.
+  // Splits over the keys until there is a workgroup per CU, of 20 tiles at
+  // least (8 waves, 2 to 3 tiles each): more splits cost more in the merge than
+  // they gain (bf16, one sequence through 16384 keys: 16 splits 31 us, 32 splits
+  // 36; 8 sequences of 16 rows through 4096: 2 splits 75, 4 splits 86).
   const int64_t units = B * Hk * p.n_rb;
   const int64_t span = tree ? M : std::min<int64_t>(M, p.rpb / p.G + 2);
   const int64_t reach = std::min(n_keys, window + span) / 32 + 2 + std::min(n_keys, sinks) / 32;
-  const int64_t want = std::max<int64_t>(1, (int64_t)device_cus() * (tile ? 1 : 4) / units);
-  p.splits = (int)std::max<int64_t>(1, std::min(want, reach / 4));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(device_cus() / units, reach / (tile ? 4 : 20)));
   const size_t rows = p.splits > 1 ? (size_t)B * Hk * p.splits * R : 0;
   p.opart_bytes = align_up(rows * D * sizeof(float), 256);
   p.ml_bytes = align_up(rows * sizeof(float2), 256);

@@ -28,9 +28,9 @@
 // row by row (0 * inf would be NaN in the matrix product).
 //
 // win_rows_kernel (this file's simplest; few rows: single tokens, short
-// chunks): bound by reading K and V.  Four waves share a workgroup's tiles, each
-// with a softmax of its own, merged in LDS at the end, so no barrier stands in
-// the loop.  A tile goes memory -> registers in whole rows (16 bytes a lane,
+// chunks): bound by reading K and V.  Eight waves share a workgroup's tiles,
+// each with a softmax of its own, merged in LDS at the end, so no barrier stands
+// in the loop.  A tile goes memory -> registers in whole rows (16 bytes a lane,
 // the next tile in flight while this one is used) -> the wave's own LDS -> MFMA
 // operands: K rows by ds_read_b128, V transposed by ds_read_b64_tr_b16.  Splits
 // over the keys fill the GPU when there are few rows; win_merge_kernel joins
@@ -100,11 +100,16 @@ __global__ void __launch_bounds__(256) win_tree_kernel(const WinArgs a, const vo
   }
 }
 
+// Eight waves: two per SIMD have 256 KiB of loads in flight between them where
+// the registers allow, and four per workgroup left the batch of 64 at 230 us, 184
+// with eight (16 spill).
+constexpr int kRowWaves = 8;
+
 // ---- few rows ------------------------------------------------------------------
 
 template <typename T, int D, int NR>
-__global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
-  constexpr int NW = 4;
+__global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs a) {
+  constexpr int NW = kRowWaves;
   constexpr int CH = D / 8;           // 16-byte chunks per key
   constexpr int KPI = 64 / CH;        // keys per load instruction
   constexpr int NL = 32 / KPI;        // load instructions per tile and half
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
     wave_lds_fence();
   }
 
-  // ---- the four waves' rows joined, 16 at a time
+  // ---- the waves' rows joined, 16 at a time
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const float lt = row_sum(ls[i]);
@@ -306,39 +311,42 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(mine + lr * OST + (16 * d + 4 * lg) * 4) = acc[i][d];
     __syncthreads();
-    constexpr int N = D / 16;  // elements per thread
-    const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * N;
-    float m = sm_m[0][rr];
+    constexpr int N = 4;  // elements per thread
+    constexpr int TPR = D / N;
+    const int rr = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N;
+    if (rr < 16) {
+      float m = sm_m[0][rr];
 #pragma unroll
-    for (int x = 1; x < NW; ++x) m = fmaxf(m, sm_m[x][rr]);
-    const float ms = m == kNegInf ? 0.f : m;
-    float l = 0.f, o[N];
+      for (int x = 1; x < NW; ++x) m = fmaxf(m, sm_m[x][rr]);
+      const float ms = m == kNegInf ? 0.f : m;
+      float l = 0.f, o[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = 0.f;
+      for (int e = 0; e < N; ++e) o[e] = 0.f;
 #pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      if (sm_l[x][rr] == 0.f) continue;  // a wave without a key of this row
-      const float f = __builtin_amdgcn_exp2f(sm_m[x][rr] - ms);
-      l += sm_l[x][rr] * f;
-      const f32x4* p = reinterpret_cast<const f32x4*>(smem + x * REGION + rr * OST + d0 * 4);
+      for (int x = 0; x < NW; ++x) {
+        if (sm_l[x][rr] == 0.f) continue;  // a wave without a key of this row
+        const float f = __builtin_amdgcn_exp2f(sm_m[x][rr] - ms);
+        l += sm_l[x][rr] * f;
+        const f32x4* p = reinterpret_cast<const f32x4*>(smem + x * REGION + rr * OST + d0 * 4);
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] += p[e / 4][e % 4] * f;
-    }
-    const int r = r0 + 16 * i + rr;
-    if (r < a.R) {
-      if (a.splits == 1) {
-        const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        for (int e = 0; e < N; ++e) o[e] += p[e / 4][e % 4] * f;
+      }
+      const int r = r0 + 16 * i + rr;
+      if (r < a.R) {
+        if (a.splits == 1) {
+          const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] *= inv;
-        store_out<N>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
-        if (d0 == 0 && a.lse != nullptr)
-          a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
-      } else {
-        const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
+          for (int e = 0; e < N; ++e) o[e] *= inv;
+          store_out<N>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
+          if (d0 == 0 && a.lse != nullptr)
+            a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+        } else {
+          const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
 #pragma unroll
-        for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(a.opart + pr * D + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
-        if (d0 == 0) a.ml[pr] = make_float2(m, l);
+          for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(a.opart + pr * D + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+          if (d0 == 0) a.ml[pr] = make_float2(m, l);
+        }
       }
     }
     __syncthreads();
@@ -351,8 +359,8 @@ __global__ void __launch_bounds__(256) win_rows_kernel(const WinArgs a) {
 // head dimension in the product is free as long as Q's agrees), V's operand is a
 // row-major element, so nothing passes through LDS but the join of the waves.
 template <int D>
-__global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
-  constexpr int NW = 4;
+__global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinArgs a) {
+  constexpr int NW = kRowWaves;
   constexpr int KC = D / 16;          // 16-byte chunks per lane and key
   constexpr int DT = D / 16;
   constexpr int OST = D + 4;
@@ -389,23 +397,44 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
 
-  for (int t = (int)((int64_t)kl.nt * split / a.splits) + wave; t < t_end; t += NW) {
+  // Lane l holds the page of key l (mod 32) of a tile, read a tile ahead.
+  auto tile_pages = [&](int tt) -> int32_t {
+    if (a.pt == nullptr || tt >= t_end) return 0;
+    return page_of(a, b, kl.read(kl.base(tt) + (lane & 31)));
+  };
+  int t = (int)((int64_t)kl.nt * split / a.splits) + wave;
+  int32_t pg = tile_pages(t);
+  for (; t < t_end; t += NW) {
     const int kb = kl.base(t);
+    // All of the tile's loads first: keys 16 h + lr of K (operand A), 16 (e / 4) +
+    // 4 lg + e % 4 of V.
+    f32x4 kf[2][KC];
+    float vf[8][DT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = 16 * h + lr;
+      const float* k = kbase + key_off(a, a.k_sp, a.k_st, kl.read(kb + i), a.pt != nullptr ? __shfl(pg, i) : 0) + 4 * lg;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kf[h][c] = *reinterpret_cast<const f32x4*>(k + 16 * c);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = 16 * (e >> 2) + 4 * lg + (e & 3);
+      const float* v = vbase + key_off(a, a.v_sp, a.v_st, kl.read(kb + i), a.pt != nullptr ? __shfl(pg, i) : 0) + lr;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vf[e][d] = v[16 * d];
+    }
+    pg = tile_pages(t + NW);
     const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
     const uint32_t keep = masked ? keep_word(a, b, row.m, row.pos, kb, n0) : ~0u;
     f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int n = kl.read(kb + 16 * h + lr);
-      const float* k = kbase + key_off(a, a.k_sp, a.k_st, n, a.pt != nullptr ? page_of(a, b, n) : 0) + 4 * lg;
-      f32x4 kf[KC];
-#pragma unroll
-      for (int c = 0; c < KC; ++c) kf[c] = *reinterpret_cast<const f32x4*>(k + 16 * c);
       s[h] = f32x4{};
 #pragma unroll
       for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][e], qf[c][e], s[h], 0, 0, 0);
+        for (int e = 0; e < 4; ++e) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[h][c][e], qf[c][e], s[h], 0, 0, 0);
     }
     float x[8];
 #pragma unroll
@@ -432,18 +461,9 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int n = kl.read(kb + 16 * (e >> 2) + 4 * lg + (e & 3));
-      const float* v = vbase + key_off(a, a.v_sp, a.v_st, n, a.pt != nullptr ? page_of(a, b, n) : 0) + lr;
-      const bool has = kl.has(kb + 16 * (e >> 2) + 4 * lg + (e & 3));
-      float vf[DT];
-#pragma unroll
-      for (int d = 0; d < DT; ++d) vf[d] = v[16 * d];
       bool odd = false;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        if (masked && !has) vf[d] = 0.f;
-        odd |= !(vf[d] - vf[d] == 0.f);
-      }
+      for (int d = 0; d < DT; ++d) odd |= !(vf[e][d] - vf[e][d] == 0.f);
       if (masked && __ballot(odd) != 0ull) {
         // Infinite or NaN entries: added to the rows that see them, and out of
         // the product.  Lane group y holds key 4 y + e % 4; this lane's
@@ -453,14 +473,14 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
-              const float o = __shfl(vf[d], 16 * y + 4 * lg + z);
+              const float o = __shfl(vf[e][d], 16 * y + 4 * lg + z);
               if (!(o - o == 0.f) && ((keep >> (16 * (e >> 2) + 4 * y + (e & 3))) & 1u)) acc[d][z] += o;
             }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) vf[d] = vf[d] - vf[d] == 0.f ? vf[d] : 0.f;
+        for (int d = 0; d < DT; ++d) vf[e][d] = vf[e][d] - vf[e][d] == 0.f ? vf[e][d] : 0.f;
       }
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[d], x[e], acc[d], 0, 0, 0);
+      for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][d], x[e], acc[d], 0, 0, 0);
     }
   }
 
@@ -472,8 +492,9 @@ __global__ void __launch_bounds__(256) win_rows_f32_kernel(const WinArgs a) {
 #pragma unroll
   for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&smem[wave][lr * OST + 16 * d + 4 * lg]) = acc[d];
   __syncthreads();
-  constexpr int N = D / 16;
-  const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * N;
+  constexpr int N = 4, TPR = D / N;
+  const int rr = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N;
+  if (rr >= 16) return;
   float m = sm_m[0][rr];
 #pragma unroll
   for (int y = 1; y < NW; ++y) m = fmaxf(m, sm_m[y][rr]);
@@ -543,11 +564,11 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
 
 template <typename T, int D>
 hipError_t launch_rows(const WinArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits));
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), block(kRowWaves * 64);
   if (a.rows_per_block == 16)
-    hipLaunchKernelGGL((win_rows_kernel<T, D, 1>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((win_rows_kernel<T, D, 1>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((win_rows_kernel<T, D, 2>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((win_rows_kernel<T, D, 2>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
@@ -555,7 +576,7 @@ template <int D>
 hipError_t launch_d(const WinArgs& a, hipStream_t s) {
   hipError_t e;
   if (a.dtype == 2) {
-    hipLaunchKernelGGL(win_rows_f32_kernel<D>, dim3((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(win_rows_f32_kernel<D>, dim3((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), dim3(kRowWaves * 64), 0, s, a);
     e = hipGetLastError();
   } else if (a.rows_per_block == 256) {
     e = launch_window_tile(a, D, s);
