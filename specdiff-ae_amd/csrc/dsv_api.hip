@@ -1884,7 +1884,7 @@ bool win_args_ok(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
 }
 
 WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys, int64_t window,
-                 int64_t sinks, bool tree, bool small_pages) {
+                 int64_t sinks, bool tree, bool no_tile) {
   WinPlan p;
   const bool in_range = B <= (1 << 20) && M <= (1 << 24) && H <= (1 << 16) && n_keys <= dsv::kWinMaxKeys;
   const int64_t R = in_range ? (H / Hk) * M : 0;
@@ -1896,7 +1896,7 @@ WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
   p.G = (int)(H / Hk);
   p.R = (int)R;
   p.MW = tree ? (int)((M + 63) / 64) : 0;
-  const bool tile = dtype != DSV_F32 && R > 64 && !small_pages;
+  const bool tile = dtype != DSV_F32 && R > 64 && !no_tile;
   p.rpb = tile ? 256 : dtype == DSV_F32 || R <= 16 ? 16 : 32;
   p.n_rb = (int)((R + p.rpb - 1) / p.rpb);
   // Splits over the keys until there is a workgroup per CU, of 20 tiles at
@@ -1922,8 +1922,10 @@ extern "C" {
 size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dtype, int64_t n_keys,
                                   int64_t window, int64_t sinks, int has_tree) {
   if (!win_args_ok(B, M, H, Hk, D, dtype, n_keys, window, sinks) || (has_tree && M > dsv::kTreeMaxM)) return 0;
+  // (Whatever pages and strides the call comes with.)
   const WinPlan p = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0, false);
-  return p.err != nullptr ? 0 : std::max<size_t>(p.total, 256);
+  const WinPlan r = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0, true);
+  return p.err != nullptr ? 0 : std::max<size_t>(std::max(p.total, r.total), 256);
 }
 
 int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_tensor* v, const dsv_tensor* page_table,
@@ -2027,7 +2029,10 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
 
   // (Beyond every key, either means all of them.)
   const int64_t W = std::min<int64_t>(window, dsv::kWinMaxKeys), S = std::min<int64_t>(sinks, dsv::kWinMaxKeys);
-  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, tree.parent != nullptr, present(page_table) && k->shape[2] < 8);
+  // The kernel for many rows reads a DMA instruction's 4 or 8 keys through one
+  // page, and a tile's 32 keys with 32-bit offsets from the first.
+  const bool no_tile = (present(page_table) && k->shape[2] < 8) || a.k_st > (1 << 25) || a.v_st > (1 << 25);
+  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, tree.parent != nullptr, no_tile);
   if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
   if ((rc = check_workspace(std::max<size_t>(p.total, 256), workspace, workspace_bytes)) != DSV_OK) return rc;
   a.dtype = q->dtype;

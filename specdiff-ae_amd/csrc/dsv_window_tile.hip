@@ -83,11 +83,6 @@ __device__ __forceinline__ const WinArgs& args_again() {
   return *(const WinArgs*)p;
 }
 
-template <int N>
-struct IC {
-  static constexpr int value = N;
-};
-
 // A wave's 32 rows once more, from memory and without matrix products, where V
 // holds infinities or NaN in keys that some of the rows do not see: in the
 // product 0 * inf would reach those rows.  A lane takes a key of 64 for the
@@ -164,6 +159,11 @@ __device__ __noinline__ void exact_rows(const WinArgs* ap, int b, int kvh, int s
   }
 }
 
+template <bool B>
+struct BoolC {
+  static constexpr bool value = B;
+};
+
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   using G = Geo<D>;
@@ -220,60 +220,64 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   // ---- DMA of one tile into its ring stage --------------------------------------
   // Instruction x of this wave covers keys [j*KPI, (j+1)*KPI) of the tile's K
   // (waves 0-3) or V half; lane p fills key j*KPI + p/CH, slot p%CH, which holds
-  // global chunk slot ^ swizzle(key).
+  // global chunk slot ^ swizzle(key).  Tile t goes into stage t & 3.
   const bool v_wave = wid >= NW / 2;
   const int64_t st2 = 2 * (v_wave ? a.v_st : a.k_st), sp2 = 2 * (v_wave ? a.v_sp : a.k_sp);
-  const char* hbase = reinterpret_cast<const char*>(v_wave ? a.v : a.k);
-  const int64_t wg_off = 2 * (v_wave ? b * a.v_sb + kvh * a.v_sh : b * a.k_sb + kvh * a.k_sh);
-  const int64_t span = v_wave ? a.v_bytes : a.k_bytes;
-  const uint32_t half = lds_addr(smem) + (uint32_t)uniform(v_wave ? G::TILE : 0);
-  uint32_t lane_off[IPW];
-  int jx[IPW];
+  const char* hbase = reinterpret_cast<const char*>(v_wave ? a.v : a.k) +
+                      2 * (v_wave ? b * a.v_sb + kvh * a.v_sh : b * a.k_sb + kvh * a.k_sh);
+  const int j0 = uniform(wid % (NW / 2) * IPW);  // this wave's first instruction of its half
+  const uint32_t dst0 = lds_addr(smem) + (uint32_t)uniform(v_wave ? G::TILE : 0) + (uint32_t)j0 * 1024;
   auto chunk_of = [&](int x, int l) {
-    const int key_t = jx[x] * G::KPI + l / CH;
+    const int key_t = (j0 + x) * G::KPI + l / CH;
     return v_wave ? v_slot(CH, key_t, l % CH) : k_slot(CH, key_t, l % CH);
   };
+  // In a tile that the block's rows see whole: a uniform 64-bit offset plus the
+  // lane's 32-bit one (from the tile's first key; paged: from the instruction's).
+  uint32_t lane_off[IPW];
 #pragma unroll
-  for (int x = 0; x < IPW; ++x) {
-    bool is_v;
-    dma_ins<D>(wid * IPW + x, is_v, jx[x]);
-    jx[x] = uniform(jx[x]);
-    lane_off[x] = (uint32_t)(lane / CH * st2) + (uint32_t)(chunk_of(x, lane) * 16);
-  }
-  const int psm = (1 << a.ps_shift) - 1;
-  // Paged: lane l holds the page of instruction x's keys in tile pgw_t0 + l.
-  int32_t pgw[IPW];
+  for (int x = 0; x < IPW; ++x)
+    lane_off[x] = (uint32_t)(((PAGED ? 0 : (j0 + x) * G::KPI) + lane / CH) * st2) + (uint32_t)(chunk_of(x, lane) * 16);
+  const uint32_t reach = (uint32_t)((PAGED ? G::KPI - 1 : 31) * st2) + 2 * D;
+  // The tiles [whole0, whole1) are such (others may be: whole() tells).
+  const int whole0 = kl.nst + (kl.lo > kl.lo_al ? max((kl.lo - kl.lo_al + 31) >> 5, 0) : 0) - t_lo;
+  const int whole1 = kl.nst + ((kl.hi - kl.lo_al) >> 5) - t_lo;
+  // Paged: lane l holds the offset of instruction x's keys in tile pgw_t0 + l.
+  uint32_t pgw_lo[IPW], pgw_hi[IPW];
   int pgw_t0 = -64;
 #pragma unroll
-  for (int x = 0; x < IPW; ++x) pgw[x] = 0;
+  for (int x = 0; x < IPW; ++x) pgw_lo[x] = pgw_hi[x] = 0;
   auto fill_pgw = [&](int t0) {
     pgw_t0 = t0;
 #pragma unroll
-    for (int x = 0; x < IPW; ++x)
-      pgw[x] = page_of(a, b, kl.read(kl.base(t_lo + min(t0 + again(lane), ntiles - 1)) + jx[x] * G::KPI));
-  };
-  auto issue_tile = [&](auto stage_c, int t) {
-    constexpr int stage = decltype(stage_c)::value;
-    // (Windows start at multiples of 64: only stage 0 starts one.)
-    if (PAGED && stage == 0 && t - pgw_t0 >= 64) fill_pgw(t);
-    const int kb = kl.base(t_lo + t);
-    const bool whole = kl.whole(kb);
-#pragma unroll
     for (int x = 0; x < IPW; ++x) {
-      const uint32_t dst = half + (uint32_t)(stage * 2 * G::TILE + jx[x] * 1024);
-      const int nb = kb + jx[x] * G::KPI;
-      if (whole) {
-        int64_t off = wg_off;
+      const int n = kl.read(kl.base(t_lo + min(t0 + again(lane), ntiles - 1)) + (j0 + x) * G::KPI);
+      const uint64_t o = (uint64_t)key_off(a, sp2, st2, n, page_of(a, b, n));
+      pgw_lo[x] = (uint32_t)o;
+      pgw_hi[x] = (uint32_t)(o >> 32);
+    }
+  };
+  auto issue_tile = [&](int t) {
+    if (PAGED && t - pgw_t0 >= 64) fill_pgw(t);
+    const uint32_t dst = dst0 + (uint32_t)(t & 3) * (2 * G::TILE);
+    const int kb = kl.base(t_lo + t);
+    if ((uint32_t)(t - whole0) < (uint32_t)(whole1 - whole0) && whole1 > whole0) {
+#pragma unroll
+      for (int x = 0; x < IPW; ++x) {
+        int64_t off;
         if (PAGED)
-          off += __builtin_amdgcn_readlane(pgw[x], t - pgw_t0) * sp2 + (nb & psm) * st2;
+          off = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)pgw_hi[x], t - pgw_t0) << 32) |
+                          (uint32_t)__builtin_amdgcn_readlane((int)pgw_lo[x], t - pgw_t0));
         else
-          off += nb * st2;
-        dma_rs<false>(dst, make_rsrc(hbase + off, rsrc_range(span, off / 2)), lane_off[x]);
-      } else {
-        // At a border: a key that some row sees, through its own page.
+          off = kb * st2;
+        dma_rs<false>(dst + x * 1024, make_rsrc(hbase + off, reach), lane_off[x]);
+      }
+    } else {
+      // At a border: a key that some row sees, through its own page.
+#pragma unroll
+      for (int x = 0; x < IPW; ++x) {
         const int l = again(lane);
-        const int n = kl.read(nb + l / CH);
-        dma_lane(dst, hbase + wg_off + key_off(a, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
+        const int n = kl.read(kb + (j0 + x) * G::KPI + l / CH);
+        dma_lane(dst + x * 1024, hbase + key_off(a, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
       }
     }
   };
@@ -286,8 +290,8 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 
   // Per-lane LDS offsets of the operand reads within a tile: K's of k-step ks is
   // kofs ^ (ks << 5) and V's of d tile dt is vofs ^ (dt << 6) (the swizzles are
-  // XORs of whole chunks), one register each instead of one per step: 12 XORs a
-  // tile, where the registers would spill.
+  // XORs of whole chunks) plus the stage: one register each, so that the loop is
+  // not unrolled over the ring and nothing spills.
   uint32_t kofs, vofs;
   {
     const int bl = lane >> 4, bi = lane & 15;
@@ -297,56 +301,62 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     vofs = vkey * (2 * D) + v_slot(CH, vkey, vcol >> 3) * 16 + (vcol & 7) * 2;
   }
 
-  auto sync = [&](auto stage3_c, int k) {
+  auto sync = [&](int k) {
     if (k + 2 < ntiles)
       wait_vmcnt<IPW>();
     else
       wait_vmcnt<0>();
     barrier_lds();
-    if (k + 3 < ntiles) issue_tile(stage3_c, k + 3);
+    if (k + 3 < ntiles) issue_tile(k + 3);
   };
 
   f32x16 s_cur = f32x16{};
-  auto read_k = [&](auto stage_c, u32x4 (&kf)[KS]) {
-    constexpr int stage = decltype(stage_c)::value;
-    const uint8_t* kt = smem + stage * 2 * G::TILE;
-    const uint32_t o = (uint32_t)again((int)kofs);
+  auto read_k = [&](int t, u32x4 (&kf)[KS]) {
+    const uint32_t o = kofs + (uint32_t)(t & 3) * (2 * G::TILE);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const u32x4*>(kt + (o ^ (ks << 5)));
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const u32x4*>(smem + (o ^ (ks << 5)));
   };
-  auto read_vh = [&](auto stage_c, int hh, u32x4 (&vf)[2][DT]) {
-    constexpr int stage = decltype(stage_c)::value;
-    const uint8_t* vt = smem + (stage * 2 + 1) * G::TILE;
-    const uint32_t o = (uint32_t)again((int)vofs);
+  // V^T operands of half hh (keys 16*hh .. 16*hh+15) of a tile.
+  auto read_vh = [&](int t, int hh, u32x4 (&vf)[2][DT]) {
+    const uint32_t o = vofs + (uint32_t)(t & 3) * (2 * G::TILE) + G::TILE;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const uint8_t* p = vt + (o ^ (dt << 6)) + hh * 16 * (2 * D);
+      const uint8_t* p = smem + (o ^ (dt << 6)) + hh * 16 * (2 * D);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * (2 * D)));
       const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
       vf[hh][dt] = u32x4{l2[0], l2[1], h2[0], h2[1]};
     }
   };
+  // The tiles [seen0, seen1) are seen whole by every row of the wave (others may be).
+  int seen0 = 0, seen1 = 0;
+  {
+    const int first = pmax - a.W + 1, last = tree ? n0 : pmin + 1;  // keys [first, last)
+    seen0 = kl.nst + max((first - kl.lo_al + 31) >> 5, 0) - t_lo;
+    seen1 = kl.nst + ((last - kl.lo_al) >> 5) - t_lo;
+  }
 
   const float scale_log2 = a.scale_log2;
 
-  auto step = [&](auto stage_c, int k) {
-    constexpr int S = decltype(stage_c)::value;
-    if (!v_wave && k > 0) sync(IC<(S + 3) & 3>{}, k);
+  auto step = [&](auto masked_c, int k) {
+    constexpr bool MASKED = decltype(masked_c)::value;
+    if (!v_wave && k > 0) sync(k);
     u32x4 kf[KS], vf[2][DT];
     u32x4 pk[2];
     {
-      read_k(IC<(S + 1) & 3>{}, kf);
-      const int kb = kl.base(t_lo + k);
-      const bool drops = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, tree);
-      uint32_t keep = ~0u;
-      if (drops) {
-        keep = keep_word(a, b, tree ? min(row0 + (again(lane) & 31), a.R - 1) / a.G : 0, again(pos), kb, n0);
+      read_k(k + 1, kf);
+      bool drops = false;
+      if constexpr (MASKED) {
+       const int kb = kl.base(t_lo + k);
+       drops = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, tree);
+       if (drops) {
+        const uint32_t keep = keep_word(a, b, tree ? min(row0 + (again(lane) & 31), a.R - 1) / a.G : 0, again(pos), kb, n0);
         // Bit v of a lane <-> key 8 * (v / 4) + 4 * lg + v % 4.
         const uint32_t vb = keep >> (again(lane) >> 5 << 2);
         const uint32_t kv = (vb & 0xFu) | ((vb >> 4) & 0xF0u) | ((vb >> 8) & 0xF00u) | ((vb >> 12) & 0xF000u);
 #pragma unroll
         for (int v = 0; v < 16; ++v) s_cur[v] = ((kv >> v) & 1u) ? s_cur[v] : kNegInf;
+       }
       }
       auto rescale = [&]() {
         const float mt = xor32_max(max16(s_cur)) * scale_log2;
@@ -359,7 +369,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
           for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
         }
       };
-      if (drops || __ballot(mx == kNegInf) != 0ull) rescale();
+      if (MASKED && (drops || __ballot(mx == kNegInf) != 0ull)) rescale();
       auto exps = [&](bool with_v) {
         const float ms = (mx == kNegInf) ? 0.f : mx;
         float ts = 0.f;
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
         for (int hh = 0; hh < 2; ++hh) {
           if (with_v) {
             __builtin_amdgcn_sched_barrier(0);
-            read_vh(IC<S>{}, hh, vf);
+            read_vh(k, hh, vf);
             __builtin_amdgcn_sched_barrier(0);
           }
           uint32_t w4[4];
@@ -388,7 +398,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
         ts = exps(false);
       }
       lsum += ts;
-      if (drops) {
+      if (MASKED && drops) {
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
@@ -397,7 +407,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
             for (int e = 0; e < 4; ++e) odd |= nonfinite2<T>(vf[hh][dt][e]);
       }
     }
-    if (v_wave) sync(IC<(S + 3) & 3>{}, k);
+    if (v_wave) sync(k);
     {
       f32x16 sn = f32x16{};
 #pragma unroll
@@ -411,9 +421,9 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   };
 
   // ---- prologue: K(0..2) and V(0..1) issued, barrier 0, S(0) ---------------------
-  if (ntiles > 0) issue_tile(IC<0>{}, 0);
-  if (ntiles > 1) issue_tile(IC<1>{}, 1);
-  if (ntiles > 2 && !v_wave) issue_tile(IC<2>{}, 2);
+  if (ntiles > 0) issue_tile(0);
+  if (ntiles > 1) issue_tile(1);
+  if (ntiles > 2 && !v_wave) issue_tile(2);
   // The Q fragments and the score scale are complete before the loop: waits
   // placed at a first use inside it would wait for the DMA in flight there.
 #pragma unroll
@@ -426,33 +436,38 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       wait_vmcnt<0>();
     barrier_lds();
     if (v_wave) {
-      if (ntiles > 2) issue_tile(IC<2>{}, 2);
+      if (ntiles > 2) issue_tile(2);
     } else {
-      if (ntiles > 3) issue_tile(IC<3>{}, 3);
+      if (ntiles > 3) issue_tile(3);
     }
     if (wave_active) {
       u32x4 kf[KS];
-      read_k(IC<0>{}, kf);
+      read_k(0, kf);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s_cur = mfma32<T>(kf[ks], qf[ks], s_cur);
     }
   }
   if (wave_active) {
-    for (int t0 = 0; t0 < ntiles; t0 += 4) {
-      step(IC<0>{}, t0);
-      if (t0 + 1 < ntiles) step(IC<1>{}, t0 + 1);
-      if (t0 + 2 < ntiles) step(IC<2>{}, t0 + 2);
-      if (t0 + 3 < ntiles) step(IC<3>{}, t0 + 3);
+    // Three loops, so that the long one in the middle holds no mask and no first
+    // maximum (one of its tiles comes before it; a row that then still has none,
+    // all its scores -inf, keeps the wave out of it).  Unrolled: the accumulators
+    // stay in place.
+    const int k0 = min(max(seen0, 0) + 1, ntiles);
+    int k = 0;
+    for (; k < k0; ++k) step(BoolC<true>{}, k);
+    if (__ballot(mx == kNegInf) == 0ull) {
+      for (; k + 4 <= seen1 && k + 4 <= ntiles; k += 4) {
+        step(BoolC<false>{}, k);
+        step(BoolC<false>{}, k + 1);
+        step(BoolC<false>{}, k + 2);
+        step(BoolC<false>{}, k + 3);
+      }
     }
+    for (; k < ntiles; ++k) step(BoolC<true>{}, k);
   } else {
     // A wave without rows does its share of the DMA and meets the barriers.  (A
     // loop of its own: tests inside the other one cost 20 registers.)
-    for (int t0 = 0; t0 < ntiles; t0 += 4) {
-      if (v_wave || t0 > 0) sync(IC<3>{}, t0);
-      if (t0 + 1 < ntiles) sync(IC<0>{}, t0 + 1);
-      if (t0 + 2 < ntiles) sync(IC<1>{}, t0 + 2);
-      if (t0 + 3 < ntiles) sync(IC<2>{}, t0 + 3);
-    }
+    for (int k = v_wave ? 0 : 1; k < ntiles; ++k) sync(k);
   }
   // K waves meet the last barrier (V waves met it after the softmax of the last tile).
   if (ntiles > 0 && !v_wave) {
