@@ -1873,7 +1873,7 @@ namespace {
 
 struct WinPlan {
   int G = 0, R = 0, MW = 0, rpb = 0, n_rb = 0, splits = 1;
-  size_t opart_bytes = 0, ml_bytes = 0, depth_bytes = 0, total = 0;
+  size_t opart_bytes = 0, ml_bytes = 0, total = 0;
   const char* err = nullptr;
 };
 
@@ -1910,8 +1910,7 @@ WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
   const size_t rows = p.splits > 1 ? (size_t)B * Hk * p.splits * R : 0;
   p.opart_bytes = align_up(rows * D * sizeof(float), 256);
   p.ml_bytes = align_up(rows * sizeof(float2), 256);
-  p.depth_bytes = tree ? align_up((size_t)B * M * sizeof(int32_t), 256) : 0;
-  p.total = p.opart_bytes + p.ml_bytes + p.depth_bytes + (tree ? align_up((size_t)B * M * p.MW * 8, 256) : 0);
+  p.total = p.opart_bytes + p.ml_bytes;
   return p;
 }
 
@@ -1996,7 +1995,6 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
     a.seqlens = cache_seqlens->data;
     a.seqlens_i64 = cache_seqlens->dtype == DSV_I64;
   }
-  dsv::WinTree tree{};
   if (present(parent)) {
     if (parent->ndim != 1 && parent->ndim != 2) return fail(DSV_ERR_INVALID, "parent must be [M] or [B, M]");
     if ((rc = check_nd(parent, "parent", parent->ndim)) != DSV_OK) return rc;
@@ -2005,10 +2003,10 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
     if (parent->ndim == 2 && parent->shape[0] != B && parent->shape[0] != 1)
       return fail(DSV_ERR_INVALID, "parent batch must be 1 or B");
     if (M > dsv::kTreeMaxM) return fail(DSV_ERR_UNSUPPORTED, "trees larger than %d nodes are not supported", dsv::kTreeMaxM);
-    tree.parent = parent->data;
-    tree.i64 = parent->dtype == DSV_I64;
-    tree.sb = (parent->ndim == 2 && parent->shape[0] > 1) ? parent->stride[0] : 0;
-    tree.sm = parent->stride[parent->ndim - 1];
+    a.parent = parent->data;
+    a.par_i64 = parent->dtype == DSV_I64;
+    a.par_sb = (parent->ndim == 2 && parent->shape[0] > 1) ? parent->stride[0] : 0;
+    a.par_sm = parent->stride[parent->ndim - 1];
   }
   if (present(lse)) {
     if ((rc = check_nd(lse, "lse", 3)) != DSV_OK) return rc;
@@ -2032,7 +2030,7 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   // The kernel for many rows reads a DMA instruction's 4 or 8 keys through one
   // page, and a tile's 32 keys with 32-bit offsets from the first.
   const bool no_tile = (present(page_table) && k->shape[2] < 8) || a.k_st > (1 << 25) || a.v_st > (1 << 25);
-  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, tree.parent != nullptr, no_tile);
+  const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, a.parent != nullptr, no_tile);
   if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
   if ((rc = check_workspace(std::max<size_t>(p.total, 256), workspace, workspace_bytes)) != DSV_OK) return rc;
   a.dtype = q->dtype;
@@ -2060,11 +2058,7 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   char* w = static_cast<char*>(workspace);
   a.opart = reinterpret_cast<float*>(w);
   a.ml = reinterpret_cast<float2*>(w + p.opart_bytes);
-  if (tree.parent != nullptr) {
-    a.depth = reinterpret_cast<const int32_t*>(w + p.opart_bytes + p.ml_bytes);
-    a.bits = reinterpret_cast<const uint64_t*>(w + p.opart_bytes + p.ml_bytes + p.depth_bytes);
-    a.MW = p.MW;
-  }
+  a.MW = p.MW;
   a.out = out->data;
   a.out_dtype = out->dtype;
   a.o_sb = out->stride[0];
@@ -2074,7 +2068,7 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   a.out_vec = (reinterpret_cast<uintptr_t>(out->data) & 15) == 0 && (B == 1 || a.o_sb % per16 == 0) &&
               (M == 1 || a.o_sm % per16 == 0) && (H == 1 || a.o_sh % per16 == 0);
   if (g_dry_run) return DSV_OK;
-  const hipError_t e = dsv::launch_window(a, tree, (int)D, static_cast<hipStream_t>(stream));
+  const hipError_t e = dsv::launch_window(a, (int)D, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "windowed attention launch");
   return DSV_OK;
 }

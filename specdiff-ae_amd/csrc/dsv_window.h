@@ -24,20 +24,15 @@ struct WinArgs {
   int B, M, H, Hk, G, R;                   // R = G * M rows per KV head, row m * G + g
   int W, S;                                // window (>= 1) and sinks, at most kWinMaxKeys
   float scale_log2;                        // log2(e) / sqrt(D)
-  const int32_t* depth;                    // tree: [B, M] depths
-  const uint64_t* bits; int MW;            // tree: [B, M, MW] visible ancestors
+  const void* parent; int par_i64;         // tree: [B, M] parents (nullptr: causal)
+  int64_t par_sb, par_sm;
+  int MW;                                  // tree: 64-bit words of a row's set
   int rows_per_block, n_rb, splits;
   float* opart;                            // [B, Hk, splits, R, D] (splits > 1), relative to the maximum
   float2* ml;                              // [B, Hk, splits, R] (maximum in log2 units, sum)
   void* out; int out_dtype, out_vec;       // out_vec: rows take 16-byte stores
   int64_t o_sb, o_sm, o_sh;
   float* lse; int64_t l_sb, l_sm, l_sh;
-};
-
-struct WinTree {
-  const void* parent;                      // nullptr: causal
-  int i64;
-  int64_t sb, sm;
 };
 
 // Keys of a sequence at most: token numbers, positions and their differences
@@ -95,6 +90,6 @@ DSV_HD WinKeys win_keys(int M, int G, int R, int W, int S, bool tree, int n0, in
 
 // The kernel for many rows (rows_per_block 256, 16-bit, pages of at least 8 keys).
 hipError_t launch_window_tile(const WinArgs& a, int D, hipStream_t s);
-hipError_t launch_window(const WinArgs& a, const WinTree& tree, int D, hipStream_t s);
+hipError_t launch_window(const WinArgs& a, int D, hipStream_t s);
 
 }  // namespace dsv

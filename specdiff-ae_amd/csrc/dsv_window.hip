@@ -73,33 +73,6 @@ __device__ __forceinline__ float row_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// ---- the tree's visibility ---------------------------------------------------
-// Depth and the visible ancestor-or-self set of every node, once per call: a
-// walk up the parents of at most M steps (a parent < 0, >= M or equal to the
-// node ends it, as in the tree split of dsv_attn.hip).
-__global__ void __launch_bounds__(256) win_tree_kernel(const WinArgs a, const void* parent, int p_i64, int64_t p_sb,
-                                                       int64_t p_sm, int32_t* depth, uint64_t* bits) {
-  __shared__ int32_t par[kTreeMaxM];
-  const int b = blockIdx.x, M = a.M;
-  for (int i = threadIdx.x; i < M; i += 256) {
-    const int64_t o = b * p_sb + (int64_t)i * p_sm;
-    const int64_t x = p_i64 ? reinterpret_cast<const int64_t*>(parent)[o] : (int64_t) reinterpret_cast<const int32_t*>(parent)[o];
-    par[i] = x < 0 || x >= M || x == i ? -1 : (int32_t)x;
-  }
-  __syncthreads();
-  const int n0 = len_of(a, b) - M;
-  for (int i = threadIdx.x; i < M; i += 256) {
-    int d = 0;
-    for (int x = par[i]; x >= 0 && d < M; x = par[x]) ++d;
-    depth[(int64_t)b * M + i] = d;
-    uint64_t* t = bits + ((int64_t)b * M + i) * a.MW;
-    for (int w = 0; w < a.MW; ++w) t[w] = 0;
-    // Ancestor at h hops: position n0 + d - h against the row's n0 + d.
-    for (int x = i, h = 0; x >= 0 && h <= d; x = par[x], ++h)
-      if (h < a.W || n0 + d - h < a.S) t[x >> 6] |= 1ull << (x & 63);
-  }
-}
-
 // Eight waves: two per SIMD have 256 KiB of loads in flight between them where
 // the registers allow, and four per workgroup left the batch of 64 at 230 us, 184
 // with eight (16 spill).
@@ -136,23 +109,33 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
   const int kvh = w % a.Hk, b = w / a.Hk;
   const int n0 = len_of(a, b) - a.M;
   const int r0 = rb * 16 * NR;
-  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, r0, 16 * NR);
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, r0, 16 * NR);
   const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
   int t = (int)((int64_t)kl.nt * split / a.splits) + wave;
 
   // This lane's rows: Q fragments (B operand): row lr, elements 32 ks + 8 lg ..
-  Row row[NR];
+  __shared__ TreeLds<16 * NR> tl;
+  int pos[NR];
   u32x4 qf[NR][KS];
   int pmin = 0x7fffffff, pmax = -0x7fffffff;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int r = min(r0 + 16 * i + lr, a.R - 1);
-    row[i] = row_of(a, b, r, n0);
-    const uint16_t* q = a.q + b * a.q_sb + (int64_t)row[i].m * a.q_sm + (int64_t)(kvh * a.G + row[i].g) * a.q_sh + 8 * lg;
+    const Row row = row_of(a, r);
+    const uint16_t* q = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh + 8 * lg;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[i][ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks);
-    pmin = min(pmin, row[i].pos);
-    pmax = max(pmax, row[i].pos);
+    pos[i] = n0 + row.m;
+  }
+  if (a.parent != nullptr) {
+    tree_rows<16 * NR, kRowWaves * 64>(a, b, n0, r0, tl);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) pos[i] = n0 + tl.depth[16 * i + lr];
+  }
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    pmin = min(pmin, pos[i]);
+    pmax = max(pmax, pos[i]);
   }
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -228,14 +211,14 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     if (t + NW < t_end) load_tile(t + NW, pg);
     pg = tile_pages(t + 2 * NW);
     // ---- mask and softmax
-    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
+    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.parent != nullptr);
     uint32_t keep[NR];
     u32x4 pf[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       keep[i] = ~0u;
       if (masked) {
-        keep[i] = keep_word(a, b, row[i].m, row[i].pos, kb, n0);
+        keep[i] = keep_word(a, tl.vis + (16 * i + lr) * kTreeMaxW, pos[i], kb, n0);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (!((keep[i] >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[i][e >> 2][e & 3] = kNegInf;
@@ -376,17 +359,23 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
   const int kvh = w % a.Hk, b = w / a.Hk;
   const int n0 = len_of(a, b) - a.M;
   const int r0 = rb * 16;
-  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, r0, 16);
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, r0, 16);
   const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
   const float* kbase = reinterpret_cast<const float*>(a.k) + b * a.k_sb + kvh * a.k_sh;
   const float* vbase = reinterpret_cast<const float*>(a.v) + b * a.v_sb + kvh * a.v_sh;
 
-  const Row row = row_of(a, b, min(r0 + lr, a.R - 1), n0);
+  __shared__ TreeLds<16> tl;
+  const Row row = row_of(a, min(r0 + lr, a.R - 1));
   f32x4 qf[KC];
   const float* q = reinterpret_cast<const float*>(a.q) + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh;
 #pragma unroll
   for (int c = 0; c < KC; ++c) qf[c] = *reinterpret_cast<const f32x4*>(q + 16 * c + 4 * lg);
-  int pmin = row.pos, pmax = row.pos;
+  int pos = n0 + row.m;
+  if (a.parent != nullptr) {
+    tree_rows<16, kRowWaves * 64>(a, b, n0, r0, tl);
+    pos = n0 + tl.depth[lr];
+  }
+  int pmin = pos, pmax = pos;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
     pmin = min(pmin, __shfl_xor(pmin, o));
@@ -425,8 +414,8 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
       for (int d = 0; d < DT; ++d) vf[e][d] = v[16 * d];
     }
     pg = tile_pages(t + NW);
-    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.bits != nullptr);
-    const uint32_t keep = masked ? keep_word(a, b, row.m, row.pos, kb, n0) : ~0u;
+    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.parent != nullptr);
+    const uint32_t keep = masked ? keep_word(a, tl.vis + lr * kTreeMaxW, pos, kb, n0) : ~0u;
     f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -538,20 +527,40 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
   const int64_t bh = x / a.R;
   const int r = (int)(x - bh * a.R);
   const int b = (int)(bh / a.Hk), kvh = (int)(bh % a.Hk);
+  // Eight splits' loads in flight (16 splits of 4096 rows: 12 us with four, 8 with
+  // eight).
+  constexpr int U = 8;
   float m = kNegInf, l = 0.f;
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t pr = (bh * a.splits + s) * a.R + r;
-    const float2 ml = a.ml[pr];
-    const f32x4 p = *reinterpret_cast<const f32x4*>(a.opart + pr * D + d0);
-    if (ml.y == 0.f) continue;
-    const float mn = fmaxf(m, ml.x);
-    const float f0 = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
-    m = mn;
-    l = l * f0 + ml.y * f1;
+  const int64_t p0 = bh * a.splits * a.R + r;
+  for (int s0 = 0; s0 < a.splits; s0 += U) {
+    float2 ml[U];
+    f32x4 p[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + p[e] * f1;
+    for (int u = 0; u < U; ++u) {
+      const int64_t pr = p0 + (int64_t)min(s0 + u, a.splits - 1) * a.R;
+      ml[u] = a.ml[pr];
+      p[u] = *reinterpret_cast<const f32x4*>(a.opart + pr * D + d0);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= a.splits) ml[u] = make_float2(kNegInf, 0.f);
+      mn = fmaxf(mn, ml[u].x);
+    }
+    const float ms = mn == kNegInf ? 0.f : mn, f0 = __builtin_amdgcn_exp2f(m - ms);
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (ml[u].y == 0.f) continue;  // a split without a key of this row
+      const float f = __builtin_amdgcn_exp2f(ml[u].x - ms);
+      l += ml[u].y * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += p[u][e] * f;
+    }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
@@ -592,14 +601,6 @@ hipError_t launch_d(const WinArgs& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_window(const WinArgs& a, const WinTree& tree, int D, hipStream_t s) {
-  if (tree.parent != nullptr) {
-    hipLaunchKernelGGL(win_tree_kernel, dim3((unsigned)a.B), dim3(256), 0, s, a, tree.parent, tree.i64, tree.sb, tree.sm,
-                       const_cast<int32_t*>(a.depth), const_cast<uint64_t*>(a.bits));
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return D == 64 ? launch_d<64>(a, s) : launch_d<128>(a, s);
-}
+hipError_t launch_window(const WinArgs& a, int D, hipStream_t s) { return D == 64 ? launch_d<64>(a, s) : launch_d<128>(a, s); }
 
 }  // namespace dsv

@@ -55,34 +55,85 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// One query row as a lane sees it.
+// One query row.
 struct Row {
-  int m, g, pos;
+  int m, g;
 };
-__device__ __forceinline__ Row row_of(const WinArgs& a, int b, int r, int n0) {
+__device__ __forceinline__ Row row_of(const WinArgs& a, int r) {
   Row w;
   w.m = r / a.G;
   w.g = r - w.m * a.G;
-  w.pos = n0 + (a.depth != nullptr ? a.depth[(int64_t)b * a.M + w.m] : w.m);
   return w;
 }
 
-// The keep word of a row for the tile at key kb: bit i = key kb + i is seen.
-__device__ __forceinline__ uint32_t keep_word(const WinArgs& a, int b, int m, int pos, int kb, int n0) {
+// A workgroup's rows of a tree, in LDS: each row's depth and the set of tree keys
+// that it sees, MW = ceil(M / 64) words.  Every workgroup walks up its rows'
+// parents by itself (about a microsecond beside the latencies of its first
+// loads; a kernel of its own before the attention took 5 us and a launch).
+template <int ROWS>
+struct TreeLds {
+  int16_t par[kTreeMaxM];
+  int depth[ROWS];
+  uint64_t vis[ROWS * kTreeMaxW];
+};
+
+// The walks, at most M steps each (a parent < 0, >= M or equal to the node ends
+// one, as in the tree split of dsv_attn.hip).  Every thread of the workgroup
+// calls it; ends with a barrier.
+template <int ROWS, int NT>
+__device__ __forceinline__ void tree_rows(const WinArgs& a, int b, int n0, int r0, TreeLds<ROWS>& t) {
+  const int M = a.M;
+  for (int i = threadIdx.x; i < M; i += NT) {
+    const int64_t o = b * a.par_sb + (int64_t)i * a.par_sm;
+    const int64_t x = a.par_i64 ? reinterpret_cast<const int64_t*>(a.parent)[o]
+                                : (int64_t) reinterpret_cast<const int32_t*>(a.parent)[o];
+    t.par[i] = x < 0 || x >= M || x == i ? (int16_t)-1 : (int16_t)x;
+  }
+  __syncthreads();
+  if (threadIdx.x < ROWS) {
+    const int m = min(r0 + (int)threadIdx.x, a.R - 1) / a.G;
+    uint64_t* vis = t.vis + threadIdx.x * kTreeMaxW;
+    for (int w = 0; w < a.MW; ++w) vis[w] = 0;
+    // The ancestor at h hops stands h positions before the row: seen for h < W.
+    uint64_t word = 0;
+    int at = m >> 6, h = 0;
+    for (int x = m; x >= 0 && h <= M; x = t.par[x], ++h) {
+      if (x >> 6 != at) {
+        vis[at] |= word;
+        word = 0;
+        at = x >> 6;
+      }
+      if (h < a.W) word |= 1ull << (x & 63);
+    }
+    vis[at] |= word;
+    const int depth = min(h - 1, M);
+    t.depth[threadIdx.x] = depth;
+    // And those at positions below the sinks' end.
+    if (n0 < a.S) {
+      h = 0;
+      for (int x = m; x >= 0 && h <= depth; x = t.par[x], ++h)
+        if (n0 + depth - h < a.S) vis[x >> 6] |= 1ull << (x & 63);
+    }
+  }
+  __syncthreads();
+}
+
+// The keep word of a row at position pos for the tile at key kb: bit i = key
+// kb + i is seen (vis: the row's tree keys, where there is a tree).
+__device__ __forceinline__ uint32_t keep_word(const WinArgs& a, const uint64_t* vis, int pos, int kb, int n0) {
   const uint32_t win = ~win_below(pos - a.W + 1 - kb) | win_below(a.S - kb);
-  if (a.bits == nullptr) return win & win_below(pos + 1 - kb);
+  if (a.parent == nullptr) return win & win_below(pos + 1 - kb);
   uint32_t keep = win & win_below(n0 - kb);
   if (kb + 32 > n0) {
     // Tree keys: bits [kb - n0, kb - n0 + 32) of the row's set.
-    const uint64_t* t = a.bits + ((int64_t)b * a.M + m) * a.MW;
     const int at = kb - n0;
     uint64_t x = 0;
     if (at < 0) {
-      x = t[0] << -at;
+      x = vis[0] << -at;
     } else if ((at >> 6) < a.MW) {
       const int i = at >> 6, sh = at & 63;
-      x = t[i] >> sh;
-      if (sh > 32 && i + 1 < a.MW) x |= t[i + 1] << (64 - sh);
+      x = vis[i] >> sh;
+      if (sh > 32 && i + 1 < a.MW) x |= vis[i + 1] << (64 - sh);
     }
     keep |= (uint32_t)x;
   }

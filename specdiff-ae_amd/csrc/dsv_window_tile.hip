@@ -88,16 +88,18 @@ __device__ __forceinline__ const WinArgs& args_again() {
 // product 0 * inf would reach those rows.  A lane takes a key of 64 for the
 // scores and D / 64 columns for the sums.
 template <typename T, int D>
-__device__ __noinline__ void exact_rows(const WinArgs* ap, int b, int kvh, int split, int rb, int t0, int t1, int row0) {
+__device__ __noinline__ void exact_rows(const WinArgs* ap, const TreeLds<256>* tl, int b, int kvh, int split, int rb, int t0,
+                                        int t1, int row0) {
   const WinArgs& a = *ap;
   const int n0 = len_of(a, b) - a.M;
-  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.bits != nullptr, n0, rb * 256, 256);
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, rb * 256, 256);
   constexpr int N = D / 64;
   const int lane = threadIdx.x & 63;
   const uint16_t* kbase = a.k + b * a.k_sb + kvh * a.k_sh;
   const uint16_t* vbase = a.v + b * a.v_sb + kvh * a.v_sh;
   for (int r = row0; r < row0 + 32 && r < a.R; ++r) {
-    const Row row = row_of(a, b, r, n0);
+    const Row row = row_of(a, r);
+    const int pos = n0 + (a.parent != nullptr ? tl->depth[r - rb * 256] : row.m);
     const int h = kvh * a.G + row.g;
     const uint16_t* q = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)h * a.q_sh;
     float m = kNegInf, l = 0.f, o[N];
@@ -106,7 +108,7 @@ __device__ __noinline__ void exact_rows(const WinArgs* ap, int b, int kvh, int s
     for (int t = t0; t < t1; t += 2) {
       const int tt = t + (lane >> 5), i = lane & 31;
       const int kb = kl.base(min(tt, t1 - 1));
-      const bool seen = tt < t1 && ((keep_word(a, b, row.m, row.pos, kb, n0) >> i) & 1u);
+      const bool seen = tt < t1 && ((keep_word(a, tl->vis + (r - rb * 256) * kTreeMaxW, pos, kb, n0) >> i) & 1u);
       const int n = kl.read(kb + i);
       const int32_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
       const uint16_t* k = kbase + key_off(a, a.k_sp, a.k_st, n, page);
@@ -174,7 +176,9 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   constexpr int IPW = 2 * G::NINS / NW;  // DMA instructions per wave and tile
   static_assert(IPW * NW == 2 * G::NINS && G::NINS % IPW == 0, "K and V DMA halves map to wave halves");
   static_assert(G::STAGES == 4 && NW * 32 * D * 2 <= G::RING, "");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[G::RING];
+  // One LDS allocation, the DMA ring at its start (destinations below 64 KiB).
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[G::RING + sizeof(TreeLds<256>)];
+  TreeLds<256>& tl = *reinterpret_cast<TreeLds<256>*>(smem + G::RING);
 
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, lj = lane & 31, lg = lane >> 5;
@@ -189,7 +193,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   w /= a.splits;
   const int kvh = w % a.Hk, b = w / a.Hk;
 
-  const bool tree = a.bits != nullptr;
+  const bool tree = a.parent != nullptr;
   const int n0 = uniform(len_of(a, b) - a.M);
   const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, tree, n0, rb * 256, 256);
   const int t_lo = (int)((int64_t)kl.nt * split / a.splits);
@@ -202,11 +206,15 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   u32x4 qf[KS];
   int pos;
   {
-    const Row row = row_of(a, b, min(r_me, a.R - 1), n0);
-    pos = row.pos;
+    const Row row = row_of(a, min(r_me, a.R - 1));
+    pos = n0 + row.m;
     const uint16_t* qp = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh + lg * 8;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + ks * 16);
+  }
+  if (tree) {
+    tree_rows<256, 512>(a, b, n0, rb * 256, tl);
+    pos = n0 + tl.depth[wid * 32 + lj];
   }
   int pmin = pos, pmax = pos;
 #pragma unroll
@@ -350,7 +358,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
        const int kb = kl.base(t_lo + k);
        drops = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, tree);
        if (drops) {
-        const uint32_t keep = keep_word(a, b, tree ? min(row0 + (again(lane) & 31), a.R - 1) / a.G : 0, again(pos), kb, n0);
+        const uint32_t keep = keep_word(a, tl.vis + (wid * 32 + (again(lane) & 31)) * kTreeMaxW, again(pos), kb, n0);
         // Bit v of a lane <-> key 8 * (v / 4) + 4 * lg + v % 4.
         const uint32_t vb = keep >> (again(lane) >> 5 << 2);
         const uint32_t kv = (vb & 0xFu) | ((vb >> 4) & 0xF0u) | ((vb >> 8) & 0xF00u) | ((vb >> 12) & 0xF000u);
@@ -486,11 +494,11 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   const int r_ep = row0 + lje;
   const bool rvalid = r_ep < z.R;
   if (__ballot(odd != 0) != 0ull) {
-    exact_rows<T, D>(&z, b, kvh, split, rb, t_lo, t_lo + ntiles, row0);
+    exact_rows<T, D>(&z, &tl, b, kvh, split, rb, t_lo, t_lo + ntiles, row0);
     return;
   }
   const float ltot = xor32_sum(lsum);
-  const Row row = row_of(z, b, min(r_ep, z.R - 1), n0);
+  const Row row = row_of(z, min(r_ep, z.R - 1));
   const int h = kvh * z.G + row.g;
   // Accumulator value v of d tile dt holds d = 32*dt + 8*(v/4) + 4*lge + v%4.
   if (z.splits > 1) {
