@@ -49,9 +49,6 @@ struct WinKeys {
   int lo, hi, sink, lo_al;
   int nst, nt;
   DSV_HD int base(int t) const { return t < nst ? 32 * t : lo_al + 32 * (t - nst); }
-  // Does any row of the block see key n?
-  DSV_HD bool has(int n) const { return n < sink || (n >= lo && n < hi); }
-  DSV_HD bool whole(int kb) const { return kb + 32 <= sink || (kb >= lo && kb + 32 <= hi); }
   // Key n, or where no row sees it one that some row does: what is read in its
   // place (its own page may be gone).
   DSV_HD int read(int n) const {

@@ -22,10 +22,10 @@
 // takes them unrounded.  Partial outputs of splits are fp32.
 //
 // Values of keys that a row does not see never reach it, whatever they hold: a
-// masked score is replaced, rows of V outside the workgroup's keys are
-// replaced by zeros, and a tile whose V holds infinities or NaN while some row
-// of the wave drops some of its keys takes a slow path that adds those entries
-// row by row (0 * inf would be NaN in the matrix product).
+// masked score is replaced, keys that no row of a workgroup sees are not read (a
+// seen one is, in their place), and where V holds infinities or NaN in a tile of
+// which some row drops keys, the rows are computed once more without matrix
+// products (exact_rows; in the product 0 * inf would be NaN).
 //
 // win_rows_kernel (this file's simplest; few rows: single tokens, short
 // chunks): bound by reading K and V.  Eight waves share a workgroup's tiles,
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
   }
 
   float mx[NR], ls[NR];
+  uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of
   f32x4 acc[NR][DT];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
@@ -196,14 +197,12 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
       }
     }
     wave_lds_fence();
-    // ---- V into LDS; rows that no row of the workgroup sees become zeros.
-    const bool edge = !kl.whole(kb);
-    uint32_t odd = 0;
+    // ---- V into LDS
+    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.parent != nullptr);
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int i = j * KPI + lane / CH;
-      if (edge && !kl.has(kb + i)) vr[j] = u32x4{0, 0, 0, 0};
-      odd |= nonfinite2<T>(vr[j][0]) | nonfinite2<T>(vr[j][1]) | nonfinite2<T>(vr[j][2]) | nonfinite2<T>(vr[j][3]);
+      if (masked) odd |= nonfinite2<T>(vr[j][0]) | nonfinite2<T>(vr[j][1]) | nonfinite2<T>(vr[j][2]) | nonfinite2<T>(vr[j][3]);
       *reinterpret_cast<u32x4*>(mine + i * VST + (lane % CH) * 16) = vr[j];
     }
     wave_lds_fence();
@@ -211,17 +210,14 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     if (t + NW < t_end) load_tile(t + NW, pg);
     pg = tile_pages(t + 2 * NW);
     // ---- mask and softmax
-    const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.parent != nullptr);
-    uint32_t keep[NR];
     u32x4 pf[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-      keep[i] = ~0u;
       if (masked) {
-        keep[i] = keep_word(a, tl.vis + (16 * i + lr) * kTreeMaxW, pos[i], kb, n0);
+        const uint32_t keep = keep_word(a, tl.vis + (16 * i + lr) * kTreeMaxW, pos[i], kb, n0);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (!((keep[i] >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[i][e >> 2][e & 3] = kNegInf;
+          if (!((keep >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[i][e >> 2][e & 3] = kNegInf;
       }
       float x[8];
 #pragma unroll
@@ -246,31 +242,6 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
       pf[i] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
     }
     // ---- O^T += V^T . P^T; element e of lane group lg is key 16 (e / 4) + 4 lg + e % 4.
-    if (masked && __ballot(odd != 0) != 0ull) {
-      // Infinite or NaN entries of V: added to the rows that see them, and out of the product.
-      for (int n = 0; n < 32; ++n) {
-        uint16_t* v = reinterpret_cast<uint16_t*>(mine + n * VST);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = unpack1<T>(v[16 * d + 4 * lg + e]);
-            const bool bad = !(x - x == 0.f);
-#pragma unroll
-            for (int i = 0; i < NR; ++i)
-              if (bad && ((keep[i] >> n) & 1u)) acc[i][d][e] += x;
-          }
-        wave_lds_fence();
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = unpack1<T>(v[16 * d + 4 * lg + e]);
-            if (lr == 0 && !(x - x == 0.f)) v[16 * d + 4 * lg + e] = 0;
-          }
-      }
-      wave_lds_fence();
-    }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const uint8_t* p = mine + (4 * lg + (lr >> 2)) * VST + (16 * d + 4 * (lr & 3)) * 2;
@@ -283,6 +254,10 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     wave_lds_fence();
   }
 
+  if (__syncthreads_or((int)(odd & 0x80008000u)) != 0) {
+    exact_rows<T, D, 16 * NR>(&args_again(), &tl, b, kvh, split, rb, (int)((int64_t)kl.nt * split / a.splits), t_end, wave, 16 * NR, NW);
+    return;
+  }
   // ---- the waves' rows joined, 16 at a time
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
@@ -382,6 +357,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
     pmax = max(pmax, __shfl_xor(pmax, o));
   }
   float mx = kNegInf, ls = 0.f;
+  bool odd = false;
   f32x4 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
@@ -448,29 +424,20 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
       x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -ms));
       ls += x[e];
     }
+    if (masked) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bool odd = false;
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) odd |= !(vf[e][d] - vf[e][d] == 0.f);
-      if (masked && __ballot(odd) != 0ull) {
-        // Infinite or NaN entries: added to the rows that see them, and out of
-        // the product.  Lane group y holds key 4 y + e % 4; this lane's
-        // accumulators are d = 16 d + 4 lg + z of row lr.
-        for (int y = 0; y < 4; ++y)
+        for (int d = 0; d < DT; ++d) odd |= !(vf[e][d] - vf[e][d] == 0.f);
+    }
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const float o = __shfl(vf[e][d], 16 * y + 4 * lg + z);
-              if (!(o - o == 0.f) && ((keep >> (16 * (e >> 2) + 4 * y + (e & 3))) & 1u)) acc[d][z] += o;
-            }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vf[e][d] = vf[e][d] - vf[e][d] == 0.f ? vf[e][d] : 0.f;
-      }
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][d], x[e], acc[d], 0, 0, 0);
-    }
+  }
+  if (__syncthreads_or((int)odd) != 0) {
+    exact_rows<float, D, 16>(&args_again(), &tl, b, kvh, split, rb, (int)((int64_t)kl.nt * split / a.splits), t_end, wave, 16, NW);
+    return;
   }
 
   const float lt = row_sum(ls);

@@ -192,4 +192,106 @@ __device__ __forceinline__ void store_out(const WinArgs& a, int64_t off, const f
   }
 }
 
+// The kernel's arguments, loaded again where they are needed: what the epilogue
+// reads does not stay in registers through the loop.
+__device__ __forceinline__ const WinArgs& args_again() {
+  typedef const WinArgs __attribute__((address_space(4))) * Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const WinArgs*)p;
+}
+
+// Rows [i0, i1) by step of a workgroup once more, by one wave, from memory and
+// without matrix products, where V holds infinities or NaN in keys that some of
+// the rows do not see: in the product 0 * inf would reach those rows.  A lane
+// takes a key of 64 for the scores and D / 64 columns for the sums.
+template <typename T>
+struct Elem {
+  typedef uint16_t type;
+  static __device__ __forceinline__ float get(uint16_t x) { return unpack1<T>(x); }
+};
+template <>
+struct Elem<float> {
+  typedef float type;
+  static __device__ __forceinline__ float get(float x) { return x; }
+};
+template <typename T, int D, int ROWS>
+__device__ __noinline__ void exact_rows(const WinArgs* ap, const TreeLds<ROWS>* tl, int b, int kvh, int split, int rb, int t0, int t1,
+                                        int i0, int i1, int step) {
+  typedef Elem<T> El;
+  typedef typename El::type E;
+  constexpr int N = D / 64;
+  const WinArgs& a = *ap;
+  const int n0 = len_of(a, b) - a.M;
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, rb * ROWS, ROWS);
+  const int lane = threadIdx.x & 63;
+  const E* kbase = reinterpret_cast<const E*>(a.k) + b * a.k_sb + kvh * a.k_sh;
+  const E* vbase = reinterpret_cast<const E*>(a.v) + b * a.v_sb + kvh * a.v_sh;
+  for (int i = i0; i < i1; i += step) {
+    const int r = rb * ROWS + i;
+    if (r >= a.R) break;
+    const Row row = row_of(a, r);
+    const int pos = n0 + (a.parent != nullptr ? tl->depth[i] : row.m);
+    const int h = kvh * a.G + row.g;
+    const E* q = reinterpret_cast<const E*>(a.q) + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)h * a.q_sh;
+    float m = kNegInf, l = 0.f, o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0.f;
+    for (int t = t0; t < t1; t += 2) {
+      const int tt = t + (lane >> 5), x = lane & 31;
+      const int kb = kl.base(min(tt, t1 - 1));
+      const bool seen = tt < t1 && ((keep_word(a, tl->vis + i * kTreeMaxW, pos, kb, n0) >> x) & 1u);
+      const int n = kl.read(kb + x);
+      const int32_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
+      const E* k = kbase + key_off(a, a.k_sp, a.k_st, n, page);
+      const int64_t vo = key_off(a, a.v_sp, a.v_st, n, page);
+      float s = kNegInf;
+      if (seen) {
+        s = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < D; ++d) s = fmaf(El::get(q[d]), El::get(k[d]), s);
+      }
+      float mt = s;
+#pragma unroll
+      for (int y = 1; y < 64; y <<= 1) mt = fmaxf(mt, __shfl_xor(mt, y));
+      const float mn = fmaxf(m, mt * a.scale_log2), ms = mn == kNegInf ? 0.f : mn;
+      const float al = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, a.scale_log2, -ms)) : 0.f;
+      float ps = p;
+#pragma unroll
+      for (int y = 1; y < 64; y <<= 1) ps += __shfl_xor(ps, y);
+      l = l * al + ps;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] *= al;
+      for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
+        const int src = __builtin_ctzll(left);
+        const float pn = __shfl(p, src);
+        const E* v = vbase + (int64_t)__shfl((long long)vo, src) + lane * N;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = fmaf(pn, El::get(v[e]), o[e]);
+      }
+    }
+    if (a.splits > 1) {
+      const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
+#pragma unroll
+      for (int e = 0; e < N; ++e) a.opart[pr * D + lane * N + e] = o[e];
+      if (lane == 0) a.ml[pr] = make_float2(m, l);
+      continue;
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const int64_t off = b * a.o_sb + (int64_t)row.m * a.o_sm + (int64_t)h * a.o_sh + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = o[e] * inv;
+      if (a.out_dtype == 2)
+        reinterpret_cast<float*>(a.out)[off + e] = x;
+      else
+        reinterpret_cast<uint16_t*>(a.out)[off + e] = (uint16_t)(a.out_dtype == 0 ? pack2<BF16>(x, x) : pack2<F16>(x, x));
+    }
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[b * a.l_sb + (int64_t)row.m * a.l_sm + (int64_t)h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+  }
+}
+
 }  // namespace dsv

@@ -74,93 +74,6 @@ __device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
 }
 
-// The kernel's arguments, loaded again where they are needed: what the epilogue
-// reads does not stay in registers through the loop.
-__device__ __forceinline__ const WinArgs& args_again() {
-  typedef const WinArgs __attribute__((address_space(4))) * Ptr;
-  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const WinArgs*)p;
-}
-
-// A wave's 32 rows once more, from memory and without matrix products, where V
-// holds infinities or NaN in keys that some of the rows do not see: in the
-// product 0 * inf would reach those rows.  A lane takes a key of 64 for the
-// scores and D / 64 columns for the sums.
-template <typename T, int D>
-__device__ __noinline__ void exact_rows(const WinArgs* ap, const TreeLds<256>* tl, int b, int kvh, int split, int rb, int t0,
-                                        int t1, int row0) {
-  const WinArgs& a = *ap;
-  const int n0 = len_of(a, b) - a.M;
-  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, rb * 256, 256);
-  constexpr int N = D / 64;
-  const int lane = threadIdx.x & 63;
-  const uint16_t* kbase = a.k + b * a.k_sb + kvh * a.k_sh;
-  const uint16_t* vbase = a.v + b * a.v_sb + kvh * a.v_sh;
-  for (int r = row0; r < row0 + 32 && r < a.R; ++r) {
-    const Row row = row_of(a, r);
-    const int pos = n0 + (a.parent != nullptr ? tl->depth[r - rb * 256] : row.m);
-    const int h = kvh * a.G + row.g;
-    const uint16_t* q = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)h * a.q_sh;
-    float m = kNegInf, l = 0.f, o[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = 0.f;
-    for (int t = t0; t < t1; t += 2) {
-      const int tt = t + (lane >> 5), i = lane & 31;
-      const int kb = kl.base(min(tt, t1 - 1));
-      const bool seen = tt < t1 && ((keep_word(a, tl->vis + (r - rb * 256) * kTreeMaxW, pos, kb, n0) >> i) & 1u);
-      const int n = kl.read(kb + i);
-      const int32_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
-      const uint16_t* k = kbase + key_off(a, a.k_sp, a.k_st, n, page);
-      const int64_t vo = key_off(a, a.v_sp, a.v_st, n, page);
-      float s = kNegInf;
-      if (seen) {
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = fmaf(unpack1<T>(q[d]), unpack1<T>(k[d]), s);
-      }
-      float mt = s;
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) mt = fmaxf(mt, __shfl_xor(mt, x));
-      const float mn = fmaxf(m, mt * a.scale_log2), ms = mn == kNegInf ? 0.f : mn;
-      const float al = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, a.scale_log2, -ms)) : 0.f;
-      float ps = p;
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) ps += __shfl_xor(ps, x);
-      l = l * al + ps;
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[e] *= al;
-      for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
-        const int src = __builtin_ctzll(left);
-        const float pn = __shfl(p, src);
-        const uint16_t* v = vbase + (int64_t)__shfl((long long)vo, src) + lane * N;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = fmaf(pn, unpack1<T>(v[e]), o[e]);
-      }
-    }
-    if (a.splits > 1) {
-      const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
-#pragma unroll
-      for (int e = 0; e < N; ++e) a.opart[pr * D + lane * N + e] = o[e];
-      if (lane == 0) a.ml[pr] = make_float2(m, l);
-      continue;
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    const int64_t off = b * a.o_sb + (int64_t)row.m * a.o_sm + (int64_t)h * a.o_sh + lane * N;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = o[e] * inv;
-      if (a.out_dtype == 2)
-        reinterpret_cast<float*>(a.out)[off + e] = x;
-      else
-        reinterpret_cast<uint16_t*>(a.out)[off + e] = (uint16_t)(a.out_dtype == 0 ? pack2<BF16>(x, x) : pack2<F16>(x, x));
-    }
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[b * a.l_sb + (int64_t)row.m * a.l_sm + (int64_t)h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
-  }
-}
-
 template <bool B>
 struct BoolC {
   static constexpr bool value = B;
@@ -494,7 +407,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   const int r_ep = row0 + lje;
   const bool rvalid = r_ep < z.R;
   if (__ballot(odd != 0) != 0ull) {
-    exact_rows<T, D>(&z, &tl, b, kvh, split, rb, t_lo, t_lo + ntiles, row0);
+    exact_rows<T, D, 256>(&z, &tl, b, kvh, split, rb, t_lo, t_lo + ntiles, wid * 32, wid * 32 + 32, 1);
     return;
   }
   const float ltot = xor32_sum(lsum);
