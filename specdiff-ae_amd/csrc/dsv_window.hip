@@ -80,7 +80,7 @@ constexpr int kRowWaves = 8;
 
 // ---- few rows ------------------------------------------------------------------
 
-template <typename T, int D, int NR>
+template <typename T, int D>
 __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs a) {
   constexpr int NW = kRowWaves;
   constexpr int CH = D / 8;           // 16-byte chunks per key
@@ -108,51 +108,38 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
   w /= a.n_rb;
   const int kvh = w % a.Hk, b = w / a.Hk;
   const int n0 = len_of(a, b) - a.M;
-  const int r0 = rb * 16 * NR;
-  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, r0, 16 * NR);
+  const int r0 = rb * 16;
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, a.parent != nullptr, n0, r0, 16);
   const int t_end = (int)((int64_t)kl.nt * (split + 1) / a.splits);
   int t = (int)((int64_t)kl.nt * split / a.splits) + wave;
 
   // This lane's rows: Q fragments (B operand): row lr, elements 32 ks + 8 lg ..
-  __shared__ TreeLds<16 * NR> tl;
-  int pos[NR];
-  u32x4 qf[NR][KS];
-  int pmin = 0x7fffffff, pmax = -0x7fffffff;
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const int r = min(r0 + 16 * i + lr, a.R - 1);
-    const Row row = row_of(a, r);
+  __shared__ TreeLds<16> tl;
+  int pos;
+  u32x4 qf[KS];
+  {
+    const Row row = row_of(a, min(r0 + lr, a.R - 1));
     const uint16_t* q = a.q + b * a.q_sb + (int64_t)row.m * a.q_sm + (int64_t)(kvh * a.G + row.g) * a.q_sh + 8 * lg;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[i][ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks);
-    pos[i] = n0 + row.m;
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks);
+    pos = n0 + row.m;
   }
   if (a.parent != nullptr) {
-    tree_rows<16 * NR, kRowWaves * 64>(a, b, n0, r0, tl);
-#pragma unroll
-    for (int i = 0; i < NR; ++i) pos[i] = n0 + tl.depth[16 * i + lr];
+    tree_rows<16, kRowWaves * 64>(a, b, n0, r0, tl);
+    pos = n0 + tl.depth[lr];
   }
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    pmin = min(pmin, pos[i]);
-    pmax = max(pmax, pos[i]);
-  }
+  int pmin = pos, pmax = pos;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
     pmin = min(pmin, __shfl_xor(pmin, o));
     pmax = max(pmax, __shfl_xor(pmax, o));
   }
 
-  float mx[NR], ls[NR];
+  float mx = kNegInf, ls = 0.f;
   uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of
-  f32x4 acc[NR][DT];
+  f32x4 acc[DT];
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    mx[i] = kNegInf;
-    ls[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{};
-  }
+  for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
 
   const uint16_t* kbase = a.k + b * a.k_sb + kvh * a.k_sh + (lane % CH) * 8;
   const uint16_t* vbase = a.v + b * a.v_sb + kvh * a.v_sh + (lane % CH) * 8;
@@ -184,16 +171,14 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     for (int j = 0; j < NL; ++j)
       *reinterpret_cast<u32x4*>(mine + (j * KPI + lane / CH) * KST + (lane % CH) * 16) = kr[j];
     wave_lds_fence();
-    f32x4 s[NR][2];
+    f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < NR; ++i) s[i][h] = f32x4{};
+      s[h] = f32x4{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(mine + (16 * h + lr) * KST + (4 * ks + lg) * 16);
-#pragma unroll
-        for (int i = 0; i < NR; ++i) s[i][h] = mfma16<T>(kf, qf[i][ks], s[i][h]);
+        s[h] = mfma16<T>(kf, qf[ks], s[h]);
       }
     }
     wave_lds_fence();
@@ -210,37 +195,33 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     if (t + NW < t_end) load_tile(t + NW, pg);
     pg = tile_pages(t + 2 * NW);
     // ---- mask and softmax
-    u32x4 pf[NR];
+    if (masked) {
+      const uint32_t keep = keep_word(a, tl.vis + lr * kTreeMaxW, pos, kb, n0);
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      if (masked) {
-        const uint32_t keep = keep_word(a, tl.vis + (16 * i + lr) * kTreeMaxW, pos[i], kb, n0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!((keep >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[i][e >> 2][e & 3] = kNegInf;
-      }
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s[i][e >> 2][e & 3];
-      float mt = x[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
-      const float mn = fmaxf(mx[i], row_max(mt) * a.scale_log2);
-      if (__ballot(mn > mx[i]) != 0ull) {
-        const float al = mx[i] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mx[i] - mn);
-        ls[i] *= al;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[i][d] *= al;
-        mx[i] = mn;
-      }
-      const float ms = mx[i] == kNegInf ? 0.f : mx[i];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -ms));
-        ls[i] += x[e];
-      }
-      pf[i] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
+      for (int e = 0; e < 8; ++e)
+        if (!((keep >> (16 * (e >> 2) + 4 * lg + (e & 3))) & 1u)) s[e >> 2][e & 3] = kNegInf;
     }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3];
+    float mt = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
+    const float mn = fmaxf(mx, row_max(mt) * a.scale_log2);
+    if (__ballot(mn > mx) != 0ull) {
+      const float al = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+      ls *= al;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] *= al;
+      mx = mn;
+    }
+    const float ms = mx == kNegInf ? 0.f : mx;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -ms));
+      ls += x[e];
+    }
+    const u32x4 pf = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
     // ---- O^T += V^T . P^T; element e of lane group lg is key 16 (e / 4) + 4 lg + e % 4.
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -248,66 +229,61 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
       const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
       const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * VST)));
       const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-      for (int i = 0; i < NR; ++i) acc[i][d] = mfma16<T>(vf, pf[i], acc[i][d]);
+      acc[d] = mfma16<T>(vf, pf, acc[d]);
     }
     wave_lds_fence();
   }
 
   if (__syncthreads_or((int)(odd & 0x80008000u)) != 0) {
-    exact_rows<T, D, 16 * NR>(&args_again(), &tl, b, kvh, split, rb, (int)((int64_t)kl.nt * split / a.splits), t_end, wave, 16 * NR, NW);
+    exact_rows<T, D, 16>(&args_again(), &tl, b, kvh, split, rb, (int)((int64_t)kl.nt * split / a.splits), t_end, wave, 16, NW);
     return;
   }
-  // ---- the waves' rows joined, 16 at a time
+  // ---- the waves' rows joined
+  const float lt = row_sum(ls);
+  if (lg == 0) {
+    sm_m[wave][lr] = mx;
+    sm_l[wave][lr] = lt;
+  }
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const float lt = row_sum(ls[i]);
-    if (lg == 0) {
-      sm_m[wave][lr] = mx[i];
-      sm_l[wave][lr] = lt;
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(mine + lr * OST + (16 * d + 4 * lg) * 4) = acc[d];
+  __syncthreads();
+  constexpr int N = 4;  // elements per thread
+  constexpr int TPR = D / N;
+  const int rr = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N;
+  if (rr < 16) {
+    float m = sm_m[0][rr];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) m = fmaxf(m, sm_m[x][rr]);
+    const float ms = m == kNegInf ? 0.f : m;
+    float l = 0.f, o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      if (sm_l[x][rr] == 0.f) continue;  // a wave without a key of this row
+      const float f = __builtin_amdgcn_exp2f(sm_m[x][rr] - ms);
+      l += sm_l[x][rr] * f;
+      const f32x4* p = reinterpret_cast<const f32x4*>(smem + x * REGION + rr * OST + d0 * 4);
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] += p[e / 4][e % 4] * f;
     }
+    const int r = r0 + rr;
+    if (r < a.R) {
+      if (a.splits == 1) {
+        const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(mine + lr * OST + (16 * d + 4 * lg) * 4) = acc[i][d];
-    __syncthreads();
-    constexpr int N = 4;  // elements per thread
-    constexpr int TPR = D / N;
-    const int rr = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N;
-    if (rr < 16) {
-      float m = sm_m[0][rr];
+        for (int e = 0; e < N; ++e) o[e] *= inv;
+        store_out<N>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
+        if (d0 == 0 && a.lse != nullptr)
+          a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+      } else {
+        const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
 #pragma unroll
-      for (int x = 1; x < NW; ++x) m = fmaxf(m, sm_m[x][rr]);
-      const float ms = m == kNegInf ? 0.f : m;
-      float l = 0.f, o[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = 0.f;
-#pragma unroll
-      for (int x = 0; x < NW; ++x) {
-        if (sm_l[x][rr] == 0.f) continue;  // a wave without a key of this row
-        const float f = __builtin_amdgcn_exp2f(sm_m[x][rr] - ms);
-        l += sm_l[x][rr] * f;
-        const f32x4* p = reinterpret_cast<const f32x4*>(smem + x * REGION + rr * OST + d0 * 4);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] += p[e / 4][e % 4] * f;
-      }
-      const int r = r0 + 16 * i + rr;
-      if (r < a.R) {
-        if (a.splits == 1) {
-          const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-          for (int e = 0; e < N; ++e) o[e] *= inv;
-          store_out<N>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
-          if (d0 == 0 && a.lse != nullptr)
-            a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
-        } else {
-          const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
-#pragma unroll
-          for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(a.opart + pr * D + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
-          if (d0 == 0) a.ml[pr] = make_float2(m, l);
-        }
+        for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(a.opart + pr * D + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+        if (d0 == 0) a.ml[pr] = make_float2(m, l);
       }
     }
-    __syncthreads();
   }
 }
 
@@ -541,10 +517,7 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
 template <typename T, int D>
 hipError_t launch_rows(const WinArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), block(kRowWaves * 64);
-  if (a.rows_per_block == 16)
-    hipLaunchKernelGGL((win_rows_kernel<T, D, 1>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((win_rows_kernel<T, D, 2>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((win_rows_kernel<T, D>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
