@@ -1490,7 +1490,7 @@ int dsv_lmhead_accept(int mode, const dsv_tensor* hidden, const dsv_tensor* weig
 namespace {
 
 struct SpecPlan {
-  int nwg = 1, step = 0, step1 = 0;
+  int nwg = 1, own = 1, step = 0, step1 = 0;
   size_t state_bytes = 0, rej_bytes = 0, total = 0;
 };
 
@@ -1499,14 +1499,17 @@ struct SpecPlan {
 bool spec_plan(int64_t T, int64_t M, int64_t V, SpecPlan& p) {
   if (M < 1 || M > dsv::kSpecMaxM || T < 1 || T > (1 << 20) || V < 1 || V > 0x7fffffff) return false;
   const int64_t waves = dsv::kSpecThreads / 64, nseg = (V + dsv::kSpecSeg - 1) / dsv::kSpecSeg;
-  const int64_t most = std::min<int64_t>((nseg + waves - 1) / waves, dsv::kSpecSlots / waves);
+  const int64_t most = std::min<int64_t>((nseg + waves - 1) / waves, 64);
   p.nwg = (int)std::max<int64_t>(1, std::min(most, (int64_t)device_cus() / T));
-  p.step = (int)((nseg + waves * p.nwg - 1) / (waves * p.nwg));
+  // A wave's segments in up to 4 slots: the draw walks one slot again.
+  const int64_t each = (nseg + waves * p.nwg - 1) / (waves * p.nwg);
+  p.own = (int)std::min<int64_t>(each, dsv::kSpecSlots / waves);
+  p.step = (int)((each + p.own - 1) / p.own);
   p.step1 = (int)((nseg + waves - 1) / waves);
   if (p.nwg > 1) {
     p.state_bytes = align_up((size_t)T * sizeof(dsv::SpecState), 256);
     p.rej_bytes = align_up((size_t)T * M * sizeof(int32_t), 256);
-    p.total = p.state_bytes + p.rej_bytes + align_up((size_t)T * p.nwg * waves * sizeof(double), 256);
+    p.total = p.state_bytes + p.rej_bytes + align_up((size_t)T * p.nwg * waves * p.own * sizeof(double), 256);
   }
   return true;
 }
@@ -1609,6 +1612,7 @@ int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft, const dsv
   a.out_info = static_cast<int64_t*>(out_info->data);
   a.oi_st = out_info->stride[0];
   a.nwg = p.nwg;
+  a.own = p.own;
   a.step = p.step;
   a.step1 = p.step1;
   if (p.total > 0) {

@@ -209,7 +209,7 @@ struct BundleArgs {
 constexpr int kSpecMaxM = 1024;            // tree nodes
 constexpr int kSpecThreads = 1024;
 constexpr int kSpecSeg = 512;              // vocabulary entries a wave sums at a time
-constexpr int kSpecSlots = 4096;           // sums of a row at most (16 per workgroup)
+constexpr int kSpecSlots = 64;             // sums of a row per workgroup at most
 struct SpecState {
   double c;                                // share of the draft's row taken from the last node's
   int32_t node, nrej;                      // last node, rejected tokens listed in rej
@@ -227,10 +227,11 @@ struct SpecArgs {
   int64_t* out_tok; int64_t ot_st;
   int64_t* out_info; int64_t oi_st;
   int nwg;                                 // workgroups per tree
-  int step, step1;                         // segments per slot: of 16 nwg slots, of 16
+  int own, step;                           // slots per wave, segments per slot
+  int step1;                               // segments per wave of one workgroup
   SpecState* state;                        // nwg > 1: [T]
   int32_t* rej;                            // [T, M]
-  double* part;                            // [T, 16 nwg]
+  double* part;                            // [T, nwg, 16 own]
 };
 
 // Arguments of the page operations.  The bookkeeping of a pool lives on the

@@ -87,29 +87,13 @@ __device__ __forceinline__ double wave_scan(double x) {
   x += dpp<0x143, 0xc>(x);
   return x;
 }
-__device__ __forceinline__ double last_lane(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
-  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-}
 
-// The inclusive scan of x over the workgroup's NW waves, and its total.
-template <int NW>
-__device__ __forceinline__ double block_scan(double x, double* scratch, double& total) {
-  const double inc = wave_scan(x), all = last_lane(inc);
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[wave] = all;
-  __syncthreads();
-  total = 0.0;
-  double before = 0.0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    if (i == wave) before = total;
-    total += scratch[i];
-  }
-  return before + inc;
+// x of a lane that the wave agrees on.
+__device__ __forceinline__ double lane_of(double x, int l) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
 // What the remaining weights of a row are: max(p - c q, 0), or p without the
@@ -176,29 +160,31 @@ __device__ __forceinline__ void weights(const Rows<E>& r, const Piece<E, N, ROWS
   }
 }
 
-// The sums of the workgroup's 16 slots (step segments each, from slot first on)
-// into LDS, their total in every thread, in a fixed order.  Bound by its VALU operations where few trees share the GPU (a CU
-// issues one per SIMD and 4 cycles, 64-bit ones slower): the check for infinite
-// entries is one maximum over all of them, and the sweep runs again with the
-// full check only if there is one.
-template <typename E, bool Q, bool CHECK, int NW>
-__device__ __forceinline__ double sweep_as(const Rows<E>& r, int first, int step, double* sums) {
-  const int lane = threadIdx.x & 63;
+// The sums of the workgroup's 16 own slots (own per wave, step segments each, from
+// slot first on) into LDS, their total in every thread, in a fixed order.  Bound by
+// what the CU takes in and by its VALU operations (one per SIMD and 4 cycles,
+// 64-bit ones slower): the check for infinite entries is one maximum over all of
+// them, and the sweep runs again with the full check only if there is one.
+template <typename E, bool Q, bool CHECK>
+__device__ __forceinline__ double sweep_as(const Rows<E>& r, int first, int own, int step, double* sums) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   typedef Piece<E, kPer, true> Pc;
-  __syncthreads();
-  for (int slot = threadIdx.x >> 6; slot < kW; slot += NW) {
-    const int64_t w0 = ((int64_t)first + slot) * step * kSpecSeg, w1 = min(w0 + (int64_t)step * kSpecSeg, r.V);
-    double s0 = 0.0, s1 = 0.0;
-    float mx = 0.f;
-    Pc p, q, pn, qn;
-    auto fetch = [&](int64_t v, Pc& x, Pc& y) {
-      x.load(r.p, v, r.V);
-      if (Q && r.c != 0.0) y.load(r.q, v, r.V);
-    };
+  const int64_t w0 = ((int64_t)first + wave * own) * step * kSpecSeg;
+  const int64_t w1 = min(w0 + (int64_t)own * step * kSpecSeg, r.V);
+  float mx = 0.f;
+  Pc p, q, pn, qn;
+  auto fetch = [&](int64_t v, Pc& x, Pc& y) {
+    x.load(r.p, v, r.V);
+    if (Q && r.c != 0.0) y.load(r.q, v, r.V);
+  };
 #pragma unroll
-    for (int k = 0; k < Pc::NV; ++k) p.x[k] = pn.x[k] = q.x[k] = qn.x[k] = (E)0.f;
-    if (w0 < w1) fetch(w0, p, q);
-    for (int64_t v = w0; v < w1; v += kSpecSeg) {
+  for (int k = 0; k < Pc::NV; ++k) p.x[k] = pn.x[k] = q.x[k] = qn.x[k] = (E)0.f;
+  if (w0 < w1) fetch(w0, p, q);
+  __syncthreads();  // the sums before these have been read
+  int64_t v = w0;
+  for (int k = 0; k < own; ++k) {
+    double s0 = 0.0, s1 = 0.0;
+    for (int j = 0; j < step && v < w1; ++j, v += kSpecSeg) {
       if (v + kSpecSeg < w1) fetch(v + kSpecSeg, pn, qn);
       double w[kPer];
       weights<E, Q, CHECK, kPer, true>(r, p, q, v, w);
@@ -214,125 +200,112 @@ __device__ __forceinline__ double sweep_as(const Rows<E>& r, int first, int step
       p = pn;
       q = qn;
     }
-    const double s = last_lane(wave_scan(s0 + s1));
-    const bool inf = __ballot(mx == __builtin_huge_valf()) != 0ull;
-    if (lane == 0) sums[slot] = inf ? __builtin_huge_val() : s;  // (marked by an infinite sum)
+    const double s = lane_of(wave_scan(s0 + s1), 63);
+    if (lane == 0) sums[wave * own + k] = s;
   }
+  // (Infinite entries are marked by an infinite sum.)
+  const bool inf = __ballot(mx == __builtin_huge_valf()) != 0ull;
+  if (lane == 0 && inf) sums[wave * own] = __builtin_huge_val();
   __syncthreads();
-  double total = 0.0;
-#pragma unroll
-  for (int i = 0; i < kW; ++i) total += sums[i];
-  return total;
+  static_assert(kSpecSlots == 64, "a lane per slot at most");
+  return lane_of(wave_scan(lane < kW * own ? sums[lane] : 0.0), 63);
 }
 
-template <typename E, bool Q, int NW>
-__device__ __forceinline__ double sweep(const Rows<E>& r, int first, int step, double* sums) {
-  const double s = sweep_as<E, Q, false, NW>(r, first, step, sums);
-  return s < __builtin_huge_val() ? s : sweep_as<E, Q, true, NW>(r, first, step, sums);
+template <typename E, bool Q>
+__device__ __forceinline__ double sweep(const Rows<E>& r, int first, int own, int step, double* sums) {
+  const double s = sweep_as<E, Q, false>(r, first, own, step, sums);
+  return s < __builtin_huge_val() ? s : sweep_as<E, Q, true>(r, first, own, step, sums);
 }
 
 // The next token from the remaining weights, whose nslot sums of step segments
-// are in LDS: the first v whose cumulative weight exceeds u W, W the total (the
-// last one with a weight if rounding left none).  Where nothing is left of the
-// weights (the target never exceeds the draft's share, or all of it was
-// rejected) it is drawn from the target's own row, and it is 0 if that has no
-// weight either.  NW waves.
-template <typename E, bool Q, int NW>
-__device__ __forceinline__ int64_t next_token(Rows<E> r, int nslot, int step, int step1, double u, double* sums,
-                                              double* scratch, int32_t* found, double* base_s) {
-  constexpr int N = 8, NT = NW * 64;  // entries per thread and round
-  double W, run;
-  int per;
-  for (int again = 0;; ++again) {
-    per = (nslot + NT - 1) / NT;
-    double mine = 0.0;
-    for (int k = 0; k < per; ++k) {
-      const int i = threadIdx.x * per + k;
-      mine += i < nslot ? sums[i] : 0.0;
-    }
-    run = block_scan<NW>(mine, scratch, W) - mine;
-    if (W > 0.0) break;
-    if (again != 0) return 0;
-    r.c = 0.0;
-    r.nrej = 0;
-    nslot = kW;
-    step = step1;
-    sweep<E, Q, NW>(r, 0, step, sums);
-  }
+// are given (in LDS or memory): the first v whose cumulative weight exceeds u W,
+// W the total (the last one with a weight if rounding left none); -1 if W is 0.
+// One wave: no barriers, and little code, which a kernel of this length fetches
+// from memory line by line (by 4 waves with block scans it took 7 us, by 16 ten).
+template <typename E, bool Q>
+__device__ __forceinline__ int64_t draw(const Rows<E>& r, const double* sums, int nslot, int step, double u) {
+  const int lane = threadIdx.x & 63;
+  const int per = (nslot + 63) / 64;
+  double mine = 0.0;
+  for (int k = 0; k < per; ++k) mine += lane * per + k < nslot ? sums[lane * per + k] : 0.0;
+  double inc = wave_scan(mine);
+  const double W = lane_of(inc, 63);
+  if (!(W > 0.0)) return -1;
   const double tau = u * W;
-  if (threadIdx.x == 0) {
-    found[0] = 0x7fffffff;
-    found[1] = -1;
-  }
-  __syncthreads();
-  // The slot: the first whose end passes tau, else the last with a weight.
-  int hit = 0x7fffffff, last = -1;
-  double hit_at = 0.0, last_at = 0.0;
+  // The lane whose slots carry the cumulative weight past tau, then the slot.
+  uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && inc > tau);
+  int owner = past != 0 ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  double run = lane_of(inc - mine, owner), base = run;
+  int slot = 0;
   for (int k = 0; k < per; ++k) {
-    const int i = threadIdx.x * per + k;
-    const double own = i < nslot ? sums[i] : 0.0;
-    if (own > 0.0) {
-      last = i;
-      last_at = run;
-      if (run + own > tau && hit == 0x7fffffff) {
-        hit = i;
-        hit_at = run;
-      }
+    const int i = owner * per + k;
+    const double s = i < nslot ? sums[i] : 0.0;
+    if (s > 0.0) {
+      slot = i;
+      base = run;
+      if (run + s > tau) break;
     }
-    run += own;
+    run += s;
   }
-  if (hit != 0x7fffffff) atomicMin(&found[0], hit);
-  if (last >= 0) atomicMax(&found[1], last);
-  __syncthreads();
-  const int slot = found[0] != 0x7fffffff ? found[0] : found[1];
-  if (slot == hit)
-    *base_s = hit_at;
-  else if (slot == last)
-    *base_s = last_at;
-  __syncthreads();
-  double base = *base_s;
   int64_t tok = 0;
-  const int64_t v1 = (int64_t)(slot + 1) * step * kSpecSeg;
-  for (int64_t v0 = (int64_t)slot * step * kSpecSeg; v0 < v1 && v0 < r.V; v0 += (int64_t)NT * N) {
-    const int64_t v = v0 + (int64_t)threadIdx.x * N, vw = v0 + (int64_t)(threadIdx.x & ~63) * N;
-    typedef Piece<E, N, false> Pc;
+  const int64_t v1 = min((int64_t)(slot + 1) * step * kSpecSeg, r.V);
+  for (int64_t v = (int64_t)slot * step * kSpecSeg; v < v1; v += kSpecSeg) {
+    typedef Piece<E, kPer, false> Pc;
     Pc p, q;
 #pragma unroll
     for (int k = 0; k < Pc::NV; ++k) q.x[k] = (E)0.f;
-    p.load(r.p, vw, r.V);
-    if (Q && r.c != 0.0) q.load(r.q, vw, r.V);
-    double w[N], mine = 0.0, total;
-    weights<E, Q, true, N, false>(r, p, q, vw, w);
+    p.load(r.p, v, r.V);
+    if (Q && r.c != 0.0) q.load(r.q, v, r.V);
+    double w[kPer];
+    weights<E, Q, true, kPer, false>(r, p, q, v, w);
+    mine = 0.0;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if (v + e >= v1) w[e] = 0.0;  // the next slot's
-      mine += w[e];
-    }
-    double cum = base + (block_scan<NW>(mine, scratch, total) - mine);
-    if (threadIdx.x == 0) {
-      found[0] = 0x7fffffff;
-      found[1] = -1;
-    }
-    __syncthreads();
-    hit = 0x7fffffff;
-    last = -1;
+    for (int e = 0; e < kPer; ++e) mine += w[e];
+    inc = wave_scan(mine);
+    some = __ballot(mine > 0.0);
+    past = __ballot(mine > 0.0 && base + inc > tau);
+    if (some != 0) {
+      owner = past != 0 ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+      // The owner's entry, in every lane for its own.
+      double cum = base + (inc - mine);
+      int at = 0;
+      bool done = false;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      cum += w[e];
-      if (w[e] > 0.0) {
-        last = threadIdx.x * N + e;
-        if (cum > tau && hit == 0x7fffffff) hit = last;
+      for (int e = 0; e < kPer; ++e) {
+        cum += w[e];
+        if (w[e] > 0.0 && !done) {
+          at = e;
+          done = cum > tau;
+        }
       }
+      tok = v + owner * kPer + __builtin_amdgcn_readlane(at, owner);
+      if (past != 0) return tok;
     }
-    if (hit != 0x7fffffff) atomicMin(&found[0], hit);
-    if (last >= 0) atomicMax(&found[1], last);
-    __syncthreads();
-    if (found[0] != 0x7fffffff) return v0 + found[0];
-    if (found[1] >= 0) tok = v0 + found[1];
-    base += total;
-    __syncthreads();
+    base += lane_of(inc, 63);
   }
   return tok;
+}
+
+// Where nothing is left of the weights (the target never exceeds the draft's
+// share, or all of it was rejected) the token is drawn from the target's own
+// row, and it is 0 if that has no weight either.  One wave, any waves beside it.
+template <typename E>
+__device__ __noinline__ int64_t draw_row(const E* p, int64_t V, double u) {
+  const Rows<E> r{p, nullptr, 0.0, nullptr, 0, V};
+  double W = 0.0;
+  for (int64_t v = 0; v < V; v += kSpecSeg) {
+    Piece<E, kPer, false> x;
+    x.load(p, v, V);
+    double w[kPer], mine = 0.0;
+    weights<E, false, true, kPer, false>(r, x, x, v, w);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) mine += w[e];
+    W += lane_of(wave_scan(mine), 63);
+  }
+  const int64_t nseg = (V + kSpecSeg - 1) / kSpecSeg;
+  if (!(W > 0.0)) return 0;
+  const int64_t t = draw<E, false>(r, &W, 1, (int)nseg, u);
+  return t < 0 ? 0 : t;
 }
 
 struct Walk {
@@ -351,8 +324,7 @@ __global__ void __launch_bounds__(kT) spec_kernel(const SpecArgs a) {
   __shared__ int32_t par[kSpecMaxM], tok[kSpecMaxM], rej[kSpecMaxM];
   __shared__ float px[kSpecMaxM], qx[kSpecMaxM], un[kSpecMaxM];
   __shared__ int16_t path[kSpecMaxM];
-  __shared__ double sums[kW], scratch[kW], base_s;
-  __shared__ int32_t found[2];
+  __shared__ double sums[kSpecSlots];
   __shared__ Walk wk;
   const E* P = reinterpret_cast<const E*>(a.target) + (int64_t)t * a.t_st;
   const E* Dp = Q ? reinterpret_cast<const E*>(a.dprobs) + (int64_t)t * a.q_st : nullptr;
@@ -445,7 +417,7 @@ __global__ void __launch_bounds__(kT) spec_kernel(const SpecArgs a) {
     if (!Q || wk.sweep == 0) break;
     if constexpr (Q) {
       const Rows<E> r{P + (int64_t)wk.node * a.t_sm, Dp + (int64_t)wk.node * a.q_sm, wk.c, rej, 0, V};
-      const double s = sweep<E, Q, kW>(r, 0, a.step1, sums);
+      const double s = sweep<E, Q>(r, 0, 1, a.step1, sums);
       if (threadIdx.x == 0) wk.mass = s;
       __syncthreads();
     }
@@ -467,13 +439,16 @@ __global__ void __launch_bounds__(kT) spec_kernel(const SpecArgs a) {
   }
   // The last node's remaining weights.
   Rows<E> r{P + (int64_t)node * a.t_sm, Q ? Dp + (int64_t)node * a.q_sm : nullptr, wk.c, rej, nrej, V};
-  sweep<E, Q, kW>(r, wg * kW, a.step, sums);
+  const int nsum = kW * a.own;
+  sweep<E, Q>(r, wg * nsum, a.own, a.step, sums);
   if (a.nwg == 1) {
-    const int64_t tok = next_token<E, Q, kW>(r, kW, a.step, a.step1, unit(un[0]), sums, scratch, found, &base_s);
+    if (threadIdx.x >= 64) return;
+    int64_t tok = draw<E, Q>(r, sums, nsum, a.step, unit(un[0]));
+    if (tok < 0) tok = draw_row<E>(r.p, V, unit(un[0]));
     if (threadIdx.x == 0) info[2] = tok;
     return;
   }
-  if (threadIdx.x < kW) a.part[((int64_t)t * a.nwg + wg) * kW + threadIdx.x] = sums[threadIdx.x];
+  if (threadIdx.x < nsum) a.part[((int64_t)t * a.nwg + wg) * nsum + threadIdx.x] = sums[threadIdx.x];
   if (wg == 0) {
     if (threadIdx.x == 0) a.state[t] = SpecState{wk.c, node, nrej};
     for (int i = threadIdx.x; i < nrej; i += kT) a.rej[(int64_t)t * M + i] = rej[i];
@@ -481,20 +456,16 @@ __global__ void __launch_bounds__(kT) spec_kernel(const SpecArgs a) {
 }
 
 // The draw from the sums that a tree's workgroups left.
-constexpr int kDW = 4;  // waves
 template <typename E, bool Q>
-__global__ void __launch_bounds__(kDW * 64) spec_draw_kernel(const SpecArgs a) {
-  const int t = blockIdx.x, nslot = a.nwg * kW;
-  __shared__ double sums[kSpecSlots], scratch[kDW], base_s;
-  __shared__ int32_t found[2];
-  for (int i = threadIdx.x; i < nslot; i += kDW * 64) sums[i] = a.part[(int64_t)t * nslot + i];
+__global__ void __launch_bounds__(64) spec_draw_kernel(const SpecArgs a) {
+  const int t = blockIdx.x, nslot = a.nwg * kW * a.own;
   const SpecState st = a.state[t];
   const double u = unit(a.uniform[(int64_t)t * a.u_st]);
   const Rows<E> r{reinterpret_cast<const E*>(a.target) + (int64_t)t * a.t_st + (int64_t)st.node * a.t_sm,
                   Q ? reinterpret_cast<const E*>(a.dprobs) + (int64_t)t * a.q_st + (int64_t)st.node * a.q_sm : nullptr,
                   st.c, a.rej + (int64_t)t * a.M, st.nrej, a.V};
-  __syncthreads();
-  const int64_t tok = next_token<E, Q, kDW>(r, nslot, a.step, a.step1, u, sums, scratch, found, &base_s);
+  int64_t tok = draw<E, Q>(r, a.part + (int64_t)t * nslot, nslot, a.step, u);
+  if (tok < 0) tok = draw_row<E>(r.p, a.V, u);
   if (threadIdx.x == 0) a.out_info[(int64_t)t * a.oi_st + 2] = tok;
 }
 
@@ -503,7 +474,7 @@ hipError_t launch_q(const SpecArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((spec_kernel<E, Q>), dim3((unsigned)(a.T * a.nwg)), dim3(kT), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nwg == 1) return e;
-  hipLaunchKernelGGL((spec_draw_kernel<E, Q>), dim3((unsigned)a.T), dim3(kDW * 64), 0, s, a);
+  hipLaunchKernelGGL((spec_draw_kernel<E, Q>), dim3((unsigned)a.T), dim3(64), 0, s, a);
   return hipGetLastError();
 }
 
