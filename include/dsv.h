@@ -558,7 +558,8 @@ size_t dsv_pages_workspace_bytes(int64_t P, int64_t B, int64_t n);
  * Sequence children[i] becomes a continuation of parents[i]: whole pages are
  * shared, a partly filled last page is copied into a page of the child's own
  * (every layer, K and V, the whole page).  Refused: indices out of range,
- * parent == child, a child that is not empty (seqlens != 0), is named twice or
+ * parent == child, a child that is not empty (seqlens != 0; its table row is
+ * overwritten, so free it first), is named twice or
  * is a parent of the same call, a parent longer than its table row.
  *   parents, children  [n] int32|int64
  */
@@ -570,9 +571,11 @@ int dsv_pages_fork(const dsv_tensor* kv_pages, const dsv_tensor* page_table,
 
 /*
  * Sequences grow to new_lens [B] int32|int64 tokens (shorter or equal ones
- * stay as they are): table entries up to the last page of the new length
- * receive free pages, seqlens the new length.  Refused: new lengths beyond the
- * table row, negative seqlens.  The new tokens' contents are the caller's.
+ * stay as they are): the table entries behind the present length and up to the
+ * last page of the new one that name no page receive free pages, seqlens the new
+ * length.  (Entries that name one keep it: seqlens may be set back after drafted
+ * tokens were rejected.)  Refused: new lengths beyond the table row, negative
+ * seqlens.  The new tokens' contents are the caller's.
  */
 int dsv_pages_extend(const dsv_tensor* page_table, const dsv_tensor* refcount,
                      const dsv_tensor* seqlens, const dsv_tensor* new_lens,

@@ -56,7 +56,7 @@ def extend(table: List[List[int]], ref: List[int], lens: List[int], new: Sequenc
     bad = sum(1 for b in grow if lens[b] < 0 or new[b] > n_log * ps)
     if bad:
         return 0, 0, bad
-    slots = [(b, j) for b in grow for j in range(-(-lens[b] // ps), -(-new[b] // ps))]
+    slots = [(b, j) for b in grow for j in range(-(-lens[b] // ps), -(-new[b] // ps)) if not 0 <= table[b][j] < len(ref)]
     free = [p for p in range(len(ref)) if ref[p] == 0]
     if len(free) < len(slots):
         return 0, len(slots) - len(free), 0

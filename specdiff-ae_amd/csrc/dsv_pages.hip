@@ -279,26 +279,60 @@ __global__ void __launch_bounds__(kCopyT) fork_kernel(const ForkArgs a, int64_t 
 
 // ---- extend ----------------------------------------------------------------
 
+// Pages that a sequence's row already names behind its tokens stay its own (those
+// of drafted tokens that were rejected); the missing ones are taken.
 __global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
   __shared__ int64_t scratch[kPW];
   __shared__ int32_t cnt[257];
-  __shared__ int32_t bad;
+  __shared__ int32_t bad, many;
   const PageBook& b = a.book;
   const int64_t ps = 1ll << b.ps_shift;
-  if (threadIdx.x == 0) bad = 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) bad = many = 0;
   __syncthreads();
   auto pages_of = [&](int64_t n) { return (n >> b.ps_shift) + ((n & (ps - 1)) != 0 ? 1 : 0); };
-  int64_t want = 0;
+  auto missing = [&](int64_t i, int64_t j) {
+    const int32_t page = b.table[i * b.t_sb + j];
+    return page < 0 || page >= b.P;
+  };
+  // Which of up to kFewPages entries from lo on are missing.
+  auto missing_few = [&](int64_t i, int64_t lo, int n) {
+    int32_t page[kFewPages];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < kFewPages; ++j) page[j] = j < n ? b.table[i * b.t_sb + lo + j] : 0;
+#pragma unroll
+    for (int j = 0; j < kFewPages; ++j) bits |= (page[j] < 0 || page[j] >= b.P ? 1u : 0u) << j;
+    return bits;
+  };
+  // The pages that sequences lack: a thread counts a few, a wave many.
+  int64_t want = 0, lo = 0, hi = 0;
+  uint32_t few = 0;
   for (int64_t i0 = 0; i0 < b.B; i0 += kPT) {
     const int64_t i = i0 + threadIdx.x;
-    int64_t need = 0;
+    lo = hi = 0;
     if (i < b.B) {
       const int64_t len = seqlen(b, i), n = get(a.newlens, i);
       if (n > len) {
-        if (len < 0 || n > b.n_log * ps)
+        if (len < 0 || n > b.n_log * ps) {
           atomicAdd(&bad, 1);
-        else
-          need = pages_of(n) - pages_of(len);
+        } else {
+          lo = pages_of(len);
+          hi = pages_of(n);
+        }
+      }
+    }
+    const bool is_many = hi - lo > kFewPages;
+    few = is_many ? 0u : missing_few(i, lo, (int)(hi - lo));
+    int64_t need = __builtin_popcount(few);
+    if (__syncthreads_or(is_many) != 0) {
+      if (threadIdx.x == 0) many = 1;
+      for (uint64_t left = __ballot(is_many); left != 0; left &= left - 1) {
+        const int src = __builtin_ctzll(left);
+        const int64_t l = __shfl((long long)lo, src), h = __shfl((long long)hi, src), s = __shfl((long long)i, src);
+        int found = 0;
+        for (int64_t j = l + lane; j - lane < h; j += 64) found += __builtin_popcountll(__ballot(j < h && missing(s, j)));
+        if (lane == src) need = found;
       }
     }
     int64_t total;
@@ -322,39 +356,47 @@ __global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
     a.info[2] = refused;
   }
   if (!go) return;
-  // A thread per sequence for a few pages, then a wave per sequence for many.
-  __shared__ int32_t many;
-  if (threadIdx.x == 0) many = 0;
-  __syncthreads();
+  const bool again = b.B > kPT;  // (else lo, hi and few are this thread's sequence's)
   for (int64_t i = threadIdx.x; i < b.B; i += kPT) {
-    const int64_t len = seqlen(b, i), n = get(a.newlens, i);
-    if (n <= len) continue;
-    const int64_t have = pages_of(len), need = pages_of(n) - have, at = a.off[i];
-    if (need > kFewPages) {
-      many = 1;
-      continue;
+    const int64_t n = get(a.newlens, i);
+    if (again) {
+      const int64_t len = seqlen(b, i);
+      lo = n > len ? pages_of(len) : 0;
+      hi = n > len ? pages_of(n) : 0;
+      few = hi - lo > kFewPages ? 0u : missing_few(i, lo, (int)(hi - lo));
     }
-    for (int j = 0; j < (int)need; ++j) {
-      const int32_t page = a.list[at + j];
-      b.table[i * b.t_sb + have + j] = page;
-      b.ref[page] = 1;
+    if (hi - lo > kFewPages) continue;
+    int64_t at = a.off[i];
+#pragma unroll
+    for (int j = 0; j < kFewPages; ++j) {
+      if ((few >> j) & 1u) {
+        const int32_t page = a.list[at++];
+        b.table[i * b.t_sb + lo + j] = page;
+        b.ref[page] = 1;
+      }
     }
-    set_seqlen(b, i, n);
+    if (n > seqlen(b, i)) set_seqlen(b, i, n);
   }
   __syncthreads();
   if (many == 0) return;
-  for (int64_t i = threadIdx.x >> 6; i < b.B; i += kPW) {
+  for (int64_t i = wave; i < b.B; i += kPW) {
     const int64_t len = seqlen(b, i), n = get(a.newlens, i);
     if (n <= len) continue;  // (those done above among them)
-    const int64_t have = pages_of(len), need = pages_of(n) - have, at = a.off[i];
-    for (int64_t j = threadIdx.x & 63; j < need; j += 64) {
-      const int32_t page = a.list[at + j];
-      b.table[i * b.t_sb + have + j] = page;
-      b.ref[page] = 1;
+    const int64_t l = pages_of(len), h = pages_of(n);
+    int64_t at = a.off[i];
+    for (int64_t j = l + lane; j - lane < h; j += 64) {
+      const bool take = j < h && missing(i, j);
+      const uint64_t all = __ballot(take);
+      if (take) {
+        const int32_t page = a.list[at + __builtin_popcountll(all & ((1ull << lane) - 1ull))];
+        b.table[i * b.t_sb + j] = page;
+        b.ref[page] = 1;
+      }
+      at += __builtin_popcountll(all);
     }
     // Every lane has read the length before it changes.
     __builtin_amdgcn_wave_barrier();
-    if ((threadIdx.x & 63) == 0) set_seqlen(b, i, n);
+    if (lane == 0) set_seqlen(b, i, n);
   }
 }
 

@@ -41,8 +41,8 @@ def fork_pages(kv_pages: torch.Tensor, page_table: torch.Tensor, refcount: torch
     Whole pages are shared (their counts grow); a partly filled last page is
     copied, in every layer, into a page of the child's own.  A parent may be
     named several times.  Refused (and then nothing is done): indices out of
-    range, a child that is not empty (``seqlens != 0``), that is named twice or
-    that is a parent of the same call.
+    range, a child that is not empty (``seqlens != 0``; its row is overwritten, so
+    free it first), that is named twice or that is a parent of the same call.
 
     Returns the int32 [3] tensor (pages taken, pages lacking, pairs refused).
     """
@@ -61,6 +61,10 @@ def fork_pages(kv_pages: torch.Tensor, page_table: torch.Tensor, refcount: torch
 def extend_pages(page_table: torch.Tensor, refcount: torch.Tensor, seqlens: torch.Tensor, new_lens: torch.Tensor,
                  page_size: int) -> torch.Tensor:
     """Grow sequences to ``new_lens`` [B] tokens; shorter or equal lengths change nothing.
+
+    Pages that a sequence's row already names behind its ``seqlens`` are used
+    before any is taken: a caller may set ``seqlens`` back after drafted tokens
+    were rejected, and the next draft finds their pages.
 
     Returns the int32 [3] tensor (pages taken, pages lacking, sequences refused:
     new lengths that the table row cannot hold).

@@ -72,6 +72,23 @@ def test_fork_extend_free(gpu):
     assert sum(p.ref) == 0
 
 
+@pytest.mark.parametrize("B", [5, 1100])
+def test_extend_keeps_pages_behind_the_length(gpu, B):
+    """Lengths set back after rejected tokens: their pages are used again, none is lost."""
+    p = Pool(gpu, B=B, P=30 * B, n_log=80, L=1, Hk=1, lens=torch.int64)
+    rng = random.Random(B)
+    for _ in range(4):
+        p.extend([min(320, n + rng.choice([0, 1, 3, 30, 33, 100])) for n in p.lens])
+        p.free([rng.randrange(B) for _ in range(B // 3)], window=9, sinks=2)
+        for b in range(B):
+            p.lens[b] = rng.randint(0, p.lens[b]) if p.lens[b] and rng.random() < 0.5 else p.lens[b]
+        p.dlens.copy_(torch.tensor(p.lens))
+        assert sum(x >= 0 for row in p.table for x in row) == sum(p.ref)
+        p.same()
+    p.free(list(range(B)))
+    assert sum(p.ref) == 0
+
+
 def test_nothing_happens_without_enough_pages(gpu):
     p = Pool(gpu, B=5, P=6, n_log=8)
     p.extend([9, 9, 0, 0, 0])
