@@ -27,8 +27,7 @@ namespace {
 
 constexpr int kPT = kPlanThreads;
 constexpr int kPW = kPT / 64;       // waves of the planning workgroup
-constexpr int kScanK = 16;          // entries per thread and scan step
-constexpr int kScanStep = kPT * kScanK;
+constexpr int kScanStep = 4 * kPT;  // pages of a scan step
 constexpr int kFewPages = 8;        // pages that one thread hands to a sequence
 
 __device__ __forceinline__ int64_t get(const PageIndex& x, int64_t i) {
@@ -45,20 +44,31 @@ __device__ __forceinline__ void set_seqlen(const PageBook& b, int64_t i, int64_t
     reinterpret_cast<int32_t*>(b.lens)[i] = (int32_t)n;
 }
 
+// x of the lane that DPP control CTRL names, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp(int64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)x >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
 // Exclusive scan of one value per thread over the planning workgroup.
 __device__ __forceinline__ int64_t scan1(int64_t x, int64_t* scratch, int64_t& total) {
+  // Shifts by 1, 2, 4, 8 inside the rows of 16, then the last lanes of rows 0 and
+  // 2, then of row 1, handed on.
   int64_t inc = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(inc, o);
-    if ((int)(threadIdx.x & 63) >= o) inc += y;
-  }
+  inc += dpp<0x111, 0xf>(inc);
+  inc += dpp<0x112, 0xf>(inc);
+  inc += dpp<0x114, 0xf>(inc);
+  inc += dpp<0x118, 0xf>(inc);
+  inc += dpp<0x142, 0xa>(inc);
+  inc += dpp<0x143, 0xc>(inc);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = inc;
   __syncthreads();
   int64_t before = 0;
   total = 0;
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < kPW; ++i) {
     if (i == (int)(threadIdx.x >> 6)) before = total;
     total += scratch[i];
@@ -66,65 +76,58 @@ __device__ __forceinline__ int64_t scan1(int64_t x, int64_t* scratch, int64_t& t
   return before + inc - x;
 }
 
-// Visits the entries of [lo, hi) that satisfy pred in ascending order: each
-// calls emit(index, rank), rank counted from 0; stops after the step in which
-// `limit` were found.  Returns how many were found (more than limit possible).
-// Entry lo + step * kScanStep + k * kPT + tid belongs to thread tid, so loads
-// are whole lines; a step is one round of 16 loads in flight.
+// The counts of this thread's four pages of the scan step at s0 (0 behind the pool).
+typedef int32_t i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ i32x4 refs_at(const PageBook& b, int64_t s0) {
+  const int64_t i = s0 + 4 * (int)threadIdx.x;
+  if (i + 4 <= b.P) return *reinterpret_cast<const i32x4*>(b.ref + i);
+  i32x4 r = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (i + e < b.P) r[e] = b.ref[i + e];
+  return r;
+}
+
+// Visits the pages of [lo, hi) whose number and count satisfy pred in ascending
+// order: each calls emit(index, rank), rank counted from 0; stops after the step
+// in which `limit` were found.  Returns how many were found (more than limit
+// possible).  Steps start at multiples of kScanStep; `first` holds the counts of
+// the first one, read once for all of a plan's scans.  What a plan of a few
+// hundred pages takes is mostly the fetching of its code from memory: four pages
+// a thread and loops that are not unrolled (16 a thread, unrolled: 2 to 4 times the
+// code; compact's plan of 2048 pages took 10 us, so 7).
 template <typename Pred, typename Emit>
-__device__ int64_t scan_entries(int64_t lo, int64_t hi, int64_t limit, int32_t* cnt, Pred pred, Emit emit) {
+__device__ __forceinline__ int64_t scan_pages(const PageBook& b, const i32x4& first, int64_t lo, int64_t hi, int64_t limit,
+                                              int32_t* cnt, Pred pred, Emit emit) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t below = (1ull << lane) - 1ull;
   int64_t found = 0;
-  for (int64_t s0 = lo; s0 < hi && found < limit; s0 += kScanStep) {
+#pragma unroll 1
+  for (int64_t s0 = lo - lo % kScanStep; s0 < hi && found < limit; s0 += kScanStep) {
+    const int64_t i = s0 + 4 * (int)threadIdx.x;
+    const i32x4 ref = s0 == 0 ? first : refs_at(b, s0);
     uint32_t bits = 0;
-    bool f[kScanK];
 #pragma unroll
-    for (int k = 0; k < kScanK; ++k) {
-      const int64_t i = s0 + k * kPT + threadIdx.x;
-      f[k] = i < hi && pred(i);
-    }
-    uint64_t mask[kScanK];
-#pragma unroll
-    for (int k = 0; k < kScanK; ++k) {
-      mask[k] = __ballot(f[k]);
-      bits |= (f[k] ? 1u : 0u) << k;
-    }
+    for (int e = 0; e < 4; ++e)
+      if (i + e >= lo && i + e < hi && pred(i + e, ref[e])) bits |= 1u << e;
+    // The number of entries before this thread's, from the bits of the numbers.
+    const int n = __builtin_popcount(bits);
+    const uint64_t b0 = __ballot(n & 1), b1 = __ballot(n & 2), b2 = __ballot(n & 4);
     __syncthreads();  // the previous step's counts have been read
-    if (lane == 0) {
-#pragma unroll
-      for (int k = 0; k < kScanK; ++k) cnt[k * kPW + wave] = __builtin_popcountll(mask[k]);
-    }
+    if (lane == 0) cnt[wave] = __builtin_popcountll(b0) + 2 * __builtin_popcountll(b1) + 4 * __builtin_popcountll(b2);
     __syncthreads();
-    // Exclusive scan of the kScanK * kPW counts by wave 0, four a lane.
-    static_assert(kScanK * kPW == 256, "four counts a lane");
-    if (wave == 0) {
-      int v[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = cnt[lane * 4 + e];
-        sum += v[e];
-      }
-      int inc = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(inc, o);
-        if (lane >= o) inc += y;
-      }
-      int run = inc - sum;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        cnt[lane * 4 + e] = run;
-        run += v[e];
-      }
-      if (lane == 63) cnt[256] = inc;
+    int before = __builtin_popcountll(b0 & below) + 2 * __builtin_popcountll(b1 & below) + 4 * __builtin_popcountll(b2 & below);
+    int all = 0;
+#pragma unroll 1
+    for (int w = 0; w < kPW; ++w) {
+      before += w < wave ? cnt[w] : 0;
+      all += cnt[w];
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kScanK; ++k)
-      if ((bits >> k) & 1u)
-        emit(s0 + k * kPT + threadIdx.x,
-             found + cnt[k * kPW + wave] + __builtin_popcountll(mask[k] & ((1ull << lane) - 1ull)));
-    found += cnt[256];
+    int64_t at = found + before;
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e)
+      if ((bits >> e) & 1u) emit(i + e, at++);
+    found += all;
   }
   return found;
 }
@@ -180,9 +183,10 @@ __device__ __forceinline__ void copy_pages(const PageData& d, const int32_t* src
 __global__ void __launch_bounds__(kPT) fork_plan_kernel(const ForkArgs a) {
   __shared__ uint32_t is_child[kPageMaxSeqs / 32], is_parent[kPageMaxSeqs / 32];
   __shared__ int64_t scratch[kPW];
-  __shared__ int32_t cnt[257];
+  __shared__ int32_t cnt[kPW];
   __shared__ int32_t bad;
   const PageBook& b = a.book;
+  const i32x4 first = refs_at(b, 0);
   const int64_t ps = 1ll << b.ps_shift;
   for (int64_t i = threadIdx.x; i < (b.B + 31) / 32; i += kPT) is_child[i] = is_parent[i] = 0;
   if (threadIdx.x == 0) bad = 0;
@@ -230,8 +234,8 @@ __global__ void __launch_bounds__(kPT) fork_plan_kernel(const ForkArgs a) {
   }
   // list[rank] = page, kept behind the pairs.
   int32_t* list = a.dst + a.n;
-  const int64_t found = scan_entries(
-      0, b.P, want, cnt, [&](int64_t i) { return b.ref[i] == 0; },
+  const int64_t found = scan_pages(
+      b, first, 0, b.P, want, cnt, [](int64_t, int32_t ref) { return ref == 0; },
       [&](int64_t i, int64_t r) {
         if (r < want) list[r] = (int32_t)i;
       });
@@ -283,10 +287,11 @@ __global__ void __launch_bounds__(kCopyT) fork_kernel(const ForkArgs a, int64_t 
 // of drafted tokens that were rejected); the missing ones are taken.
 __global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
   __shared__ int64_t scratch[kPW];
-  __shared__ int32_t cnt[257];
+  __shared__ int32_t cnt[kPW];
   __shared__ int32_t bad, many;
   const PageBook& b = a.book;
   const int64_t ps = 1ll << b.ps_shift;
+  const i32x4 first = refs_at(b, 0);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) bad = many = 0;
   __syncthreads();
@@ -343,8 +348,8 @@ __global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
   __syncthreads();
   const int refused = bad;
   const int64_t limit = refused == 0 ? want : 0;
-  const int64_t found = scan_entries(
-      0, b.P, limit, cnt, [&](int64_t i) { return b.ref[i] == 0; },
+  const int64_t found = scan_pages(
+      b, first, 0, b.P, limit, cnt, [](int64_t, int32_t ref) { return ref == 0; },
       [&](int64_t i, int64_t r) {
         if (r < limit) a.list[r] = (int32_t)i;
       });
@@ -367,13 +372,11 @@ __global__ void __launch_bounds__(kPT) extend_kernel(const ExtendArgs a) {
     }
     if (hi - lo > kFewPages) continue;
     int64_t at = a.off[i];
-#pragma unroll
-    for (int j = 0; j < kFewPages; ++j) {
-      if ((few >> j) & 1u) {
-        const int32_t page = a.list[at++];
-        b.table[i * b.t_sb + lo + j] = page;
-        b.ref[page] = 1;
-      }
+#pragma unroll 1
+    for (uint32_t left = few; left != 0; left &= left - 1) {
+      const int32_t page = a.list[at++];
+      b.table[i * b.t_sb + lo + __builtin_ctz(left)] = page;
+      b.ref[page] = 1;
     }
     if (n > seqlen(b, i)) set_seqlen(b, i, n);
   }
@@ -427,28 +430,25 @@ __global__ void __launch_bounds__(256) free_kernel(const FreeArgs a) {
 // free pages below n.
 __global__ void __launch_bounds__(kPT) compact_plan_kernel(const CompactArgs a) {
   __shared__ int64_t scratch[kPW];
-  __shared__ int32_t cnt[257];
+  __shared__ int32_t cnt[kPW];
   const PageBook& b = a.book;
+  const i32x4 first = refs_at(b, 0);
   int64_t mine = 0;
-  for (int64_t i0 = 0; i0 < b.P; i0 += kScanStep) {
-    int32_t v[kScanK];
+#pragma unroll 1
+  for (int64_t s0 = 0; s0 < b.P; s0 += kScanStep) {
+    const i32x4 ref = s0 == 0 ? first : refs_at(b, s0);
 #pragma unroll
-    for (int k = 0; k < kScanK; ++k) {
-      const int64_t i = i0 + k * kPT + threadIdx.x;
-      v[k] = i < b.P ? b.ref[i] : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < kScanK; ++k) mine += v[k] > 0 ? 1 : 0;
+    for (int e = 0; e < 4; ++e) mine += ref[e] > 0 ? 1 : 0;
   }
   int64_t n;
   scan1(mine, scratch, n);
-  const int64_t holes = scan_entries(
-      0, n, b.P, cnt, [&](int64_t i) { return b.ref[i] <= 0; }, [&](int64_t i, int64_t r) { a.dst[r] = (int32_t)i; });
-  const int64_t moved = scan_entries(
-      n, b.P, b.P, cnt,
-      [&](int64_t i) {
+  const int64_t holes = scan_pages(
+      b, first, 0, n, b.P, cnt, [](int64_t, int32_t ref) { return ref <= 0; }, [&](int64_t i, int64_t r) { a.dst[r] = (int32_t)i; });
+  const int64_t moved = scan_pages(
+      b, first, n, b.P, b.P, cnt,
+      [&](int64_t i, int32_t ref) {
         a.to[i] = (int32_t)i;
-        return b.ref[i] > 0;
+        return ref > 0;
       },
       [&](int64_t i, int64_t r) { a.src[r] = (int32_t)i; });
   (void)holes;  // equal: n pages are in use, those below n and the moved ones
