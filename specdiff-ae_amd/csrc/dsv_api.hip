@@ -1906,6 +1906,11 @@ WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
   const bool tile = dtype != DSV_F32 && R > 16 && !no_tile;
   p.rpb = tile ? 256 : 16;
   p.n_rb = (int)((R + p.rpb - 1) / p.rpb);
+  if (B * Hk * p.n_rb >= (1 << 23)) {
+    // (512 threads each; a launch counts fewer than 2^32.)
+    p.err = "batch x key heads x blocks of rows beyond 2^23 - 1";
+    return p;
+  }
   // Splits over the keys until there is a workgroup per CU, of 20 tiles at
   // least (8 waves, 2 to 3 tiles each): more splits cost more in the merge than
   // they gain (bf16, one sequence through 16384 keys: 16 splits 31 us, 32 splits

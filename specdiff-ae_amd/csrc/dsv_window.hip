@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     pos = n0 + row.m;
   }
   if (a.parent != nullptr) {
-    tree_rows<16, kRowWaves * 64>(a, b, n0, r0, tl);
+    tree_rows<16, kRowWaves * 64>(a, TreeParents<kRowWaves * 64>(a, b), n0, r0, tl);
     pos = n0 + tl.depth[lr];
   }
   int pmin = pos, pmax = pos;
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
   for (int c = 0; c < KC; ++c) qf[c] = *reinterpret_cast<const f32x4*>(q + 16 * c + 4 * lg);
   int pos = n0 + row.m;
   if (a.parent != nullptr) {
-    tree_rows<16, kRowWaves * 64>(a, b, n0, r0, tl);
+    tree_rows<16, kRowWaves * 64>(a, TreeParents<kRowWaves * 64>(a, b), n0, r0, tl);
     pos = n0 + tl.depth[lr];
   }
   int pmin = pos, pmax = pos;

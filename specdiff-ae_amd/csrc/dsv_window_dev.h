@@ -77,19 +77,42 @@ struct TreeLds {
   uint64_t vis[ROWS * kTreeMaxW];
 };
 
-// The walks, at most M steps each (a parent < 0, >= M or equal to the node ends
-// one, as in the tree split of dsv_attn.hip).  Every thread of the workgroup
-// calls it; ends with a barrier.
-template <int ROWS, int NT>
-__device__ __forceinline__ void tree_rows(const WinArgs& a, int b, int n0, int r0, TreeLds<ROWS>& t) {
-  const int M = a.M;
-  for (int i = threadIdx.x; i < M; i += NT) {
-    const int64_t o = b * a.par_sb + (int64_t)i * a.par_sm;
-    const int64_t x = a.par_i64 ? reinterpret_cast<const int64_t*>(a.parent)[o]
-                                : (int64_t) reinterpret_cast<const int32_t*>(a.parent)[o];
-    t.par[i] = x < 0 || x >= M || x == i ? (int16_t)-1 : (int16_t)x;
+// A barrier behind the waves' LDS operations alone: loads into LDS stay in flight.
+__device__ __forceinline__ void barrier_after_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// This thread's parents, of up to kTreeMaxM in the workgroup (a parent < 0, >= M or
+// equal to the node: -1); none for b < 0.
+template <int NT>
+struct TreeParents {
+  static constexpr int N = (kTreeMaxM + NT - 1) / NT;
+  int16_t p[N];
+  __device__ __forceinline__ TreeParents(const WinArgs& a, int b) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = k * NT + (int)threadIdx.x;
+      p[k] = -1;
+      if (b < 0 || i >= a.M) continue;
+      const int64_t o = b * a.par_sb + (int64_t)i * a.par_sm;
+      const int64_t x = a.par_i64 ? reinterpret_cast<const int64_t*>(a.parent)[o]
+                                  : (int64_t) reinterpret_cast<const int32_t*>(a.parent)[o];
+      if (x >= 0 && x < a.M && x != i) p[k] = (int16_t)x;
+    }
   }
-  __syncthreads();
+};
+
+// The walks, at most M steps each.  Every thread of the workgroup calls it; ends
+// with a barrier.
+template <int ROWS, int NT>
+__device__ __forceinline__ void tree_rows(const WinArgs& a, const TreeParents<NT>& mine, int n0, int r0, TreeLds<ROWS>& t) {
+  const int M = a.M;
+#pragma unroll
+  for (int k = 0; k < TreeParents<NT>::N; ++k)
+    if (k * NT + (int)threadIdx.x < M) t.par[k * NT + threadIdx.x] = mine.p[k];
+  barrier_after_lds();
   if (threadIdx.x < ROWS) {
     const int m = min(r0 + (int)threadIdx.x, a.R - 1) / a.G;
     uint64_t* vis = t.vis + threadIdx.x * kTreeMaxW;
@@ -115,7 +138,7 @@ __device__ __forceinline__ void tree_rows(const WinArgs& a, int b, int n0, int r
         if (n0 + depth - h < a.S) vis[x >> 6] |= 1ull << (x & 63);
     }
   }
-  __syncthreads();
+  barrier_after_lds();
 }
 
 // The keep word of a row at position pos for the tile at key kb: bit i = key

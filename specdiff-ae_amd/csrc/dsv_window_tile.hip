@@ -125,18 +125,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + ks * 16);
   }
-  if (tree) {
-    tree_rows<256, 512>(a, b, n0, rb * 256, tl);
-    pos = n0 + tl.depth[wid * 32 + lj];
-  }
-  int pmin = pos, pmax = pos;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    pmin = min(pmin, __shfl_xor(pmin, o));
-    pmax = max(pmax, __shfl_xor(pmax, o));
-  }
-  pmin = uniform(pmin);
-  pmax = uniform(pmax);
+  const TreeParents<512> parents(a, tree ? b : -1);
 
   // ---- DMA of one tile into its ring stage --------------------------------------
   // Instruction x of this wave covers keys [j*KPI, (j+1)*KPI) of the tile's K
@@ -249,15 +238,9 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       vf[hh][dt] = u32x4{l2[0], l2[1], h2[0], h2[1]};
     }
   };
-  // The tiles [seen0, seen1) are seen whole by every row of the wave (others may be).
-  int seen0 = 0, seen1 = 0;
-  {
-    const int first = pmax - a.W + 1, last = tree ? n0 : pmin + 1;  // keys [first, last)
-    seen0 = kl.nst + max((first - kl.lo_al + 31) >> 5, 0) - t_lo;
-    seen1 = kl.nst + ((last - kl.lo_al) >> 5) - t_lo;
-  }
-
   const float scale_log2 = a.scale_log2;
+
+  int pmin = pos, pmax = pos;  // of the wave's rows
 
   auto step = [&](auto masked_c, int k) {
     constexpr bool MASKED = decltype(masked_c)::value;
@@ -345,6 +328,26 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   if (ntiles > 0) issue_tile(0);
   if (ntiles > 1) issue_tile(1);
   if (ntiles > 2 && !v_wave) issue_tile(2);
+  // The tree is walked while the first tiles come in.
+  if (tree) {
+    tree_rows<256, 512>(a, parents, n0, rb * 256, tl);
+    pos = n0 + tl.depth[wid * 32 + lj];
+  }
+  pmin = pmax = pos;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    pmin = min(pmin, __shfl_xor(pmin, o));
+    pmax = max(pmax, __shfl_xor(pmax, o));
+  }
+  pmin = uniform(pmin);
+  pmax = uniform(pmax);
+  // The tiles [seen0, seen1) are seen whole by every row of the wave (others may be).
+  int seen0 = 0, seen1 = 0;
+  {
+    const int first = pmax - a.W + 1, last = tree ? n0 : pmin + 1;  // keys [first, last)
+    seen0 = kl.nst + max((first - kl.lo_al + 31) >> 5, 0) - t_lo;
+    seen1 = kl.nst + ((last - kl.lo_al) >> 5) - t_lo;
+  }
   // The Q fragments and the score scale are complete before the loop: waits
   // placed at a first use inside it would wait for the DMA in flight there.
 #pragma unroll
