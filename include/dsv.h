@@ -84,6 +84,8 @@ int dsv_set_timing_events(void* start_event, void* stop_event);
  * own address arithmetic, and fail with DSV_ERR_INVALID naming the first
  * access outside the extent of its argument (pointers are only compared,
  * never dereferenced, so the call runs on machines without a GPU).
+ * dsv_window_attention, dsv_spec_accept and the dsv_pages_* calls validate and
+ * plan only; their kernels' addresses are not walked.
  * dsv_dry_run_checks() returns the number of checks the last dry run made.
  */
 int dsv_set_dry_run(int enable);
@@ -248,7 +250,8 @@ int dsv_tree_verify_noalloc(const dsv_tensor* q, const dsv_tensor* k,
  * Workspace of dsv_window_attention for queries [B, M, H, D] of dtype
  * (dsv_dtype) over a cache of n_keys keys with Hk heads.  0 on invalid
  * arguments and on sizes that the call refuses: batch > 2^20, query heads >
- * 65536, keys > 2^30, H / Hk * M > 2^24, B * H * M > 2^30 (DSV_ERR_UNSUPPORTED).
+ * 65536, keys > 2^30, H / Hk * M > 2^24, B * H * M > 2^30, or 2^23 and more
+ * blocks of 16 or 256 rows (DSV_ERR_UNSUPPORTED).
  */
 size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk,
                                   int64_t D, int dtype, int64_t n_keys,
@@ -588,7 +591,7 @@ int dsv_pages_extend(const dsv_tensor* page_table, const dsv_tensor* refcount,
  * window > 0: the pages that no later token sees through a sliding window of
  * that many tokens with `sinks` first tokens that stay visible
  * (dsv_window_attention): those that start at or behind token `sinks` and end
- * before token seqlens - window + 2; lengths stay.
+ * with token seqlens - window at the latest; lengths stay.
  *   seqs [n] int32|int64: entries out of range are skipped, a sequence named
  *   twice is freed once
  */

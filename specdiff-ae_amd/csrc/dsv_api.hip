@@ -1901,7 +1901,7 @@ WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
   p.R = (int)R;
   p.MW = tree ? (int)((M + 63) / 64) : 0;
   // Blocks of 256 rows from 17 rows on (32 sequences of 24 rows through 4096 keys:
-  // 108 us, in blocks of 16 or 32 113 and more; of 64 rows 122 against 196), of 16
+  // 108 us, in blocks of 16 113; of 64 rows 122 against 196), of 16
   // below (64 sequences of 16 rows: 198 us, 219 in blocks of 256) and in fp32.
   const bool tile = dtype != DSV_F32 && R > 16 && !no_tile;
   p.rpb = tile ? 256 : 16;

@@ -12,9 +12,11 @@
 // Split.  fork and compact are two launches: a plan by one workgroup (who gets
 // which page: prefix sums over the counts, 4 bytes a page), then the copies by
 // the whole chip.  extend is the plan alone, free one launch over the entries.
-// The plan is latency, a few passes of 64 KiB; the copies are bound by HBM:
-// each page is read and written once, in 16-byte pieces, eight in flight per
-// thread.
+// The plan is latency (fork and extend 5 to 7 us, compact of 2048 pages 7); the
+// copies are bound by HBM: each page is read and written once, in 16-byte pieces,
+// eight in flight per thread.  92 pages of 2 MiB of 23 parents: 57 us, 6.8 TB/s of
+// reads and writes together (a parent's page comes from the cache after the first
+// time); 507 pages of 512 KiB moved: 101 to 114 us, 4.7 to 5.2 TB/s.
 //
 // Reference: core/kv_cache/paged_kv.py:81-166 (allocation, sharing with copy
 // on write, release) and :364-402 (defragmentation) keep this on the host.

@@ -1,6 +1,5 @@
 // dsv_window.h — launch arguments and key geometry of the windowed attention
-// (dsv_window.hip), shared by the kernels, the host's plan and the CPU tests'
-// emulation of it.
+// (dsv_window.hip, dsv_window_tile.hip).
 #pragma once
 
 #include <stdint.h>

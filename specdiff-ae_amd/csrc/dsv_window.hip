@@ -27,14 +27,17 @@
 // which some row drops keys, the rows are computed once more without matrix
 // products (exact_rows; in the product 0 * inf would be NaN).
 //
-// win_rows_kernel (this file's simplest; few rows: single tokens, short
-// chunks): bound by reading K and V.  Eight waves share a workgroup's tiles,
-// each with a softmax of its own, merged in LDS at the end, so no barrier stands
-// in the loop.  A tile goes memory -> registers in whole rows (16 bytes a lane,
-// the next tile in flight while this one is used) -> the wave's own LDS -> MFMA
-// operands: K rows by ds_read_b128, V transposed by ds_read_b64_tr_b16.  Splits
-// over the keys fill the GPU when there are few rows; win_merge_kernel joins
-// them.
+// win_rows_kernel (up to 16 rows: single tokens, short chunks): bound by
+// reading K and V.  Eight waves share a workgroup's tiles, each with a softmax of
+// its own, merged in LDS at the end, so no barrier stands in the loop.  A tile
+// goes memory -> registers in whole rows (16 bytes a lane, the next tile in flight
+// while this one is used) -> the wave's own LDS -> MFMA operands: K rows by
+// ds_read_b128, V transposed by ds_read_b64_tr_b16.  Splits over the keys fill
+// the GPU when there are few rows; win_merge_kernel joins them.  64 sequences of
+// one token through 4096 keys (32 query heads, 8 key heads of 128, pages of 64):
+// 181 us, 5.4 TB/s, the rate of a large copy.  One sequence through 1024 keys:
+// 17.5 us, a chain of latencies (arguments, length, page, four tiles a wave) that
+// the call's host path of 17 us covers.
 //
 // Reference context: runtime/attention_compat.py:103-132 (the cache call whose
 // layouts are kept), runtime/cache_state.py:52-66 (the tree behind the prefix),
@@ -73,9 +76,9 @@ __device__ __forceinline__ float row_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Eight waves: two per SIMD have 256 KiB of loads in flight between them where
-// the registers allow, and four per workgroup left the batch of 64 at 230 us, 184
-// with eight (16 spill).
+// Eight waves, two per SIMD, each with a tile's loads in flight: the batch of 64
+// above takes 181 us; with four waves a workgroup it took 230, and 16 do not have
+// the registers (they spill).
 constexpr int kRowWaves = 8;
 
 // ---- few rows ------------------------------------------------------------------
@@ -292,6 +295,9 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
 // step.  K's operand takes a lane's 16 bytes as four k-steps (the order of the
 // head dimension in the product is free as long as Q's agrees), V's operand is a
 // row-major element, so nothing passes through LDS but the join of the waves.
+// Three chunks of 37 rows through 777 keys (14 query heads, 2 key heads of 64):
+// 21 us, of which 102 workgroups of three or four tiles a wave spend half in
+// fp32 MFMA (a tile: 64 of 32 cycles) and the rest in the latencies before.
 template <int D>
 __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinArgs a) {
   constexpr int NW = kRowWaves;

@@ -6,7 +6,9 @@ Module layout mirrors the reference package ``diffspec``:
   runtime.bundle_verifier    FusedBundleVerifier, PagedBundleVerifier
   core.bundle_scheduler      BundleScheduler, TreeDescriptorBuilder, bundle_row_order,
                              bundle_row_order_device
-  draft.tree_verification    verify / verify_new, tree_accept, evaluate_tree
+  runtime.window_attention   window_attn_with_kvcache
+  core.kv_cache              fork_pages, extend_pages, free_pages, compact_pages
+  draft.tree_verification    verify / verify_new, tree_accept, speculative_accept, evaluate_tree
 All compute runs in libdsv.so (HIP kernels for gfx950 behind a C ABI).
 """
 

@@ -56,6 +56,8 @@ def window_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     if q.dim() != 4 or k_cache.dim() != 4:
         raise ValueError(f"q and the caches must be 4-d (got {tuple(q.shape)} and {tuple(k_cache.shape)})")
     B, M, H, D = q.shape
+    if page_table is not None and page_table.dim() not in (1, 2):
+        raise ValueError(f"page_table must be [n_pages] or [B, n_pages] (got {tuple(page_table.shape)})")
     if page_table is not None:
         Hk, cap = k_cache.shape[1], page_table.shape[-1] * k_cache.shape[2]
     else:

@@ -20,9 +20,9 @@ def dry(dsv_lib):
 
 
 def call(lib, B=2, M=3, H=4, Hk=2, D=64, N=40, window=9, sinks=2, n_keys=-1, nbytes=1 << 23, ws=None, **kw):
-    t = dict(q=torch.zeros(B, M, H, D), k=torch.zeros(B, N, Hk, D), v=torch.zeros(B, N, Hk, D), table=None, lens=None,
-             parent=None, out=torch.zeros(B, M, H, D), lse=torch.zeros(B, H, M))
-    t.update(kw)
+    sizes = dict(q=(B, M, H, D), k=(B, N, Hk, D), v=(B, N, Hk, D), out=(B, M, H, D), lse=(B, H, M))
+    t = {x: kw[x] if x in kw else torch.zeros(sizes[x]) if x in sizes else None
+         for x in ("q", "k", "v", "table", "lens", "parent", "out", "lse")}
     d = {x: _ext.desc(y) for x, y in t.items()}
     ptr = (WS.data_ptr() + 255) // 256 * 256 if ws is None else ws
     return lib.dsv_window_attention(d["q"], d["k"], d["v"], d["table"], d["lens"], n_keys, window, sinks, d["parent"],
@@ -54,6 +54,9 @@ def test_accepts_and_refuses(dry):
     assert call(dry, B=1, M=1025, parent=i32(1025)) == UNSUPPORTED
     assert call(dry, B=1, M=(1 << 24) + 1, H=1, Hk=1, q=big.expand(1, (1 << 24) + 1, 1, 64),
                 out=big.clone().expand(1, (1 << 24) + 1, 1, 64), lse=None) == UNSUPPORTED
+    wide, kv = big.expand(1 << 20, 1, 8, 64), big.expand(1 << 20, 40, 8, 64)  # 2^23 workgroups
+    assert call(dry, B=1 << 20, M=1, H=8, Hk=8, q=wide, out=big.clone().expand(1 << 20, 1, 8, 64),
+                k=kv, v=kv, lse=None) == UNSUPPORTED
     assert call(dry, ws=0) == WORKSPACE
     assert call(dry, nbytes=0) == WORKSPACE
     assert call(dry, ws=(WS.data_ptr() + 255) // 256 * 256 + 64) == WORKSPACE
@@ -68,7 +71,7 @@ def test_workspace_sizes(dsv_lib):
     for bad in [(0, 1, 4, 2, 64, 0, 10, 4, 0, 0), (1, 0, 4, 2, 64, 0, 10, 4, 0, 0), (1, 1, 4, 3, 64, 0, 10, 4, 0, 0),
                 (1, 1, 4, 2, 80, 0, 10, 4, 0, 0), (1, 1, 4, 2, 64, 3, 10, 4, 0, 0), (1, 1, 4, 2, 64, 0, -1, 4, 0, 0),
                 (1, 1, 4, 2, 64, 0, 10, 0, 0, 0), (1, 1, 4, 2, 64, 0, 10, 4, -1, 0), (1, 1025, 4, 2, 64, 0, 10, 4, 0, 1),
-                ((1 << 20) + 1, 1, 4, 2, 64, 0, 10, 4, 0, 0)]:
+                ((1 << 20) + 1, 1, 4, 2, 64, 0, 10, 4, 0, 0), (1 << 20, 1, 8, 8, 64, 0, 10, 4, 0, 0)]:
         assert n(*bad) == 0, bad
 
 
