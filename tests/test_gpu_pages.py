@@ -176,6 +176,7 @@ def test_strided_pool(gpu):
     rows = torch.full((4, 9), -7, dtype=torch.int32, device=gpu)
     rows[:, :6] = p.dtable
     p.dtable = rows[:, :6]
+    p.dref = torch.zeros(P + 1, dtype=torch.int32, device=gpu)[1:]  # 4-byte aligned
     p.extend([10, 3, 0, 0])
     p.fork([0, 1], [2, 3])
     p.free([0])

@@ -223,12 +223,13 @@ def test_masks_of_scores(gpu):
     assert torch.equal(torch.isnan(lse[0]).all(0), sees)
 
 
-def test_strides_and_output_types(gpu):
+@pytest.mark.parametrize("M", [5, 70])
+def test_strides_and_output_types(gpu, M):
     """Heads before tokens, padded rows, shared tables, an int64 table, every output type."""
-    c = Case(gpu, 2, 5, 6, 2, 64, [120, 77], BF16, 16, seed=5)
+    c = Case(gpu, 2, M, 6, 2, 64, [120, 77], BF16, 16, seed=5)
     want = c.check(50, 3)
-    big = torch.zeros(2, 6, 7, 80, dtype=BF16, device=gpu)
-    qv = big[:, :, 1:6, :64].transpose(1, 2)
+    big = torch.zeros(2, 6, M + 2, 80, dtype=BF16, device=gpu)
+    qv = big[:, :, 1:M + 1, :64].transpose(1, 2)
     qv.copy_(c.q)
     pool = torch.zeros(2, c.k.shape[0], 16, 2, 72, dtype=BF16, device=gpu)
     kv, vv = (pool[i, ..., :64].transpose(1, 2) for i in range(2))
@@ -245,19 +246,20 @@ def test_strides_and_output_types(gpu):
     c.check(50, 3, result=got)
 
 
-def test_c_abi_strided_outputs(gpu, dsv_lib):
+@pytest.mark.parametrize("M", [5, 70])
+def test_c_abi_strided_outputs(gpu, dsv_lib, M):
     """Outputs at strides of their own: rows between theirs stay as they were."""
     from diffspec_mi355x import _ext
     for dtype in (BF16, F32):
-        c = Case(gpu, 2, 5, 6, 2, 64, [120, 3], dtype, 0, seed=6)
+        c = Case(gpu, 2, M, 6, 2, 64, [120, 3], dtype, 0, seed=6)
         for pad in (1, 8):
-            big = torch.full((2, 6, 6, 64 + pad), 7.0, dtype=dtype, device=gpu)
+            big = torch.full((2, M + 1, 6, 64 + pad), 7.0, dtype=dtype, device=gpu)
             out = big[:, 1:, :, :64]
-            lbig = torch.full((2, 5, 7), 7.0, device=gpu)
+            lbig = torch.full((2, M, 7), 7.0, device=gpu)
             lse = lbig[:, :, :6].transpose(1, 2)
             d = _ext.desc
             lens = torch.tensor(c.lens, device=gpu)
-            n = dsv_lib.dsv_window_workspace_bytes(2, 5, 6, 2, 64, d(c.q).dtype, 120, 50, 3, 0)
+            n = dsv_lib.dsv_window_workspace_bytes(2, M, 6, 2, 64, d(c.q).dtype, 120, 50, 3, 0)
             ws = _ext.workspace(n, gpu)
             rc = dsv_lib.dsv_window_attention(d(c.q), d(c.k), d(c.v), d(None), d(lens), -1, 50, 3, d(None), d(out), d(lse),
                                               ws.data_ptr(), n, _ext.stream_of(gpu))
@@ -266,21 +268,22 @@ def test_c_abi_strided_outputs(gpu, dsv_lib):
             assert bool((big[:, 0] == 7).all()) and bool((big[..., 64:] == 7).all()) and bool((lbig[:, :, 6:] == 7).all())
 
 
-def test_long_cache_beyond_32_bits(gpu):
+@pytest.mark.parametrize("M", [4, 40])
+def test_long_cache_beyond_32_bits(gpu, M):
     """Offsets past 2^32 bytes into the cache, dense and paged."""
     N = 1 << 20
     k = torch.zeros(1, N, 16, 128, dtype=BF16, device=gpu)   # 4 GiB a half
     v = torch.zeros_like(k)
-    c = Case(gpu, 1, 4, 32, 16, 128, [64], BF16, 0, seed=7)
+    c, window = Case(gpu, 1, M, 32, 16, 128, [64], BF16, 0, seed=7), 62 - M
     k[:, N - 61:N], v[:, N - 61:N] = c.k[:, 3:], c.v[:, 3:]
     k[:, :3], v[:, :3] = c.k[:, :3], c.v[:, :3]
     # The last 61 keys and 3 sinks are the small cache's 64 keys.
-    a = window_attn_with_kvcache(c.q, k, v, 58, 3, return_softmax_lse=True)
-    small = window_attn_with_kvcache(c.q, c.k, c.v, 58, 3, return_softmax_lse=True)
+    a = window_attn_with_kvcache(c.q, k, v, window, 3, return_softmax_lse=True)
+    small = window_attn_with_kvcache(c.q, c.k, c.v, window, 3, return_softmax_lse=True)
     assert torch.allclose(a[0].float(), small[0].float(), rtol=2 ** -7, atol=2 ** -7)
     assert torch.allclose(a[1], small[1], rtol=1e-5, atol=1e-5)
     pages = lambda x: x.view(N // 64, 64, 16, 128).transpose(1, 2)  # noqa: E731
-    b = window_attn_with_kvcache(c.q, pages(k), pages(v), 58, 3, None, torch.arange(N // 64, device=gpu), None, True)
+    b = window_attn_with_kvcache(c.q, pages(k), pages(v), window, 3, None, torch.arange(N // 64, device=gpu), None, True)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
