@@ -1495,11 +1495,15 @@ struct SpecPlan {
 };
 
 // Workgroups per tree: one per CU in all, at most so many that each wave has a
-// segment of the row.
+// segment of the row.  One up to 32768 entries: its sweep is longer by at most 2 us,
+// and the second launch costs the caller 2.5 (4 chains over pairs of rows, us in a
+// graph and called: 16384 entries 8.1 and 15.9 by one workgroup, 8.8 and 18.6 by
+// several; 32000 10.4 and 16.0, 8.9 and 18.5; 64000 14.4 and 15.8, 8.7 and 18.4;
+// 128256 22.6 and 22.9, 9.1 and 18.0).
 bool spec_plan(int64_t T, int64_t M, int64_t V, SpecPlan& p) {
   if (M < 1 || M > dsv::kSpecMaxM || T < 1 || T > (1 << 20) || V < 1 || V > 0x7fffffff) return false;
   const int64_t waves = dsv::kSpecThreads / 64, nseg = (V + dsv::kSpecSeg - 1) / dsv::kSpecSeg;
-  const int64_t most = std::min<int64_t>((nseg + waves - 1) / waves, 64);
+  const int64_t most = nseg <= 64 ? 1 : std::min<int64_t>((nseg + waves - 1) / waves, 64);
   p.nwg = (int)std::max<int64_t>(1, std::min(most, (int64_t)device_cus() / T));
   // A wave's segments in up to 4 slots: the draw walks one slot again.
   const int64_t each = (nseg + waves * p.nwg - 1) / (waves * p.nwg);

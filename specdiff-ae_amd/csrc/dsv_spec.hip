@@ -25,10 +25,10 @@
 // us), so with few trees a row is shared out over several workgroups of 16
 // waves, each walking the tree by itself (no wait stands between the walk and
 // the sweep), and a second launch, one workgroup a tree, draws from their sums;
-// with a tree per CU the one workgroup draws as well.  64 chains of 5 over 128256
-// fp32 entries: one workgroup each 33 us, four each 19 (16.5 + 3.8).  A wave sums a
-// contiguous slot of the row, 8 entries a lane at a time with the next ones in
-// flight.
+// with a tree per CU, or a short row, the one workgroup draws as well.  64 chains of
+// 5 over 128256 fp32 entries: one workgroup each 27 us, four each 19.5 (16.5 + 3.8).
+// A wave sums a contiguous slot of the row, 8 entries a lane at a time with the next
+// ones in flight.
 //
 // Reference context: draft/tree_verification.py:100-182 (the walk whose
 // outputs are kept alike: path, tokens, winner, accept length, next token).

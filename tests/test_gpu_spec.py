@@ -45,7 +45,8 @@ def check(gpu, p, q, draft, parent, u):
 @pytest.mark.parametrize("sampled", [True, False])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,M,V,chain", [(1, 1, 1, False), (1, 2, 2, True), (3, 6, 4096, True), (2, 6, 4097, True),
-                                         (4, 17, 129, False), (2, 64, 5003, False), (1, 70, 8191, False)])
+                                         (4, 17, 129, False), (2, 64, 5003, False), (1, 70, 8191, False),
+                                         (2, 17, 32768, False), (3, 17, 32769, False), (200, 3, 33333, True)])
 def test_rule(gpu, T, M, V, chain, dtype, sampled):
     check(gpu, *make(T, M, V, dtype, sampled, seed=T * 100 + M, chain=chain))
 
@@ -84,13 +85,14 @@ def test_1024_nodes_and_unordered_trees(gpu):
     check(gpu, p, q, draft, parent, u)
 
 
-def test_strides_and_unaligned_rows(gpu):
+@pytest.mark.parametrize("V", [4500, 50001])
+def test_strides_and_unaligned_rows(gpu, V):
     """Rows of an odd stride at an odd offset, reversed-order views of the small inputs."""
-    p, q, draft, parent, u = make(3, 9, 4500, torch.bfloat16, True, seed=21)
-    big = torch.zeros(3, 10, 4507, dtype=torch.bfloat16, device=gpu)
-    pv = big[:, 1:, 3:4503]
+    p, q, draft, parent, u = make(3, 9, V, torch.bfloat16, True, seed=21)
+    big = torch.zeros(3, 10, V + 7, dtype=torch.bfloat16, device=gpu)
+    pv = big[:, 1:, 3:V + 3]
     pv.copy_(p)
-    qv = torch.zeros(9, 3, 4501, dtype=torch.bfloat16, device=gpu)[:, :, 1:].transpose(0, 1)
+    qv = torch.zeros(9, 3, V + 1, dtype=torch.bfloat16, device=gpu)[:, :, 1:].transpose(0, 1)
     qv.copy_(q)
     want = check(gpu, p, q, draft, parent, u)
     got = speculative_accept(pv, draft.to(gpu).t().contiguous().t(), parent.to(gpu), u.to(gpu).t().contiguous().t(), qv)
@@ -98,8 +100,9 @@ def test_strides_and_unaligned_rows(gpu):
         assert torch.equal(want[k], got[k])
 
 
-def test_edges(gpu):
-    V, M = 50, 4
+@pytest.mark.parametrize("V", [50, 40007])
+def test_edges(gpu, V):
+    M = 4
     p = torch.full((6, M, V), 1.0 / V)
     q = p.clone()
     draft = torch.tensor([[0, 3, 4, 5]] * 6)
@@ -128,9 +131,9 @@ def test_edges(gpu):
     check(gpu, p, q, draft, parent, torch.full((6, M), 0.99))
 
 
-def test_draw_at_both_ends(gpu):
+@pytest.mark.parametrize("V", [3 * 4096 + 5, 128 * 512 + 77])
+def test_draw_at_both_ends(gpu, V):
     """The next token for the smallest and largest numbers, weights in the first and last sub-block only."""
-    V = 3 * 4096 + 5
     p = torch.zeros(4, 1, V)
     p[:2, 0, 2], p[:2, 0, V - 1] = 0.25, 0.75
     p[2:, 0, 4095], p[2:, 0, 4096] = 0.5, 0.5
