@@ -136,13 +136,13 @@ struct Piece {
 
 // Weights of this lane's entries of the wave's piece at v0.  CHECK: infinite
 // entries count as 0; without it they are assumed absent (negative ones and NaN
-// are 0 either way: one maximum).
+// are 0 either way, p's by the maximum behind the product).
 template <typename E, bool Q, bool CHECK, int N, bool ROWS>
 __device__ __forceinline__ void weights(const Rows<E>& r, const Piece<E, N, ROWS>& p, const Piece<E, N, ROWS>& q, int64_t v0,
                                         double (&w)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    w[e] = (double)(CHECK ? prob(p.at(e)) : fmaxf(p.at(e), 0.f));
+    w[e] = (double)(CHECK ? prob(p.at(e)) : (Q ? p.at(e) : fmaxf(p.at(e), 0.f)));
     if constexpr (Q) w[e] = fmax(fma(-r.c, (double)(CHECK ? prob(q.at(e)) : fmaxf(q.at(e), 0.f)), w[e]), 0.0);
   }
   if constexpr (!Q) {
