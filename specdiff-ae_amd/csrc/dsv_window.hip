@@ -83,7 +83,7 @@ constexpr int kRowWaves = 8;
 
 // ---- few rows ------------------------------------------------------------------
 
-template <typename T, int D>
+template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs a) {
   constexpr int NW = kRowWaves;
   constexpr int CH = D / 8;           // 16-byte chunks per key
@@ -148,20 +148,18 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
   const uint16_t* vbase = a.v + b * a.v_sb + kvh * a.v_sh + (lane % CH) * 8;
   // Lane l holds the page of key l (mod 32) of a tile, read a tile ahead.
   auto tile_pages = [&](int tt) -> int32_t {
-    if (a.pt == nullptr || tt >= t_end) return 0;
+    if (!PAGED || tt >= t_end) return 0;
     return page_of(a, b, kl.read(kl.base(tt) + (lane & 31)));
   };
   u32x4 kr[NL], vr[NL];
+  // It works out that key's offsets for the others.
   auto load_tile = [&](int tt, int32_t pg) {
-    const int kb = kl.base(tt);
+    const int n = kl.read(kl.base(tt) + (lane & 31));
+    const long long ko = key_off(a, PAGED, a.k_sp, a.k_st, n, pg), vo = key_off(a, PAGED, a.v_sp, a.v_st, n, pg);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int i = j * KPI + lane / CH;
-      const int n = kl.read(kb + i);
-      const int32_t page = a.pt != nullptr ? __shfl(pg, i) : 0;
-      kr[j] = *reinterpret_cast<const u32x4*>(kbase + key_off(a, a.k_sp, a.k_st, n, page));
-      vr[j] = *reinterpret_cast<const u32x4*>(vbase + key_off(a, a.v_sp, a.v_st, n, page));
-    }
+    for (int j = 0; j < NL; ++j) kr[j] = *reinterpret_cast<const u32x4*>(kbase + __shfl(ko, j * KPI + lane / CH));
+#pragma unroll
+    for (int j = 0; j < NL; ++j) vr[j] = *reinterpret_cast<const u32x4*>(vbase + __shfl(vo, j * KPI + lane / CH));
   };
 
   int32_t pg = tile_pages(t);
@@ -293,12 +291,13 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
 // ---- fp32 ------------------------------------------------------------------------
 // The same walk over tiles with v_mfma_f32_16x16x4_f32, 16 rows and 32 keys a
 // step.  K's operand takes a lane's 16 bytes as four k-steps (the order of the
-// head dimension in the product is free as long as Q's agrees), V's operand is a
-// row-major element, so nothing passes through LDS but the join of the waves.
+// head dimension in the product is free as long as Q's agrees), V's operand a
+// lane's 16 bytes as four tiles of columns (tile d's row i is column 64 (d / 4) + 4 i
+// + d % 4), so nothing passes through LDS but the join of the waves.
 // Three chunks of 37 rows through 777 keys (14 query heads, 2 key heads of 64):
 // 21 us, of which 102 workgroups of three or four tiles a wave spend half in
 // fp32 MFMA (a tile: 64 of 32 cycles) and the rest in the latencies before.
-template <int D>
+template <int D, bool PAGED>
 __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinArgs a) {
   constexpr int NW = kRowWaves;
   constexpr int KC = D / 16;          // 16-byte chunks per lane and key
@@ -346,43 +345,51 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
 
   // Lane l holds the page of key l (mod 32) of a tile, read a tile ahead.
   auto tile_pages = [&](int tt) -> int32_t {
-    if (a.pt == nullptr || tt >= t_end) return 0;
+    if (!PAGED || tt >= t_end) return 0;
     return page_of(a, b, kl.read(kl.base(tt) + (lane & 31)));
   };
   int t = (int)((int64_t)kl.nt * split / a.splits) + wave;
-  int32_t pg = tile_pages(t);
-  for (; t < t_end; t += NW) {
-    const int kb = kl.base(t);
-    // All of the tile's loads first: keys 16 h + lr of K (operand A), 16 (e / 4) +
-    // 4 lg + e % 4 of V.
-    f32x4 kf[2][KC];
-    float vf[8][DT];
+  // Keys 16 h + lr of K (operand A), 16 (e / 4) + 4 lg + e % 4 of V; the next tile's
+  // are loaded as soon as this one's have been used.
+  f32x4 kf[2][KC];
+  f32x4 vf[8][DT / 4];
+  // Lane l works out the offsets of key l (mod 32) for the others.
+  auto load_k = [&](int tt, int32_t pg) {
+    const long long ko = key_off(a, PAGED, a.k_sp, a.k_st, kl.read(kl.base(tt) + (lane & 31)), pg);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int i = 16 * h + lr;
-      const float* k = kbase + key_off(a, a.k_sp, a.k_st, kl.read(kb + i), a.pt != nullptr ? __shfl(pg, i) : 0) + 4 * lg;
+      const float* k = kbase + __shfl(ko, 16 * h + lr) + 4 * lg;
 #pragma unroll
       for (int c = 0; c < KC; ++c) kf[h][c] = *reinterpret_cast<const f32x4*>(k + 16 * c);
     }
+  };
+  auto load_v = [&](int tt, int32_t pg) {
+    const long long vo = key_off(a, PAGED, a.v_sp, a.v_st, kl.read(kl.base(tt) + (lane & 31)), pg);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int i = 16 * (e >> 2) + 4 * lg + (e & 3);
-      const float* v = vbase + key_off(a, a.v_sp, a.v_st, kl.read(kb + i), a.pt != nullptr ? __shfl(pg, i) : 0) + lr;
+      const float* v = vbase + __shfl(vo, 16 * (e >> 2) + 4 * lg + (e & 3)) + 4 * lr;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vf[e][d] = v[16 * d];
+      for (int d = 0; d < DT / 4; ++d) vf[e][d] = *reinterpret_cast<const f32x4*>(v + 64 * d);
     }
-    pg = tile_pages(t + NW);
+  };
+  int32_t pg = tile_pages(t);
+  if (t < t_end) {
+    load_k(t, pg);
+    load_v(t, pg);
+  }
+  pg = tile_pages(t + NW);
+  for (; t < t_end; t += NW) {
+    const int kb = kl.base(t);
     const bool masked = !kl.seen_by_all(kb, pmin, pmax, a.W, a.S, n0, a.parent != nullptr);
     const uint32_t keep = masked ? keep_word(a, tl.vis + lr * kTreeMaxW, pos, kb, n0) : ~0u;
-    f32x4 s[2];
+    f32x4 s[2] = {f32x4{}, f32x4{}};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[h] = f32x4{};
+    for (int c = 0; c < KC; ++c)
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[h][c][e], qf[c][e], s[h], 0, 0, 0);
-    }
+        for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[h][c][e], qf[c][e], s[h], 0, 0, 0);
+    if (t + NW < t_end) load_k(t + NW, pg);
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -410,12 +417,14 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
 #pragma unroll
       for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) odd |= !(vf[e][d] - vf[e][d] == 0.f);
+        for (int d = 0; d < DT; ++d) odd |= !(vf[e][d / 4][d % 4] - vf[e][d / 4][d % 4] == 0.f);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][d], x[e], acc[d], 0, 0, 0);
+      for (int d = 0; d < DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][d / 4][d % 4], x[e], acc[d], 0, 0, 0);
+    if (t + NW < t_end) load_v(t + NW, pg);
+    pg = tile_pages(t + 2 * NW);
   }
   if (__syncthreads_or((int)odd) != 0) {
     exact_rows<float, D, 16>(&args_again(), &tl, b, kvh, split, rb, (int)((int64_t)kl.nt * split / a.splits), t_end, wave, 16, NW);
@@ -428,7 +437,11 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
     sm_l[wave][lr] = lt;
   }
 #pragma unroll
-  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&smem[wave][lr * OST + 16 * d + 4 * lg]) = acc[d];
+  for (int d = 0; d < DT; d += 4)
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      *reinterpret_cast<f32x4*>(&smem[wave][lr * OST + 16 * d + 16 * lg + 4 * v]) =
+          f32x4{acc[d][v], acc[d + 1][v], acc[d + 2][v], acc[d + 3][v]};
   __syncthreads();
   constexpr int N = 4, TPR = D / N;
   const int rr = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N;
@@ -523,7 +536,20 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
 template <typename T, int D>
 hipError_t launch_rows(const WinArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), block(kRowWaves * 64);
-  hipLaunchKernelGGL((win_rows_kernel<T, D>), grid, block, 0, s, a);
+  if (a.pt != nullptr)
+    hipLaunchKernelGGL((win_rows_kernel<T, D, true>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((win_rows_kernel<T, D, false>), grid, block, 0, s, a);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_rows_f32(const WinArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), block(kRowWaves * 64);
+  if (a.pt != nullptr)
+    hipLaunchKernelGGL((win_rows_f32_kernel<D, true>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((win_rows_f32_kernel<D, false>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
@@ -531,8 +557,7 @@ template <int D>
 hipError_t launch_d(const WinArgs& a, hipStream_t s) {
   hipError_t e;
   if (a.dtype == 2) {
-    hipLaunchKernelGGL(win_rows_f32_kernel<D>, dim3((unsigned)((int64_t)a.B * a.Hk * a.n_rb * a.splits)), dim3(kRowWaves * 64), 0, s, a);
-    e = hipGetLastError();
+    e = launch_rows_f32<D>(a, s);
   } else if (a.rows_per_block == 256) {
     e = launch_window_tile(a, D, s);
   } else {

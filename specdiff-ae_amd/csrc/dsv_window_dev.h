@@ -164,8 +164,8 @@ __device__ __forceinline__ uint32_t keep_word(const WinArgs& a, const uint64_t* 
 }
 
 // Element offset of key n of the K or V half, for its physical page.
-__device__ __forceinline__ int64_t key_off(const WinArgs& a, int64_t sp, int64_t st, int n, int32_t page) {
-  return a.pt != nullptr ? page * sp + (n & ((1 << a.ps_shift) - 1)) * st : n * st;
+__device__ __forceinline__ int64_t key_off(const WinArgs& a, bool paged, int64_t sp, int64_t st, int n, int32_t page) {
+  return paged ? page * sp + (n & ((1 << a.ps_shift) - 1)) * st : n * st;
 }
 __device__ __forceinline__ int32_t page_of(const WinArgs& a, int b, int n) {
   const int64_t i = (int64_t)b * a.pt_sb + (n >> a.ps_shift);
@@ -265,9 +265,10 @@ __device__ __noinline__ void exact_rows(const WinArgs* ap, const TreeLds<ROWS>* 
       const int kb = kl.base(min(tt, t1 - 1));
       const bool seen = tt < t1 && ((keep_word(a, tl->vis + i * kTreeMaxW, pos, kb, n0) >> x) & 1u);
       const int n = kl.read(kb + x);
-      const int32_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
-      const E* k = kbase + key_off(a, a.k_sp, a.k_st, n, page);
-      const int64_t vo = key_off(a, a.v_sp, a.v_st, n, page);
+      const bool paged = a.pt != nullptr;
+      const int32_t page = paged ? page_of(a, b, n) : 0;
+      const E* k = kbase + key_off(a, paged, a.k_sp, a.k_st, n, page);
+      const int64_t vo = key_off(a, paged, a.v_sp, a.v_st, n, page);
       float s = kNegInf;
       if (seen) {
         s = 0.f;

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 #pragma unroll
     for (int x = 0; x < IPW; ++x) {
       const int n = kl.read(kl.base(t_lo + min(t0 + again(lane), ntiles - 1)) + (j0 + x) * G::KPI);
-      const uint64_t o = (uint64_t)key_off(a, sp2, st2, n, page_of(a, b, n));
+      const uint64_t o = (uint64_t)key_off(a, PAGED, sp2, st2, n, page_of(a, b, n));
       pgw_lo[x] = (uint32_t)o;
       pgw_hi[x] = (uint32_t)(o >> 32);
     }
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       for (int x = 0; x < IPW; ++x) {
         const int l = again(lane);
         const int n = kl.read(kb + (j0 + x) * G::KPI + l / CH);
-        dma_lane(dst + x * 1024, hbase + key_off(a, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
+        dma_lane(dst + x * 1024, hbase + key_off(a, PAGED, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
       }
     }
   };
