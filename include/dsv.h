@@ -248,8 +248,8 @@ int dsv_tree_verify_noalloc(const dsv_tensor* q, const dsv_tensor* k,
 
 /*
  * Workspace of dsv_window_attention for queries [B, M, H, D] of dtype
- * (dsv_dtype) over a cache of n_keys keys with Hk heads.  0 on invalid
- * arguments and on sizes that the call refuses: batch > 2^20, query heads >
+ * (dsv_dtype) over a cache of n_keys keys with Hk heads.  0 where the call needs
+ * none, on invalid arguments and on sizes that it refuses: batch > 2^20, query heads >
  * 65536, keys > 2^30, H / Hk * M > 2^24, B * H * M > 2^30, or 2^23 and more
  * blocks of 16 or 256 rows (DSV_ERR_UNSUPPORTED).
  */
@@ -490,8 +490,8 @@ int dsv_bundle_order(const dsv_tensor* parent, int64_t bundle_size,
 /* Verification of drafted tokens from given random numbers                   */
 /* ------------------------------------------------------------------------- */
 
-/* Workspace for dsv_spec_accept with T trees of M nodes over vocab V (0 on
- * invalid sizes). */
+/* Workspace for dsv_spec_accept with T trees of M nodes over vocab V (0 where
+ * it needs none and on invalid sizes). */
 size_t dsv_spec_workspace_bytes(int64_t T, int64_t M, int64_t V);
 
 /*

@@ -1534,7 +1534,7 @@ extern "C" {
 
 size_t dsv_spec_workspace_bytes(int64_t T, int64_t M, int64_t V) {
   SpecPlan p;
-  return spec_plan(T, M, V, p) ? std::max<size_t>(p.total, 256) : 0;
+  return spec_plan(T, M, V, p) ? p.total : 0;
 }
 
 int dsv_spec_accept(const dsv_tensor* target, const dsv_tensor* draft, const dsv_tensor* parent,
@@ -1940,7 +1940,7 @@ size_t dsv_window_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t Hk, i
   // (Whatever pages and strides the call comes with.)
   const WinPlan p = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0, false);
   const WinPlan r = win_plan(B, M, H, Hk, D, dtype, n_keys, window, sinks, has_tree != 0, true);
-  return p.err != nullptr ? 0 : std::max<size_t>(std::max(p.total, r.total), 256);
+  return p.err != nullptr ? 0 : std::max(p.total, r.total);
 }
 
 int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_tensor* v, const dsv_tensor* page_table,
@@ -2048,7 +2048,7 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   const bool no_tile = (present(page_table) && k->shape[2] < 8) || a.k_st > (1 << 25) || a.v_st > (1 << 25);
   const WinPlan p = win_plan(B, M, H, Hk, D, q->dtype, n, W, S, a.parent != nullptr, no_tile);
   if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
-  if ((rc = check_workspace(std::max<size_t>(p.total, 256), workspace, workspace_bytes)) != DSV_OK) return rc;
+  if (p.total > 0 && (rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
   a.dtype = q->dtype;
   a.q = static_cast<const uint16_t*>(q->data);
   a.q_sb = q->stride[0];
@@ -2071,9 +2071,11 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   a.rows_per_block = p.rpb;
   a.n_rb = p.n_rb;
   a.splits = p.splits;
-  char* w = static_cast<char*>(workspace);
-  a.opart = reinterpret_cast<float*>(w);
-  a.ml = reinterpret_cast<float2*>(w + p.opart_bytes);
+  if (p.total > 0) {
+    char* w = static_cast<char*>(workspace);
+    a.opart = reinterpret_cast<float*>(w);
+    a.ml = reinterpret_cast<float2*>(w + p.opart_bytes);
+  }
   a.MW = p.MW;
   a.out = out->data;
   a.out_dtype = out->dtype;

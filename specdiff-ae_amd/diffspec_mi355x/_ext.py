@@ -177,9 +177,20 @@ def stream_of(device: torch.device) -> ctypes.c_void_p:
         torch.cuda.current_device() if device.index is None else device.index))
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """Context in which launches go to ``device`` (a no-op where it is current)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def scratch(nbytes: int, device: torch.device):
+    """(tensor that holds the workspace, its address), nothing where none is needed."""
+    if nbytes == 0:
+        return None, None
+    ws = workspace(nbytes, device)
+    return ws, ws.data_ptr()
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

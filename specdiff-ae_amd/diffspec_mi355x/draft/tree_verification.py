@@ -204,10 +204,11 @@ def speculative_accept(target_probs: torch.Tensor, draft: torch.Tensor, parent: 
         path = torch.empty((T, M), dtype=torch.int64, device=dev)
         tokens = torch.empty((T, M), dtype=torch.int64, device=dev)
         info = torch.empty((T, 4), dtype=torch.int64, device=dev)
-        ws = _ext.workspace(lib.dsv_spec_workspace_bytes(T, M, V), dev)
+        n_ws = lib.dsv_spec_workspace_bytes(T, M, V)
+        ws, ws_ptr = _ext.scratch(n_ws, dev)
         rc = lib.dsv_spec_accept(_ext.desc(target_probs), _ext.desc(draft), _ext.desc(parent), _ext.desc(uniform),
                                  _ext.desc(draft_probs), _ext.desc(path), _ext.desc(tokens), _ext.desc(info),
-                                 ws.data_ptr(), ws.numel(), _ext.stream_of(dev))
+                                 ws_ptr, n_ws, _ext.stream_of(dev))
     _ext.check(rc, "speculative_accept")
     return {"path": path, "tokens": tokens, "info": info}
 

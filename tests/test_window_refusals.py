@@ -57,9 +57,12 @@ def test_accepts_and_refuses(dry):
     wide, kv = big.expand(1 << 20, 1, 8, 64), big.expand(1 << 20, 40, 8, 64)  # 2^23 workgroups
     assert call(dry, B=1 << 20, M=1, H=8, Hk=8, q=wide, out=big.clone().expand(1 << 20, 1, 8, 64),
                 k=kv, v=kv, lse=None) == UNSUPPORTED
-    assert call(dry, ws=0) == WORKSPACE
-    assert call(dry, nbytes=0) == WORKSPACE
-    assert call(dry, ws=(WS.data_ptr() + 255) // 256 * 256 + 64) == WORKSPACE
+    many = dict(B=1, N=8192, window=8192)  # (keys shared out over workgroups)
+    assert call(dry, **many) == 0
+    assert call(dry, ws=0, **many) == WORKSPACE
+    assert call(dry, nbytes=0, **many) == WORKSPACE
+    assert call(dry, ws=(WS.data_ptr() + 255) // 256 * 256 + 64, **many) == WORKSPACE
+    assert call(dry, ws=0, nbytes=0) == 0  # none needed
     q = f(2, 3, 4, 64)
     assert call(dry, q=q, out=q) == INVALID
     assert call(dry, lse=q.view(-1)[:24].view(2, 4, 3), q=q) == INVALID
@@ -67,7 +70,8 @@ def test_accepts_and_refuses(dry):
 
 def test_workspace_sizes(dsv_lib):
     n = dsv_lib.dsv_window_workspace_bytes
-    assert n(1, 1, 32, 8, 128, _ext.DSV_BF16, 5000, 1024, 4, 0) > 0
+    assert n(1, 1, 32, 8, 128, _ext.DSV_BF16, 50000, 8192, 4, 0) > 0
+    assert n(1, 1, 32, 8, 128, _ext.DSV_BF16, 50000, 512, 4, 0) == 0
     for bad in [(0, 1, 4, 2, 64, 0, 10, 4, 0, 0), (1, 0, 4, 2, 64, 0, 10, 4, 0, 0), (1, 1, 4, 3, 64, 0, 10, 4, 0, 0),
                 (1, 1, 4, 2, 80, 0, 10, 4, 0, 0), (1, 1, 4, 2, 64, 3, 10, 4, 0, 0), (1, 1, 4, 2, 64, 0, -1, 4, 0, 0),
                 (1, 1, 4, 2, 64, 0, 10, 0, 0, 0), (1, 1, 4, 2, 64, 0, 10, 4, -1, 0), (1, 1025, 4, 2, 64, 0, 10, 4, 0, 1),
