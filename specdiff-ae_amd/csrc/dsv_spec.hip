@@ -21,14 +21,13 @@
 //
 // Layout.  The acceptance tests read two scalars a node; all M nodes' are
 // gathered at once and wave 0 walks in LDS.  The last row's sweep is the large
-// read.  One CU takes in about 45 GB/s (a row pair of 128256 fp32 entries: 23
-// us), so with few trees a row is shared out over several workgroups of 16
-// waves, each walking the tree by itself (no wait stands between the walk and
-// the sweep), and a second launch, one workgroup a tree, draws from their sums;
-// with a tree per CU, or a short row, the one workgroup draws as well.  64 chains of
-// 5 over 128256 fp32 entries: one workgroup each 27 us, four each 19.5 (16.5 + 3.8).
-// A wave sums a contiguous slot of the row, 8 entries a lane at a time with the next
-// ones in flight.
+// read.  One CU sweeps a row pair of 128256 entries in about 17 us, so with few
+// trees a long row is shared out over several workgroups of 16 waves, each walking
+// the tree by itself (no wait stands between the walk and the sweep), and a second
+// launch, one wave a tree, draws from their sums; with a tree per CU, or a short
+// row, the one workgroup draws as well.  64 chains of 5 over 128256 fp32 entries:
+// one workgroup each 27 us, four each 19.5 (16.5 + 3.8).  A wave sums a contiguous
+// slot of the row, 8 entries a lane at a time with the next ones in flight.
 //
 // Reference context: draft/tree_verification.py:100-182 (the walk whose
 // outputs are kept alike: path, tokens, winner, accept length, next token).
@@ -162,9 +161,10 @@ __device__ __forceinline__ void weights(const Rows<E>& r, const Piece<E, N, ROWS
 
 // The sums of the workgroup's 16 own slots (own per wave, step segments each, from
 // slot first on) into LDS, their total in every thread, in a fixed order.  Bound by
-// what the CU takes in and by its VALU operations (one per SIMD and 4 cycles,
-// 64-bit ones slower): the check for infinite entries is one maximum over all of
-// them, and the sweep runs again with the full check only if there is one.
+// its VALU operations, 64-bit ones among them (a pair of 64000 entries takes one
+// workgroup 4 us more than of 32000, in bf16 as in fp32): the check for infinite
+// entries is one maximum over all of them, and the sweep runs again with the full
+// check only if there is one.
 template <typename E, bool Q, bool CHECK>
 __device__ __forceinline__ double sweep_as(const Rows<E>& r, int first, int own, int step, double* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

@@ -35,9 +35,9 @@
 // ds_read_b128, V transposed by ds_read_b64_tr_b16.  Splits over the keys fill
 // the GPU when there are few rows; win_merge_kernel joins them.  64 sequences of
 // one token through 4096 keys (32 query heads, 8 key heads of 128, pages of 64):
-// 181 us, 5.4 TB/s, the rate of a large copy.  One sequence through 1024 keys:
-// 17.5 us, a chain of latencies (arguments, length, page, four tiles a wave) that
-// the call's host path of 17 us covers.
+// 179 us, 5.5 TB/s, the rate of a large copy.  One sequence through 1024 keys: 15
+// us, a chain of latencies (arguments, length, page, four tiles a wave).  (Each lane
+// computing the offsets of the keys that it loads took 17.5: 64-bit products.)
 //
 // Reference context: runtime/attention_compat.py:103-132 (the cache call whose
 // layouts are kept), runtime/cache_state.py:52-66 (the tree behind the prefix),
@@ -77,7 +77,7 @@ __device__ __forceinline__ float row_sum(float x) {
 }
 
 // Eight waves, two per SIMD, each with a tile's loads in flight: the batch of 64
-// above takes 181 us; with four waves a workgroup it took 230, and 16 do not have
+// above takes 179 us; with four waves a workgroup it took 230, and 16 do not have
 // the registers (they spill).
 constexpr int kRowWaves = 8;
 
@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
 // lane's 16 bytes as four tiles of columns (tile d's row i is column 64 (d / 4) + 4 i
 // + d % 4), so nothing passes through LDS but the join of the waves.
 // Three chunks of 37 rows through 777 keys (14 query heads, 2 key heads of 64):
-// 21 us, of which 102 workgroups of three or four tiles a wave spend half in
-// fp32 MFMA (a tile: 64 of 32 cycles) and the rest in the latencies before.
+// 20 us, of which 102 workgroups of three or four tiles a wave spend 4.5 before the
+// first tile and a third in fp32 MFMA (a tile: 64 of 32 cycles, two waves a SIMD).
 template <int D, bool PAGED>
 __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinArgs a) {
   constexpr int NW = kRowWaves;
