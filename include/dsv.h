@@ -84,8 +84,9 @@ int dsv_set_timing_events(void* start_event, void* stop_event);
  * own address arithmetic, and fail with DSV_ERR_INVALID naming the first
  * access outside the extent of its argument (pointers are only compared,
  * never dereferenced, so the call runs on machines without a GPU).
- * dsv_window_attention, dsv_spec_accept and the dsv_pages_* calls validate and
- * plan only; their kernels' addresses are not walked.
+ * dsv_window_attention walks the keys of its row blocks in the same way (many
+ * blocks, tiles and rows by samples).  dsv_spec_accept and the dsv_pages_* calls
+ * validate and plan only.
  * dsv_dry_run_checks() returns the number of checks the last dry run made.
  */
 int dsv_set_dry_run(int enable);

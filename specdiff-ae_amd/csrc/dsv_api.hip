@@ -2085,7 +2085,18 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   const int per16 = 16 / elem_size(out->dtype);
   a.out_vec = (reinterpret_cast<uintptr_t>(out->data) & 15) == 0 && (B == 1 || a.o_sb % per16 == 0) &&
               (M == 1 || a.o_sm % per16 == 0) && (H == 1 || a.o_sh % per16 == 0);
-  if (g_dry_run) return DSV_OK;
+  if (g_dry_run) {
+    dsv::WinExtents ex;
+    ex.q = ins[0], ex.k = ins[1], ex.v = ins[2], ex.pt = ins[3], ex.lens = ins[4], ex.parent = ins[5];
+    ex.out = extent_of("out", out);
+    ex.lse = extent_of("lse", lse);
+    ex.ws = extent_raw("workspace", workspace, (int64_t)workspace_bytes);
+    std::string err;
+    int64_t checks = 0;
+    const int bad = dsv::emulate_window(a, (int)D, ex, err, &checks);
+    g_dry_checks = checks;
+    return bad ? fail(DSV_ERR_INVALID, "dry run: %s", err.c_str()) : DSV_OK;
+  }
   const hipError_t e = dsv::launch_window(a, (int)D, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "windowed attention launch");
   return DSV_OK;

@@ -31,4 +31,15 @@ struct AttnExtents {
 int emulate_attention(const AttnArgs& a, const MergeArgs& m, int D, bool dmask, bool f32, const AttnExtents& ex,
                       std::string& err, int64_t* n_checked);
 
+struct WinArgs;
+struct WinExtents {
+  Extent q{"q", 0, 0}, k{"k", 0, 0}, v{"v", 0, 0}, pt{"page_table", 0, 0};
+  Extent lens{"cache_seqlens", 0, 0}, parent{"parent", 0, 0};
+  Extent out{"out", 0, 0}, lse{"lse", 0, 0}, ws{"workspace", 0, 0};
+};
+
+// The same for the windowed attention (the lengths, which the host does not know,
+// at their ends), and that every key that a row sees lies in exactly one tile.
+int emulate_window(const WinArgs& a, int D, const WinExtents& ex, std::string& err, int64_t* n_checked);
+
 }  // namespace dsv

@@ -9,6 +9,7 @@
 // not known on the host: the kernel clamps page ids into [0, n_phys), so both
 // ends of that range are checked (offsets are monotone in the page id).
 
+#include <algorithm>
 #include <cstdio>
 #include <string>
 #include <vector>
@@ -16,6 +17,7 @@
 #include "dsv_attn_f32_geo.h"
 #include "dsv_attn_geo.h"
 #include "dsv_check.h"
+#include "dsv_window.h"
 
 namespace dsv {
 
@@ -357,6 +359,99 @@ void check_merge(const MergeArgs& m, const AttnExtents& ex, Checker& ck) {
   }
 }
 
+// Of n things: all, or where there are many the first, the last and some between.
+std::vector<int> sample(int n) {
+  std::vector<int> x;
+  if (n <= 24) {
+    for (int i = 0; i < n; ++i) x.push_back(i);
+  } else {
+    for (int i : {0, 1, 2, 3, n / 4, n / 2, n / 2 + 1, n - n / 4, n - 4, n - 3, n - 2, n - 1}) x.push_back(i);
+  }
+  return x;
+}
+
+// The keys of a block of rows of a sequence of len tokens.
+void check_window_block(const WinArgs& a, int D, const WinExtents& ex, int b, int kvh, int rb, int len, Checker& ck) {
+  const int es = a.dtype == 2 ? 4 : 2, n0 = len - a.M;
+  const bool tree = a.parent != nullptr, paged = a.pt != nullptr;
+  const int r0 = rb * a.rows_per_block, r1 = std::min(r0 + a.rows_per_block, a.R);
+  const WinKeys kl = win_keys(a.M, a.G, a.R, a.W, a.S, tree, n0, r0, a.rows_per_block);
+  if (!ck.cond(kl.nt >= 0 && (kl.nt == 0 || (kl.lo < kl.hi && kl.hi <= len)), "window: keys of a block")) return;
+  for (int t : sample(kl.nt)) {
+    const bool whole = t >= kl.first_whole() && t < kl.end_whole();
+    for (int i = 0; i < 32; ++i) {
+      const int n = kl.read(kl.base(t) + i);
+      if (!ck.cond(n >= 0 && n < len, "window: a key behind the sequence is read") ||
+          !ck.cond(!whole || n == kl.base(t) + i, "window: a tile that counts as whole is not"))
+        return;
+      if (paged) {
+        const int ib = a.pt_i64 ? 8 : 4;
+        ck.range(ex.pt, elem_addr(a.pt, b * a.pt_sb + (n >> a.ps_shift), ib), ib, "window: page table entry");
+      }
+      for (int64_t page : {(int64_t)0, paged ? a.n_phys - 1 : 0}) {
+        const int64_t in = paged ? n & ((1 << a.ps_shift) - 1) : n;
+        ck.range(ex.k, elem_addr(a.k, b * a.k_sb + page * a.k_sp + kvh * a.k_sh + in * a.k_st, es), (int64_t)D * es, "window: K row");
+        ck.range(ex.v, elem_addr(a.v, b * a.v_sb + page * a.v_sp + kvh * a.v_sh + in * a.v_st, es), (int64_t)D * es, "window: V row");
+      }
+      if (!ck.ok) return;
+    }
+  }
+  // Every key that a row sees, in one tile (trees: a row anywhere from n0 on).
+  if ((int64_t)kl.nt * 32 > 1 << 16 || kl.nt == 0) return;
+  std::vector<uint8_t> in(len + 64, 0);
+  for (int t = 0; t < kl.nt; ++t)
+    for (int i = 0; i < 32; ++i)
+      if (kl.base(t) + i < len) ++in[kl.base(t) + i];
+  for (int r : {r0, (r0 + r1) / 2, r1 - 1}) {
+    for (int pos : {tree ? n0 : n0 + r / a.G, tree ? n0 + a.M - 1 : n0 + r / a.G}) {
+      for (int n = 0; n < len; ++n) {
+        const bool sees = tree ? (n >= n0 || n > pos - a.W || n < a.S) : (n <= pos && (n > pos - a.W || n < a.S));
+        if (!ck.cond(in[n] <= 1 && (in[n] == 1 || !sees), "window: a key that a row sees is in no tile, or in two")) return;
+      }
+      for (int t = 0; t < kl.nt; ++t) {
+        const int kb = kl.base(t);
+        if (!kl.seen_by_all(kb, pos, pos, a.W, a.S, n0, tree) && !(t >= kl.first_seen(pos, a.W) && t < kl.end_seen(pos, n0, tree)))
+          continue;
+        for (int n = kb; n < kb + 32; ++n)
+          if (!ck.cond((tree ? n < n0 : n <= pos) && (n > pos - a.W || n < a.S), "window: an unmasked tile holds a key that a row does not see"))
+            return;
+      }
+    }
+  }
+}
+
+void check_window(const WinArgs& a, int D, const WinExtents& ex, Checker& ck) {
+  const int es = a.dtype == 2 ? 4 : 2, oes = a.out_dtype == 2 ? 4 : 2;
+  for (int b : sample(a.B)) {
+    if (a.seqlens != nullptr) ck.range(ex.lens, elem_addr(a.seqlens, b, a.seqlens_i64 ? 8 : 4), a.seqlens_i64 ? 8 : 4, "window: length");
+    for (int m : sample(a.M)) {
+      if (a.parent != nullptr) {
+        const int pb = a.par_i64 ? 8 : 4;
+        ck.range(ex.parent, elem_addr(a.parent, b * a.par_sb + m * a.par_sm, pb), pb, "window: parent");
+      }
+      for (int h : sample(a.H)) {
+        ck.range(ex.q, elem_addr(a.q, b * a.q_sb + m * a.q_sm + h * a.q_sh, es), (int64_t)D * es, "window: Q row");
+        ck.range(ex.out, elem_addr(a.out, b * a.o_sb + m * a.o_sm + h * a.o_sh, oes), (int64_t)D * oes, "window: output row");
+        if (a.lse != nullptr) ck.range(ex.lse, elem_addr(a.lse, b * a.l_sb + m * a.l_sm + h * a.l_sh, 4), 4, "window: lse");
+      }
+    }
+  }
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.B * a.Hk * a.splits * a.R;
+    ck.range(ex.ws, (uintptr_t)a.opart, rows * D * 4, "window: partial rows");
+    ck.range(ex.ws, (uintptr_t)a.ml, rows * 8, "window: partial sums");
+    ck.cond((uintptr_t)a.ml >= (uintptr_t)a.opart + (uintptr_t)(rows * D * 4), "window: partial rows and sums overlap");
+  }
+  ck.cond((int64_t)a.n_rb * a.rows_per_block >= a.R, "window: rows without a block");
+  const int n = (int)a.n_keys;
+  for (int len : {0, 1, a.M - 1, a.M, a.M + 1, a.M + a.W, n / 2 + 1, n - 1, n}) {
+    if (len < 0 || len > n || (a.seqlens == nullptr && len != n)) continue;
+    for (int rb : sample(a.n_rb))
+      for (int b : {0, a.B - 1})
+        if (ck.ok) check_window_block(a, D, ex, b, b == 0 ? 0 : a.Hk - 1, rb, len, ck);
+  }
+}
+
 }  // namespace
 
 int emulate_attention(const AttnArgs& a, const MergeArgs& m, int D, bool dmask, bool f32, const AttnExtents& ex,
@@ -369,6 +464,13 @@ int emulate_attention(const AttnArgs& a, const MergeArgs& m, int D, bool dmask, 
   else
     ck.cond(false, "unsupported head_dim in emulation");
   if (ck.ok && a.direct == 0) check_merge(m, ex, ck);
+  if (n_checked) *n_checked = ck.n_checked;
+  return ck.ok ? 0 : -1;
+}
+
+int emulate_window(const WinArgs& a, int D, const WinExtents& ex, std::string& err, int64_t* n_checked) {
+  Checker ck{&err};
+  check_window(a, D, ex, ck);
   if (n_checked) *n_checked = ck.n_checked;
   return ck.ok ? 0 : -1;
 }

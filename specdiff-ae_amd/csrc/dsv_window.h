@@ -55,6 +55,17 @@ struct WinKeys {
     n = n > lo ? n : lo;
     return n < hi ? n : hi - 1;
   }
+  // The tiles [first_whole(), end_whole()) hold only keys that some row sees (others
+  // may): the window's.
+  DSV_HD int first_whole() const { return nst + (lo > lo_al ? (lo - lo_al + 31) >> 5 : 0); }
+  DSV_HD int end_whole() const { return nst + ((hi - lo_al) >> 5); }
+  // The tiles [first_seen(), end_seen()) are seen whole by every row between
+  // positions pmin and pmax (others may be).
+  DSV_HD int first_seen(int pmax, int W) const {
+    const int x = (pmax - W + 1 - lo_al + 31) >> 5;
+    return nst + (x > 0 ? x : 0);
+  }
+  DSV_HD int end_seen(int pmin, int n0, bool tree) const { return nst + (((tree ? n0 : pmin + 1) - lo_al) >> 5); }
   // Is every key of the tile seen by every row between positions pmin and pmax?
   DSV_HD bool seen_by_all(int kb, int pmin, int pmax, int W, int S, int n0, bool tree) const {
     return (tree ? kb + 32 <= n0 : kb + 31 <= pmin) && (kb > pmax - W || kb + 32 <= S);

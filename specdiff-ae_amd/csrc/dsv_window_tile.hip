@@ -157,8 +157,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     lane_off[x] = (uint32_t)(((PAGED ? 0 : (j0 + x) * G::KPI) + lane / CH) * st2) + (uint32_t)(chunk_of(x, lane) * 16);
   const uint32_t reach = (uint32_t)((PAGED ? G::KPI - 1 : 31) * st2) + 2 * D;
   // The tiles [whole0, whole1) are such (others may be: whole() tells).
-  const int whole0 = kl.nst + (kl.lo > kl.lo_al ? max((kl.lo - kl.lo_al + 31) >> 5, 0) : 0) - t_lo;
-  const int whole1 = kl.nst + ((kl.hi - kl.lo_al) >> 5) - t_lo;
+  const int whole0 = kl.first_whole() - t_lo, whole1 = kl.end_whole() - t_lo;
   // Paged: lane l holds the offset of instruction x's keys in tile pgw_t0 + l.
   uint32_t pgw_lo[IPW], pgw_hi[IPW];
   int pgw_t0 = -64;
@@ -350,12 +349,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   pmin = uniform(pmin);
   pmax = uniform(pmax);
   // The tiles [seen0, seen1) are seen whole by every row of the wave (others may be).
-  int seen0 = 0, seen1 = 0;
-  {
-    const int first = pmax - a.W + 1, last = tree ? n0 : pmin + 1;  // keys [first, last)
-    seen0 = kl.nst + max((first - kl.lo_al + 31) >> 5, 0) - t_lo;
-    seen1 = kl.nst + ((last - kl.lo_al) >> 5) - t_lo;
-  }
+  const int seen0 = kl.first_seen(pmax, a.W) - t_lo, seen1 = kl.end_seen(pmin, n0, tree) - t_lo;
   // The Q fragments and the score scale are complete before the loop: waits
   // placed at a first use inside it would wait for the DMA in flight there.
 #pragma unroll

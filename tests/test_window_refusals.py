@@ -68,6 +68,34 @@ def test_accepts_and_refuses(dry):
     assert call(dry, lse=q.view(-1)[:24].view(2, 4, 3), q=q) == INVALID
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_every_address_and_key(dry, seed):
+    """The kernels' key geometry and addresses, walked on the host: in range, every seen key in one tile."""
+    rng = np.random.default_rng(seed)
+    pick = lambda *x: x[int(rng.integers(len(x)))]  # noqa: E731
+    B, Hk, G, D = pick(1, 3), pick(1, 2), pick(1, 2, 7, 16), pick(64, 128)
+    M, N = int(pick(1, 2, 5, 31, 64, 200)), int(pick(1, 33, 200, 700))
+    dt = pick(torch.bfloat16, torch.float16, torch.float32)
+    kw = dict(B=B, M=M, H=Hk * G, Hk=Hk, D=D, window=int(pick(1, 7, 32, 100, 1000)), sinks=int(pick(0, 1, 31, 33, 90)),
+              q=torch.zeros(B, M, Hk * G, D, dtype=dt), nbytes=(1 << 24) - 256)
+    if rng.random() < 0.5:
+        page = int(pick(1, 4, 16, 64))
+        n_log = -(-N // page)
+        kv = torch.zeros(2, 5, Hk, page, D, dtype=dt)
+        kw.update(k=kv[0], v=kv[1], table=torch.zeros((B, n_log) if rng.random() < 0.7 else (n_log,), dtype=pick(torch.int32, torch.int64)))
+    else:
+        kv = torch.zeros(2, B, N, Hk, D + 8, dtype=dt)[..., :D]
+        kw.update(k=kv[0], v=kv[1])
+    if rng.random() < 0.8:
+        kw.update(lens=torch.zeros(B, dtype=torch.int32))
+    if rng.random() < 0.4:
+        kw.update(parent=torch.zeros((B, M), dtype=torch.int64))
+    if rng.random() < 0.3:
+        kw.update(n_keys=max(1, N // 2))
+    assert call(dry, **kw) == 0, _ext.last_error()
+    assert dry.dsv_dry_run_checks() > 0
+
+
 def test_workspace_sizes(dsv_lib):
     n = dsv_lib.dsv_window_workspace_bytes
     assert n(1, 1, 32, 8, 128, _ext.DSV_BF16, 50000, 8192, 4, 0) > 0
