@@ -578,7 +578,8 @@ int dsv_pages_fork(const dsv_tensor* kv_pages, const dsv_tensor* page_table,
  * stay as they are): the table entries behind the present length and up to the
  * last page of the new one that name no page receive free pages, seqlens the new
  * length.  (Entries that name one keep it: seqlens may be set back after drafted
- * tokens were rejected.)  Refused: new lengths beyond the table row, negative
+ * tokens were rejected, though not below tokens shared with another sequence,
+ * whose pages are the other's too.)  Refused: new lengths beyond the table row, negative
  * seqlens.  The new tokens' contents are the caller's.
  */
 int dsv_pages_extend(const dsv_tensor* page_table, const dsv_tensor* refcount,

@@ -64,7 +64,8 @@ def extend_pages(page_table: torch.Tensor, refcount: torch.Tensor, seqlens: torc
 
     Pages that a sequence's row already names behind its ``seqlens`` are used
     before any is taken: a caller may set ``seqlens`` back after drafted tokens
-    were rejected, and the next draft finds their pages.
+    were rejected, and the next draft finds their pages.  (Not below tokens that
+    it shares with another sequence: the pages are the other's too.)
 
     Returns the int32 [3] tensor (pages taken, pages lacking, sequences refused:
     new lengths that the table row cannot hold).

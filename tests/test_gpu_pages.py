@@ -89,6 +89,22 @@ def test_extend_keeps_pages_behind_the_length(gpu, B):
     assert sum(p.ref) == 0
 
 
+def test_empty_lists_and_strided_indices(gpu):
+    p = Pool(gpu, B=4, P=12, n_log=4)
+    p.extend([5, 0, 9, 0])
+    p.fork([], [])
+    p.free([])
+    p.extend([0, 0, 0, 0])
+    wide = torch.tensor([0, 7, 2, 7], device=gpu)
+    kids = torch.tensor([1, 7, 3, 7], device=gpu)
+    oracle.fork(p.kv, p.table, p.ref, p.lens, [0, 2], [1, 3], p.ps)
+    fork_pages(p.dkv, p.dtable, p.dref, p.dlens, wide[::2], kids[::2])
+    p.same()
+    oracle.free(p.table, p.ref, p.lens, [0, 2], p.ps)
+    free_pages(p.dtable, p.dref, p.dlens, wide[::2], p.ps)
+    p.same()
+
+
 def test_nothing_happens_without_enough_pages(gpu):
     p = Pool(gpu, B=5, P=6, n_log=8)
     p.extend([9, 9, 0, 0, 0])

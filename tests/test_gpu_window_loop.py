@@ -193,3 +193,50 @@ def test_loop_captured(gpu):
         for k, v in {**got, "kv": p.kv, "table": p.dtable, "ref": p.dref, "lens": p.dlens}.items():
             # (Bytes: pages that nobody wrote hold NaN.)
             assert torch.equal(v.contiguous().view(torch.uint8), want[i][k].contiguous().view(torch.uint8)), (i, k)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that share keys and rows out over workgroups, on two streams at once, as one after the other."""
+    g = torch.Generator().manual_seed(2)
+    q = [torch.randn((2, m, 8, 64), generator=g).to(torch.bfloat16).to(gpu) for m in (1, 40)]
+    k, v = (torch.randn((2, 4000, 2, 64), generator=g).to(torch.bfloat16).to(gpu) for _ in range(2))
+    probs = [torch.softmax(torch.randn((3, 6, 60000), generator=g), -1).to(gpu) for _ in range(2)]
+    draft = torch.randint(0, 60000, (3, 6), generator=g).to(gpu)
+    parent = torch.arange(-1, 4, device=gpu).expand(3, -1)
+    uniform = torch.rand((3, 6), generator=g).to(gpu)
+
+    def run(i):
+        out, lse = window_attn_with_kvcache(q[i], k, v, 3000, 4, return_softmax_lse=True)
+        return out, lse, speculative_accept(probs[i], draft, parent, uniform, probs[1 - i])["info"]
+
+    want = [run(0), run(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("M", [5, 60])
+def test_forms_of_the_tree(gpu, M):
+    """One tree for all sequences or one each, int32 or int64, at any stride: the same result."""
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn((3, M, 8, 64), generator=g).to(torch.bfloat16).to(gpu)
+    k, v = (torch.randn((3, 300, 2, 64), generator=g).to(torch.bfloat16).to(gpu) for _ in range(2))
+    lens = torch.tensor([300, M, M + 31], device=gpu)
+    par = torch.tensor(wl.make_tree(M, max_depth=M, max_outdeg=3, seed=5)[0], device=gpu)
+    f = lambda p: window_attn_with_kvcache(q, k, v, 100, 7, lens, parent=p, return_softmax_lse=True)  # noqa: E731
+    want = f(par)
+    wide = torch.full((3, 2 * M + 1), 99, dtype=torch.int64, device=gpu)
+    wide[:, 1::2] = par
+    for p in (par.int(), par[None], par.int().expand(3, -1), par.repeat(3, 1), wide[:, 1::2]):
+        got = f(p)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = window_attn_with_kvcache(q[:1], k[:1], v[:1], 100, 7, 300, parent=par)
+    assert torch.equal(one[0], want[0][0])
