@@ -227,6 +227,25 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     if (k + 3 < ntiles) issue_tile(k + 3);
   };
 
+  // The same in the long loop, where three tiles follow and the third is whole.
+  int64_t next_off = 0;  // dense: that tile's offset
+  auto sync_steady = [&](int k) {
+    wait_vmcnt<IPW>();
+    barrier_lds();
+    const int t = k + 3;
+    if (PAGED && t - pgw_t0 >= 64) fill_pgw(t);
+    const uint32_t dst = dst0 + (uint32_t)(t & 3) * (2 * G::TILE);
+#pragma unroll
+    for (int x = 0; x < IPW; ++x) {
+      int64_t off = next_off;
+      if (PAGED)
+        off = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)pgw_hi[x], t - pgw_t0) << 32) |
+                        (uint32_t)__builtin_amdgcn_readlane((int)pgw_lo[x], t - pgw_t0));
+      dma_rs<false>(dst + x * 1024, make_rsrc(hbase + off, reach), lane_off[x]);
+    }
+    next_off += 32 * st2;
+  };
+
   f32x16 s_cur = f32x16{};
   auto read_k = [&](int t, u32x4 (&kf)[KS]) {
     const uint32_t o = kofs + (uint32_t)(t & 3) * (2 * G::TILE);
@@ -251,7 +270,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 
   auto step = [&](auto masked_c, int k) {
     constexpr bool MASKED = decltype(masked_c)::value;
-    if (!v_wave && k > 0) sync(k);
+    if (!v_wave && (!MASKED || k > 0)) MASKED ? sync(k) : sync_steady(k);
     u32x4 kf[KS], vf[2][DT];
     u32x4 pk[2];
     {
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
             for (int e = 0; e < 4; ++e) odd |= nonfinite2<T>(vf[hh][dt][e]);
       }
     }
-    if (v_wave) sync(k);
+    if (v_wave) MASKED ? sync(k) : sync_steady(k);
     {
       f32x16 sn = f32x16{};
 #pragma unroll
@@ -382,7 +401,9 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     int k = 0;
     for (; k < k0; ++k) step(BoolC<true>{}, k);
     if (__ballot(mx == kNegInf) == 0ull) {
-      for (; k + 4 <= seen1 && k + 4 <= ntiles; k += 4) {
+      if (!PAGED) next_off = (int64_t)kl.base(t_lo + min(k + 3, ntiles - 1)) * st2;
+      const int k1 = k + 3 >= whole0 ? min(seen1, min(whole1, ntiles) - 3) : 0;
+      for (; k + 4 <= k1; k += 4) {
         step(BoolC<false>{}, k);
         step(BoolC<false>{}, k + 1);
         step(BoolC<false>{}, k + 2);

@@ -333,3 +333,22 @@ def test_streams_and_graphs(gpu):
         torch.cuda.synchronize()
         assert torch.equal(outs[0][0], eager[0]) and torch.equal(outs[0][1], eager[1])
         assert torch.equal(outs[1][0], want[2][0]) and torch.equal(outs[1][1], want[2][1])
+
+
+@pytest.mark.parametrize("M,page,D", [(20, 16, 64), (20, 8, 128), (3, 64, 128)])
+def test_many_tiles_of_one_split(gpu, M, page, D):
+    """A workgroup per CU, each over about 90 tiles: paged as dense bit by bit, some heads against float64."""
+    lens, window, sinks = [3001, 2950, 64, 2999, 3000, 0, 1500, 2960], 2900, 40
+    c = Case(gpu, 8, M, 32, 32, D, lens, BF16, page, seed=M + D)
+    lens_t = torch.tensor(lens, device=gpu)
+    dense = [x[c.table.long()].transpose(2, 3).reshape(8, -1, 32, D) for x in (c.k, c.v)]
+    a = window_attn_with_kvcache(c.q, c.k, c.v, window, sinks, lens_t, c.table, None, True)
+    b = window_attn_with_kvcache(c.q, *dense, window, sinks, lens_t, None, None, True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for i, h in ((0, 5), (3, 31), (6, 0)):
+        keys = oracle.visible(M, lens[i], window, sinks)
+        k, v = (x[i, :, h:h + 1].double().cpu().numpy() for x in dense)
+        want, wl_, absum, reach = oracle.attend(c.q[i, :, h:h + 1].double().cpu().numpy(), k, v, keys)
+        tol, ltol = bounds(BF16, BF16, want, wl_, absum, reach, window + sinks, D, np.abs(v).max())
+        assert (np.abs(a[0][i, :, h:h + 1].double().cpu().numpy() - want) <= tol).all()
+        assert (np.abs(a[1][i, h:h + 1].double().cpu().numpy() - wl_) <= ltol).all()
