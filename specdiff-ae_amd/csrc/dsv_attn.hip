@@ -109,26 +109,7 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i
 }
 
 
-// LDS-DMA: 16 bytes per lane, lane l lands at LDS m0 + 16*l.  K/V bytes are
-// read once per verify step: the loads are marked non-temporal (nt).
-// Through a buffer resource (hardware range check; out-of-range lanes read 0).
-__device__ __forceinline__ void dma_buf(uint32_t lds, const void* base, uint32_t range, uint32_t voff) {
-  const uint64_t p = (uint64_t)base;
-  i32x4 r;
-  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
-  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
-  r[2] = __builtin_amdgcn_readfirstlane((int)range);
-  r[3] = 0x00020000;
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(m0), "v"(voff), "s"(r)
-               : "memory", "m0");
-}
-// With a full per-lane address (keys clamped to valid ones by the caller).
-__device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(m0), "v"(vaddr) : "memory", "m0");
-}
-
+// K/V bytes are read once per verify step: the DMA loads are non-temporal.
 
 // Does element (i, j) of a dense tree-mask block keep the key?
 __device__ __forceinline__ bool tmask_keep(const AttnArgs& a, int b, int i, int j) {
@@ -440,7 +421,7 @@ __global__ void __launch_bounds__(512, 2) attn_splitk_kernel(const AttnArgs a) {
           const int c = is_v ? v_slot(CH, key_t, slot) : k_slot(CH, key_t, slot);
           vo = (uint32_t)(fast_lane_elem(src, is_v, nb, fast_lane_key(src, kb, kend, j, G::KPI, kii), c) * 2);
         }
-        dma_buf(dst, base + be, rsrc_range(is_v ? src.v_bytes : src.k_bytes, be), vo);
+        dma_rs(dst, make_rsrc(base + be, rsrc_range(is_v ? src.v_bytes : src.k_bytes, be)), vo);
       } else {
         const int c = is_v ? v_slot(CH, key_t, slot) : k_slot(CH, key_t, slot);
         const int64_t n = lane_key(src, kb, kend, key_t);

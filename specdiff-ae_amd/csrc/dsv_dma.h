@@ -1,11 +1,18 @@
-// dsv_dma.h — LDS-DMA helpers shared by the attention kernel and the fused
-// lm_head on gfx950.
+// dsv_dma.h — LDS-DMA helpers shared by the attention kernels on gfx950.
 //
 // buffer_load_dwordx4 ... offen lds moves 16 bytes per lane from global
 // memory straight into LDS: lane l of the instruction lands at LDS address
 // m0 + 16*l.  The source goes through a buffer resource (base, byte range):
 // the hardware checks every lane's offset against the range and returns
 // zeros past it.  Callers keep every destination below 64 KiB.
+//
+// Wait states: the hardware does not hold these loads back for a write of m0 by
+// the instruction before (one wait state is needed), nor for a resource whose
+// SGPRs a VALU instruction wrote (five: the compiler restores spilled SGPRs by
+// v_readlane), and the compiler looks for neither inside an asm block.  So each
+// block waits itself: s_mov of m0 and s_nop 3 make five.  (Four wait states more
+// measured 0.6%: a verify step over a 64K prefix 82.9 us, 83.4; a windowed chunk of
+// 8192 rows 536, 540.)
 #pragma once
 
 #include "dsv_internal.h"
@@ -40,11 +47,21 @@ __device__ __forceinline__ void dma_rs(uint32_t lds, i32x4 r_in, uint32_t voff) 
   for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r_in[i]);
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(m0), "v"(voff), "s"(r)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(m0), "v"(voff), "s"(r)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(r)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(r)
                  : "memory", "m0");
+}
+
+// The same from a full address per lane (valid ones: nothing is checked).
+template <bool NT = true>
+__device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(m0), "v"(vaddr) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
 }
 
 // Wait until at most N of this wave's vector-memory operations are pending.

@@ -75,14 +75,6 @@ __device__ __forceinline__ int again(int x) {
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// LDS-DMA of 16 bytes per lane; lane l lands at lds + 16 l.  From a per-lane
-// address, or from a uniform base plus a 32-bit lane offset through a buffer
-// resource whose range ends with the tensor.
-__device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
-}
-
 template <bool B>
 struct BoolC {
   static constexpr bool value = B;
@@ -195,7 +187,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       for (int x = 0; x < IPW; ++x) {
         const int l = again(lane);
         const int n = kl.read(kb + (j0 + x) * G::KPI + l / CH);
-        dma_lane(dst + x * 1024, hbase + key_off(a, PAGED, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
+        dma_lane<false>(dst + x * 1024, hbase + key_off(a, PAGED, sp2, st2, n, PAGED ? page_of(a, b, n) : 0) + chunk_of(x, l) * 16);
       }
     }
   };
