@@ -1901,6 +1901,9 @@ WinPlan win_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t D, int dty
             "key heads x rows <= 2^24, batch x query heads x rows <= 2^30)";
     return p;
   }
+  // (Beyond every key, either means all of them.)
+  window = std::min(window, dsv::kWinMaxKeys);
+  sinks = std::min(sinks, dsv::kWinMaxKeys);
   p.G = (int)(H / Hk);
   p.R = (int)R;
   p.MW = tree ? (int)((M + 63) / 64) : 0;
@@ -2041,7 +2044,7 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
       return fail(DSV_ERR_INVALID, "out or lse overlaps %s", in.name);
   if (overlap(extent_of("out", out), extent_of("lse", lse))) return fail(DSV_ERR_INVALID, "out overlaps lse");
 
-  // (Beyond every key, either means all of them.)
+  // (As win_plan takes them.)
   const int64_t W = std::min<int64_t>(window, dsv::kWinMaxKeys), S = std::min<int64_t>(sinks, dsv::kWinMaxKeys);
   // The kernel for many rows reads a DMA instruction's 4 or 8 keys through one
   // page, and a tile's 32 keys with 32-bit offsets from the first.

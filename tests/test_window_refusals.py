@@ -107,6 +107,22 @@ def test_workspace_sizes(dsv_lib):
         assert n(*bad) == 0, bad
 
 
+@pytest.mark.parametrize("big", [1 << 30, 1 << 62, (1 << 63) - 70, (1 << 63) - 2, (1 << 63) - 1])
+@pytest.mark.parametrize("M,tree", [(1, False), (5, False), (64, True), (300, False)])
+def test_workspace_of_a_window_beyond_every_key(dry, M, tree, big):
+    """The queried number of bytes is what the call asks for, up to the largest window and sinks; all mean every key."""
+    N = 50000
+    kv, q = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16).expand(1, N, 8, 128), torch.zeros(1, M, 32, 128, dtype=torch.bfloat16)
+    size = lambda w, s: dry.dsv_window_workspace_bytes(1, M, 32, 8, 128, _ext.DSV_BF16, N, w, s, int(tree))  # noqa: E731
+    assert size(big, 0) == size(N + M, 0) > 0
+    for window, sinks in [(big, 0), (9, big), (big, big)]:
+        n = size(window, sinks)
+        ws = torch.empty(n + 256, dtype=torch.uint8)
+        ptr = (ws.data_ptr() + 255) // 256 * 256
+        assert call(dry, B=1, M=M, H=32, Hk=8, D=128, q=q, k=kv, v=kv, window=window, sinks=sinks, nbytes=n, ws=ptr, lse=None,
+                    out=torch.zeros_like(q), parent=torch.zeros(M, dtype=torch.int32) if tree else None) == 0, _ext.last_error()
+
+
 def test_python_refusals(dsv_lib):
     q, k = torch.zeros(1, 2, 4, 64), torch.zeros(1, 9, 2, 64)
     with pytest.raises(RuntimeError):
