@@ -104,7 +104,7 @@ struct TreeParents {
   }
 };
 
-// The walks, at most M steps each.  Every thread of the workgroup calls it; ends
+// The walks, at most M nodes each (a row that leads into a cycle has depth M - 1).  Every thread of the workgroup calls it; ends
 // with a barrier.
 template <int ROWS, int NT>
 __device__ __forceinline__ void tree_rows(const WinArgs& a, const TreeParents<NT>& mine, int n0, int r0, TreeLds<ROWS>& t) {
@@ -120,7 +120,7 @@ __device__ __forceinline__ void tree_rows(const WinArgs& a, const TreeParents<NT
     // The ancestor at h hops stands h positions before the row: seen for h < W.
     uint64_t word = 0;
     int at = m >> 6, h = 0;
-    for (int x = m; x >= 0 && h <= M; x = t.par[x], ++h) {
+    for (int x = m; x >= 0 && h < M; x = t.par[x], ++h) {
       if (x >> 6 != at) {
         vis[at] |= word;
         word = 0;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void tree_rows(const WinArgs& a, const TreeParents<NT
       if (h < a.W) word |= 1ull << (x & 63);
     }
     vis[at] |= word;
-    const int depth = min(h - 1, M);
+    const int depth = h - 1;
     t.depth[threadIdx.x] = depth;
     // And those at positions below the sinks' end.
     if (n0 < a.S) {

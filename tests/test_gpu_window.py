@@ -146,6 +146,16 @@ def test_tree_shapes(gpu):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,H", [(70, 4), (12, 2)])
+def test_cyclic_tree_in_a_long_window(gpu, M, H, dtype):
+    """Nodes whose parents form one cycle: a walk ends after M nodes, at depth M - 1 (every prefix border shows it)."""
+    cycle = [M - 1] + list(range(M - 1))
+    c = Case(gpu, 1, M, H, 2, 64, [M + 100], dtype, 16, seed=M)
+    for window, sinks in [(100, 0), (M + 1, 3), (M - 1, 0), (30, M + 100 - 5), (1, 100 + M - 1), (1, 100 + M)]:
+        c.check(window, sinks, cycle)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_lengths(gpu, dtype):
     """Lengths as an int, a 0-d and an int64 tensor, None; beyond the cache; a window beyond every length."""
     c = Case(gpu, 2, 3, 4, 2, 64, [100, 100], dtype, 16, cap=112)
