@@ -17,8 +17,9 @@
 // positions, so a mask costs no memory.
 //
 // Scores, sums and running maxima are fp32 (log2 domain); the probabilities
-// are rounded to the inputs' 16-bit type for the second matrix product (off by
-// half a step of values at most one, the inputs' own rounding); their sum
+// are rounded to the inputs' 16-bit type for the second matrix product, the type
+// of the values that they weigh (off by half a step of each: 2^-8 of it in bf16,
+// 2^-11 in fp16, which holds them times a power of two, see kProbShift); their sum
 // takes them unrounded.  Partial outputs of splits are fp32.
 //
 // Values of keys that a row does not see never reach it, whatever they hold: a
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
   constexpr int NL = 32 / KPI;        // load instructions per tile and half
   constexpr int KS = D / 32;          // k-steps of Q.K^T
   constexpr int DT = D / 16;          // d tiles of P.V
+  constexpr int SHIFT = kProbShift<T, 15>;  // (the maximum is exact: probabilities are at most 2^15)
   // Row strides of the LDS images: K rows shift by 4 banks a key (b128 reads
   // of 16 keys), V rows by 8 (transposed reads of 16 keys x 32 bytes): free of
   // bank conflicts.  K, then V, then the wave's partial output use one region.
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
       for (int d = 0; d < DT; ++d) acc[d] *= al;
       mx = mn;
     }
-    const float ms = mx == kNegInf ? 0.f : mx;
+    const float ms = mx == kNegInf ? 0.f : mx - (float)SHIFT;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -ms));
@@ -239,8 +241,11 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
     exact_rows<T, D, 16>(&args_again(), &tl, b, kvh, split, rb, (int)((int64_t)kl.nt * split / a.splits), t_end, wave, 16, NW);
     return;
   }
-  // ---- the waves' rows joined
-  const float lt = row_sum(ls);
+  // ---- the waves' rows joined (sums as without the factor: by exact products)
+  constexpr float kBack = 1.f / (1 << SHIFT);
+  const float lt = row_sum(ls) * kBack;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] *= kBack;
   if (lg == 0) {
     sm_m[wave][lr] = mx;
     sm_l[wave][lr] = lt;

@@ -47,6 +47,15 @@ __device__ __forceinline__ uint32_t nonfinite2<F16>(uint32_t x) {
   return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
+// fp16 probabilities are held times 2^N of this, N the power that a kernel's own
+// bound on them leaves room for: below 2^-14 fp16 loses bits and below 2^-25 all of
+// them, and a key 17 above 2^18 others (whose sum is 2^18 e^-17 = 0.01 of its own
+// weight) would hide them.  bf16 has fp32's range.
+template <typename T, int N>
+constexpr int kProbShift = 0;
+template <int N>
+constexpr int kProbShift<F16, N> = N;
+
 // Lanes of a wave read LDS that other lanes of it wrote (LDS operations of a
 // wave execute in order; this keeps the compiler from moving them).
 __device__ __forceinline__ void wave_lds_fence() {

@@ -30,11 +30,15 @@ namespace dsv {
 
 namespace {
 
-// The running maximum used for the exponentials may lag the true one by this
-// much (log2 units), and, on unmasked tiles, a lane's probabilities may sum up to
-// 2^kSumTau before the tile is redone: every probability then stays below what
-// its 16-bit type holds (f16: 65504).
+// The running maximum used for the exponentials may lag the true one by kRescaleTau
+// (log2 units) on masked tiles; unmasked ones are redone with the true one when a
+// lane's 16 probabilities sum to more than kSumBound.  fp16 probabilities (times
+// 2^10) stay below what the type holds either way: 2^(10 + 5) and kSumBound, and
+// with the true maximum a lane sums to 2^14 at most, so nothing is redone twice.
+template <typename T>
 constexpr float kRescaleTau = 8.0f;
+template <>
+constexpr float kRescaleTau<F16> = 5.0f;
 template <typename T>
 constexpr float kSumBound = 65536.f;
 template <>
@@ -87,6 +91,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
   constexpr int CH = G::CH;
+  constexpr int SHIFT = kProbShift<T, 10>;
   constexpr int IPW = 2 * G::NINS / NW;  // DMA instructions per wave and tile
   static_assert(IPW * NW == 2 * G::NINS && G::NINS % IPW == 0, "K and V DMA halves map to wave halves");
   static_assert(G::STAGES == 4 && NW * 32 * D * 2 <= G::RING, "");
@@ -281,9 +286,9 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
         for (int v = 0; v < 16; ++v) s_cur[v] = ((kv >> v) & 1u) ? s_cur[v] : kNegInf;
        }
       }
-      auto rescale = [&]() {
+      auto rescale = [&](float tau) {
         const float mt = xor32_max(max16(s_cur)) * scale_log2;
-        if (__ballot(mt > mx + kRescaleTau) != 0ull) {
+        if (__ballot(mt > mx + tau) != 0ull) {
           const float mn = __builtin_elementwise_maximum(mx, mt);
           const float al = (mn == mx) ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
           mx = mn;
@@ -292,9 +297,9 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
           for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
         }
       };
-      if (MASKED && (drops || __ballot(mx == kNegInf) != 0ull)) rescale();
+      if (MASKED && (drops || __ballot(mx == kNegInf) != 0ull)) rescale(kRescaleTau<T>);
       auto exps = [&](bool with_v) {
-        const float ms = (mx == kNegInf) ? 0.f : mx;
+        const float ms = (mx == kNegInf) ? 0.f : mx - (float)SHIFT;
         float ts = 0.f;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
       };
       float ts = exps(true);
       if (!drops && __ballot(!(ts <= kSumBound<T>)) != 0ull) {
-        rescale();
+        rescale(0.f);
         ts = exps(false);
       }
       lsum += ts;
@@ -429,7 +434,11 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
     exact_rows<T, D, 256>(&z, &tl, b, kvh, split, rb, t_lo, t_lo + ntiles, wid * 32, wid * 32 + 32, 1);
     return;
   }
-  const float ltot = xor32_sum(lsum);
+  // (Sums as without the factor: by exact products.)
+  constexpr float kBack = 1.f / (1 << SHIFT);
+  const float ltot = xor32_sum(lsum) * kBack;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] *= kBack;
   const Row row = row_of(z, min(r_ep, z.R - 1));
   const int h = kvh * z.G + row.g;
   // Accumulator value v of d tile dt holds d = 32*dt + 8*(v/4) + 4*lge + v%4.
