@@ -2059,8 +2059,6 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   a.q_sh = q->stride[2];
   a.k = static_cast<const uint16_t*>(k->data);
   a.v = static_cast<const uint16_t*>(v->data);
-  a.k_bytes = span_bytes(k);
-  a.v_bytes = span_bytes(v);
   a.n_keys = n;
   a.B = (int)B;
   a.M = (int)M;

@@ -444,7 +444,8 @@ __global__ void __launch_bounds__(kPT) compact_plan_kernel(const CompactArgs a) 
   }
   int64_t n;
   scan1(mine, scratch, n);
-  const int64_t holes = scan_pages(
+  // (As many as are moved: n pages are in use, those below n and the moved ones.)
+  scan_pages(
       b, first, 0, n, b.P, cnt, [](int64_t, int32_t ref) { return ref <= 0; }, [&](int64_t i, int64_t r) { a.dst[r] = (int32_t)i; });
   const int64_t moved = scan_pages(
       b, first, n, b.P, b.P, cnt,
@@ -453,7 +454,6 @@ __global__ void __launch_bounds__(kPT) compact_plan_kernel(const CompactArgs a) 
         return ref > 0;
       },
       [&](int64_t i, int64_t r) { a.src[r] = (int32_t)i; });
-  (void)holes;  // equal: n pages are in use, those below n and the moved ones
   __syncthreads();
   for (int64_t r = threadIdx.x; r < moved; r += kPT) {
     const int32_t s = a.src[r], d = a.dst[r];

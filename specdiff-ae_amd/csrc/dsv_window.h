@@ -15,7 +15,6 @@ struct WinArgs {
   int64_t q_sb, q_sm, q_sh;
   const uint16_t* k; int64_t k_sb, k_sp, k_sh, k_st;
   const uint16_t* v; int64_t v_sb, v_sp, v_sh, v_st;
-  int64_t k_bytes, v_bytes;                // spans of the views
   const void* pt; int pt_i64, ps_shift;    // page table (nullptr: dense)
   int64_t pt_sb, n_phys;
   const void* seqlens; int seqlens_i64;    // optional [B]
@@ -29,7 +28,7 @@ struct WinArgs {
   int rows_per_block, n_rb, splits;
   float* opart;                            // [B, Hk, splits, R, D] (splits > 1), relative to the maximum
   float2* ml;                              // [B, Hk, splits, R] (maximum in log2 units, sum)
-  void* out; int out_dtype, out_vec;       // out_vec: rows take 16-byte stores
+  void* out; int out_dtype, out_vec;       // out_vec: rows take vector stores
   int64_t o_sb, o_sm, o_sh;
   float* lse; int64_t l_sb, l_sm, l_sh;
 };

@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
         for (int e = 0; e < N; ++e) o[e] *= inv;
-        store_out<N>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
+        store_out(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
         if (d0 == 0 && a.lse != nullptr)
           a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
       } else {
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] *= inv;
-    store_out<N>(a, b * a.o_sb + mm * a.o_sm + hh * a.o_sh + d0, o);
+    store_out(a, b * a.o_sb + mm * a.o_sm + hh * a.o_sh + d0, o);
     if (d0 == 0 && a.lse != nullptr)
       a.lse[b * a.l_sb + mm * a.l_sm + hh * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
   } else {
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= inv;
   const int mm = r / a.G, h = kvh * a.G + r - mm * a.G;
-  store_out<4>(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
+  store_out(a, b * a.o_sb + mm * a.o_sm + h * a.o_sh + d0, o);
   if (d0 == 0 && a.lse != nullptr)
     a.lse[b * a.l_sb + mm * a.l_sm + h * a.l_sh] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
 }

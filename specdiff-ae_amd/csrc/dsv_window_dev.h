@@ -193,34 +193,28 @@ __device__ __forceinline__ int len_of(const WinArgs& a, int b) {
   return (int)n;
 }
 
-// Writes N consecutive output elements.
-template <int N>
-__device__ __forceinline__ void store_out(const WinArgs& a, int64_t off, const float (&x)[N]) {
-  static_assert(N == 4 || N == 8, "");
+// Writes four consecutive output elements.
+__device__ __forceinline__ void store_out(const WinArgs& a, int64_t off, const float (&x)[4]) {
   if (a.out_dtype == 2) {
     float* o = reinterpret_cast<float*>(a.out) + off;
     if (a.out_vec) {
-#pragma unroll
-      for (int i = 0; i < N; i += 4) *reinterpret_cast<f32x4*>(o + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+      *reinterpret_cast<f32x4*>(o) = f32x4{x[0], x[1], x[2], x[3]};
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = x[i];
+      for (int i = 0; i < 4; ++i) o[i] = x[i];
     }
     return;
   }
   uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + off;
-  uint32_t w[N / 2];
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i)
+  for (int i = 0; i < 2; ++i)
     w[i] = a.out_dtype == 0 ? pack2<BF16>(x[2 * i], x[2 * i + 1]) : pack2<F16>(x[2 * i], x[2 * i + 1]);
   if (a.out_vec) {
-    if constexpr (N == 8)
-      *reinterpret_cast<u32x4*>(o) = u32x4{w[0], w[1], w[2], w[3]};
-    else
-      *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
+    *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    for (int i = 0; i < 4; ++i) o[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
   }
 }
 

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const float x[4] = {acc[dt][4 * q4] * inv, acc[dt][4 * q4 + 1] * inv, acc[dt][4 * q4 + 2] * inv, acc[dt][4 * q4 + 3] * inv};
-        store_out<4>(a, off + 32 * dt + 8 * q4 + 4 * lge, x);
+        store_out(a, off + 32 * dt + 8 * q4 + 4 * lge, x);
       }
     return;
   }
