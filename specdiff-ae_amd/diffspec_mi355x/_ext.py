@@ -171,10 +171,16 @@ def require_gpu(*tensors: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+# The current stream's handle without the Stream object around it, which takes 2 us
+# a call.  No public function gives it: where a torch build lacks this one, the
+# object's is used.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device: torch.device) -> ctypes.c_void_p:
-    # (The handle itself: building the Stream object around it took 2 us a call.)
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(
-        torch.cuda.current_device() if device.index is None else device.index))
+    if _raw_stream is None:
+        return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return ctypes.c_void_p(_raw_stream(torch.cuda.current_device() if device.index is None else device.index))
 
 
 _HERE = contextlib.nullcontext()
@@ -182,7 +188,7 @@ _HERE = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """Context in which launches go to ``device`` (a no-op where it is current)."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def scratch(nbytes: int, device: torch.device):
