@@ -191,6 +191,11 @@ def on_device(device: torch.device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def i64(x) -> int:
+    """An integer argument as the C ABI takes it: beyond 64 bits the nearest end (ctypes would drop the high bits)."""
+    return min(max(int(x), -1 << 63), (1 << 63) - 1)
+
+
 def scratch(nbytes: int, device: torch.device):
     """(tensor that holds the workspace, its address), nothing where none is needed."""
     if nbytes == 0:

@@ -76,7 +76,7 @@ def extend_pages(page_table: torch.Tensor, refcount: torch.Tensor, seqlens: torc
         info = torch.empty(3, dtype=torch.int32, device=dev)
         ws = _page_ws(lib, refcount, page_table, 0, dev)
         rc = lib.dsv_pages_extend(_ext.desc(page_table), _ext.desc(refcount), _ext.desc(seqlens), _ext.desc(new_lens),
-                                  int(page_size), _ext.desc(info), ws.data_ptr(), ws.numel(), _ext.stream_of(dev))
+                                  _ext.i64(page_size), _ext.desc(info), ws.data_ptr(), ws.numel(), _ext.stream_of(dev))
     _ext.check(rc, "extend_pages")
     return info
 
@@ -97,7 +97,7 @@ def free_pages(page_table: torch.Tensor, refcount: torch.Tensor, seqlens: torch.
     lib = _ext.load()
     with _ext.on_device(dev):
         rc = lib.dsv_pages_free(_ext.desc(page_table), _ext.desc(refcount), _ext.desc(seqlens), _ext.desc(seqs),
-                                int(page_size), int(window or 0), int(sinks), _ext.stream_of(dev))
+                                _ext.i64(page_size), _ext.i64(window or 0), _ext.i64(sinks), _ext.stream_of(dev))
     _ext.check(rc, "free_pages")
 
 

@@ -62,7 +62,7 @@ def window_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         Hk, cap = k_cache.shape[1], page_table.shape[-1] * k_cache.shape[2]
     else:
         Hk, cap = k_cache.shape[2], k_cache.shape[1]
-    n = cap
+    n, window, sinks = cap, _ext.i64(window), _ext.i64(sinks)
     if lens is not None:
         if lens.dim() == 0:
             lens = lens.reshape(1).expand(B).contiguous()
@@ -78,10 +78,10 @@ def window_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         out = torch.empty((B, M, H, D), dtype=out_dtype or q.dtype, device=dev)
         lse = torch.empty((B, H, M), dtype=torch.float32, device=dev) if return_softmax_lse else None
         q_d = _ext.desc(q)
-        n_ws = lib.dsv_window_workspace_bytes(B, M, H, Hk, D, q_d.dtype, n, int(window), int(sinks), int(parent is not None))
+        n_ws = lib.dsv_window_workspace_bytes(B, M, H, Hk, D, q_d.dtype, n, window, sinks, int(parent is not None))
         ws, ws_ptr = _ext.scratch(n_ws, dev)
         rc = lib.dsv_window_attention(q_d, _ext.desc(k_cache), _ext.desc(v_cache), _ext.desc(page_table),
-                                      _ext.desc(lens), n, int(window), int(sinks), _ext.desc(parent), _ext.desc(out),
+                                      _ext.desc(lens), n, window, sinks, _ext.desc(parent), _ext.desc(out),
                                       _ext.desc(lse), ws_ptr, n_ws, _ext.stream_of(dev))
     _ext.check(rc, "window_attn_with_kvcache")
     return (out, lse) if return_softmax_lse else out

@@ -140,6 +140,16 @@ def test_free_behind_the_window(gpu, sinks, window):
     assert sum(p.ref) == 0
 
 
+@pytest.mark.parametrize("huge", [1 << 62, 1 << 63, (1 << 64) + 1])
+def test_free_behind_a_window_beyond_64_bits(gpu, huge):
+    """Nothing lies behind a window (or outside sinks) beyond every token."""
+    p = Pool(gpu, B=2, P=40, n_log=20)
+    p.extend([79, 33])
+    p.free([0, 1], window=huge)
+    p.free([0, 1], window=1, sinks=huge)
+    assert sum(p.ref) == 20 + 9
+
+
 @pytest.mark.parametrize("dtype,ps,Hk,D,L", [(torch.bfloat16, 16, 8, 128, 2), (torch.float16, 1, 1, 8, 1),
                                              (torch.float32, 8, 3, 20, 3), (torch.bfloat16, 64, 5, 72, 1)])
 def test_random_calls(gpu, dtype, ps, Hk, D, L):

@@ -162,3 +162,17 @@ def test_hidden_tree_values_shared_out(gpu, dsv_lib, dtype):
     fixed = out[0].clone()
     fixed[0, sees, 2:, 7] = ref[0, sees, 2:, 7]
     c.check(window, sinks, parent, result=(fixed, out[1]))
+
+
+@pytest.mark.parametrize("M", [1, 40])
+@pytest.mark.parametrize("huge", [(1 << 63) - 1, 1 << 63, (1 << 64) + 9, 10 ** 30])
+def test_windows_beyond_64_bits(gpu, huge, M):
+    """A window or sinks beyond every key mean all of them, however large the number."""
+    c = Case(gpu, 2, M, 8, 2, 64, [1500, 1500], BF16, 16, seed=M)
+    want = c.check(1500, 0)
+    for window, sinks in ((huge, 0), (1, huge)):
+        got = window_attn_with_kvcache(c.q, c.k, c.v, window, sinks, 1500, c.table, None, True)
+        assert torch.allclose(got[0].float(), want[0].float(), rtol=2 ** -6, atol=2 ** -6)
+        c.check(1500, 0, result=got)
+    with pytest.raises(RuntimeError):
+        window_attn_with_kvcache(c.q, c.k, c.v, -huge, 0, 1500, c.table)

@@ -133,6 +133,11 @@ def test_python_refuses_cpu_tensors(dsv_lib):
         speculative_accept(torch.zeros(1, 2, 4), torch.zeros(1, 2), torch.zeros(1, 1), torch.zeros(1, 2))
 
 
+def test_integers_beyond_64_bits():
+    assert [_ext.i64(x) for x in (0, -5, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 9, -2 ** 63 - 1, np.int64(7))] == \
+        [0, -5, 2 ** 63 - 1, 2 ** 63 - 1, 2 ** 63 - 1, -2 ** 63, 7]
+
+
 def test_oracle_keeps_the_targets_distribution():
     """The rule itself, over every draft and the numbers integrated: P(first token) is the target's row."""
     rng = np.random.default_rng(0)
