@@ -396,8 +396,9 @@ void check_window_block(const WinArgs& a, int D, const WinExtents& ex, int b, in
       if (!ck.ok) return;
     }
   }
-  // Every key that a row sees, in one tile (trees: a row anywhere from n0 on).
-  if ((int64_t)kl.nt * 32 > 1 << 16 || kl.nt == 0) return;
+  // Every key that a row sees, in one tile (trees: a row anywhere from n0 on); not
+  // in caches so long that the walk over their keys takes seconds.
+  if ((int64_t)kl.nt * 32 > 1 << 16 || kl.nt == 0 || len > 1 << 20) return;
   std::vector<uint8_t> in(len + 64, 0);
   for (int t = 0; t < kl.nt; ++t)
     for (int i = 0; i < 32; ++i)

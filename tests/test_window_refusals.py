@@ -1,5 +1,7 @@
 """Refusals and key geometry of the windowed attention (CPU only: nothing is launched)."""
 
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -94,6 +96,16 @@ def test_every_address_and_key(dry, seed):
         kw.update(n_keys=max(1, N // 2))
     assert call(dry, **kw) == 0, _ext.last_error()
     assert dry.dsv_dry_run_checks() > 0
+
+
+@pytest.mark.parametrize("M", [1, 64])
+def test_dry_run_of_the_longest_cache(dry, M):
+    """2^30 keys: the tiles' addresses are walked, not every key of the cache."""
+    kv, q = torch.zeros(1, 1, 1, 64).expand(1, 1 << 30, 2, 64), torch.zeros(1, M, 4, 64)
+    t0 = time.monotonic()
+    assert call(dry, B=1, M=M, q=q, k=kv, v=kv, lens=torch.zeros(1, dtype=torch.int32), window=512, sinks=4) == 0, _ext.last_error()
+    assert dry.dsv_dry_run_checks() > 0
+    assert time.monotonic() - t0 < 20.0  # (milliseconds; minutes if every key were walked)
 
 
 def test_workspace_sizes(dsv_lib):
