@@ -26,7 +26,10 @@
 // the tree by itself (no wait stands between the walk and the sweep), and a second
 // launch, one wave a tree, draws from their sums; with a tree per CU, or a short
 // row, the one workgroup draws as well.  64 chains of 5 over 128256 fp32 entries:
-// one workgroup each 27 us, four each 19.5 (16.5 + 3.8).  A wave sums a contiguous
+// one workgroup each 27 us, four each 19.5 (16.5 + 3.8).  The mass that a further
+// sibling's test needs is not shared out: every workgroup of the tree sweeps the
+// whole row for it (sampled trees of 64 nodes over 128256 entries, in a graph: one
+// 23 to 25 us, four 38 to 48).  A wave sums a contiguous
 // slot of the row, 8 entries a lane at a time with the next ones in flight.
 //
 // Reference context: draft/tree_verification.py:100-182 (the walk whose

@@ -36,8 +36,10 @@
 // ds_read_b128, V transposed by ds_read_b64_tr_b16.  Splits over the keys fill
 // the GPU when there are few rows; win_merge_kernel joins them.  64 sequences of
 // one token through 4096 keys (32 query heads, 8 key heads of 128, pages of 64):
-// 179 us, 5.5 TB/s, the rate of a large copy.  One sequence through 1024 keys: 15
-// us, a chain of latencies (arguments, length, page, four tiles a wave).  (Each lane
+// 179 us, 5.5 TB/s, 88% of what a kernel that only reads reaches (6.2).  One
+// sequence through 1024 keys: 15 us, 5 of them arguments, length and page; in the
+// rest 8 workgroups read 0.5 MB each, what one CU fetches (more workgroups would
+// need the merge, a launch more).  (Each lane
 // computing the offsets of the keys that it loads took 17.5: 64-bit products.)
 //
 // Reference context: runtime/attention_compat.py:103-132 (the cache call whose

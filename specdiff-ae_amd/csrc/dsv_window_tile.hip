@@ -15,12 +15,12 @@
 //
 // Bound by the matrix products and the softmax between them, about 1.0 us a tile
 // of 256 rows and D = 128 with all CUs at work.  8192 rows through 4096 keys (32
-// query heads, 8 key heads of 128, bf16): 512 us, 1.07 PFLOP/s, seven eighths of
-// what a large library product reaches (529 with the tests of each barrier's loads
-// in the long loop).  Two trees of 64 nodes through 8192 keys
-// (one block of rows per key head, 16 splits): 39 us, of which the 16 tiles take
-// 19, arguments, length, pages and first tile 7, the fp32 partials 3 and the
-// launch the rest; the merge follows with 8.
+// query heads, 8 key heads of 128, bf16): 504 to 536 us by card, 1.03 to 1.09
+// PFLOP/s, 84 to 89% of what a large library product reaches (on one card 512, and
+// 529 with the tests of each barrier's loads in the long loop).  Two trees of 64
+// nodes through 8192 keys (one block of rows per key head, 16 splits): 39 us, of
+// which the 16 tiles take 19, arguments, length, pages and first tile 7, the fp32
+// partials 3 and the launch the rest; the merge follows with 8.
 
 #include "dsv_attn_geo.h"
 #include "dsv_dma.h"
