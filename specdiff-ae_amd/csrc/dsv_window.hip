@@ -26,7 +26,8 @@
 // masked score is replaced, keys that no row of a workgroup sees are not read (a
 // seen one is, in their place), and where V holds infinities or NaN in a tile of
 // which some row drops keys, the rows are computed once more without matrix
-// products (exact_rows; in the product 0 * inf would be NaN).
+// products (exact_rows; in the product 0 * inf would be NaN).  So are rows whose
+// scores are beyond 2^22, where the exponents lose their last bits before the point.
 //
 // win_rows_kernel (up to 16 rows: single tokens, short chunks): bound by
 // reading K and V.  Eight waves share a workgroup's tiles, each with a softmax of
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
   }
 
   float mx = kNegInf, ls = 0.f;
-  uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of
+  uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of, far scores
   f32x4 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_kernel(const WinArgs 
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= al;
       mx = mn;
+      odd |= far_score(mx) ? 0x80008000u : 0u;
     }
     const float ms = mx == kNegInf ? 0.f : mx - (float)SHIFT;
 #pragma unroll
@@ -413,6 +415,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) win_rows_f32_kernel(const WinA
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= al;
       mx = mn;
+      odd |= far_score(mx);
     }
     const float ms = mx == kNegInf ? 0.f : mx;
 #pragma unroll

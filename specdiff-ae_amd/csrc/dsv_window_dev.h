@@ -56,6 +56,14 @@ constexpr int kProbShift = 0;
 template <int N>
 constexpr int kProbShift<F16, N> = N;
 
+// A running maximum from here on: the product of a score and the exponent's scale is
+// off by 2^-24 of itself, so a probability by 2^0.25 at 2^22 (a factor that a row's
+// sum shares) and by more than fp16, later fp32, holds beyond.  Such rows are
+// computed by exact_rows, which takes differences of scores.
+__device__ __forceinline__ bool far_score(float m) {
+  return fabsf(m) >= 4194304.f && fabsf(m) < __builtin_huge_valf();
+}
+
 // Lanes of a wave read LDS that other lanes of it wrote (LDS operations of a
 // wave execute in order; this keeps the compiler from moving them).
 __device__ __forceinline__ void wave_lds_fence() {
@@ -229,8 +237,10 @@ __device__ __forceinline__ const WinArgs& args_again() {
 
 // Rows [i0, i1) by step of a workgroup once more, by one wave, from memory and
 // without matrix products, where V holds infinities or NaN in keys that some of
-// the rows do not see: in the product 0 * inf would reach those rows.  A lane
-// takes a key of 64 for the scores and D / 64 columns for the sums.
+// the rows do not see (in the product 0 * inf would reach those rows), or where a
+// row's scores are so large that their product with the exponent's scale is off by
+// powers of two (the maximum is held and subtracted as a score).  A lane takes a key
+// of 64 for the scores and D / 64 columns for the sums.
 template <typename T>
 struct Elem {
   typedef uint16_t type;
@@ -281,10 +291,10 @@ __device__ __noinline__ void exact_rows(const WinArgs* ap, const TreeLds<ROWS>* 
       float mt = s;
 #pragma unroll
       for (int y = 1; y < 64; y <<= 1) mt = fmaxf(mt, __shfl_xor(mt, y));
-      const float mn = fmaxf(m, mt * a.scale_log2), ms = mn == kNegInf ? 0.f : mn;
-      const float al = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      const float mn = fmaxf(m, mt), ms = mn == kNegInf ? 0.f : mn;
+      const float al = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
       m = mn;
-      const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, a.scale_log2, -ms)) : 0.f;
+      const float p = seen ? __builtin_amdgcn_exp2f((s - ms) * a.scale_log2) : 0.f;
       float ps = p;
 #pragma unroll
       for (int y = 1; y < 64; y <<= 1) ps += __shfl_xor(ps, y);
@@ -299,6 +309,7 @@ __device__ __noinline__ void exact_rows(const WinArgs* ap, const TreeLds<ROWS>* 
         for (int e = 0; e < N; ++e) o[e] = fmaf(pn, El::get(v[e]), o[e]);
       }
     }
+    m *= a.scale_log2;
     if (a.splits > 1) {
       const int64_t pr = ((int64_t)(b * a.Hk + kvh) * a.splits + split) * a.R + r;
 #pragma unroll

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
 
   f32x16 acc[DT];
   float mx = kNegInf, lsum = 0.f;
-  uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of
+  uint32_t odd = 0;  // infinite or NaN entries of V in tiles that some row drops keys of, far scores
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
 
@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(512, 2) win_tile_kernel(const WinArgs a) {
           const float mn = __builtin_elementwise_maximum(mx, mt);
           const float al = (mn == mx) ? 1.f : __builtin_amdgcn_exp2f(mx - mn);
           mx = mn;
+          odd |= far_score(mx) ? 1u : 0u;
           lsum *= al;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;

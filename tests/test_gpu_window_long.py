@@ -176,3 +176,32 @@ def test_windows_beyond_64_bits(gpu, huge, M):
         c.check(1500, 0, result=got)
     with pytest.raises(RuntimeError):
         window_attn_with_kvcache(c.q, c.k, c.v, -huge, 0, 1500, c.table)
+
+
+@pytest.mark.parametrize("dtype,power", [(F16, 9), (F16, 11), (F16, 12), (F16, 13), (F16, 15), (BF16, 11), (BF16, 13), (BF16, 16),
+                                         (BF16, 20), (BF16, 40), (F32, 11), (F32, 13), (F32, 16), (F32, 20), (F32, 40)])
+@pytest.mark.parametrize("level", [0.25, 0.2744140625, 0.3056640625, 0.33203125])
+@pytest.mark.parametrize("M,H,B", [(1, 2, 1), (3, 2, 150), (40, 1, 1), (200, 1, 1), (20, 1, 260)])
+def test_scores_beyond_the_exponents_resolution(gpu, dtype, power, level, M, H, B):
+    """Scores around 2^(2 power + 1), whose product with the exponent's scale is off by more than a probability may be.
+
+    One key's score is twice the next one's, so its value is the output: off by
+    the rounding of its probability and the output's own; the score is exact (equal
+    powers of two, eight bits of level) and the log-sum-exp two fp32 products of it.
+    """
+    N, D, window = 1500, 64, 1200
+    g = torch.Generator().manual_seed(power)
+    sign = torch.where(torch.rand((1, 1, H, 1), generator=g) < 0.5, -1.0, 1.0)
+    q = (2.0 ** power * sign).expand(B, M, H, D).to(dtype).to(gpu)
+    k = torch.zeros((1, N, H, D), dtype=dtype)
+    top = N - M - 40
+    for n, f in ((top - 900, level / 4), (top - 500, level / 2), (top, level)):
+        k[0, n] = (f * 2.0 ** power * sign[0, 0]).expand(H, D).to(dtype)
+    v = torch.randn((1, N, H, D), generator=g).to(dtype)
+    k, v = k.to(gpu), v.to(gpu)
+    out, lse = window_attn_with_kvcache(q, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), window, 0, return_softmax_lse=True)
+    want = v[0, top].double().expand(B, M, H, D)
+    step = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    assert bool(((out.double() - want).abs() <= want.abs() * (2.02 * step + 2.0 ** -20)).all())
+    score = float((q[0, 0, 0].double() * k[0, top, 0].double()).sum()) / D ** 0.5
+    assert bool(((lse.double() - score).abs() <= score * 2.0 ** -21).all())
