@@ -63,6 +63,16 @@ def test_large_vocabulary(gpu):
     check(gpu, *make(2, 5, 128256, torch.bfloat16, False, seed=10))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,gap", [(1, 0.8), (4, 3.0)])
+def test_sampled_trees_over_a_large_vocabulary(gpu, T, gap, dtype):
+    """Siblings' masses where a row is shared out over workgroups, each of which sums the whole row for them."""
+    p, q, draft, parent, u = make(T, 13, 128256, dtype, True, seed=T, gap=gap, peak=1.0)
+    check(gpu, p, q, draft, parent, u)
+    # Every number the largest: all siblings of every node on the way are tested that the rule can reject.
+    check(gpu, p, q, draft, parent, torch.full_like(u, 0.99999994))
+
+
 def test_1024_nodes_and_unordered_trees(gpu):
     """A child may have a lower index than its parent; malformed parents belong to nobody."""
     p, q, draft, parent, u = make(2, 1024, 40, torch.float32, True, seed=3, peak=1.0)
