@@ -85,8 +85,8 @@ int dsv_set_timing_events(void* start_event, void* stop_event);
  * access outside the extent of its argument (pointers are only compared,
  * never dereferenced, so the call runs on machines without a GPU).
  * dsv_window_attention walks the keys of its row blocks in the same way (many
- * blocks, tiles and rows by samples).  dsv_spec_accept and the dsv_pages_* calls
- * validate and plan only.
+ * blocks, tiles and rows by samples).  dsv_spec_accept, the dsv_pages_* calls,
+ * dsv_token_slots and the dsv_latent_* calls validate and plan only.
  * dsv_dry_run_checks() returns the number of checks the last dry run made.
  */
 int dsv_set_dry_run(int enable);
@@ -610,6 +610,124 @@ int dsv_pages_free(const dsv_tensor* page_table, const dsv_tensor* refcount,
 int dsv_pages_compact(const dsv_tensor* kv_pages, const dsv_tensor* page_table,
                       const dsv_tensor* refcount, dsv_tensor* info,
                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* A cache of one latent vector per token                                     */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Models with latent attention keep, of every token, one vector that all heads
+ * share and a small rotated key part: a cache row of dc + dr entries, rows [P, page,
+ * dc + dr] of a page pool or [B, N, dc + dr] of a dense cache.  (For dsv_pages_fork and
+ * dsv_pages_compact a pool [L, P, page, dc + dr] is viewed as [L, 2, P, 1, page,
+ * (dc + dr) / 2], the halves of a row in the place of K and V.)
+ */
+
+/*
+ * Block tables and slot maps of a step's requests, in place of the per-token host
+ * bookkeeping of PagedKVCache.write_kv (core/kv_cache/paged_kv.py:168-223).  Request i
+ * is sequence seqs[i], whose last new_lens[i] tokens of seqlens (dsv_pages_extend has
+ * given them pages) are new; in request order they stand at cu_seqlens[i] ..
+ * cu_seqlens[i + 1].
+ *   page_table  [B, n_logical] int32, innermost stride 1;  page_size a power of two
+ *   seqlens     [B] int32|int64, contiguous (clamped to the table's tokens)
+ *   new_lens    [n] int32|int64 (clamped to the sequence's length)
+ *   seqs        optional [n] int32|int64 (ndim 0: request i is sequence i); a
+ *               sequence out of range is an empty request
+ *   slots       [capacity] int64: page * page_size + offset of every new token, -1
+ *               where the table names no page and behind the last token
+ *   positions, requests  [capacity] int32: its position and request (-1 behind the
+ *               last); tokens beyond the capacity are left out
+ *   cu_seqlens  [n + 1] int32 (at most 2^31 - 1)
+ *   block_table [n, n_logical] int32: the requests' page lists, -1 behind their lengths
+ *   lens        [n] int32: the requests' lengths
+ * B, n <= 2^17; capacity <= 2^30; table rows below 2^31 tokens.
+ */
+int dsv_token_slots(const dsv_tensor* page_table, const dsv_tensor* seqlens,
+                    const dsv_tensor* new_lens, const dsv_tensor* seqs,
+                    int64_t page_size, dsv_tensor* slots,
+                    dsv_tensor* positions, dsv_tensor* requests,
+                    dsv_tensor* cu_seqlens, dsv_tensor* block_table,
+                    dsv_tensor* lens, void* stream);
+
+/*
+ * Rows of T new tokens enter a latent cache: cache[slots[t]] = [c_t normalised | k_pe_t
+ * rotated], the queries' rotated parts are rotated in the same launch.  Stands to a
+ * latent cache as dsv_kv_append does to a K/V cache; everything is computed in fp32 and
+ * rounded once.
+ *   c           [T, dc], k_pe [T, dr]: bf16|f16|f32, dtype of the cache; dc a multiple of
+ *               16 bytes, dr of 32 bytes, both <= 2048 entries
+ *   norm_weight optional [dc], same dtype: c * norm_weight / sqrt(mean(c^2) + eps)
+ *   cos, sin    optional [n_pos, dr], float32 or the cache's dtype: x * cos + p * sin,
+ *               p = (-x[dr/2:], x[:dr/2]) or, interleaved != 0, (-x[1], x[0], -x[3], ..)
+ *   positions   optional [T] int32|int64: row of cos and sin (clamped to the table;
+ *               ndim 0: row t)
+ *   slots       [T] int32|int64; tokens whose slot is out of range are not stored.  A
+ *               slot may be named once (named twice it holds a mixture)
+ *   cache       [P, page, dc + dr] (page a power of two; slot = page number * page +
+ *               offset) or [S, dc + dr]
+ *   q_pe, q_out optional [T, H, dr]: rotated for every token; q_out may be q_pe itself
+ * T <= 2^26, T * (1 + H) * dr / 16 (fp32: 8) <= 2^31.  No other overlap of an input and
+ * an output.
+ */
+int dsv_latent_append(const dsv_tensor* c, const dsv_tensor* k_pe,
+                      const dsv_tensor* norm_weight, float eps,
+                      const dsv_tensor* cos, const dsv_tensor* sin,
+                      const dsv_tensor* positions, int interleaved,
+                      const dsv_tensor* slots, const dsv_tensor* cache,
+                      const dsv_tensor* q_pe, dsv_tensor* q_out, void* stream);
+
+/*
+ * Workspace of the two calls below for queries [B, M, H, .] of dtype over n_keys keys;
+ * v_dim is the outputs' width.  0 where the call needs none, on invalid arguments and on
+ * sizes that it refuses: batch > 2^20, heads > 65536, keys > 2^30, rows per key head
+ * (absorbed M * H, expanded M) > 2^24, B * H * M > 2^30, or 2^23 and more blocks of
+ * rows (DSV_ERR_UNSUPPORTED).
+ */
+size_t dsv_latent_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t v_dim,
+                                  int dtype, int64_t n_keys, int has_tree,
+                                  int expanded);
+
+/*
+ * Attention over a latent cache in its absorbed form: the queries are in the latent
+ * space already, a cache row is every head's key and its first v_dim entries every
+ * head's value.  Otherwise the contract of dsv_window_attention without a window: the M
+ * queries are the last M of len_b tokens, causal, or the nodes of a tree.
+ *   q            [B, M, H, v_dim + dr] bf16|f16|f32; v_dim 256 or 512, dr 32 or 64
+ *   kv           [B, N, v_dim + dr], or pages [P, page, v_dim + dr] with page_table
+ *                [n_pages] or [B, n_pages] int32|int64 (page a power of two; entries
+ *                are clamped to the pool)
+ *   cache_seqlens optional [B] int32|int64: len_b, clamped to [0, n_keys]
+ *   n_keys       < 0 (or beyond the cache): all that the cache holds
+ *   softmax_scale > 0
+ *   parent       optional [M] or [B, M] int32|int64, M <= 1024 (dsv_tree_verify)
+ *   out          [B, M, H, v_dim] bf16|f16|f32;  lse optional [B, H, M] f32
+ * A query without a key (len_b < M) gets out = 0 and lse = -inf; with a tree every query
+ * of such a sequence does.  Rows that a query does not see never affect it, whatever
+ * they hold.  out and lse may not overlap an input.
+ */
+int dsv_latent_attention(const dsv_tensor* q, const dsv_tensor* kv,
+                         int64_t v_dim, const dsv_tensor* page_table,
+                         const dsv_tensor* cache_seqlens, int64_t n_keys,
+                         double softmax_scale, const dsv_tensor* parent,
+                         dsv_tensor* out, dsv_tensor* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * The same attention in its expanded form, for prompts and chunks of them: keys and
+ * values per head as the expansion of the latent rows gives them, the rotated key part
+ * shared by the heads.
+ *   q     [B, M, H, dn + dr] bf16|f16|f32; dn 64 or 128, dr 32 or 64
+ *   k, v  [B, N, H, dn];  k_pe [B, N, dr]
+ *   cache_seqlens, n_keys, softmax_scale, out [B, M, H, dn], lse: as above
+ *   causal != 0: query m of sequence b sees keys n <= len_b - M + m, else all n < len_b
+ */
+int dsv_latent_expanded(const dsv_tensor* q, const dsv_tensor* k,
+                        const dsv_tensor* k_pe, const dsv_tensor* v,
+                        const dsv_tensor* cache_seqlens, int64_t n_keys,
+                        int causal, double softmax_scale, dsv_tensor* out,
+                        dsv_tensor* lse, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

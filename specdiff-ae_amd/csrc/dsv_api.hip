@@ -6,6 +6,7 @@
 #include "dsv_attn_geo.h"
 #include "dsv_check.h"
 #include "dsv_internal.h"
+#include "dsv_latent.h"
 #include "dsv_window.h"
 
 #include <algorithm>
@@ -2101,6 +2102,509 @@ int dsv_window_attention(const dsv_tensor* q, const dsv_tensor* k, const dsv_ten
   const hipError_t e = dsv::launch_window(a, (int)D, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "windowed attention launch");
   return DSV_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Slot maps and the latent cache's append
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// An int32 or int64 array that the call writes: contiguous, of n entries.
+int check_list(const dsv_tensor* t, const char* name, int dtype, int64_t n) {
+  if (t == nullptr || t->ndim != 1 || t->shape[0] != 0) {
+    const int rc = check_nd(t, name, 1);
+    if (rc != DSV_OK) return rc;
+  }
+  if (t->dtype != dtype || t->shape[0] != n || (n > 1 && t->stride[0] != 1))
+    return fail(DSV_ERR_INVALID, "%s must be contiguous %s [%lld]", name, dt_name(dtype), (long long)n);
+  return DSV_OK;
+}
+
+// Outputs may share no byte with an input or with each other.
+int check_apart(const Extent* outs, int n_outs, const Extent* ins, int n_ins) {
+  for (int i = 0; i < n_outs; ++i) {
+    for (int j = 0; j < n_ins; ++j)
+      if (overlap(outs[i], ins[j])) return fail(DSV_ERR_INVALID, "%s overlaps %s", outs[i].name, ins[j].name);
+    for (int j = i + 1; j < n_outs; ++j)
+      if (overlap(outs[i], outs[j])) return fail(DSV_ERR_INVALID, "%s overlaps %s", outs[i].name, outs[j].name);
+  }
+  return DSV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsv_token_slots(const dsv_tensor* page_table, const dsv_tensor* seqlens, const dsv_tensor* new_lens,
+                    const dsv_tensor* seqs, int64_t page_size, dsv_tensor* slots, dsv_tensor* positions,
+                    dsv_tensor* requests, dsv_tensor* cu_seqlens, dsv_tensor* block_table, dsv_tensor* lens,
+                    void* stream) {
+  int rc;
+  dsv::SlotArgs a{};
+  if ((rc = check_nd(page_table, "page_table", 2)) != DSV_OK) return rc;
+  if (page_table->dtype != DSV_I32 || (page_table->shape[1] > 1 && page_table->stride[1] != 1))
+    return fail(DSV_ERR_INVALID, "page_table must be int32 [B, n_logical] with innermost stride 1");
+  const int sh = log2_exact(page_size);
+  if (sh < 0) return fail(DSV_ERR_UNSUPPORTED, "page_size %lld must be a power of two", (long long)page_size);
+  a.table = static_cast<const int32_t*>(page_table->data);
+  a.t_sb = page_table->stride[0];
+  a.B = page_table->shape[0];
+  a.n_log = page_table->shape[1];
+  a.ps_shift = sh;
+  if (a.B > dsv::kPageMaxSeqs) return fail(DSV_ERR_UNSUPPORTED, "more than %d sequences", dsv::kPageMaxSeqs);
+  if (a.n_log > 0x7fffffff >> sh) return fail(DSV_ERR_UNSUPPORTED, "page_table rows beyond 2^31 - 1 tokens");
+  if ((rc = check_nd(seqlens, "seqlens", 1)) != DSV_OK) return rc;
+  if ((seqlens->dtype != DSV_I32 && seqlens->dtype != DSV_I64) || seqlens->shape[0] != a.B || (a.B > 1 && seqlens->stride[0] != 1))
+    return fail(DSV_ERR_INVALID, "seqlens must be contiguous int32 or int64 [B]");
+  a.lens = seqlens->data;
+  a.lens_i64 = seqlens->dtype == DSV_I64;
+  if (new_lens == nullptr || new_lens->ndim != 1) return fail(DSV_ERR_INVALID, "new_lens must be a 1-d tensor");
+  const int64_t n = new_lens->shape[0];
+  if (n > dsv::kPageMaxSeqs) return fail(DSV_ERR_UNSUPPORTED, "more than %d requests", dsv::kPageMaxSeqs);
+  if ((rc = check_index(new_lens, "new_lens", n, nullptr, 0, a.news)) != DSV_OK) return rc;
+  if (present(seqs)) {
+    if ((rc = check_index(seqs, "seqs", n, nullptr, 0, a.seqs)) != DSV_OK) return rc;
+  } else if (n != a.B) {
+    return fail(DSV_ERR_INVALID, "new_lens must have an entry per sequence (%lld) where no seqs are given", (long long)a.B);
+  }
+  a.n = (int)n;
+  if (slots == nullptr || slots->ndim != 1) return fail(DSV_ERR_INVALID, "slots must be a 1-d tensor");
+  a.cap = slots->shape[0];
+  if (a.cap > ((int64_t)1 << 30)) return fail(DSV_ERR_UNSUPPORTED, "a capacity of more than 2^30 tokens");
+  if ((rc = check_list(slots, "slots", DSV_I64, a.cap)) != DSV_OK) return rc;
+  if ((rc = check_list(positions, "positions", DSV_I32, a.cap)) != DSV_OK) return rc;
+  if ((rc = check_list(requests, "requests", DSV_I32, a.cap)) != DSV_OK) return rc;
+  if ((rc = check_list(cu_seqlens, "cu_seqlens", DSV_I32, n + 1)) != DSV_OK) return rc;
+  if ((rc = check_list(lens, "lens", DSV_I32, n)) != DSV_OK) return rc;
+  if (block_table == nullptr || block_table->ndim != 2 || block_table->dtype != DSV_I32 || block_table->shape[0] != n ||
+      block_table->shape[1] != a.n_log || (a.n_log > 1 && block_table->stride[1] != 1) ||
+      (n > 1 && block_table->stride[0] < a.n_log))
+    return fail(DSV_ERR_INVALID, "block_table must be int32 [n, n_logical] with innermost stride 1");
+  if (n > 0 && a.n_log > 0 && (rc = check_nd(block_table, "block_table", 2)) != DSV_OK) return rc;
+  const Extent outs[6] = {extent_of("slots", slots), extent_of("positions", positions), extent_of("requests", requests),
+                          extent_of("cu_seqlens", cu_seqlens), extent_of("block_table", block_table), extent_of("lens", lens)};
+  const Extent ins[4] = {extent_of("page_table", page_table), extent_of("seqlens", seqlens), extent_of("new_lens", new_lens),
+                         extent_of("seqs", seqs)};
+  if ((rc = check_apart(outs, 6, ins, 4)) != DSV_OK) return rc;
+  a.slots = static_cast<int64_t*>(slots->data);
+  a.pos = static_cast<int32_t*>(positions->data);
+  a.req = static_cast<int32_t*>(requests->data);
+  a.cu = static_cast<int32_t*>(cu_seqlens->data);
+  a.block = static_cast<int32_t*>(block_table->data);
+  a.b_sb = block_table->stride[0];
+  a.out_lens = static_cast<int32_t*>(lens->data);
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_slots(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "slot map launch");
+  return DSV_OK;
+}
+
+int dsv_latent_append(const dsv_tensor* c, const dsv_tensor* k_pe, const dsv_tensor* norm_weight, float eps,
+                      const dsv_tensor* cos, const dsv_tensor* sin, const dsv_tensor* positions, int interleaved,
+                      const dsv_tensor* slots, const dsv_tensor* cache, const dsv_tensor* q_pe, dsv_tensor* q_out,
+                      void* stream) {
+  int rc;
+  dsv::LatentAppendArgs a{};
+  if ((rc = check_nd(cache, "cache", cache != nullptr && cache->ndim == 2 ? 2 : 3)) != DSV_OK) return rc;
+  if ((rc = check_vec16(cache, "cache")) != DSV_OK) return rc;
+  auto rows = [&](const dsv_tensor* t, const char* name, int nd) -> int {
+    int r;
+    if (t == nullptr || t->ndim != nd) return fail(DSV_ERR_INVALID, "%s must be a %d-d tensor", name, nd);
+    for (int i = 0; i < nd; ++i)
+      if (t->shape[i] == 0) return fail(DSV_ERR_INVALID, "%s is empty", name);
+    if ((r = check_nd(t, name, nd)) != DSV_OK) return r;
+    if ((r = check_vec16(t, name)) != DSV_OK) return r;
+    if (t->dtype != cache->dtype) return fail(DSV_ERR_INVALID, "%s must have the cache's dtype", name);
+    return DSV_OK;
+  };
+  if ((rc = rows(c, "c", 2)) != DSV_OK) return rc;
+  if ((rc = rows(k_pe, "k_pe", 2)) != DSV_OK) return rc;
+  const int64_t T = c->shape[0], dc = c->shape[1], dr = k_pe->shape[1];
+  const int es = elem_size(cache->dtype), nd = cache->ndim;
+  if (k_pe->shape[0] != T) return fail(DSV_ERR_INVALID, "c and k_pe must have the same tokens");
+  if ((dc * es) % 16 != 0 || (dr * es) % 32 != 0)
+    return fail(DSV_ERR_UNSUPPORTED, "rows of %lld + %lld entries (the latent part a multiple of 16 bytes, the rotated part of 32)",
+                (long long)dc, (long long)dr);
+  if (dc > 2048 || dr > 2048) return fail(DSV_ERR_UNSUPPORTED, "rows wider than 2048 + 2048 entries");
+  if (cache->shape[nd - 1] != dc + dr)
+    return fail(DSV_ERR_INVALID, "cache rows hold %lld entries, c and k_pe %lld", (long long)cache->shape[nd - 1], (long long)(dc + dr));
+  a.dtype = cache->dtype;
+  a.T = T;
+  a.dc = (int)dc;
+  a.dr = (int)dr;
+  a.c = c->data;
+  a.c_st = c->stride[0];
+  a.pe = k_pe->data;
+  a.pe_st = k_pe->stride[0];
+  a.eps = eps;
+  if (present(norm_weight)) {
+    if ((rc = rows(norm_weight, "norm_weight", 1)) != DSV_OK) return rc;
+    if (norm_weight->shape[0] != dc) return fail(DSV_ERR_INVALID, "norm_weight must be [%lld]", (long long)dc);
+    if (!(eps >= 0.f) || !(eps < 3.4e38f)) return fail(DSV_ERR_INVALID, "eps must be finite and >= 0");
+    a.w = norm_weight->data;
+  }
+  if (present(cos) != present(sin)) return fail(DSV_ERR_INVALID, "cos and sin go together");
+  if (present(cos)) {
+    for (const dsv_tensor* t : {cos, sin}) {
+      const char* nm = t == cos ? "cos" : "sin";
+      if ((rc = check_nd(t, nm, 2)) != DSV_OK) return rc;
+      if ((rc = check_vec16(t, nm)) != DSV_OK) return rc;
+      if (t->shape[1] != dr || t->shape[0] < 1 || t->shape[0] != cos->shape[0])
+        return fail(DSV_ERR_INVALID, "cos and sin must be [n_pos, %lld]", (long long)dr);
+      if (t->dtype != cos->dtype || (t->dtype != DSV_F32 && t->dtype != a.dtype))
+        return fail(DSV_ERR_INVALID, "cos and sin must both be float32 or of the cache's dtype");
+    }
+    a.cos = cos->data;
+    a.sin = sin->data;
+    a.cos_st = cos->stride[0];
+    a.sin_st = sin->stride[0];
+    a.tab_f32 = cos->dtype == DSV_F32;
+    a.n_pos = cos->shape[0];
+    if (present(positions)) {
+      dsv::PageIndex x{};
+      if ((rc = check_index(positions, "positions", T, nullptr, 0, x)) != DSV_OK) return rc;
+      if (T > 1 && x.stride != 1) return fail(DSV_ERR_INVALID, "positions must be contiguous");
+      a.pos = x.p;
+      a.pos_i64 = x.is64;
+    } else if (a.n_pos != T) {
+      return fail(DSV_ERR_INVALID, "cos and sin must have a row per token where no positions are given");
+    }
+  } else if (present(positions)) {
+    return fail(DSV_ERR_INVALID, "positions without cos and sin");
+  }
+  a.interleaved = interleaved != 0;
+  {
+    dsv::PageIndex x{};
+    if ((rc = check_index(slots, "slots", T, nullptr, 0, x)) != DSV_OK) return rc;
+    if (T > 1 && x.stride != 1) return fail(DSV_ERR_INVALID, "slots must be contiguous");
+    a.slots = x.p;
+    a.slots_i64 = x.is64;
+  }
+  a.cache = cache->data;
+  a.s_t = cache->stride[nd - 2];
+  // Rows that share bytes would be written into each other.
+  if (cache->shape[nd - 2] > 1 && a.s_t < dc + dr) return fail(DSV_ERR_INVALID, "cache rows overlap");
+  if (nd == 3) {
+    const int sh = log2_exact(cache->shape[1]);
+    if (sh < 0) return fail(DSV_ERR_UNSUPPORTED, "page_size %lld must be a power of two", (long long)cache->shape[1]);
+    if (cache->shape[0] > 0x7fffffff) return fail(DSV_ERR_UNSUPPORTED, "more than 2^31 - 1 pages");
+    a.s_p = cache->stride[0];
+    if (cache->shape[0] > 1 && a.s_p < (cache->shape[1] - 1) * a.s_t + dc + dr) return fail(DSV_ERR_INVALID, "cache pages overlap");
+    a.ps_shift = sh;
+    a.n_slots = cache->shape[0] << sh;
+  } else {
+    a.ps_shift = 62;
+    a.n_slots = cache->shape[0];
+  }
+  if (present(q_pe) != present(q_out)) return fail(DSV_ERR_INVALID, "q_pe and q_out go together");
+  bool in_place = false;
+  if (present(q_pe)) {
+    if ((rc = rows(q_pe, "q_pe", 3)) != DSV_OK) return rc;
+    if ((rc = rows(q_out, "q_out", 3)) != DSV_OK) return rc;
+    for (int i = 0; i < 3; ++i)
+      if (q_out->shape[i] != q_pe->shape[i]) return fail(DSV_ERR_INVALID, "q_out must have q_pe's shape");
+    if (q_pe->shape[0] != T || q_pe->shape[2] != dr) return fail(DSV_ERR_INVALID, "q_pe must be [%lld, H, %lld]", (long long)T, (long long)dr);
+    if (q_pe->shape[1] > (1 << 16)) return fail(DSV_ERR_UNSUPPORTED, "more than 65536 heads");
+    a.H = (int)q_pe->shape[1];
+    a.q = q_pe->data;
+    a.q_st = q_pe->stride[0];
+    a.q_sh = q_pe->stride[1];
+    a.qo = q_out->data;
+    a.qo_st = q_out->stride[0];
+    a.qo_sh = q_out->stride[1];
+    // Rows of the output apart from each other: heads within tokens or tokens within heads.
+    const int64_t H = a.H, st = T > 1 ? a.qo_st : -1, sh = H > 1 ? a.qo_sh : -1;
+    const bool ok = (st < 0 || st >= dr) && (sh < 0 || sh >= dr) && (st < 0 || sh < 0 || st >= (H - 1) * sh + dr || sh >= (T - 1) * st + dr);
+    if (!ok) return fail(DSV_ERR_INVALID, "q_out rows overlap");
+    // A thread reads what it writes: row for row in place is safe.
+    in_place = a.qo == a.q && a.qo_st == a.q_st && a.qo_sh == a.q_sh;
+  }
+  if (T > ((int64_t)1 << 26) || T * (1 + a.H) * (dr * es / 32) > ((int64_t)1 << 31))
+    return fail(DSV_ERR_UNSUPPORTED, "more than 2^26 tokens or 2^31 chunk pairs of rotated rows");
+  const Extent outs[2] = {extent_of("cache", cache), extent_of("q_out", q_out)};
+  const Extent ins[8] = {extent_of("c", c), extent_of("k_pe", k_pe), extent_of("norm_weight", norm_weight), extent_of("cos", cos),
+                         extent_of("sin", sin), extent_of("positions", positions), extent_of("slots", slots),
+                         in_place ? Extent{"q_pe", 0, 0} : extent_of("q_pe", q_pe)};
+  if ((rc = check_apart(outs, 2, ins, 8)) != DSV_OK) return rc;
+  if (g_dry_run) return DSV_OK;
+  const hipError_t e = dsv::launch_latent_append(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "latent append launch");
+  return DSV_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Latent attention
+// ---------------------------------------------------------------------------
+
+namespace {
+
+struct LatPlan {
+  int G = 0, R = 0, MW = 0, rpb = 0, n_rb = 0, W = 1, kt = 0;
+  size_t opart_bytes = 0, ml_bytes = 0, total = 0;
+  const char* err = nullptr;
+};
+
+LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dtype, int64_t n_keys, bool tree) {
+  LatPlan p;
+  const bool in_range = B <= (1 << 20) && M <= (1 << 24) && H <= (1 << 16) && n_keys <= dsv::kLatMaxKeys;
+  const int64_t R = in_range ? (H / Hk) * M : 0;
+  if (!in_range || R > ((int64_t)1 << 24) || B * Hk * R > ((int64_t)1 << 30)) {
+    p.err = "sizes beyond the latent attention's range (batch <= 2^20, heads <= 65536, keys <= 2^30, rows per key head "
+            "<= 2^24, batch x heads x rows <= 2^30)";
+    return p;
+  }
+  const bool expanded = Hk == H && dv <= 128;
+  p.G = (int)(H / Hk);
+  p.R = (int)R;
+  p.MW = tree ? (int)((M + 63) / 64) : 0;
+  if (dtype == DSV_F32) {
+    p.rpb = 16;
+    p.kt = dsv::kLatTileF32;
+  } else if (expanded) {
+    p.rpb = 256;
+    p.kt = dsv::kLatTileExp;
+  } else {
+    p.rpb = R > 32 ? 64 : (R > 16 ? 32 : 16);
+    p.kt = dsv::kLatTile;
+    // The trees' sets of a block of 64 rows have room for 576 words.
+    if (p.rpb == 64 && std::min<int64_t>(64, 63 / p.G + 2) * p.MW > 576) p.rpb = 32;
+  }
+  p.n_rb = (int)((R + p.rpb - 1) / p.rpb);
+  const int64_t units = Hk * p.n_rb;
+  if (units >= (1 << 23)) {
+    // (512 threads each; a launch counts fewer than 2^32.)
+    p.err = "key heads x blocks of rows beyond 2^23 - 1";
+    return p;
+  }
+  // Ranges: as many workgroups as fill the CUs one to four times, whichever leaves
+  // fewest idle in the last turn; of two tiles at least.
+  const int64_t cus = device_cus();
+  int64_t W = 1;
+  if (units < 4 * cus) {
+    double best = 0;
+    for (int64_t k = 1; k <= 4; ++k) {
+      const int64_t w = cus * k / units;
+      const double use = (double)(units * w) / (double)(cus * k);
+      if (w >= 1 && use > best + 0.04) {
+        best = use;
+        W = w;
+      }
+    }
+  }
+  const int64_t tiles = B * ((n_keys + p.kt - 1) / p.kt);
+  W = std::max<int64_t>(1, std::min<int64_t>(W, tiles / 2));
+  p.W = (int)W;
+  const size_t rows = W > 1 ? (size_t)units * W * 2 * p.rpb : 0;
+  p.opart_bytes = align_up(rows * dv * sizeof(float), 256);
+  p.ml_bytes = align_up(rows * sizeof(float2), 256);
+  p.total = p.opart_bytes + p.ml_bytes;
+  return p;
+}
+
+// The lengths, the tree, the outputs and the plan of both forms; then the launch.
+int lat_common(dsv::LatArgs& a, const dsv_tensor* q, const dsv_tensor* seqlens, int64_t n, const dsv_tensor* parent, double scale,
+               dsv_tensor* out, dsv_tensor* lse, const Extent* ins, int n_ins, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  const int64_t B = q->shape[0], M = q->shape[1], H = q->shape[2];
+  if (!(scale > 0) || !(scale < 3.4e38)) return fail(DSV_ERR_INVALID, "the softmax scale must be finite and > 0");
+  if ((rc = check_nd(out, "out", 4)) != DSV_OK) return rc;
+  if (out->shape[0] != B || out->shape[1] != M || out->shape[2] != H || out->shape[3] != a.dv)
+    return fail(DSV_ERR_INVALID, "out must be [B, M, H, %d]", a.dv);
+  if (out->dtype != DSV_BF16 && out->dtype != DSV_F16 && out->dtype != DSV_F32)
+    return fail(DSV_ERR_INVALID, "out dtype must be bf16, f16 or f32");
+  if (out->stride[3] != 1) return fail(DSV_ERR_INVALID, "out innermost stride must be 1");
+  if (present(seqlens)) {
+    if ((rc = check_nd(seqlens, "cache_seqlens", 1)) != DSV_OK) return rc;
+    if ((seqlens->dtype != DSV_I32 && seqlens->dtype != DSV_I64) || seqlens->shape[0] != B || (B > 1 && seqlens->stride[0] != 1))
+      return fail(DSV_ERR_INVALID, "cache_seqlens must be a contiguous int32 or int64 [B] tensor");
+    a.seqlens = seqlens->data;
+    a.seqlens_i64 = seqlens->dtype == DSV_I64;
+  }
+  if (present(parent)) {
+    if (parent->ndim != 1 && parent->ndim != 2) return fail(DSV_ERR_INVALID, "parent must be [M] or [B, M]");
+    if ((rc = check_nd(parent, "parent", parent->ndim)) != DSV_OK) return rc;
+    if (parent->dtype != DSV_I32 && parent->dtype != DSV_I64) return fail(DSV_ERR_INVALID, "parent must be int32 or int64");
+    if (parent->shape[parent->ndim - 1] != M) return fail(DSV_ERR_INVALID, "parent must have M entries per tree");
+    if (parent->ndim == 2 && parent->shape[0] != B && parent->shape[0] != 1)
+      return fail(DSV_ERR_INVALID, "parent batch must be 1 or B");
+    if (M > dsv::kTreeMaxM) return fail(DSV_ERR_UNSUPPORTED, "trees larger than %d nodes are not supported", dsv::kTreeMaxM);
+    a.parent = parent->data;
+    a.par_i64 = parent->dtype == DSV_I64;
+    a.par_sb = (parent->ndim == 2 && parent->shape[0] > 1) ? parent->stride[0] : 0;
+    a.par_sm = parent->stride[parent->ndim - 1];
+  }
+  if (present(lse)) {
+    if ((rc = check_nd(lse, "lse", 3)) != DSV_OK) return rc;
+    if (lse->dtype != DSV_F32 || lse->shape[0] != B || lse->shape[1] != H || lse->shape[2] != M)
+      return fail(DSV_ERR_INVALID, "lse must be float32 [B, H, M]");
+    a.lse = static_cast<float*>(lse->data);
+    a.l_sb = lse->stride[0];
+    a.l_sh = lse->stride[1];
+    a.l_sm = lse->stride[2];
+  }
+  // Rows are written while others' inputs are still read.
+  const Extent outs[2] = {extent_of("out", out), extent_of("lse", lse)};
+  if ((rc = check_apart(outs, 2, ins, n_ins)) != DSV_OK) return rc;
+  const LatPlan p = lat_plan(B, M, H, a.Hk, a.dv, a.dtype, n, a.parent != nullptr);
+  if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
+  if (p.total > 0 && (rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+  a.q = q->data;
+  a.q_sb = q->stride[0];
+  a.q_sm = q->stride[1];
+  a.q_sh = q->stride[2];
+  a.n_keys = n;
+  a.B = (int)B;
+  a.M = (int)M;
+  a.H = (int)H;
+  a.G = p.G;
+  a.R = p.R;
+  a.MW = p.MW;
+  a.rpb = p.rpb;
+  a.n_rb = p.n_rb;
+  a.W = p.W;
+  a.scale_log2 = (float)(1.4426950408889634 * scale);
+  if (!(a.scale_log2 > 0.f)) return fail(DSV_ERR_INVALID, "the softmax scale is too small for float32");
+  if (p.total > 0) {
+    char* w = static_cast<char*>(workspace);
+    a.opart = reinterpret_cast<float*>(w);
+    a.ml = reinterpret_cast<float2*>(w + p.opart_bytes);
+  }
+  a.out = out->data;
+  a.out_dtype = out->dtype;
+  a.o_sb = out->stride[0];
+  a.o_sm = out->stride[1];
+  a.o_sh = out->stride[2];
+  const int per16 = 16 / elem_size(out->dtype);
+  a.out_vec = (reinterpret_cast<uintptr_t>(out->data) & 15) == 0 && (B == 1 || a.o_sb % per16 == 0) &&
+              (M == 1 || a.o_sm % per16 == 0) && (H == 1 || a.o_sh % per16 == 0);
+  if (g_dry_run) return DSV_OK;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e = a.dtype == DSV_F32 ? dsv::launch_latent_f32(a, s)
+                 : p.kt == dsv::kLatTileExp && p.rpb == 256 ? dsv::launch_latent_tile(a, s)
+                                                            : dsv::launch_latent(a, s);
+  if (e == hipSuccess) e = dsv::launch_latent_merge(a, p.kt, s);
+  if (e != hipSuccess) return hip_fail(e, "latent attention launch");
+  return DSV_OK;
+}
+
+int lat_query(const dsv_tensor* q) {
+  int rc;
+  if ((rc = check_nd(q, "q", 4)) != DSV_OK) return rc;
+  if ((rc = check_vec16(q, "q")) != DSV_OK) return rc;
+  if (q->shape[0] < 1 || q->shape[1] < 1 || q->shape[2] < 1) return fail(DSV_ERR_INVALID, "q must hold at least one query");
+  return DSV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dsv_latent_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t v_dim, int dtype, int64_t n_keys, int has_tree,
+                                  int expanded) {
+  if (B < 1 || M < 1 || H < 1 || v_dim < 1 || dtype < DSV_BF16 || dtype > DSV_F32 || n_keys < 0 ||
+      (has_tree && M > dsv::kTreeMaxM) || !(expanded ? dsv::expanded_widths((int)std::min<int64_t>(v_dim, 4096), 64)
+                                                     : dsv::latent_widths((int)std::min<int64_t>(v_dim, 4096), 64)))
+    return 0;
+  const LatPlan p = lat_plan(B, M, H, expanded ? H : 1, v_dim, dtype, n_keys, has_tree != 0);
+  return p.err != nullptr ? 0 : p.total;
+}
+
+int dsv_latent_attention(const dsv_tensor* q, const dsv_tensor* kv, int64_t v_dim, const dsv_tensor* page_table,
+                         const dsv_tensor* cache_seqlens, int64_t n_keys, double softmax_scale, const dsv_tensor* parent,
+                         dsv_tensor* out, dsv_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = lat_query(q)) != DSV_OK) return rc;
+  if ((rc = check_nd(kv, "kv_cache", 3)) != DSV_OK) return rc;
+  if ((rc = check_vec16(kv, "kv_cache")) != DSV_OK) return rc;
+  const int64_t B = q->shape[0], D = q->shape[3];
+  if (kv->dtype != q->dtype) return fail(DSV_ERR_INVALID, "q and kv_cache must share a dtype");
+  if (kv->shape[2] != D) return fail(DSV_ERR_INVALID, "kv_cache rows hold %lld entries, q's %lld", (long long)kv->shape[2], (long long)D);
+  if (v_dim < 1 || v_dim > D) return fail(DSV_ERR_INVALID, "v_dim must be in [1, %lld]", (long long)D);
+  if (D > 4096 || !dsv::latent_widths((int)v_dim, (int)(D - v_dim)))
+    return fail(DSV_ERR_UNSUPPORTED, "rows of %lld + %lld entries are not supported (256 or 512, and 32 or 64)", (long long)v_dim,
+                (long long)(D - v_dim));
+  dsv::LatArgs a{};
+  int64_t cap = 0;
+  dsv::LatSrc src{};
+  src.p = kv->data;
+  src.st = kv->stride[1];
+  if (present(page_table)) {
+    if (kv->shape[0] < 1 || kv->shape[0] > 0x7fffffff) return fail(DSV_ERR_INVALID, "the pool must hold 1 to 2^31 - 1 pages");
+    const int sh = log2_exact(kv->shape[1]);
+    if (sh < 0) return fail(DSV_ERR_UNSUPPORTED, "page_size %lld must be a power of two", (long long)kv->shape[1]);
+    if (page_table->ndim != 1 && page_table->ndim != 2) return fail(DSV_ERR_INVALID, "page_table must be 1-d or 2-d");
+    if ((rc = check_nd(page_table, "page_table", page_table->ndim)) != DSV_OK) return rc;
+    if (page_table->dtype != DSV_I32 && page_table->dtype != DSV_I64)
+      return fail(DSV_ERR_INVALID, "page_table must be int32 or int64");
+    if (page_table->ndim == 2 && page_table->shape[0] != B && page_table->shape[0] != 1)
+      return fail(DSV_ERR_INVALID, "page_table batch must be 1 or B");
+    const int64_t npt = page_table->shape[page_table->ndim - 1];
+    if (npt > 1 && page_table->stride[page_table->ndim - 1] != 1)
+      return fail(DSV_ERR_INVALID, "page_table innermost stride must be 1");
+    src.sp = kv->stride[0];
+    a.pt = page_table->data;
+    a.pt_i64 = page_table->dtype == DSV_I64;
+    a.ps_shift = std::min(sh, 30);  // (keys are below 2^30)
+    a.pt_sb = (page_table->ndim == 2 && page_table->shape[0] > 1) ? page_table->stride[0] : 0;
+    a.n_phys = kv->shape[0];
+    cap = npt > ((int64_t)1 << 40) >> sh ? (int64_t)1 << 40 : npt << sh;
+  } else {
+    if (kv->shape[0] != B) return fail(DSV_ERR_INVALID, "kv_cache batch differs from q");
+    src.sb = B > 1 ? kv->stride[0] : 0;
+    cap = kv->shape[1];
+  }
+  const int64_t n = n_keys < 0 || n_keys > cap ? cap : n_keys;
+  a.dtype = q->dtype;
+  a.dn = (int)v_dim;
+  a.dr = (int)(D - v_dim);
+  a.dv = (int)v_dim;
+  a.kn = a.kr = a.v = src;
+  a.kr.p = static_cast<const char*>(kv->data) + v_dim * elem_size(kv->dtype);
+  a.Hk = 1;
+  a.causal = 1;
+  const Extent ins[5] = {extent_of("q", q), extent_of("kv_cache", kv), extent_of("page_table", page_table),
+                         extent_of("cache_seqlens", cache_seqlens), extent_of("parent", parent)};
+  return lat_common(a, q, cache_seqlens, n, parent, softmax_scale, out, lse, ins, 5, workspace, workspace_bytes, stream);
+}
+
+int dsv_latent_expanded(const dsv_tensor* q, const dsv_tensor* k, const dsv_tensor* k_pe, const dsv_tensor* v,
+                        const dsv_tensor* cache_seqlens, int64_t n_keys, int causal, double softmax_scale, dsv_tensor* out,
+                        dsv_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = lat_query(q)) != DSV_OK) return rc;
+  const int64_t B = q->shape[0], H = q->shape[2], D = q->shape[3];
+  struct In { const dsv_tensor* t; const char* name; int nd; };
+  for (const In& x : {In{k, "k", 4}, In{k_pe, "k_pe", 3}, In{v, "v", 4}}) {
+    if ((rc = check_nd(x.t, x.name, x.nd)) != DSV_OK) return rc;
+    if ((rc = check_vec16(x.t, x.name)) != DSV_OK) return rc;
+    if (x.t->dtype != q->dtype) return fail(DSV_ERR_INVALID, "q and %s must share a dtype", x.name);
+    if (x.t->shape[0] != B) return fail(DSV_ERR_INVALID, "%s batch differs from q", x.name);
+    if (x.t->shape[1] != k->shape[1]) return fail(DSV_ERR_INVALID, "k, k_pe and v must hold the same tokens");
+    if (x.nd == 4 && x.t->shape[2] != H) return fail(DSV_ERR_INVALID, "%s must have q's heads", x.name);
+  }
+  const int64_t dn = k->shape[3], dr = k_pe->shape[2];
+  if (dn + dr != D) return fail(DSV_ERR_INVALID, "q rows hold %lld entries, k and k_pe %lld", (long long)D, (long long)(dn + dr));
+  if (v->shape[3] != dn || dn > 4096 || dr > 4096 || !dsv::expanded_widths((int)dn, (int)dr))
+    return fail(DSV_ERR_UNSUPPORTED, "heads of %lld + %lld entries and values of %lld are not supported (64 or 128 and 32 or 64, "
+                "values as wide as the first part)", (long long)dn, (long long)dr, (long long)v->shape[3]);
+  dsv::LatArgs a{};
+  a.dtype = q->dtype;
+  a.dn = a.dv = (int)dn;
+  a.dr = (int)dr;
+  a.kn = dsv::LatSrc{k->data, B > 1 ? k->stride[0] : 0, 0, k->stride[2], k->stride[1]};
+  a.kr = dsv::LatSrc{k_pe->data, B > 1 ? k_pe->stride[0] : 0, 0, 0, k_pe->stride[1]};
+  a.v = dsv::LatSrc{v->data, B > 1 ? v->stride[0] : 0, 0, v->stride[2], v->stride[1]};
+  a.Hk = (int)std::min<int64_t>(H, 1 << 17);
+  a.causal = causal != 0;
+  const int64_t n = n_keys < 0 || n_keys > k->shape[1] ? k->shape[1] : n_keys;
+  const Extent ins[5] = {extent_of("q", q), extent_of("k", k), extent_of("k_pe", k_pe), extent_of("v", v),
+                         extent_of("cache_seqlens", cache_seqlens)};
+  return lat_common(a, q, cache_seqlens, n, nullptr, softmax_scale, out, lse, ins, 5, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -287,6 +287,41 @@ struct CompactArgs {
   int32_t* state;                          // [2]: pages in use, pairs
 };
 
+// Arguments of the slot maps: places in the page pool of the requests' new tokens.
+constexpr int kSlotInline = 2048;          // requests that one launch handles
+struct SlotArgs {
+  const int32_t* table; int64_t t_sb;      // page_table [B, n_log]
+  int64_t B, n_log;
+  const void* lens; int lens_i64;          // [B]
+  PageIndex news, seqs;                    // [n]; seqs.p nullptr: request i is sequence i
+  int n, ps_shift;
+  int64_t cap;
+  int64_t* slots; int32_t* pos; int32_t* req;  // [cap]
+  int32_t* cu;                             // [n + 1]
+  int32_t* block; int64_t b_sb;            // [n, n_log]
+  int32_t* out_lens;                       // [n]
+};
+
+// Arguments of the latent append: norm, rotation and scatter of new rows.
+struct LatentAppendArgs {
+  int dtype;                               // dsv_dtype of c, k_pe, cache, weight, q
+  int64_t T;
+  int dc, dr;
+  const void* c; int64_t c_st;             // [T, dc]
+  const void* pe; int64_t pe_st;           // [T, dr]
+  const void* w; float eps;                // optional [dc] norm weight
+  const void* cos; const void* sin; int64_t cos_st, sin_st;  // optional [n_pos, dr]
+  int tab_f32; int64_t n_pos;
+  const void* pos; int pos_i64;            // optional [T]: row of the tables (nullptr: t)
+  int interleaved;
+  const void* slots; int slots_i64;        // [T]
+  void* cache; int64_t s_p, s_t;           // pages of 2^ps_shift rows
+  int64_t n_slots; int ps_shift;           // (dense: one page, ps_shift 62)
+  const void* q; int64_t q_st, q_sh;       // optional [T, H, dr]
+  void* qo; int64_t qo_st, qo_sh;
+  int H;
+};
+
 // Arguments of the lm_head fused with the acceptance statistics.
 constexpr int kLmKS = 4;                   // 16-element MFMA sub-steps per step
 constexpr int kLmVocab = 256;              // vocabulary rows per workgroup
@@ -343,6 +378,8 @@ hipError_t launch_fork(const ForkArgs& a, hipStream_t s);
 hipError_t launch_extend(const ExtendArgs& a, hipStream_t s);
 hipError_t launch_free(const FreeArgs& a, hipStream_t s);
 hipError_t launch_compact(const CompactArgs& a, hipStream_t s);
+hipError_t launch_slots(const SlotArgs& a, hipStream_t s);
+hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t s);
 // Vocabulary ranges of the acceptance statistics: sets a.chunk and a.nchunk
 // from the logits layout, T, M, V and the GPU's CU count.
 void accept_chunking(AcceptArgs& a, int cus);

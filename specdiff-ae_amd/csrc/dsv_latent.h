@@ -1,0 +1,84 @@
+// dsv_latent.h — launch arguments and work sharing of the latent attention
+// (dsv_latent.hip, dsv_latent_tile.hip, dsv_latent_f32.hip).
+#pragma once
+
+#include <stdint.h>
+
+#include "dsv_attn_geo.h"
+#include "dsv_internal.h"
+
+namespace dsv {
+
+// One of the key or value arrays: element (b, h, n) at p + b*sb + h*sh + n*st, or,
+// in a page pool, page*sp + (n mod page size)*st (element strides).
+struct LatSrc {
+  const void* p;
+  int64_t sb, sp, sh, st;
+};
+
+struct LatArgs {
+  int dtype;                               // dsv_dtype of q, keys and values
+  int dn, dr, dv;                          // widths: keys without their rotated part, that part, values
+  const void* q;
+  int64_t q_sb, q_sm, q_sh;
+  LatSrc kn, kr, v;
+  const void* pt; int pt_i64, ps_shift;    // page table (nullptr: dense)
+  int64_t pt_sb, n_phys;
+  const void* seqlens; int seqlens_i64;    // optional [B]
+  int64_t n_keys;                          // keys of the cache (lengths are clamped to it)
+  int B, M, H, Hk, G, R;                   // R = G * M rows per key head, row m * G + g
+  int causal;
+  float scale_log2;                        // log2(e) * softmax scale
+  const void* parent; int par_i64;         // tree: [B, M] parents (nullptr: none)
+  int64_t par_sb, par_sm;
+  int MW;                                  // tree: 64-bit words of a row's set
+  int rpb, n_rb, W;                        // rows per block, blocks, ranges (see LatRange)
+  float* opart;                            // [Hk, n_rb, W, 2, rpb, dv], relative to the maximum
+  float2* ml;                              // [Hk, n_rb, W, 2, rpb] (maximum as a score, sum)
+  void* out; int out_dtype, out_vec;       // out_vec: rows take vector stores
+  int64_t o_sb, o_sm, o_sh;
+  float* lse; int64_t l_sb, l_sm, l_sh;
+};
+
+// Keys of a sequence at most (token numbers are 32-bit, byte offsets are not).
+constexpr int64_t kLatMaxKeys = (int64_t)1 << 30;
+
+// Keys [0, lat_end) are those that some row of block rb sees.
+DSV_HD int lat_end(const LatArgs& a, int len, int rb) {
+  const int n0 = len - a.M;
+  if (!a.causal) return len;
+  if (a.parent != nullptr) return n0 < 0 ? 0 : len;
+  const int rl = ((rb + 1) * a.rpb < a.R ? (rb + 1) * a.rpb : a.R) - 1;
+  const int e = n0 + rl / a.G + 1;
+  return e > 0 ? e : 0;
+}
+
+// The tiles of kt keys of block rb in a sequence: at least one, so that every
+// sequence's rows are somebody's.
+DSV_HD int lat_tiles(const LatArgs& a, int len, int rb, int kt) {
+  const int t = (int)(((int64_t)lat_end(a, len, rb) + kt - 1) / kt);
+  return t > 0 ? t : 1;
+}
+
+// Work sharing.  For each unit (key head, block of rows) the sequences' tiles
+// stand in one line, which W workgroups share out evenly: range j is
+// [total * j / W, total * (j + 1) / W).  A range holds pieces of one or more
+// sequences.  Where a piece is all of its sequence's tiles the workgroup writes
+// the output, else a partial: number 0 for the piece that the range begins with,
+// 1 for another, which its end cuts (so at most two per range).
+DSV_HD int64_t lat_cut(int64_t total, int j, int W) { return total * j / W; }
+DSV_HD int lat_range_of(int64_t total, int64_t tile, int W) { return (int)(((tile + 1) * W - 1) / total); }
+
+// Shapes that the kernels are built for.
+bool latent_widths(int dc, int dr);
+bool expanded_widths(int dn, int dr);
+
+hipError_t launch_latent(const LatArgs& a, hipStream_t s);
+hipError_t launch_latent_tile(const LatArgs& a, hipStream_t s);
+hipError_t launch_latent_f32(const LatArgs& a, hipStream_t s);
+hipError_t launch_latent_merge(const LatArgs& a, int kt, hipStream_t s);
+
+// Keys per tile of the three kernels.
+constexpr int kLatTile = 64, kLatTileExp = 32, kLatTileF32 = 64;
+
+}  // namespace dsv

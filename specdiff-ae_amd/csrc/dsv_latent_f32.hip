@@ -1,0 +1,206 @@
+// dsv_latent_f32.hip — latent attention in fp32, absorbed and expanded, on gfx950.
+//
+// The mathematics of dsv_latent.hip with keys of two parts, [kn | kr], and values of
+// their own: absorbed, all three are the cache row (kr its end, v its beginning);
+// expanded, kn and v are a head's and kr is shared.  Blocks of 16 rows of a key head,
+// tiles of 64 keys.  Every product is an fp32 matrix product (16x16x4): wave w of four
+// computes the scores of 16 keys and then a quarter of the output's columns.  Operands
+// come straight from the caches (a wave's load takes 16 rows x 64 bytes), because the
+// matrix products at a sixteenth of the 16-bit rate leave time for it: no copy in LDS
+// but the probabilities, held in fp32, and the tile's addresses.
+
+#include "dsv_latent_dev.h"
+
+namespace dsv {
+
+namespace {
+
+constexpr float kTau = 8.0f;
+
+template <int DN, int DR, int DV>
+__global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
+  constexpr int KT = kLatTileF32, ROWS = 16;
+  constexpr int SN = DN / 16, SR = DR / 16, CB = DV / 64;
+  constexpr int PST = KT + 4;  // floats per row of probabilities
+  __shared__ __attribute__((aligned(16))) float p_lds[ROWS * PST];
+  __shared__ uint64_t vis[ROWS * (kTreeMaxM / 64)];
+  __shared__ int16_t par[kTreeMaxM];
+  __shared__ int64_t voff[KT];
+  __shared__ float red[4][ROWS];
+  __shared__ uint32_t flag[4];
+  __shared__ LatSpan span;
+
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  int w = (int)blockIdx.x;
+  const int rb = w % a.n_rb;
+  w /= a.n_rb;
+  const int kvh = w % a.Hk, rj = w / a.Hk;
+  lat_line<256>(a, rb, KT, rj, -1, span);
+  const int64_t total = span.total;
+  const int64_t start = lat_cut(total, rj, a.W), stop = lat_cut(total, rj + 1, a.W);
+  int b = __builtin_amdgcn_readfirstlane(span.b);
+  int t0 = __builtin_amdgcn_readfirstlane(span.off);
+  if (start >= stop) return;
+
+  const int m_lo = rb * ROWS / a.G, m_hi = (min((rb + 1) * ROWS, a.R) - 1) / a.G;
+  const int row = rb * ROWS + li, r_me = min(row, a.R - 1), m_me = r_me / a.G, h_me = kvh * a.G + r_me - m_me * a.G;
+  const float scale = a.scale_log2;
+
+  for (int64_t at = start; at < stop;) {
+    const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
+    const int tiles = lat_tiles(a, len, rb, KT);
+    const int t1 = (int)min((int64_t)tiles, t0 + (stop - at));
+    LatPiece pc;
+    pc.b = b;
+    pc.len = len;
+    pc.t0 = t0;
+    pc.t1 = t1;
+    pc.slot = t0 == 0 && t1 == tiles ? -1 : (((int64_t)kvh * a.n_rb + rb) * a.W + rj) * 2 + (at == start ? 0 : 1);
+    const int end = lat_end(a, len, rb);
+    if (a.parent != nullptr) lat_tree<256>(a, b, m_lo, m_hi - m_lo + 1, par, vis);
+    const float* kn = reinterpret_cast<const float*>(a.kn.p) + b * a.kn.sb + kvh * a.kn.sh;
+    const float* kr = reinterpret_cast<const float*>(a.kr.p) + b * a.kr.sb + kvh * a.kr.sh;
+    const float* vb = reinterpret_cast<const float*>(a.v.p) + b * a.v.sb + kvh * a.v.sh;
+
+    // A lane holds four consecutive entries of its row per step of 16 (the order of the
+    // reduction is the same for both operands).
+    f32x4 qf[SN + SR];
+    const float* q = reinterpret_cast<const float*>(a.q) + b * a.q_sb + (int64_t)m_me * a.q_sm + (int64_t)h_me * a.q_sh + lg * 4;
+#pragma unroll
+    for (int s = 0; s < SN + SR; ++s) qf[s] = *reinterpret_cast<const f32x4*>(q + s * 16);
+    f32x4 acc[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) acc[c] = f32x4{};
+    float mx = kNegInf, ls = 0.f;
+    bool odd = false;
+
+    for (int t = t0; t < t1 && end > 0; ++t) {
+      const int kb = t * KT;
+      // ---- scores of this wave's 16 keys -----------------------------------------------
+      const int n = min(kb + wid * 16 + li, end - 1);
+      const int64_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
+      const float* k1 = kn + key_off(a, a.kn, n, page) + lg * 4;
+      const float* k2 = kr + key_off(a, a.kr, n, page) + lg * 4;
+      if (lg == 0) voff[wid * 16 + li] = key_off(a, a.v, n, page);
+      f32x4 s{};
+#pragma unroll
+      for (int x = 0; x < SN + SR; ++x) {
+        const f32x4 kf = *reinterpret_cast<const f32x4*>(x < SN ? k1 + x * 16 : k2 + (x - SN) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[x][e], s, 0, 0, 0);
+      }
+      const bool whole = lat_whole(a, len, m_lo, kb, KT);
+      if (!whole) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (!lat_sees(a, len, m_me, vis + (m_me - m_lo) * a.MW, kb + wid * 16 + 4 * lg + v)) s[v] = kNegInf;
+      }
+      // ---- probabilities ---------------------------------------------------------------
+      float ps = 0.f;
+      auto probs = [&]() {
+        const float m0 = mx == kNegInf ? 0.f : mx;
+        float p[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) p[v] = __builtin_amdgcn_exp2f((s[v] - m0) * scale);
+        ps = (p[0] + p[1]) + (p[2] + p[3]);
+        *reinterpret_cast<f32x4*>(p_lds + li * PST + wid * 16 + lg * 4) = f32x4{p[0], p[1], p[2], p[3]};
+      };
+      const float m4 = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      probs();
+      const bool over = __ballot((m4 - mx) * scale > kTau) != 0ull;
+      if (lane == 0) flag[wid] = over ? 1 : 0;
+      __syncthreads();
+      if ((flag[0] | flag[1] | flag[2] | flag[3]) != 0) {
+        float mw = fmaxf(m4, __shfl_xor(m4, 16));
+        mw = fmaxf(mw, __shfl_xor(mw, 32));
+        if (lg == 0) red[wid][li] = mw;
+        __syncthreads();
+        const float mn = fmaxf(mx, fmaxf(fmaxf(red[0][li], red[1][li]), fmaxf(red[2][li], red[3][li])));
+        const float al = mn == mx ? 1.f : __builtin_amdgcn_exp2f((mx - mn) * scale);
+        mx = mn;
+        ls *= al;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[c] *= al;
+        probs();
+        __syncthreads();
+      }
+      ls += ps;
+      // ---- this wave's columns -----------------------------------------------------------
+      const float* vc = vb + wid * (DV / 4) + li;
+#pragma unroll 4
+      for (int k4 = 0; k4 < KT / 4; ++k4) {
+        const float pf = p_lds[li * PST + k4 * 4 + lg];
+        const float* vr = vc + voff[k4 * 4 + lg];
+        float vf[CB];
+#pragma unroll
+        for (int c = 0; c < CB; ++c) vf[c] = vr[c * 16];
+        if (!whole && m_hi > m_lo) {
+#pragma unroll
+          for (int c = 0; c < CB; ++c) odd |= !(fabsf(vf[c]) < __builtin_huge_valf());
+        }
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[c], pf, acc[c], 0, 0, 0);
+      }
+      __syncthreads();
+    }
+
+    // ---- the piece's results ---------------------------------------------------------
+    float lw = ls + __shfl_xor(ls, 16);
+    lw += __shfl_xor(lw, 32);
+    if (lg == 0) red[wid][li] = lw;
+    const bool any = __ballot(odd) != 0ull;
+    if (lane == 0) flag[wid] = any ? 1 : 0;
+    __syncthreads();
+    if ((flag[0] | flag[1] | flag[2] | flag[3]) != 0) {
+      lat_exact_rows<float, DV>(lat_args(), pc, kvh, rb, KT, m_lo, vis, wid, ROWS, 4);
+    } else if (row < a.R) {
+      const float l = red[0][li] + red[1][li] + red[2][li] + red[3][li];
+      if (pc.slot >= 0) {
+        const int64_t prow = pc.slot * ROWS + li;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) *reinterpret_cast<f32x4*>(a.opart + prow * DV + wid * (DV / 4) + c * 16 + lg * 4) = acc[c];
+        if (wid == 0 && lg == 0) a.ml[prow] = make_float2(mx, l);
+      } else {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const int64_t off = b * a.o_sb + (int64_t)m_me * a.o_sm + (int64_t)h_me * a.o_sh + wid * (DV / 4) + lg * 4;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          const float x[4] = {acc[c][0] * inv, acc[c][1] * inv, acc[c][2] * inv, acc[c][3] * inv};
+          store4(a, off + c * 16, x);
+        }
+        if (wid == 0 && lg == 0 && a.lse != nullptr)
+          a.lse[b * a.l_sb + (int64_t)m_me * a.l_sm + (int64_t)h_me * a.l_sh] = lat_lse(a, mx, l);
+      }
+    }
+    __syncthreads();
+    at += t1 - t0;
+    t0 = 0;
+    ++b;
+  }
+}
+
+template <int DN, int DR, int DV>
+void launch_w(const LatArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.n_rb * a.Hk * a.W));
+  hipLaunchKernelGGL((latent_f32_kernel<DN, DR, DV>), grid, dim3(256), 0, s, a);
+}
+
+template <int DN>
+void launch_dr(const LatArgs& a, hipStream_t s) {
+  a.dr == 64 ? launch_w<DN, 64, DN>(a, s) : launch_w<DN, 32, DN>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_latent_f32(const LatArgs& a, hipStream_t s) {
+  switch (a.dn) {
+    case 64: launch_dr<64>(a, s); break;
+    case 128: launch_dr<128>(a, s); break;
+    case 256: launch_dr<256>(a, s); break;
+    default: launch_dr<512>(a, s); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace dsv

@@ -23,8 +23,8 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libdsv.so"
 OBJ_DIR = LIB_DIR / "obj"
 
-SOURCES = ["dsv_attn.hip", "dsv_attn_f32.hip", "dsv_merge.hip", "dsv_accept.hip", "dsv_sample.hip", "dsv_commit.hip", "dsv_append.hip", "dsv_bundle.hip", "dsv_window.hip", "dsv_window_tile.hip", "dsv_spec.hip", "dsv_pages.hip", "dsv_lmhead.hip", "dsv_check.hip", "dsv_api.hip"]
-HEADERS = ["dsv_internal.h", "dsv_attn_geo.h", "dsv_attn_f32_geo.h", "dsv_check.h", "dsv_stats.h", "dsv_dma.h", "dsv_window.h", "dsv_window_dev.h"]
+SOURCES = ["dsv_attn.hip", "dsv_attn_f32.hip", "dsv_merge.hip", "dsv_accept.hip", "dsv_sample.hip", "dsv_commit.hip", "dsv_append.hip", "dsv_bundle.hip", "dsv_window.hip", "dsv_window_tile.hip", "dsv_spec.hip", "dsv_pages.hip", "dsv_slots.hip", "dsv_latent_append.hip", "dsv_latent.hip", "dsv_latent_tile.hip", "dsv_latent_f32.hip", "dsv_lmhead.hip", "dsv_check.hip", "dsv_api.hip"]
+HEADERS = ["dsv_internal.h", "dsv_attn_geo.h", "dsv_attn_f32_geo.h", "dsv_check.h", "dsv_stats.h", "dsv_dma.h", "dsv_window.h", "dsv_window_dev.h", "dsv_latent.h", "dsv_latent_dev.h"]
 
 ARCH = "gfx950"
 COMMON_FLAGS = [
@@ -65,7 +65,7 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(out, flush=True)
 
 
-def build(verbose: bool = False, jobs: int = 4) -> Path:
+def build(verbose: bool = False, jobs: int = 8) -> Path:
     """Compile every HIP source for gfx950 and link libdsv.so. Always rebuilds."""
     hipcc = _hipcc()
     OBJ_DIR.mkdir(parents=True, exist_ok=True)

@@ -91,6 +91,11 @@ SIGNATURES = {
     "dsv_pages_extend": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _V, _SZ, _V]),
     "dsv_pages_free": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _V]),
     "dsv_pages_compact": (ctypes.c_int, [_P, _P, _P, _P, _V, _SZ, _V]),
+    "dsv_token_slots": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _V]),
+    "dsv_latent_append": (ctypes.c_int, [_P, _P, _P, ctypes.c_float, _P, _P, _P, ctypes.c_int, _P, _P, _P, _P, _V]),
+    "dsv_latent_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, ctypes.c_int, _I64, ctypes.c_int, ctypes.c_int]),
+    "dsv_latent_attention": (ctypes.c_int, [_P, _P, _I64, _P, _P, _I64, ctypes.c_double, _P, _P, _P, _V, _SZ, _V]),
+    "dsv_latent_expanded": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, ctypes.c_int, ctypes.c_double, _P, _P, _V, _SZ, _V]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,4 +1,4 @@
-"""Page operations of a paged KV cache on MI355X: fork, extend, free, compact.
+"""Page operations of a paged KV cache on MI355X: fork, extend, free, compact, slot maps.
 
 The reference's ``PagedKVCache`` (``diffspec/core/kv_cache/paged_kv.py``) keeps
 allocation, sharing and defragmentation in host code (:81-166, :364-402).
@@ -12,7 +12,8 @@ round trip:
   * ``refcount``   [P] int32, how many table entries name a page (0 = free);
   * ``seqlens``    [B] int32/int64, the tokens of each sequence.
 
-All four calls change these tensors in place.  Pages are taken lowest first,
+``token_slots`` reads them: where the tokens of a step's requests stand in the
+pool.  The other four calls change these tensors in place.  Pages are taken lowest first,
 for requests in ascending order.  ``fork_pages`` and ``extend_pages`` either do
 all that is asked or change nothing; the int32 tensor they return holds
 (pages taken, pages lacking, requests refused), which a caller may read when
@@ -21,13 +22,13 @@ it next synchronises anyway.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Dict, Optional
 
 import torch
 
 from ... import _ext
 
-__all__ = ["fork_pages", "extend_pages", "free_pages", "compact_pages"]
+__all__ = ["fork_pages", "extend_pages", "free_pages", "compact_pages", "token_slots"]
 
 
 def _page_ws(lib, refcount: torch.Tensor, page_table: torch.Tensor, n: int, dev) -> torch.Tensor:
@@ -115,3 +116,44 @@ def compact_pages(kv_pages: torch.Tensor, page_table: torch.Tensor, refcount: to
                                    ws.data_ptr(), ws.numel(), _ext.stream_of(dev))
     _ext.check(rc, "compact_pages")
     return info
+
+
+def token_slots(page_table: torch.Tensor, seqlens: torch.Tensor, new_lens: torch.Tensor, page_size: int, capacity: int,
+                seqs: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
+    """Block tables and slot maps of a step's requests, built on the device.
+
+    Request ``i`` is sequence ``seqs[i]`` (int32/int64 [n]; None: request ``i`` is
+    sequence ``i``), whose last ``new_lens[i]`` of ``seqlens`` tokens are new
+    (``extend_pages`` has given them pages).  In place of the reference's per-token host
+    bookkeeping (``PagedKVCache.write_kv``, paged_kv.py:168-223).
+
+    Args:
+        capacity: tokens that the lists hold, whatever the lengths (which the host need
+            not know); tokens beyond it are left out.
+
+    Returns a dict:
+        slots [capacity] int64: the new tokens' places, page * page_size + offset, in
+            request order (-1 where the table names no page and behind the last token),
+            as ``append_latent_kv`` takes them;
+        positions, requests [capacity] int32: their positions and requests (-1 behind
+            the last);
+        cu_seqlens [n + 1] int32: where each request's tokens begin;
+        block_table [n, n_logical] int32 and lens [n] int32: the requests' page lists
+            (-1 behind their lengths) and lengths, as the attention calls take them.
+    """
+    dev = _ext.require_gpu(page_table, seqlens, new_lens, seqs)
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be [B, n_logical] (got {tuple(page_table.shape)})")
+    if not 0 <= int(capacity) <= 1 << 30:
+        raise ValueError(f"capacity must be in [0, 2^30] (got {capacity})")
+    n, cap = new_lens.numel(), int(capacity)
+    lib = _ext.load()
+    with _ext.on_device(dev):
+        out = {"slots": torch.empty(cap, dtype=torch.int64, device=dev)}
+        for key, shape in (("positions", (cap,)), ("requests", (cap,)), ("cu_seqlens", (n + 1,)),
+                           ("block_table", (n, page_table.shape[1])), ("lens", (n,))):
+            out[key] = torch.empty(shape, dtype=torch.int32, device=dev)
+        rc = lib.dsv_token_slots(_ext.desc(page_table), _ext.desc(seqlens), _ext.desc(new_lens), _ext.desc(seqs),
+                                 _ext.i64(page_size), *[_ext.desc(t) for t in out.values()], _ext.stream_of(dev))
+    _ext.check(rc, "token_slots")
+    return out
