@@ -4,7 +4,7 @@
 // memory straight into LDS: lane l of the instruction lands at LDS address
 // m0 + 16*l.  The source goes through a buffer resource (base, byte range):
 // the hardware checks every lane's offset against the range and returns
-// zeros past it.  Callers keep every destination below 64 KiB.
+// zeros past it.  (Measured: destinations over all of the CU's 160 KiB work.)
 //
 // Wait states: the hardware does not hold these loads back for a write of m0 by
 // the instruction before (one wait state is needed), nor for a resource whose
@@ -62,6 +62,19 @@ __device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(m0), "v"(vaddr) : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
+}
+
+// The same from a uniform address plus a 32-bit byte offset per lane (valid ones).
+template <bool NT = true>
+__device__ __forceinline__ void dma_off(uint32_t lds, const void* base, uint32_t voff) {
+  const uint64_t p = (uint64_t)base;
+  const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32) |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(m0), "v"(voff), "s"(u) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff), "s"(u) : "memory", "m0");
 }
 
 // Wait until at most N of this wave's vector-memory operations are pending.

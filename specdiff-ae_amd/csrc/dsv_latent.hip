@@ -62,6 +62,13 @@ __device__ __forceinline__ float groups_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// x, computed again at every use: what is derived from it is not held in registers
+// across the loop.
+__device__ __forceinline__ uint32_t again(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // LDS image of a tile: the rows' first dc entries, then their last dr.  Chunk c (16
 // bytes) of key k stands at slot c ^ swz(k): 16 keys read at one chunk (scores) and
 // four keys read at two neighbouring chunks (values, transposed) fall on distinct
@@ -91,13 +98,17 @@ struct LatLds {
 template <typename T, int DC, int DR, int ROWS>
 __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   using L = LatLds<DC, DR, ROWS>;
+  // Scores: KG groups of KB x 16 keys, RG groups of QR x 16 rows, a wave each.
+  constexpr int RG = ROWS == 64 ? 2 : 1, KG = 4 / RG, KB = 4 / KG, QR = ROWS / 16 / RG;
   constexpr int KT = L::KT, RB = ROWS / 16, KSN = DC / 32, KSR = DR / 32, KS = KSN + KSR;
   constexpr int CB = DC / 64;              // blocks of 16 output columns per wave
   constexpr int SHIFT = kProbShift<T, 10>;
   constexpr int KPI = 1024 / L::NB;        // keys per DMA instruction of the first part
   constexpr int IPN = 16 / KPI;            // such instructions per wave and tile
+  static_assert(KPI <= 2, "");
   constexpr int KPR = 1024 / L::RB;        // the same of the second part
   constexpr int IPR = 16 * L::RB / 1024;
+  static_assert(L::TILE % 1024 == 0, "XORs within a row leave the buffer alone");
   static_assert(sizeof(L) <= 163840, "LDS of a CU");
   static_assert(2 * kTreeMaxM <= ROWS * KT * 2, "the parents are staged in p");
   __shared__ __attribute__((aligned(1024))) L lds;
@@ -119,17 +130,16 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   if (start >= stop) return;
 
   const int m_lo = rb * ROWS / a.G, m_hi = (min((rb + 1) * ROWS, a.R) - 1) / a.G;
-  int mrow[RB];  // the position of this lane's row in each block of 16
-#pragma unroll
-  for (int i = 0; i < RB; ++i) mrow[i] = min(rb * ROWS + i * 16 + li, a.R - 1) / a.G;
-
   // Operand addresses within a tile (the swizzles are XORs of whole chunks).
-  const int key = wid * 16 + li;
-  const uint32_t kofs = key * L::NB + ((lg ^ swz_n(key)) << 4);
-  const uint32_t rofs = KT * L::NB + key * L::RB + ((lg ^ swz_r<DR>(key)) << 4);
+  const int kg = wid % KG, rg = wid / KG;
+  const uint32_t qofs = li * L::NB + ((lg ^ swz_n(li)) << 4);
+  const uint32_t qrofs = KT * L::NB + li * L::RB + ((lg ^ swz_r<DR>(li)) << 4);
+  const uint32_t kofs = kg * KB * 16 * L::NB + qofs, rofs = kg * KB * 16 * L::RB + qrofs;
   const int vkey = 4 * lg + (li >> 2);
   const uint32_t vofs = vkey * L::NB + (((wid * (DC / 32) + ((li & 3) >> 1)) ^ swz_n(vkey)) << 4) + (li & 1) * 8;
-  const uint32_t pw = li * 128 + (((wid >> 1) * 4 + lg) ^ (li >> 1)) * 16 + (wid & 1) * 8;
+  // Probabilities: of 32 keys, lane group g holds 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3 as
+  // one chunk, which is the order in which the values are read.
+  const uint32_t pw = rg * QR * 2048 + li * 128 + (((kg * KB >> 1) * 4 + lg) ^ (li >> 1)) * 16 + (KB == 1 ? (kg & 1) * 8 : 0);
   const uint32_t pr = li * 128 + ((lg ^ (li >> 1)) << 4);
   const uint32_t ring0 = lds_addr(lds.ring);
   const float scale = a.scale_log2;
@@ -149,54 +159,72 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 
     if (a.parent != nullptr) lat_tree<256>(a, b, m_lo, m_hi - m_lo + 1, reinterpret_cast<int16_t*>(lds.p), lds.vis);
 
-    // ---- DMA of a tile: wave w loads keys [16w, 16w + 16) --------------------------
-    // Keys at or behind the end are replaced by the last one (no row sees them).
-    auto issue = [&](int t) {
-      const int kb = t * KT + wid * 16;
-      const int n = min(kb + li, end - 1);
-      const int64_t off = 2 * key_off(a, a.kn, n, a.pt != nullptr ? page_of(a, b, n) : 0);
-      const uint32_t dst = ring0 + (uint32_t)(t & 1) * L::TILE + wid * 16 * L::NB;
+    // ---- DMA of 16 rows of this wave into a buffer: lane l knows row l % 16 ----------
+    auto issue_rows = [&](int buf, const char* src, int64_t off) {
+      const uint32_t dst = ring0 + (uint32_t)buf * L::TILE + wid * 16 * L::NB;
+      const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
+      const uint32_t ln = again(lane);
+      auto row = [&](int k) {
+        return src + (((int64_t)__builtin_amdgcn_readlane(hi, k) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, k));
+      };
+      // (One instruction's address at a time: the registers are full.)
 #pragma unroll
       for (int x = 0; x < IPN; ++x) {
-        const int k = x * KPI + lane / (64 / KPI);
-        const int64_t o = __shfl((long long)off, k);
-        dma_lane<false>(dst + x * 1024, base + o + (((lane % (64 / KPI)) ^ swz_n(k)) << 4));
+        if constexpr (KPI == 1) {
+          dma_off<false>(dst + x * 1024, row(x), (ln ^ swz_n(x)) << 4);
+        } else {
+          const int k = 2 * x + (lane >> 5);
+          const char* r = lane < 32 ? row(2 * x) : row(2 * x + 1);
+          dma_lane<false>(dst + x * 1024, r + (((lane & 31) ^ swz_n(k)) << 4));
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const uint32_t dst2 = ring0 + (uint32_t)(t & 1) * L::TILE + KT * L::NB + wid * 16 * L::RB;
+      const uint32_t dst2 = ring0 + (uint32_t)buf * L::TILE + KT * L::NB + wid * 16 * L::RB;
 #pragma unroll
       for (int x = 0; x < IPR; ++x) {
         const int k = x * KPR + lane / (64 / KPR);
         const int64_t o = __shfl((long long)off, k);
-        dma_lane<false>(dst2 + x * 1024, base + o + L::NB + (((lane % (64 / KPR)) ^ swz_r<DR>(k)) << 4));
+        dma_lane<false>(dst2 + x * 1024, src + o + L::NB + (((lane % (64 / KPR)) ^ swz_r<DR>(k)) << 4));
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
+    // A tile's keys; those at or behind the end are replaced by the last one (no row
+    // sees them).
+    auto issue = [&](int t) {
+      const int n = min(t * KT + wid * 16 + li, end - 1);
+      issue_rows(t & 1, base, 2 * key_off(a, a.kn, n, a.pt != nullptr ? page_of(a, b, n) : 0));
+    };
 
-    u32x4 qf[RB][KS];
+    u32x4 qf[QR][KS];
     f32x4 acc[RB][CB];
-    float mx[RB], ls[RB];
+    float mx[RB], ls[QR];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       mx[i] = kNegInf;
-      ls[i] = 0.f;
 #pragma unroll
       for (int c = 0; c < CB; ++c) acc[i][c] = f32x4{};
     }
+#pragma unroll
+    for (int i = 0; i < QR; ++i) ls[i] = 0.f;
     uint32_t odd = 0;
     if (end > 0) {
       issue(t0);
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const int r = min(rb * ROWS + i * 16 + li, a.R - 1);
-        const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_sb + (int64_t)mrow[i] * a.q_sm +
-                            (int64_t)(r - mrow[i] * a.G) * a.q_sh + lg * 8;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qf[i][ks] = *reinterpret_cast<const u32x4*>(q + ks * 32);
+      // The queries come through the other buffer (a load that ends in registers would
+      // be waited for at its first use, in the loop, and the tiles in flight with it).
+      if (wid * 16 < ROWS) {
+        const int r = min(rb * ROWS + wid * 16 + li, a.R - 1), m = r / a.G;
+        issue_rows((t0 + 1) & 1, reinterpret_cast<const char*>(a.q), 2 * (b * a.q_sb + (int64_t)m * a.q_sm + (int64_t)(r - m * a.G) * a.q_sh));
       }
+      wait_vmcnt<0>();
+      barrier_lds();
+      const uint8_t* qt = lds.ring + ((t0 + 1) & 1) * L::TILE;
 #pragma unroll
-      for (int i = 0; i < RB; ++i)
+      for (int i = 0; i < QR; ++i)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[i][ks]));
-
+        for (int ks = 0; ks < KS; ++ks)
+          qf[i][ks] = ks < KSN ? *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * 16 * L::NB + (qofs ^ (ks << 6)))
+                               : *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * 16 * L::RB + (qrofs ^ ((ks - KSN) << 6)));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       for (int t = t0; t < t1; ++t) {
         // The other buffer is free once every wave is done with tile t - 1.
         barrier_lds();
@@ -206,47 +234,81 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         } else {
           wait_vmcnt<0>();
         }
+        // (Waves that share keys wait for each other's loads.)
+        if constexpr (KB > 1) barrier_lds();
         asm volatile("" ::: "memory");
-        const uint8_t* tile = lds.ring + (t & 1) * L::TILE;
-        // ---- scores of this wave's 16 keys (its own loads: no barrier) ----------------
-        f32x4 s[RB];
+        const uint32_t stage = (uint32_t)(t & 1) * L::TILE;
+        // ---- scores of this wave's keys and rows ----------------------------------------
+        f32x4 s[QR][KB];
 #pragma unroll
-        for (int i = 0; i < RB; ++i) s[i] = f32x4{};
+        for (int i = 0; i < QR; ++i)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 kf = ks < KSN ? *reinterpret_cast<const u32x4*>(tile + (kofs ^ (ks << 6)))
-                                    : *reinterpret_cast<const u32x4*>(tile + (rofs ^ ((ks - KSN) << 6)));
+          for (int k = 0; k < KB; ++k) s[i][k] = f32x4{};
+        const uint32_t ko = again(kofs) + stage, ro = again(rofs) + stage;
+        auto read_k = [&](int x) {
+          const int ks = x / KB, k = x % KB;
+          return ks < KSN ? *reinterpret_cast<const u32x4*>(lds.ring + (ko ^ (ks << 6)) + k * 16 * L::NB)
+                          : *reinterpret_cast<const u32x4*>(lds.ring + (ro ^ ((ks - KSN) << 6)) + k * 16 * L::RB);
+        };
+        u32x4 kf[4];
 #pragma unroll
-          for (int i = 0; i < RB; ++i) s[i] = mfma16<T>(kf, qf[i][ks], s[i]);
+        for (int x = 0; x < 3; ++x) kf[x] = read_k(x);
+#pragma unroll
+        for (int x = 0; x < KS * KB; ++x) {
+          if (x + 3 < KS * KB) kf[(x + 3) % 4] = read_k(x + 3);
+#pragma unroll
+          for (int i = 0; i < QR; ++i) s[i][x % KB] = mfma16<T>(kf[x % 4], qf[i][x / KB], s[i][x % KB]);
+          __builtin_amdgcn_sched_barrier(0);
         }
         const int kb = t * KT;
         const bool whole = lat_whole(a, len, m_lo, kb, KT);
         if (!whole) {
+          // (Loops, so that it costs no registers.)
+          uint32_t keep = 0;
+#pragma unroll 1
+          for (int i = 0; i < QR; ++i) {
+            const int m = min(rb * ROWS + (rg * QR + i) * 16 + li, a.R - 1) / a.G;
+#pragma unroll 1
+            for (int v = 0; v < 4 * KB; ++v)
+              keep |= (lat_sees(a, len, m, lds.vis + (m - m_lo) * a.MW, kb + (kg * KB + v / 4) * 16 + 4 * lg + v % 4) ? 1u : 0u)
+                      << (4 * KB * i + v);
+          }
 #pragma unroll
-          for (int i = 0; i < RB; ++i)
+          for (int i = 0; i < QR; ++i)
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (!lat_sees(a, len, mrow[i], lds.vis + (mrow[i] - m_lo) * a.MW, kb + wid * 16 + 4 * lg + v)) s[i][v] = kNegInf;
+            for (int v = 0; v < 4 * KB; ++v) s[i][v / 4][v % 4] = ((keep >> (4 * KB * i + v)) & 1u) ? s[i][v / 4][v % 4] : kNegInf;
         }
         // ---- probabilities, relative to the maximum so far ------------------------------
-        float ps[RB];
+        float ps[QR];
+        auto top = [&](int i) {
+          float m = fmaxf(fmaxf(s[i][0][0], s[i][0][1]), fmaxf(s[i][0][2], s[i][0][3]));
+          if constexpr (KB > 1) m = fmaxf(m, fmaxf(fmaxf(s[i][KB - 1][0], s[i][KB - 1][1]), fmaxf(s[i][KB - 1][2], s[i][KB - 1][3])));
+          return m;
+        };
+        auto max_of = [&](int i) { return RG > 1 && rg != 0 ? mx[QR * (RG - 1) + i] : mx[i]; };
         auto probs = [&]() {
 #pragma unroll
-          for (int i = 0; i < RB; ++i) {
-            const float m0 = mx[i] == kNegInf ? 0.f : mx[i];
-            float p[4];
+          for (int i = 0; i < QR; ++i) {
+            const float m = max_of(i), m0 = m == kNegInf ? 0.f : m;
+            float p[4 * KB], sum = 0.f;
+            uint32_t w2[2 * KB];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) p[v] = __builtin_amdgcn_exp2f(fmaf(s[i][v] - m0, scale, (float)SHIFT));
-            ps[i] = (p[0] + p[1]) + (p[2] + p[3]);
-            *reinterpret_cast<u32x2*>(lds.p + i * 2048 + pw) = u32x2{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3])};
+            for (int v = 0; v < 4 * KB; ++v) {
+              p[v] = __builtin_amdgcn_exp2f(fmaf(s[i][v / 4][v % 4] - m0, scale, (float)SHIFT));
+              sum += p[v];
+            }
+#pragma unroll
+            for (int v = 0; v < 2 * KB; ++v) w2[v] = pack2<T>(p[2 * v], p[2 * v + 1]);
+            ps[i] = sum;
+            if constexpr (KB == 1)
+              *reinterpret_cast<u32x2*>(lds.p + i * 2048 + pw) = u32x2{w2[0], w2[1]};
+            else
+              *reinterpret_cast<u32x4*>(lds.p + i * 2048 + pw) = u32x4{w2[0], w2[1], w2[2 * KB - 2], w2[2 * KB - 1]};
           }
         };
         bool over = false;
 #pragma unroll
-        for (int i = 0; i < RB; ++i) {
-          const float m4 = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
-          over |= (m4 - mx[i]) * scale > kLatTau<T>;
-        }
+        for (int i = 0; i < QR; ++i) over |= (top(i) - max_of(i)) * scale > kLatTau<T>;
         probs();
         if (lane == 0) lds.flag[wid] = 0;
         if (__ballot(over) != 0ull && lane == 0) lds.flag[wid] = 1;
@@ -254,18 +316,19 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         const u32x4 fl = *reinterpret_cast<const u32x4*>(lds.flag);
         if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0) {
 #pragma unroll
-          for (int i = 0; i < RB; ++i) {
-            const float m4 = groups_max(fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
-            if (lg == 0) lds.red[wid][i * 16 + li] = m4;
+          for (int i = 0; i < QR; ++i) {
+            const float m = groups_max(top(i));
+            if (lg == 0) lds.red[kg][(rg * QR + i) * 16 + li] = m;
           }
           barrier_after_lds();
 #pragma unroll
           for (int i = 0; i < RB; ++i) {
-            const int r = i * 16 + li;
-            const float mn = fmaxf(mx[i], fmaxf(fmaxf(lds.red[0][r], lds.red[1][r]), fmaxf(lds.red[2][r], lds.red[3][r])));
+            float mn = mx[i];
+#pragma unroll
+            for (int k = 0; k < KG; ++k) mn = fmaxf(mn, lds.red[k][i * 16 + li]);
             const float al = mn == mx[i] ? 1.f : __builtin_amdgcn_exp2f((mx[i] - mn) * scale);
             mx[i] = mn;
-            ls[i] *= al;
+            if (i / QR == rg) ls[i % QR] *= al;
 #pragma unroll
             for (int c = 0; c < CB; ++c) acc[i][c] *= al;
           }
@@ -273,24 +336,33 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
           barrier_after_lds();
         }
 #pragma unroll
-        for (int i = 0; i < RB; ++i) ls[i] += ps[i];
+        for (int i = 0; i < QR; ++i) ls[i] += ps[i];
         // ---- this wave's columns -------------------------------------------------------
+        u32x4 pf[2][RB], vf[3];
+        const uint32_t vo = again(vofs) + stage;
+        auto read_p = [&](int k2) {
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          u32x4 pf[RB];
+          for (int i = 0; i < RB; ++i) pf[k2][i] = *reinterpret_cast<const u32x4*>(lds.p + i * 2048 + (pr ^ (k2 << 6)));
+        };
+        auto read_v = [&](int x) {
+          const uint8_t* vp = lds.ring + (vo ^ ((x % CB) << 5)) + x / CB * 32 * L::NB;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 16 * L::NB));
+          const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+          return u32x4{l2[0], l2[1], h2[0], h2[1]};
+        };
+        read_p(0);
+        vf[0] = read_v(0);
+        vf[1] = read_v(1);
 #pragma unroll
-          for (int i = 0; i < RB; ++i) pf[i] = *reinterpret_cast<const u32x4*>(lds.p + i * 2048 + (pr ^ (k2 << 6)));
+        for (int x = 0; x < 2 * CB; ++x) {
+          if (x == CB - 2) read_p(1);
+          if (x + 2 < 2 * CB) vf[(x + 2) % 3] = read_v(x + 2);
+          const u32x4 v = vf[x % 3];
+          if (!whole && m_hi > m_lo) odd |= nonfinite2<T>(v[0]) | nonfinite2<T>(v[1]) | nonfinite2<T>(v[2]) | nonfinite2<T>(v[3]);
 #pragma unroll
-          for (int c = 0; c < CB; ++c) {
-            const uint8_t* vp = tile + (vofs ^ (c << 5)) + k2 * 32 * L::NB;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 16 * L::NB));
-            const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-            const u32x4 vf = u32x4{l2[0], l2[1], h2[0], h2[1]};
-            if (!whole && m_hi > m_lo) odd |= nonfinite2<T>(vf[0]) | nonfinite2<T>(vf[1]) | nonfinite2<T>(vf[2]) | nonfinite2<T>(vf[3]);
-#pragma unroll
-            for (int i = 0; i < RB; ++i) acc[i][c] = mfma16<T>(vf, pf[i], acc[i][c]);
-          }
+          for (int i = 0; i < RB; ++i) acc[i][x % CB] = mfma16<T>(v, pf[x / CB][i], acc[i][x % CB]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -299,9 +371,9 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
     constexpr float kBack = 1.f / (1 << SHIFT);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
+    for (int i = 0; i < QR; ++i) {
       const float x = groups_sum(ls[i]);
-      if (lg == 0) lds.red[wid][i * 16 + li] = x;
+      if (lg == 0) lds.red[kg][(rg * QR + i) * 16 + li] = x;
     }
     if (lane == 0) lds.flag[wid] = 0;
     if (__ballot(odd != 0) != 0ull && lane == 0) lds.flag[wid] = 1;
@@ -313,7 +385,10 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
         const int r = i * 16 + li, row = rb * ROWS + r;
-        const float l = (lds.red[0][r] + lds.red[1][r] + lds.red[2][r] + lds.red[3][r]) * kBack;
+        float l = 0.f;
+#pragma unroll
+        for (int k = 0; k < KG; ++k) l += lds.red[k][r];
+        l *= kBack;
         if (row >= a.R) continue;
         if (pc.slot >= 0) {
           const int64_t prow = pc.slot * ROWS + r;
@@ -324,15 +399,15 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
           continue;
         }
         const float inv = l > 0.f ? kBack / l : (l == 0.f ? 0.f : l);
-        const int h = row - mrow[i] * a.G;
-        const int64_t off = b * a.o_sb + (int64_t)mrow[i] * a.o_sm + (int64_t)h * a.o_sh + wid * (DC / 4) + lg * 4;
+        const int m = row / a.G, h = row - m * a.G;
+        const int64_t off = b * a.o_sb + (int64_t)m * a.o_sm + (int64_t)h * a.o_sh + wid * (DC / 4) + lg * 4;
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
           const float x[4] = {acc[i][c][0] * inv, acc[i][c][1] * inv, acc[i][c][2] * inv, acc[i][c][3] * inv};
           store4(a, off + c * 16, x);
         }
         if (wid == 0 && lg == 0 && a.lse != nullptr)
-          a.lse[b * a.l_sb + (int64_t)mrow[i] * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, mx[i], l);
+          a.lse[b * a.l_sb + (int64_t)m * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, mx[i], l);
       }
     }
     // Stores are done before the next piece counts its loads.
