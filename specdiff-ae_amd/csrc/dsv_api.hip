@@ -2396,7 +2396,11 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
       }
     }
   }
-  const int64_t tiles = B * ((n_keys + p.kt - 1) / p.kt);
+  const int64_t tiles = B * std::max<int64_t>(1, (n_keys + p.kt - 1) / p.kt);
+  if (tiles >= ((int64_t)1 << 31)) {
+    p.err = "batch x keys beyond 2^31 tiles of 32 or 64 keys";
+    return p;
+  }
   W = std::max<int64_t>(1, std::min<int64_t>(W, tiles / 2));
   p.W = (int)W;
   const size_t rows = W > 1 ? (size_t)units * W * 2 * p.rpb : 0;

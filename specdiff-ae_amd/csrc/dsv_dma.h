@@ -65,16 +65,15 @@ __device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
 }
 
 // The same from a uniform address plus a 32-bit byte offset per lane (valid ones).
-template <bool NT = true>
-__device__ __forceinline__ void dma_off(uint32_t lds, const void* base, uint32_t voff) {
-  const uint64_t p = (uint64_t)base;
-  const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32) |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+// SALU: the address was made by scalar instructions, so that one wait state is enough.
+template <bool NT = true, bool SALU = false>
+__device__ __forceinline__ void dma_off(uint32_t lds, uint64_t base, uint32_t voff) {
+  static_assert(!NT, "");
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
-  if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(m0), "v"(voff), "s"(u) : "memory", "m0");
+  if constexpr (SALU)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff), "s"(base) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff), "s"(u) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff), "s"(base) : "memory", "m0");
 }
 
 // Wait until at most N of this wave's vector-memory operations are pending.

@@ -56,18 +56,25 @@ DSV_HD int lat_end(const LatArgs& a, int len, int rb) {
 // The tiles of kt keys of block rb in a sequence: at least one, so that every
 // sequence's rows are somebody's.
 DSV_HD int lat_tiles(const LatArgs& a, int len, int rb, int kt) {
-  const int t = (int)(((int64_t)lat_end(a, len, rb) + kt - 1) / kt);
+  const int t = (int)((unsigned)(lat_end(a, len, rb) + kt - 1) / (unsigned)kt);
   return t > 0 ? t : 1;
 }
 
 // Work sharing.  For each unit (key head, block of rows) the sequences' tiles
-// stand in one line, which W workgroups share out evenly: range j is
-// [total * j / W, total * (j + 1) / W).  A range holds pieces of one or more
-// sequences.  Where a piece is all of its sequence's tiles the workgroup writes
-// the output, else a partial: number 0 for the piece that the range begins with,
-// 1 for another, which its end cuts (so at most two per range).
-DSV_HD int64_t lat_cut(int64_t total, int j, int W) { return total * j / W; }
-DSV_HD int lat_range_of(int64_t total, int64_t tile, int W) { return (int)(((tile + 1) * W - 1) / total); }
+// stand in one line, which W workgroups share out evenly: the first total % W ranges
+// hold a tile more than the others.  A range holds pieces of one or more sequences.
+// Where a piece is all of its sequence's tiles the workgroup writes the output, else a
+// partial: number 0 for the piece that the range begins with, 1 for another, which its
+// end cuts (so at most two per range).  The line is below 2^31 tiles.
+struct LatCut {
+  int q, r;  // total / W, total % W
+  DSV_HD LatCut(int total, int W) : q(total / W), r(total - q * W) {}
+  DSV_HD int begin(int j) const { return j * q + (j < r ? j : r); }
+  DSV_HD int range_of(int tile) const {
+    const int head = r * (q + 1);
+    return tile < head ? tile / (q + 1) : r + (tile - head) / q;
+  }
+};
 
 // Shapes that the kernels are built for.
 bool latent_widths(int dc, int dr);

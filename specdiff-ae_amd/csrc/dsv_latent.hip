@@ -42,23 +42,39 @@ constexpr float kLatTau = 8.0f;
 template <>
 constexpr float kLatTau<F16> = 5.0f;
 
+// Products: 16x16x32 into four values a lane, 32x32x16 into sixteen.
 template <typename T>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
-template <>
-__device__ __forceinline__ f32x4 mfma16<BF16>(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (__is_same(T, BF16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-template <>
-__device__ __forceinline__ f32x4 mfma16<F16>(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+template <typename T>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (__is_same(T, BF16))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+template <bool WIDE>
+struct LatAcc {
+  typedef f32x4 type;
+};
+template <>
+struct LatAcc<true> {
+  typedef f32x16 type;
+};
 
+// Over the lanes that hold one row (TR lanes apart).
+template <int TR>
 __device__ __forceinline__ float groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
+  if constexpr (TR == 16) x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
 }
+template <int TR>
 __device__ __forceinline__ float groups_sum(float x) {
-  x += __shfl_xor(x, 16);
+  if constexpr (TR == 16) x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
 }
 
@@ -70,10 +86,9 @@ __device__ __forceinline__ uint32_t again(uint32_t x) {
 }
 
 // LDS image of a tile: the rows' first dc entries, then their last dr.  Chunk c (16
-// bytes) of key k stands at slot c ^ swz(k): 16 keys read at one chunk (scores) and
-// four keys read at two neighbouring chunks (values, transposed) fall on distinct
-// banks.
-__device__ __forceinline__ int swz_n(int key) { return ((key & 7) << 1) | ((key >> 3) & 1); }
+// bytes) of key k stands at slot c ^ swz(k): keys read at one chunk (scores) and four
+// keys read at neighbouring chunks (values, transposed) fall on distinct banks.
+__device__ __forceinline__ int swz_n(int key) { return ((key & 3) << 2) | ((key >> 2) & 3); }
 template <int DR>
 __device__ __forceinline__ int swz_r(int key) {
   return DR == 64 ? (key >> 1) & 7 : (key >> 2) & 3;
@@ -85,36 +100,190 @@ struct LatLds {
   static constexpr int NB = DC * 2, RB = DR * 2;
   static constexpr int TILE = KT * (NB + RB);
   // Sets of tree keys: a block's rows of H heads belong to at most ROWS nodes, of
-  // H >= 2 heads to ROWS / 2 + 1 (lat_block).
+  // H >= 2 heads to ROWS / 2 + 1 (the plan sees to it).
   static constexpr int VIS = 36 * (kTreeMaxM / 64) * 8;
-  uint8_t ring[2 * TILE];
+  uint8_t ring[2 * TILE];          // tiles; at the end the output rows in fp32
   uint8_t p[ROWS * KT * 2];
   uint64_t vis[VIS / 8];
   float red[4][ROWS];
+  float m[ROWS];
   uint32_t flag[4];
   LatSpan span;
+  static_assert(TILE % 1024 == 0, "XORs within a row leave the buffer alone");
+  static_assert(ROWS * DC * 4 <= 2 * TILE, "");
+  static_assert(2 * kTreeMaxM <= ROWS * KT * 2, "the parents are staged in p");
+};
+
+// DMA of one wave's 16 rows of a tile: keys [16w, 16w + 16).  (Instructions are what a
+// lone wave on a SIMD is short of: one is issued every four cycles at most.)
+template <int DC, int DR>
+struct LatLoader {
+  using L = LatLds<DC, DR, 16>;
+  static constexpr int KPI = 1024 / L::NB;         // keys per instruction of the first part
+  static constexpr int IPN = 16 / KPI;             // such instructions per tile
+  static constexpr int KPR = 1024 / L::RB;         // the same of the second part
+  static constexpr int IPR = 16 * L::RB / 1024;
+  static constexpr int N = IPN + IPR;
+  static_assert(KPI <= 2, "");
+  const LatArgs& a;
+  int wid, lane;
+  uint32_t dstn, dstr;
+  bool run_ok;                                     // a wave's 16 keys lie at even, 32-bit distances
+  int b, end;
+  uint64_t base;
+  int32_t pwin;                                    // lane l: physical page of the sequence's page pw0 + l
+  int pw0;
+
+  __device__ __forceinline__ LatLoader(const LatArgs& args, int w, int l, uint32_t ring) : a(args), wid(w), lane(l) {
+    dstn = ring + w * 16 * L::NB;
+    dstr = ring + L::KT * L::NB + w * 16 * L::RB;
+    run_ok = (a.pt == nullptr || a.ps_shift >= 4) && a.kn.st <= (1 << 24);
+  }
+  __device__ __forceinline__ void sequence(int b_, int end_) {
+    b = b_;
+    end = end_;
+    base = (uint64_t)a.kn.p + 2 * (b * a.kn.sb);
+    pw0 = -64;
+  }
+  // Rows at even distances from a uniform address.
+  __device__ __forceinline__ void run(uint32_t buf, uint64_t addr) {
+    const uint32_t ln = again(lane), st2 = (uint32_t)(2 * a.kn.st);
+    uint64_t r = addr;
+#pragma unroll
+    for (int x = 0; x < IPN; ++x) {
+      const uint32_t k = ln / (64 / KPI), c = ln % (64 / KPI);
+      dma_off<false, true>(dstn + buf + x * 1024, r, (KPI > 1 ? k * st2 : 0) + ((c ^ swz_n(x * KPI + (KPI > 1 ? k : 0))) << 4));
+      r += (uint64_t)KPI * st2;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int x = 0; x < IPR; ++x) {
+      const uint32_t k = x * KPR + ln / (64 / KPR), c = ln % (64 / KPR);
+      dma_off<false, true>(dstr + buf + x * 1024, addr + L::NB, k * st2 + ((c ^ swz_r<DR>(k)) << 4));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // Rows anywhere: lane l knows the address of row l % 16.
+  __device__ __forceinline__ void rows(uint32_t buf, uint64_t addr) {
+    const uint32_t ln = again(lane);
+#pragma unroll 1
+    for (int x = 0; x < IPN; ++x) {
+      const int k = x * KPI + ln / (64 / KPI);
+      const char* r = (const char*)__shfl((long long)addr, k);
+      dma_lane<false>(dstn + buf + x * 1024, r + (((ln % (64 / KPI)) ^ swz_n(k)) << 4));
+    }
+#pragma unroll 1
+    for (int x = 0; x < IPR; ++x) {
+      const int k = x * KPR + ln / (64 / KPR);
+      const char* r = (const char*)__shfl((long long)addr, k);
+      dma_lane<false>(dstr + buf + x * 1024, r + L::NB + (((ln % (64 / KPR)) ^ swz_r<DR>(k)) << 4));
+    }
+  }
+  // Keys [kb, kb + 64) into a buffer; those at or behind the end are replaced by the last
+  // one (no row sees them).  Page numbers are kept in a window: a load at the use would be
+  // waited for, and the tiles in flight with it.
+  template <bool FIRST>
+  __device__ __forceinline__ void issue(uint32_t buf, int kb) {
+    const int n0 = min(kb + wid * 16, end - 1), n1 = min(kb + wid * 16 + 15, end - 1);
+    if (a.pt != nullptr) {
+      const int p0 = n0 >> a.ps_shift, p1 = n1 >> a.ps_shift;
+      if (FIRST || p0 < pw0 || p1 >= pw0 + 64) {
+        pw0 = p0;
+        pwin = (int32_t)page_of(a, b, (int)min((int64_t)(p0 + lane) << a.ps_shift, (int64_t)end - 1));
+        asm volatile("" : "+v"(pwin));  // (waited for here)
+      }
+    }
+    if (!FIRST && run_ok && n1 == n0 + 15) {
+      const int64_t pg = a.pt != nullptr ? __builtin_amdgcn_readlane(pwin, (n0 >> a.ps_shift) - pw0) : 0;
+      const uint64_t at = base + 2 * key_off(a, a.kn, n0, pg);
+      run(buf, ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32) |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at));
+    } else {
+      const int n = min(n0 + (lane & 15), end - 1);
+      rows(buf, base + 2 * key_off(a, a.kn, n, a.pt != nullptr ? __shfl(pwin, (n >> a.ps_shift) - pw0) : 0));
+    }
+  }
+  // The query rows [row0, row0 + n); those behind the last are replaced by it.
+  __device__ __forceinline__ void queries(uint32_t buf, int row0, int n) {
+    if (wid * 16 >= n) return;
+    const int r = min(row0 + wid * 16 + (lane & 15), a.R - 1), m = r / a.G;
+    rows(buf, (uint64_t)a.q + 2 * (b * a.q_sb + (int64_t)m * a.q_sm + (int64_t)(r - m * a.G) * a.q_sh));
+  }
+};
+
+// Rows of a block from LDS (fp32, chunk c of row r at c ^ (r & 15)) into the output or a
+// partial: a wave takes a row at a time.  l: [groups][ROWS] sums, red.
+template <int DC, int ROWS, int GROUPS>
+__device__ __forceinline__ void lat_store_rows(const LatArgs& a, const LatPiece& pc, int rb, const uint8_t* acc, const float* m,
+                                               const float (*red)[ROWS], float back) {
+  constexpr int N = DC / 64;
+  const int lane = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < ROWS; r += 4) {
+    const int row = rb * ROWS + r;
+    if (row >= a.R) break;
+    float l = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) l += red[g][r];
+    l *= back;
+    float x[N];
+#pragma unroll
+    for (int c = 0; c < N / 4; ++c) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(acc + r * DC * 4 + (((lane * (N / 4) + c) ^ (r & 15)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * c + e] = v[e];
+    }
+    if (pc.slot >= 0) {
+      const int64_t pr = pc.slot * ROWS + r;
+#pragma unroll
+      for (int c = 0; c < N / 4; ++c)
+        *reinterpret_cast<f32x4*>(a.opart + pr * DC + lane * N + 4 * c) = f32x4{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]} * back;
+      if (lane == 0) a.ml[pr] = make_float2(m[r], l);
+      continue;
+    }
+    const float inv = l > 0.f ? back / l : (l == 0.f ? 0.f : l);
+    const int pos = row / a.G, h = row - pos * a.G;
+    const int64_t off = b_off(a, pc.b, pos, h) + lane * N;
+#pragma unroll
+    for (int c = 0; c < N / 4; ++c) {
+      const float y[4] = {x[4 * c] * inv, x[4 * c + 1] * inv, x[4 * c + 2] * inv, x[4 * c + 3] * inv};
+      store4(a, off + 4 * c, y);
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[pc.b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m[r], l);
+  }
+}
+
+template <int ROWS, bool WIDE>
+struct LatShape;
+// 16x16x32 products.  Scores: wave w has keys [16w, 16w + 16) for all rows.
+template <int ROWS>
+struct LatShape<ROWS, false> {
+  static constexpr int KG = 4, RG = 1, QR = ROWS / 16, RB = ROWS / 16, TR = 16;
+};
+// 32x32x16 products, of 64 rows: wave w has keys [32 (w % 2), + 32) for rows [32 (w / 2), + 32).
+template <>
+struct LatShape<64, true> {
+  static constexpr int KG = 2, RG = 2, QR = 1, RB = 2, TR = 32;
 };
 
 template <typename T, int DC, int DR, int ROWS>
 __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   using L = LatLds<DC, DR, ROWS>;
-  // Scores: KG groups of KB x 16 keys, RG groups of QR x 16 rows, a wave each.
-  constexpr int RG = ROWS == 64 ? 2 : 1, KG = 4 / RG, KB = 4 / KG, QR = ROWS / 16 / RG;
-  constexpr int KT = L::KT, RB = ROWS / 16, KSN = DC / 32, KSR = DR / 32, KS = KSN + KSR;
-  constexpr int CB = DC / 64;              // blocks of 16 output columns per wave
+  using Loader = LatLoader<DC, DR>;
+  constexpr bool WIDE = ROWS == 64;
+  using S = LatShape<ROWS, WIDE>;
+  // TR rows a product; scores of QR such row groups per wave, outputs of all RB.
+  constexpr int KT = L::KT, KG = S::KG, QR = S::QR, RB = S::RB, TR = S::TR;
+  constexpr int DS = WIDE ? 16 : 32;               // depth of a product
+  constexpr int KSN = DC / DS, KSR = DR / DS, KS = KSN + KSR;
+  constexpr int CB = DC / 4 / TR;                  // output tiles of TR columns per wave
+  constexpr int NV = WIDE ? 16 : 4;                // values of a product's result per lane
   constexpr int SHIFT = kProbShift<T, 10>;
-  constexpr int KPI = 1024 / L::NB;        // keys per DMA instruction of the first part
-  constexpr int IPN = 16 / KPI;            // such instructions per wave and tile
-  static_assert(KPI <= 2, "");
-  constexpr int KPR = 1024 / L::RB;        // the same of the second part
-  constexpr int IPR = 16 * L::RB / 1024;
-  static_assert(L::TILE % 1024 == 0, "XORs within a row leave the buffer alone");
+  using Acc = typename LatAcc<WIDE>::type;
   static_assert(sizeof(L) <= 163840, "LDS of a CU");
-  static_assert(2 * kTreeMaxM <= ROWS * KT * 2, "the parents are staged in p");
   __shared__ __attribute__((aligned(1024))) L lds;
 
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int lane = threadIdx.x & 63, li = lane & (TR - 1), lg = lane / TR;
 
   // Dispatch ids go round-robin over the 8 XCDs: give each a contiguous eighth, so
   // that the row blocks of a range, which read the same keys, share an L2.
@@ -122,32 +291,38 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   const int w = (nblk & 7) == 0 ? (int)(blockIdx.x & 7) * (nblk >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
   const int rb = w % a.n_rb, rj = w / a.n_rb;
 
-  lat_line<256>(a, rb, KT, rj, -1, lds.span);
-  const int64_t total = lds.span.total;
-  const int64_t start = lat_cut(total, rj, a.W), stop = lat_cut(total, rj + 1, a.W);
+  const LatCut cut(lat_line<256>(a, rb, KT, rj, -1, lds.span), a.W);
+  const int start = cut.begin(rj), stop = cut.begin(rj + 1);
+  if (start >= stop) return;
   int b = __builtin_amdgcn_readfirstlane(lds.span.b);
   int t0 = __builtin_amdgcn_readfirstlane(lds.span.off);
-  if (start >= stop) return;
 
   const int m_lo = rb * ROWS / a.G, m_hi = (min((rb + 1) * ROWS, a.R) - 1) / a.G;
+
   // Operand addresses within a tile (the swizzles are XORs of whole chunks).
   const int kg = wid % KG, rg = wid / KG;
   const uint32_t qofs = li * L::NB + ((lg ^ swz_n(li)) << 4);
   const uint32_t qrofs = KT * L::NB + li * L::RB + ((lg ^ swz_r<DR>(li)) << 4);
-  const uint32_t kofs = kg * KB * 16 * L::NB + qofs, rofs = kg * KB * 16 * L::RB + qrofs;
-  const int vkey = 4 * lg + (li >> 2);
-  const uint32_t vofs = vkey * L::NB + (((wid * (DC / 32) + ((li & 3) >> 1)) ^ swz_n(vkey)) << 4) + (li & 1) * 8;
-  // Probabilities: of 32 keys, lane group g holds 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3 as
-  // one chunk, which is the order in which the values are read.
-  const uint32_t pw = rg * QR * 2048 + li * 128 + (((kg * KB >> 1) * 4 + lg) ^ (li >> 1)) * 16 + (KB == 1 ? (kg & 1) * 8 : 0);
-  const uint32_t pr = li * 128 + ((lg ^ (li >> 1)) << 4);
-  const uint32_t ring0 = lds_addr(lds.ring);
+  const uint32_t kofs = kg * (KT / KG) * L::NB + qofs, rofs = kg * (KT / KG) * L::RB + qrofs;
+  uint32_t vofs;
+  {
+    const int bl = lane >> 4, bi = lane & 15;
+    const int vkey = 4 * (WIDE ? bl >> 1 : bl) + (bi >> 2), vcol = wid * (DC / 4) + (WIDE ? 16 * (bl & 1) : 0) + 4 * (bi & 3);
+    vofs = vkey * L::NB + (((vcol >> 3) ^ swz_n(vkey)) << 4) + (vcol & 7) * 2;
+  }
+  // Probabilities: a row's chunk holds what a lane needs for a product, of keys that the
+  // reading of the values gives it: of 16 keys (WIDE) 4g .. 4g + 3 and 8 + 4g .., which
+  // are a lane's own scores; of 32 keys 4g .. 4g + 3 and 16 + 4g ...
+  const int prow = rg * QR * TR + li, psw = (li >> 1) & 7;
+  const uint32_t pw = prow * 128 + (((WIDE ? kg * 4 + lg : (kg >> 1) * 4 + lg) ^ psw) << 4) + (WIDE ? 0 : (kg & 1) * 8);
+  const uint32_t pr = li * 128 + ((lg ^ psw) << 4);
   const float scale = a.scale_log2;
+  Loader ld(a, wid, lane, lds_addr(lds.ring));
 
-  for (int64_t at = start; at < stop;) {
+  for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
     const int tiles = lat_tiles(a, len, rb, KT);
-    const int t1 = (int)min((int64_t)tiles, t0 + (stop - at));
+    const int t1 = min(tiles, t0 + (stop - at));
     LatPiece pc;
     pc.b = b;
     pc.len = len;
@@ -155,261 +330,224 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
     pc.t1 = t1;
     pc.slot = t0 == 0 && t1 == tiles ? -1 : ((int64_t)rb * a.W + rj) * 2 + (at == start ? 0 : 1);
     const int end = lat_end(a, len, rb);
-    const char* base = reinterpret_cast<const char*>(a.kn.p) + 2 * (b * a.kn.sb);
+    ld.sequence(b, end);
 
     if (a.parent != nullptr) lat_tree<256>(a, b, m_lo, m_hi - m_lo + 1, reinterpret_cast<int16_t*>(lds.p), lds.vis);
 
-    // ---- DMA of 16 rows of this wave into a buffer: lane l knows row l % 16 ----------
-    auto issue_rows = [&](int buf, const char* src, int64_t off) {
-      const uint32_t dst = ring0 + (uint32_t)buf * L::TILE + wid * 16 * L::NB;
-      const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
-      const uint32_t ln = again(lane);
-      auto row = [&](int k) {
-        return src + (((int64_t)__builtin_amdgcn_readlane(hi, k) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, k));
-      };
-      // (One instruction's address at a time: the registers are full.)
-#pragma unroll
-      for (int x = 0; x < IPN; ++x) {
-        if constexpr (KPI == 1) {
-          dma_off<false>(dst + x * 1024, row(x), (ln ^ swz_n(x)) << 4);
-        } else {
-          const int k = 2 * x + (lane >> 5);
-          const char* r = lane < 32 ? row(2 * x) : row(2 * x + 1);
-          dma_lane<false>(dst + x * 1024, r + (((lane & 31) ^ swz_n(k)) << 4));
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const uint32_t dst2 = ring0 + (uint32_t)buf * L::TILE + KT * L::NB + wid * 16 * L::RB;
-#pragma unroll
-      for (int x = 0; x < IPR; ++x) {
-        const int k = x * KPR + lane / (64 / KPR);
-        const int64_t o = __shfl((long long)off, k);
-        dma_lane<false>(dst2 + x * 1024, src + o + L::NB + (((lane % (64 / KPR)) ^ swz_r<DR>(k)) << 4));
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    // A tile's keys; those at or behind the end are replaced by the last one (no row
-    // sees them).
-    auto issue = [&](int t) {
-      const int n = min(t * KT + wid * 16 + li, end - 1);
-      issue_rows(t & 1, base, 2 * key_off(a, a.kn, n, a.pt != nullptr ? page_of(a, b, n) : 0));
-    };
-
     u32x4 qf[QR][KS];
-    f32x4 acc[RB][CB];
+    Acc acc[RB][CB];
     float mx[RB], ls[QR];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       mx[i] = kNegInf;
 #pragma unroll
-      for (int c = 0; c < CB; ++c) acc[i][c] = f32x4{};
+      for (int c = 0; c < CB; ++c) acc[i][c] = Acc{};
     }
 #pragma unroll
     for (int i = 0; i < QR; ++i) ls[i] = 0.f;
     uint32_t odd = 0;
     if (end > 0) {
-      issue(t0);
-      // The queries come through the other buffer (a load that ends in registers would
-      // be waited for at its first use, in the loop, and the tiles in flight with it).
-      if (wid * 16 < ROWS) {
-        const int r = min(rb * ROWS + wid * 16 + li, a.R - 1), m = r / a.G;
-        issue_rows((t0 + 1) & 1, reinterpret_cast<const char*>(a.q), 2 * (b * a.q_sb + (int64_t)m * a.q_sm + (int64_t)(r - m * a.G) * a.q_sh));
-      }
+      // The queries come through the other buffer (a load that ends in registers would be
+      // waited for at its first use, in the loop, and the tiles in flight with it).
+      ld.template issue<true>((uint32_t)(t0 & 1) * L::TILE, t0 * KT);
+      const uint32_t other = (uint32_t)((t0 + 1) & 1) * L::TILE;
+      ld.queries(other, rb * ROWS, ROWS);
       wait_vmcnt<0>();
       barrier_lds();
-      const uint8_t* qt = lds.ring + ((t0 + 1) & 1) * L::TILE;
+      const uint8_t* qt = lds.ring + other;
 #pragma unroll
       for (int i = 0; i < QR; ++i)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          qf[i][ks] = ks < KSN ? *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * 16 * L::NB + (qofs ^ (ks << 6)))
-                               : *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * 16 * L::RB + (qrofs ^ ((ks - KSN) << 6)));
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      for (int t = t0; t < t1; ++t) {
-        // The other buffer is free once every wave is done with tile t - 1.
-        barrier_lds();
-        if (t + 1 < t1) {
-          issue(t + 1);
-          wait_vmcnt<IPN + IPR>();
-        } else {
-          wait_vmcnt<0>();
+        for (int ks = 0; ks < KS; ++ks) {
+          const int x = ks < KSN ? ks * DS / 8 : (ks - KSN) * DS / 8;
+          qf[i][ks] = ks < KSN ? *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * TR * L::NB + (qofs ^ ((x & 15) << 4)) + (x >> 4) * 256)
+                               : *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * TR * L::RB + (qrofs ^ (x << 4)));
         }
-        // (Waves that share keys wait for each other's loads.)
-        if constexpr (KB > 1) barrier_lds();
-        asm volatile("" ::: "memory");
-        const uint32_t stage = (uint32_t)(t & 1) * L::TILE;
-        // ---- scores of this wave's keys and rows ----------------------------------------
-        f32x4 s[QR][KB];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    for (int t = t0; t < t1 && end > 0; ++t) {
+      // The other buffer is free once every wave is done with tile t - 1.
+      barrier_lds();
+      if (t + 1 < t1) {
+        ld.template issue<false>((uint32_t)((t + 1) & 1) * L::TILE, (t + 1) * KT);
+        wait_vmcnt<Loader::N>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      const uint32_t stage = (uint32_t)(t & 1) * L::TILE;
+      if constexpr (WIDE) barrier_lds();  // (waves that share keys wait for each other's loads)
+      asm volatile("" ::: "memory");
+      // ---- scores of this wave's keys and rows ----------------------------------------
+      Acc s[QR];
+#pragma unroll
+      for (int i = 0; i < QR; ++i) s[i] = Acc{};
+      const uint32_t ko = again(kofs) + stage, ro = again(rofs) + stage;
+      // The swizzle reaches the 16 chunks of 256 bytes; beyond, an offset.
+      auto read_k = [&](int ks) {
+        const int x = ks < KSN ? ks * DS / 8 : (ks - KSN) * DS / 8;
+        return ks < KSN ? *reinterpret_cast<const u32x4*>(lds.ring + (ko ^ ((x & 15) << 4)) + (x >> 4) * 256)
+                        : *reinterpret_cast<const u32x4*>(lds.ring + (ro ^ (x << 4)));
+      };
+      constexpr int KA = 6;  // operands ahead
+      u32x4 kf[KA + 1];
+#pragma unroll
+      for (int x = 0; x < KA; ++x) kf[x] = read_k(x);
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        if (x + KA < KS) kf[(x + KA) % (KA + 1)] = read_k(x + KA);
+#pragma unroll
+        for (int i = 0; i < QR; ++i) s[i] = mfma<T>(kf[x % (KA + 1)], qf[i][x], s[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const int kb = t * KT;
+      const bool whole = lat_whole(a, len, m_lo, kb, KT);
+      // Value v of a result is key 8 (v / 4) + 4 lg + v % 4 of the wave's.
+      if (!whole) {
+        uint32_t keep = 0;
+#pragma unroll 1
+        for (int i = 0; i < QR; ++i) {
+          const int m = min(rb * ROWS + (rg * QR + i) * TR + li, a.R - 1) / a.G;
+#pragma unroll 1
+          for (int v = 0; v < NV; ++v)
+            keep |= (lat_sees(a, len, m, lds.vis + (m - m_lo) * a.MW, kb + kg * (KT / KG) + 8 * (v / 4) + 4 * lg + v % 4) ? 1u : 0u)
+                    << (NV * i + v);
+        }
 #pragma unroll
         for (int i = 0; i < QR; ++i)
 #pragma unroll
-          for (int k = 0; k < KB; ++k) s[i][k] = f32x4{};
-        const uint32_t ko = again(kofs) + stage, ro = again(rofs) + stage;
-        auto read_k = [&](int x) {
-          const int ks = x / KB, k = x % KB;
-          return ks < KSN ? *reinterpret_cast<const u32x4*>(lds.ring + (ko ^ (ks << 6)) + k * 16 * L::NB)
-                          : *reinterpret_cast<const u32x4*>(lds.ring + (ro ^ ((ks - KSN) << 6)) + k * 16 * L::RB);
-        };
-        u32x4 kf[4];
+          for (int v = 0; v < NV; ++v) s[i][v] = ((keep >> (NV * i + v)) & 1u) ? s[i][v] : kNegInf;
+      }
+      // ---- probabilities, relative to the maximum so far ------------------------------
+      float ps[QR];
+      auto top = [&](int i) {
+        float m = s[i][0];
 #pragma unroll
-        for (int x = 0; x < 3; ++x) kf[x] = read_k(x);
+        for (int v = 1; v < NV; ++v) m = fmaxf(m, s[i][v]);
+        return m;
+      };
+      auto max_of = [&](int i) { return WIDE && rg != 0 ? mx[RB - 1] : mx[i]; };
+      auto probs = [&]() {
 #pragma unroll
-        for (int x = 0; x < KS * KB; ++x) {
-          if (x + 3 < KS * KB) kf[(x + 3) % 4] = read_k(x + 3);
+        for (int i = 0; i < QR; ++i) {
+          const float m = max_of(i), m0 = m == kNegInf ? 0.f : m;
+          float sum = 0.f;
+          uint32_t w2[NV / 2];
 #pragma unroll
-          for (int i = 0; i < QR; ++i) s[i][x % KB] = mfma16<T>(kf[x % 4], qf[i][x / KB], s[i][x % KB]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        const int kb = t * KT;
-        const bool whole = lat_whole(a, len, m_lo, kb, KT);
-        if (!whole) {
-          // (Loops, so that it costs no registers.)
-          uint32_t keep = 0;
-#pragma unroll 1
-          for (int i = 0; i < QR; ++i) {
-            const int m = min(rb * ROWS + (rg * QR + i) * 16 + li, a.R - 1) / a.G;
-#pragma unroll 1
-            for (int v = 0; v < 4 * KB; ++v)
-              keep |= (lat_sees(a, len, m, lds.vis + (m - m_lo) * a.MW, kb + (kg * KB + v / 4) * 16 + 4 * lg + v % 4) ? 1u : 0u)
-                      << (4 * KB * i + v);
+          for (int v = 0; v < NV / 2; ++v) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * v] - m0, scale, (float)SHIFT));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * v + 1] - m0, scale, (float)SHIFT));
+            sum += p0 + p1;
+            w2[v] = pack2<T>(p0, p1);
           }
-#pragma unroll
-          for (int i = 0; i < QR; ++i)
-#pragma unroll
-            for (int v = 0; v < 4 * KB; ++v) s[i][v / 4][v % 4] = ((keep >> (4 * KB * i + v)) & 1u) ? s[i][v / 4][v % 4] : kNegInf;
-        }
-        // ---- probabilities, relative to the maximum so far ------------------------------
-        float ps[QR];
-        auto top = [&](int i) {
-          float m = fmaxf(fmaxf(s[i][0][0], s[i][0][1]), fmaxf(s[i][0][2], s[i][0][3]));
-          if constexpr (KB > 1) m = fmaxf(m, fmaxf(fmaxf(s[i][KB - 1][0], s[i][KB - 1][1]), fmaxf(s[i][KB - 1][2], s[i][KB - 1][3])));
-          return m;
-        };
-        auto max_of = [&](int i) { return RG > 1 && rg != 0 ? mx[QR * (RG - 1) + i] : mx[i]; };
-        auto probs = [&]() {
-#pragma unroll
-          for (int i = 0; i < QR; ++i) {
-            const float m = max_of(i), m0 = m == kNegInf ? 0.f : m;
-            float p[4 * KB], sum = 0.f;
-            uint32_t w2[2 * KB];
-#pragma unroll
-            for (int v = 0; v < 4 * KB; ++v) {
-              p[v] = __builtin_amdgcn_exp2f(fmaf(s[i][v / 4][v % 4] - m0, scale, (float)SHIFT));
-              sum += p[v];
-            }
-#pragma unroll
-            for (int v = 0; v < 2 * KB; ++v) w2[v] = pack2<T>(p[2 * v], p[2 * v + 1]);
-            ps[i] = sum;
-            if constexpr (KB == 1)
-              *reinterpret_cast<u32x2*>(lds.p + i * 2048 + pw) = u32x2{w2[0], w2[1]};
-            else
-              *reinterpret_cast<u32x4*>(lds.p + i * 2048 + pw) = u32x4{w2[0], w2[1], w2[2 * KB - 2], w2[2 * KB - 1]};
+          ps[i] = sum;
+          if constexpr (WIDE) {
+            *reinterpret_cast<u32x4*>(lds.p + pw) = u32x4{w2[0], w2[1], w2[2], w2[3]};
+            *reinterpret_cast<u32x4*>(lds.p + (pw ^ 32)) = u32x4{w2[NV / 2 - 4], w2[NV / 2 - 3], w2[NV / 2 - 2], w2[NV / 2 - 1]};
+          } else {
+            *reinterpret_cast<u32x2*>(lds.p + i * 2048 + pw) = u32x2{w2[0], w2[1]};
           }
-        };
-        bool over = false;
+        }
+      };
+      bool over = false;
 #pragma unroll
-        for (int i = 0; i < QR; ++i) over |= (top(i) - max_of(i)) * scale > kLatTau<T>;
-        probs();
-        if (lane == 0) lds.flag[wid] = 0;
-        if (__ballot(over) != 0ull && lane == 0) lds.flag[wid] = 1;
+      for (int i = 0; i < QR; ++i) over |= (top(i) - max_of(i)) * scale > kLatTau<T>;
+      probs();
+      const uint32_t up = __ballot(over) != 0ull ? 1 : 0;
+      if (lane == 0) lds.flag[wid] = up;
+      // The first operands of the output come while the waves meet.
+      constexpr int PK = KT / DS, VA = 3;
+      u32x4 pf[RB], pn[RB], vf[VA + 1];
+      const uint32_t vo = again(vofs) + stage;
+      auto read_p = [&](int k, u32x4 (&f)[RB]) {
+#pragma unroll
+        for (int i = 0; i < RB; ++i) f[i] = *reinterpret_cast<const u32x4*>(lds.p + i * TR * 128 + (pr ^ (k * DS * 2)));
+      };
+      auto read_v = [&](int x) {
+        const uint8_t* vp = lds.ring + x / CB * DS * L::NB;
+        const uint32_t o = vo ^ ((x % CB) * TR * 2), o8 = DS == 16 ? o ^ 32 : o;  // (the swizzle of keys 8 on)
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + o));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + o8 + DS / 2 * L::NB));
+        const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+        return u32x4{l2[0], l2[1], h2[0], h2[1]};
+      };
+      barrier_after_lds();
+      const u32x4 fl = *reinterpret_cast<const u32x4*>(lds.flag);
+      read_p(0, pf);
+#pragma unroll
+      for (int x = 0; x < VA; ++x) vf[x] = read_v(x);
+      if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0) {
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+          const float m = groups_max<TR>(top(i));
+          if (lg == 0) lds.red[kg][(rg * QR + i) * TR + li] = m;
+        }
         barrier_after_lds();
-        const u32x4 fl = *reinterpret_cast<const u32x4*>(lds.flag);
-        if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0) {
 #pragma unroll
-          for (int i = 0; i < QR; ++i) {
-            const float m = groups_max(top(i));
-            if (lg == 0) lds.red[kg][(rg * QR + i) * 16 + li] = m;
-          }
-          barrier_after_lds();
+        for (int i = 0; i < RB; ++i) {
+          float mn = mx[i];
 #pragma unroll
-          for (int i = 0; i < RB; ++i) {
-            float mn = mx[i];
+          for (int k = 0; k < KG; ++k) mn = fmaxf(mn, lds.red[k][i * TR + li]);
+          const float al = mn == mx[i] ? 1.f : __builtin_amdgcn_exp2f((mx[i] - mn) * scale);
+          mx[i] = mn;
+          if (i / QR == rg) ls[i % QR] *= al;
 #pragma unroll
-            for (int k = 0; k < KG; ++k) mn = fmaxf(mn, lds.red[k][i * 16 + li]);
-            const float al = mn == mx[i] ? 1.f : __builtin_amdgcn_exp2f((mx[i] - mn) * scale);
-            mx[i] = mn;
-            if (i / QR == rg) ls[i % QR] *= al;
-#pragma unroll
-            for (int c = 0; c < CB; ++c) acc[i][c] *= al;
-          }
-          probs();
-          barrier_after_lds();
+          for (int c = 0; c < CB; ++c) acc[i][c] *= al;
         }
+        probs();
+        barrier_after_lds();
+        read_p(0, pf);
+      }
 #pragma unroll
-        for (int i = 0; i < QR; ++i) ls[i] += ps[i];
-        // ---- this wave's columns -------------------------------------------------------
-        u32x4 pf[2][RB], vf[3];
-        const uint32_t vo = again(vofs) + stage;
-        auto read_p = [&](int k2) {
+      for (int i = 0; i < QR; ++i) ls[i] += ps[i];
+      // ---- this wave's columns -------------------------------------------------------
+      const bool look = !whole && m_hi > m_lo;
 #pragma unroll
-          for (int i = 0; i < RB; ++i) pf[k2][i] = *reinterpret_cast<const u32x4*>(lds.p + i * 2048 + (pr ^ (k2 << 6)));
-        };
-        auto read_v = [&](int x) {
-          const uint8_t* vp = lds.ring + (vo ^ ((x % CB) << 5)) + x / CB * 32 * L::NB;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 16 * L::NB));
-          const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-          return u32x4{l2[0], l2[1], h2[0], h2[1]};
-        };
-        read_p(0);
-        vf[0] = read_v(0);
-        vf[1] = read_v(1);
+      for (int x = 0; x < PK * CB; ++x) {
+        if (x % CB == 0 && x / CB + 1 < PK) read_p(x / CB + 1, (x / CB) % 2 ? pf : pn);
+        if (x + VA < PK * CB) vf[(x + VA) % (VA + 1)] = read_v(x + VA);
+        const u32x4 v = vf[x % (VA + 1)];
 #pragma unroll
-        for (int x = 0; x < 2 * CB; ++x) {
-          if (x == CB - 2) read_p(1);
-          if (x + 2 < 2 * CB) vf[(x + 2) % 3] = read_v(x + 2);
-          const u32x4 v = vf[x % 3];
-          if (!whole && m_hi > m_lo) odd |= nonfinite2<T>(v[0]) | nonfinite2<T>(v[1]) | nonfinite2<T>(v[2]) | nonfinite2<T>(v[3]);
-#pragma unroll
-          for (int i = 0; i < RB; ++i) acc[i][x % CB] = mfma16<T>(v, pf[x / CB][i], acc[i][x % CB]);
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < RB; ++i) acc[i][x % CB] = mfma<T>(v, (x / CB) % 2 ? pn[i] : pf[i], acc[i][x % CB]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (look) {
+#pragma unroll 1
+        for (int x = 0; x < PK * CB; ++x) {
+          const u32x4 v = read_v(x);
+          odd |= nonfinite2<T>(v[0]) | nonfinite2<T>(v[1]) | nonfinite2<T>(v[2]) | nonfinite2<T>(v[3]);
         }
       }
     }
 
     // ---- the piece's results ---------------------------------------------------------
-    constexpr float kBack = 1.f / (1 << SHIFT);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < QR; ++i) {
-      const float x = groups_sum(ls[i]);
-      if (lg == 0) lds.red[kg][(rg * QR + i) * 16 + li] = x;
+      const float x = groups_sum<TR>(ls[i]);
+      if (lg == 0) lds.red[kg][(rg * QR + i) * TR + li] = x;
     }
-    if (lane == 0) lds.flag[wid] = 0;
-    if (__ballot(odd != 0) != 0ull && lane == 0) lds.flag[wid] = 1;
+    if (wid == 0 && lg == 0) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) lds.m[i * TR + li] = mx[i];
+    }
+    const uint32_t any = __ballot(odd != 0) != 0ull ? 1 : 0;
+    if (lane == 0) lds.flag[wid] = any;
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int q4 = 0; q4 < NV / 4; ++q4) {
+          const int r = i * TR + li, ch = wid * (DC / 16) + c * (TR / 4) + 2 * q4 + lg;
+          *reinterpret_cast<f32x4*>(lds.ring + r * DC * 4 + ((ch ^ (r & 15)) << 4)) =
+              f32x4{acc[i][c][4 * q4], acc[i][c][4 * q4 + 1], acc[i][c][4 * q4 + 2], acc[i][c][4 * q4 + 3]};
+        }
     __syncthreads();
     const u32x4 fl = *reinterpret_cast<const u32x4*>(lds.flag);
-    if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0) {
+    if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0)
       lat_exact_rows<T, DC>(lat_args(), pc, 0, rb, KT, m_lo, lds.vis, wid, ROWS, 4);
-    } else {
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const int r = i * 16 + li, row = rb * ROWS + r;
-        float l = 0.f;
-#pragma unroll
-        for (int k = 0; k < KG; ++k) l += lds.red[k][r];
-        l *= kBack;
-        if (row >= a.R) continue;
-        if (pc.slot >= 0) {
-          const int64_t prow = pc.slot * ROWS + r;
-#pragma unroll
-          for (int c = 0; c < CB; ++c)
-            *reinterpret_cast<f32x4*>(a.opart + prow * DC + wid * (DC / 4) + c * 16 + lg * 4) = acc[i][c] * kBack;
-          if (wid == 0 && lg == 0) a.ml[prow] = make_float2(mx[i], l);
-          continue;
-        }
-        const float inv = l > 0.f ? kBack / l : (l == 0.f ? 0.f : l);
-        const int m = row / a.G, h = row - m * a.G;
-        const int64_t off = b * a.o_sb + (int64_t)m * a.o_sm + (int64_t)h * a.o_sh + wid * (DC / 4) + lg * 4;
-#pragma unroll
-        for (int c = 0; c < CB; ++c) {
-          const float x[4] = {acc[i][c][0] * inv, acc[i][c][1] * inv, acc[i][c][2] * inv, acc[i][c][3] * inv};
-          store4(a, off + c * 16, x);
-        }
-        if (wid == 0 && lg == 0 && a.lse != nullptr)
-          a.lse[b * a.l_sb + (int64_t)m * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, mx[i], l);
-      }
-    }
+    else
+      lat_store_rows<DC, ROWS, KG>(a, pc, rb, lds.ring, lds.m, lds.red, 1.f / (1 << SHIFT));
     // Stores are done before the next piece counts its loads.
     wait_vmcnt<0>();
     __syncthreads();
@@ -431,11 +569,12 @@ __device__ __forceinline__ void merge_rows(const LatArgs& a, int kt, int64_t x, 
   const int rb = (int)(x % a.n_rb);
   x /= a.n_rb;
   const int kvh = (int)(x % a.Hk), b = (int)(x / a.Hk);
-  lat_line<256>(a, rb, kt, 0, b, span);
-  const int64_t total = span.total, at = span.at;
+  const int total = lat_line<256>(a, rb, kt, 0, b, span), at = span.at;
   const int tiles = lat_tiles(a, len_of(a, b), rb, kt);
-  const int j0 = lat_range_of(total, at, a.W), j1 = lat_range_of(total, at + tiles - 1, a.W);
+  const LatCut cut(total, a.W);
+  const int j0 = cut.range_of(at), j1 = cut.range_of(at + tiles - 1);
   if (j0 == j1) return;  // one piece: written by its workgroup
+  const int which0 = cut.begin(j0) >= at ? 0 : 1;
   const int lane = threadIdx.x & 63;
   const int i = part * 4 + (threadIdx.x >> 6), row = rb * a.rpb + i;
   if (row >= a.R) return;
@@ -450,10 +589,9 @@ __device__ __forceinline__ void merge_rows(const LatArgs& a, int kt, int64_t x, 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = min(s0 + u, j1);
-      const int64_t begin = lat_cut(total, j, a.W);
-      const int64_t pr = ((unit * a.W + j) * 2 + (begin >= at ? 0 : 1)) * a.rpb + i;
-      // (Ranges of nothing, where there are more ranges than tiles, hold no partial.)
-      const bool none = s0 + u > j1 || begin == lat_cut(total, j + 1, a.W);
+      // (A range behind the first one begins with this sequence.)
+      const int64_t pr = ((unit * a.W + j) * 2 + (j == j0 ? which0 : 0)) * a.rpb + i;
+      const bool none = s0 + u > j1;
       ml[u] = none ? make_float2(kNegInf, 0.f) : a.ml[pr];
 #pragma unroll
       for (int e = 0; e < N; ++e) p[u][e] = none ? 0.f : a.opart[pr * DV + lane * N + e];

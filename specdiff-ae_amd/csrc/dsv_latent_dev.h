@@ -30,30 +30,32 @@ __device__ __forceinline__ int64_t key_off(const LatArgs& a, const LatSrc& s, in
 
 // Where a workgroup's range begins (or a sequence's tiles lie): filled by one thread.
 struct LatSpan {
-  int64_t total, at;   // tiles of the line, tiles before
-  int64_t wave[16];    // scratch of the scan
+  int at;              // tiles before a sequence
   int b, off;          // sequence, tile within it
+  int wave[16];        // scratch of the scan
 };
 
-// The line of a unit's tiles over the sequences: `total`, and the sequence and tile
-// at which range j begins (find_b < 0), or the place of sequence find_b (`at`).
+// The line of a unit's tiles over the sequences: returns their number, and finds the
+// sequence and tile at which range j begins (find_b < 0; none for a range of nothing),
+// or the place of sequence find_b (`at`).
 // Every thread of the workgroup calls it; ends with a barrier.
 template <int NT>
-__device__ __forceinline__ void lat_line(const LatArgs& a, int rb, int kt, int j, int find_b, LatSpan& s) {
+__device__ __forceinline__ int lat_line(const LatArgs& a, int rb, int kt, int j, int find_b, LatSpan& s) {
   const int per = (a.B + NT - 1) / NT;
   const int lo = min((int)threadIdx.x * per, a.B), hi = min(lo + per, a.B);
-  int64_t sum = 0;
+  int sum = 0;
   for (int b = lo; b < hi; ++b) sum += lat_tiles(a, len_of(a, b), rb, kt);
-  int64_t pre = sum;
+  int pre = sum, total = 0;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  if (a.B > 1) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t x = __shfl_up((long long)pre, o);
-    if (lane >= o) pre += x;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(pre, o);
+      if (lane >= o) pre += x;
+    }
   }
-  if (lane == 63) s.wave[wid] = pre;
+  if (lane == (a.B > 1 ? 63 : 0)) s.wave[wid] = pre;
   __syncthreads();
-  int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) {
     if (w < wid) pre += s.wave[w];
@@ -64,19 +66,18 @@ __device__ __forceinline__ void lat_line(const LatArgs& a, int rb, int kt, int j
     if (find_b >= lo && find_b < hi) {
       for (int b = lo; b < find_b; ++b) pre += lat_tiles(a, len_of(a, b), rb, kt);
       s.at = pre;
-      s.total = total;
     }
   } else {
-    const int64_t start = lat_cut(total, j, a.W);
+    const int start = LatCut(total, a.W).begin(j);
     if (start >= pre && start < pre + sum) {
       int b = lo;
       for (int t; start >= pre + (t = lat_tiles(a, len_of(a, b), rb, kt)); ++b) pre += t;
       s.b = b;
-      s.off = (int)(start - pre);
-      s.total = total;
+      s.off = start - pre;
     }
   }
   __syncthreads();
+  return total;
 }
 
 // The trees of a workgroup: parents of one sequence's nodes and, of the nodes
@@ -141,6 +142,11 @@ __device__ __forceinline__ void store4(const LatArgs& a, int64_t off, const floa
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
   }
+}
+
+// Element offset of an output row.
+__device__ __forceinline__ int64_t b_off(const LatArgs& a, int b, int m, int h) {
+  return b * a.o_sb + (int64_t)m * a.o_sm + (int64_t)h * a.o_sh;
 }
 
 // ln sum exp of a row from its maximum (a score) and its sum relative to it.

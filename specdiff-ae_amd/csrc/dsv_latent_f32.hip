@@ -36,21 +36,21 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
   const int rb = w % a.n_rb;
   w /= a.n_rb;
   const int kvh = w % a.Hk, rj = w / a.Hk;
-  lat_line<256>(a, rb, KT, rj, -1, span);
-  const int64_t total = span.total;
-  const int64_t start = lat_cut(total, rj, a.W), stop = lat_cut(total, rj + 1, a.W);
+  const int total = lat_line<256>(a, rb, KT, rj, -1, span);
+  const LatCut cut(total, a.W);
+  const int start = cut.begin(rj), stop = cut.begin(rj + 1);
+  if (start >= stop) return;
   int b = __builtin_amdgcn_readfirstlane(span.b);
   int t0 = __builtin_amdgcn_readfirstlane(span.off);
-  if (start >= stop) return;
 
   const int m_lo = rb * ROWS / a.G, m_hi = (min((rb + 1) * ROWS, a.R) - 1) / a.G;
   const int row = rb * ROWS + li, r_me = min(row, a.R - 1), m_me = r_me / a.G, h_me = kvh * a.G + r_me - m_me * a.G;
   const float scale = a.scale_log2;
 
-  for (int64_t at = start; at < stop;) {
+  for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
     const int tiles = lat_tiles(a, len, rb, KT);
-    const int t1 = (int)min((int64_t)tiles, t0 + (stop - at));
+    const int t1 = min(tiles, t0 + (stop - at));
     LatPiece pc;
     pc.b = b;
     pc.len = len;

@@ -105,12 +105,12 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
   w /= a.W;
   const int rb = a.n_rb - 1 - w % a.n_rb, kvh = w / a.n_rb;
 
-  lat_line<512>(a, rb, KT, rj, -1, lds.span);
-  const int64_t total = lds.span.total;
-  const int64_t start = lat_cut(total, rj, a.W), stop = lat_cut(total, rj + 1, a.W);
+  const int total = lat_line<512>(a, rb, KT, rj, -1, lds.span);
+  const LatCut cut(total, a.W);
+  const int start = cut.begin(rj), stop = cut.begin(rj + 1);
+  if (start >= stop) return;
   int b = __builtin_amdgcn_readfirstlane(lds.span.b);
   int tb = __builtin_amdgcn_readfirstlane(lds.span.off);
-  if (start >= stop) return;
 
   const int row0 = rb * 256 + wid * 32;
   const bool wave_active = row0 < a.R;
@@ -131,10 +131,10 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     vofs = L::KN + L::KR + vkey * (2 * DV) + (((vcol >> 3) ^ vswz<CHV>(vkey)) << 4) + (vcol & 7) * 2;
   }
 
-  for (int64_t at = start; at < stop;) {
+  for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
     const int tiles = lat_tiles(a, len, rb, KT);
-    const int te = (int)min((int64_t)tiles, tb + (stop - at));
+    const int te = min(tiles, tb + (stop - at));
     LatPiece pc;
     pc.b = b;
     pc.len = len;
