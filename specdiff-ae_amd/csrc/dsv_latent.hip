@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   static_assert(sizeof(L) <= 163840, "LDS of a CU");
   __shared__ __attribute__((aligned(1024))) L lds;
 
+  lat_touch_args();
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, li = lane & (TR - 1), lg = lane / TR;
 
@@ -364,6 +365,11 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
                                : *reinterpret_cast<const u32x4*>(qt + (rg * QR + i) * TR * L::RB + (qrofs ^ (x << 4)));
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // (The upper half of the registers: products read it, other instructions do not.)
+      if constexpr (WIDE && DC == 512) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+a"(qf[0][ks]));
+      }
     }
     for (int t = t0; t < t1 && end > 0; ++t) {
       // The other buffer is free once every wave is done with tile t - 1.
@@ -630,6 +636,7 @@ __device__ __forceinline__ void merge_rows(const LatArgs& a, int kt, int64_t x, 
 template <int DV>
 __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int kt, int64_t n) {
   __shared__ LatSpan span;
+  lat_touch_args();
   for (int64_t x = blockIdx.x; x < n; x += gridDim.x) {
     merge_rows<DV>(a, kt, x, span);
     __syncthreads();

@@ -163,6 +163,20 @@ __device__ __forceinline__ const LatArgs* lat_args() {
   return (const LatArgs*)p;
 }
 
+// Touches every line of the arguments at once: they lie in host memory, and a load at
+// each first use costs a round trip of its own.
+__device__ __forceinline__ void lat_touch_args() {
+  typedef const uint32_t __attribute__((address_space(4))) * Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  constexpr int LINES = (sizeof(LatArgs) + 63) / 64;
+  static_assert(LINES <= 8, "");
+  uint32_t x[LINES];
+#pragma unroll
+  for (int i = 0; i < LINES; ++i) x[i] = p[min(i * 16, (int)sizeof(LatArgs) / 4 - 1)];
+#pragma unroll
+  for (int i = 0; i < LINES; ++i) asm volatile("" ::"s"(x[i]));
+}
+
 // One piece of a range: tiles [t0, t1) of sequence b of len keys, `slot` its
 // partial (-1: the piece is all of its sequence's tiles).
 struct LatPiece {

@@ -37,6 +37,11 @@ COMMON_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 
+# Matrix products whose results stay in the registers that other instructions reach:
+# the kernel rescales them, and copies to the other half and back took 256 instructions a
+# tile (its queries, which only products read, are put there instead).
+FILE_FLAGS = {"dsv_latent.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def _hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -73,7 +78,7 @@ def build(verbose: bool = False, jobs: int = 8) -> Path:
 
     def compile_one(src: str) -> Path:
         obj = OBJ_DIR / (Path(src).stem + ".o")
-        _run([hipcc, *COMMON_FLAGS, *inc, "-c", str(CSRC_DIR / src), "-o", str(obj)], verbose)
+        _run([hipcc, *COMMON_FLAGS, *FILE_FLAGS.get(src, []), *inc, "-c", str(CSRC_DIR / src), "-o", str(obj)], verbose)
         return obj
 
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
