@@ -2344,7 +2344,7 @@ int dsv_latent_append(const dsv_tensor* c, const dsv_tensor* k_pe, const dsv_ten
 namespace {
 
 struct LatPlan {
-  int G = 0, R = 0, MW = 0, rpb = 0, n_rb = 0, W = 1, kt = 0;
+  int G = 0, R = 0, MW = 0, rpb = 0, n_rb = 0, W = 1, sh = 0;
   size_t opart_bytes = 0, ml_bytes = 0, total = 0;
   const char* err = nullptr;
 };
@@ -2358,19 +2358,19 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
             "<= 2^24, batch x heads x rows <= 2^30)";
     return p;
   }
-  const bool expanded = Hk == H && dv <= 128;
+  const bool expanded = dv <= 128;
   p.G = (int)(H / Hk);
   p.R = (int)R;
   p.MW = tree ? (int)((M + 63) / 64) : 0;
   if (dtype == DSV_F32) {
     p.rpb = 16;
-    p.kt = dsv::kLatTileF32;
+    p.sh = dsv::kLatTileF32;
   } else if (expanded) {
     p.rpb = 256;
-    p.kt = dsv::kLatTileExp;
+    p.sh = dsv::kLatTileExp;
   } else {
     p.rpb = R > 32 ? 64 : (R > 16 ? 32 : 16);
-    p.kt = dsv::kLatTile;
+    p.sh = dsv::kLatTile;
     // The trees' sets of a block of 64 rows have room for 576 words.
     if (p.rpb == 64 && std::min<int64_t>(64, 63 / p.G + 2) * p.MW > 576) p.rpb = 32;
   }
@@ -2396,7 +2396,7 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
       }
     }
   }
-  const int64_t tiles = B * std::max<int64_t>(1, (n_keys + p.kt - 1) / p.kt);
+  const int64_t tiles = B * std::max<int64_t>(1, (n_keys + (1 << p.sh) - 1) >> p.sh);
   if (tiles >= ((int64_t)1 << 31)) {
     p.err = "batch x keys beyond 2^31 tiles of 32 or 64 keys";
     return p;
@@ -2457,6 +2457,7 @@ int lat_common(dsv::LatArgs& a, const dsv_tensor* q, const dsv_tensor* seqlens, 
   const LatPlan p = lat_plan(B, M, H, a.Hk, a.dv, a.dtype, n, a.parent != nullptr);
   if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
   if (p.total > 0 && (rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
+  const bool expanded = a.dv <= 128;
   a.q = q->data;
   a.q_sb = q->stride[0];
   a.q_sm = q->stride[1];
@@ -2489,9 +2490,9 @@ int lat_common(dsv::LatArgs& a, const dsv_tensor* q, const dsv_tensor* seqlens, 
   if (g_dry_run) return DSV_OK;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e = a.dtype == DSV_F32 ? dsv::launch_latent_f32(a, s)
-                 : p.kt == dsv::kLatTileExp && p.rpb == 256 ? dsv::launch_latent_tile(a, s)
+                 : expanded                ? dsv::launch_latent_tile(a, s)
                                                             : dsv::launch_latent(a, s);
-  if (e == hipSuccess) e = dsv::launch_latent_merge(a, p.kt, s);
+  if (e == hipSuccess) e = dsv::launch_latent_merge(a, p.sh, s);
   if (e != hipSuccess) return hip_fail(e, "latent attention launch");
   return DSV_OK;
 }

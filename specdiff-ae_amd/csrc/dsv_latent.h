@@ -43,22 +43,21 @@ struct LatArgs {
 // Keys of a sequence at most (token numbers are 32-bit, byte offsets are not).
 constexpr int64_t kLatMaxKeys = (int64_t)1 << 30;
 
-// Keys [0, lat_end) are those that some row of block rb sees.
-DSV_HD int lat_end(const LatArgs& a, int len, int rb) {
-  const int n0 = len - a.M;
-  if (!a.causal) return len;
-  if (a.parent != nullptr) return n0 < 0 ? 0 : len;
-  const int rl = ((rb + 1) * a.rpb < a.R ? (rb + 1) * a.rpb : a.R) - 1;
-  const int e = n0 + rl / a.G + 1;
-  return e > 0 ? e : 0;
-}
-
-// The tiles of kt keys of block rb in a sequence: at least one, so that every
-// sequence's rows are somebody's.
-DSV_HD int lat_tiles(const LatArgs& a, int len, int rb, int kt) {
-  const int t = (int)((unsigned)(lat_end(a, len, rb) + kt - 1) / (unsigned)kt);
-  return t > 0 ? t : 1;
-}
+// Keys [0, end(len)) of a sequence are those that some row of a block sees; in tiles of
+// 2^sh, at least one, so that every sequence's rows are somebody's.
+struct LatEnd {
+  int off, least;   // end = len + off, none below `least` tokens
+  DSV_HD LatEnd(const LatArgs& a, int rb) {
+    const int rl = ((rb + 1) * a.rpb < a.R ? (rb + 1) * a.rpb : a.R) - 1;
+    off = a.causal && a.parent == nullptr ? rl / a.G + 1 - a.M : 0;
+    least = a.parent != nullptr ? a.M : -off;
+  }
+  DSV_HD int operator()(int len) const { return len >= least ? len + off : 0; }
+  DSV_HD int tiles(int len, int sh) const {
+    const int t = (operator()(len) + (1 << sh) - 1) >> sh;
+    return t > 0 ? t : 1;
+  }
+};
 
 // Work sharing.  For each unit (key head, block of rows) the sequences' tiles
 // stand in one line, which W workgroups share out evenly: the first total % W ranges
@@ -83,9 +82,9 @@ bool expanded_widths(int dn, int dr);
 hipError_t launch_latent(const LatArgs& a, hipStream_t s);
 hipError_t launch_latent_tile(const LatArgs& a, hipStream_t s);
 hipError_t launch_latent_f32(const LatArgs& a, hipStream_t s);
-hipError_t launch_latent_merge(const LatArgs& a, int kt, hipStream_t s);
+hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s);
 
-// Keys per tile of the three kernels.
-constexpr int kLatTile = 64, kLatTileExp = 32, kLatTileF32 = 64;
+// Keys per tile of the three kernels, as powers of two.
+constexpr int kLatTile = 6, kLatTileExp = 5, kLatTileF32 = 6;
 
 }  // namespace dsv

@@ -96,7 +96,7 @@ __device__ __forceinline__ int swz_r(int key) {
 
 template <int DC, int DR, int ROWS>
 struct LatLds {
-  static constexpr int KT = kLatTile;
+  static constexpr int KT = 1 << kLatTile;
   static constexpr int NB = DC * 2, RB = DR * 2;
   static constexpr int TILE = KT * (NB + RB);
   // Sets of tree keys: a block's rows of H heads belong to at most ROWS nodes, of
@@ -212,12 +212,14 @@ struct LatLoader {
 };
 
 // Rows of a block from LDS (fp32, chunk c of row r at c ^ (r & 15)) into the output or a
-// partial: a wave takes a row at a time.  l: [groups][ROWS] sums, red.
+// partial: a wave takes a row at a time.  red: [groups][ROWS] sums.
 template <int DC, int ROWS, int GROUPS>
 __device__ __forceinline__ void lat_store_rows(const LatArgs& a, const LatPiece& pc, int rb, const uint8_t* acc, const float* m,
                                                const float (*red)[ROWS], float back) {
   constexpr int N = DC / 64;
   const int lane = threadIdx.x & 63;
+  const bool part = pc.slot >= 0;
+#pragma unroll 1
   for (int r = threadIdx.x >> 6; r < ROWS; r += 4) {
     const int row = rb * ROWS + r;
     if (row >= a.R) break;
@@ -225,30 +227,42 @@ __device__ __forceinline__ void lat_store_rows(const LatArgs& a, const LatPiece&
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) l += red[g][r];
     l *= back;
-    float x[N];
-#pragma unroll
-    for (int c = 0; c < N / 4; ++c) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(acc + r * DC * 4 + (((lane * (N / 4) + c) ^ (r & 15)) << 4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * c + e] = v[e];
-    }
-    if (pc.slot >= 0) {
-      const int64_t pr = pc.slot * ROWS + r;
-#pragma unroll
-      for (int c = 0; c < N / 4; ++c)
-        *reinterpret_cast<f32x4*>(a.opart + pr * DC + lane * N + 4 * c) = f32x4{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]} * back;
-      if (lane == 0) a.ml[pr] = make_float2(m[r], l);
-      continue;
-    }
-    const float inv = l > 0.f ? back / l : (l == 0.f ? 0.f : l);
     const int pos = row / a.G, h = row - pos * a.G;
-    const int64_t off = b_off(a, pc.b, pos, h) + lane * N;
-#pragma unroll
-    for (int c = 0; c < N / 4; ++c) {
-      const float y[4] = {x[4 * c] * inv, x[4 * c + 1] * inv, x[4 * c + 2] * inv, x[4 * c + 3] * inv};
-      store4(a, off + 4 * c, y);
+    const int64_t pr = pc.slot * ROWS + r;
+    const int64_t off = part ? pr * DC : b_off(a, pc.b, pos, h);
+    const float f = part ? back : l > 0.f ? back / l : (l == 0.f ? 0.f : l);
+    if (lane == 0) {
+      if (part)
+        a.ml[pr] = make_float2(m[r], l);
+      else if (a.lse != nullptr)
+        a.lse[pc.b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m[r], l);
     }
-    if (lane == 0 && a.lse != nullptr) a.lse[pc.b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m[r], l);
+    auto chunk = [&](int c) { return *reinterpret_cast<const f32x4*>(acc + r * DC * 4 + ((c ^ (r & 15)) << 4)) * f; };
+    if (part || (a.out_dtype == 2 && a.out_vec)) {
+      float* o = (part ? a.opart : reinterpret_cast<float*>(a.out)) + off;
+#pragma unroll
+      for (int c = 0; c < N / 4; ++c) *reinterpret_cast<f32x4*>(o + (c * 64 + lane) * 4) = chunk(c * 64 + lane);
+    } else if (a.out_vec) {
+      uint32_t w[N / 2];
+#pragma unroll
+      for (int c = 0; c < N / 4; ++c) {
+        const f32x4 x = chunk(lane * (N / 4) + c);
+        w[2 * c] = a.out_dtype == 0 ? pack2<BF16>(x[0], x[1]) : pack2<F16>(x[0], x[1]);
+        w[2 * c + 1] = a.out_dtype == 0 ? pack2<BF16>(x[2], x[3]) : pack2<F16>(x[2], x[3]);
+      }
+      uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + off + lane * N;
+      if constexpr (N == 8)
+        *reinterpret_cast<u32x4*>(o) = u32x4{w[0], w[1], w[N / 2 - 2], w[N / 2 - 1]};
+      else
+        *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
+    } else {
+      // (An output whose rows take no vector stores: element by element.)
+#pragma unroll 1
+      for (int d = lane; d < DC; d += 64) {
+        const float x = *reinterpret_cast<const float*>(acc + r * DC * 4 + (((d >> 2) ^ (r & 15)) << 4) + (d & 3) * 4) * f;
+        store1(a, off + d, x);
+      }
+    }
   }
 }
 
@@ -292,7 +306,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   const int w = (nblk & 7) == 0 ? (int)(blockIdx.x & 7) * (nblk >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
   const int rb = w % a.n_rb, rj = w / a.n_rb;
 
-  const LatCut cut(lat_line<256>(a, rb, KT, rj, -1, lds.span), a.W);
+  const LatEnd ends(a, rb);
+  const LatCut cut(lat_line<256>(a, ends, kLatTile, rj, -1, lds.span), a.W);
   const int start = cut.begin(rj), stop = cut.begin(rj + 1);
   if (start >= stop) return;
   int b = __builtin_amdgcn_readfirstlane(lds.span.b);
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 
   for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
-    const int tiles = lat_tiles(a, len, rb, KT);
+    const int tiles = ends.tiles(len, kLatTile);
     const int t1 = min(tiles, t0 + (stop - at));
     LatPiece pc;
     pc.b = b;
@@ -330,7 +345,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
     pc.t0 = t0;
     pc.t1 = t1;
     pc.slot = t0 == 0 && t1 == tiles ? -1 : ((int64_t)rb * a.W + rj) * 2 + (at == start ? 0 : 1);
-    const int end = lat_end(a, len, rb);
+    const int end = ends(len);
     ld.sequence(b, end);
 
     if (a.parent != nullptr) lat_tree<256>(a, b, m_lo, m_hi - m_lo + 1, reinterpret_cast<int16_t*>(lds.p), lds.vis);
@@ -564,82 +579,88 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 }
 
 // ---- the partials joined -------------------------------------------------------------
-// A workgroup takes (sequence, unit, 4 rows) at a time: 64 lanes a row, DV / 64 columns
-// each.
+// A workgroup takes (sequence, unit, 4 rows) at a time, a wave a row of DV / 64 values a
+// lane, eight partials in flight.
 template <int DV>
-__device__ __forceinline__ void merge_rows(const LatArgs& a, int kt, int64_t x, LatSpan& span) {
-  constexpr int N = DV / 64;
-  const int parts = a.rpb / 4;
-  const int part = (int)(x % parts);
-  x /= parts;
-  const int rb = (int)(x % a.n_rb);
-  x /= a.n_rb;
-  const int kvh = (int)(x % a.Hk), b = (int)(x / a.Hk);
-  const int total = lat_line<256>(a, rb, kt, 0, b, span), at = span.at;
-  const int tiles = lat_tiles(a, len_of(a, b), rb, kt);
-  const LatCut cut(total, a.W);
-  const int j0 = cut.range_of(at), j1 = cut.range_of(at + tiles - 1);
-  if (j0 == j1) return;  // one piece: written by its workgroup
-  const int which0 = cut.begin(j0) >= at ? 0 : 1;
-  const int lane = threadIdx.x & 63;
-  const int i = part * 4 + (threadIdx.x >> 6), row = rb * a.rpb + i;
-  if (row >= a.R) return;
-  constexpr int U = 8;  // partials in flight
-  float m = kNegInf, l = 0.f, o[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) o[e] = 0.f;
-  const int64_t unit = (int64_t)kvh * a.n_rb + rb;
-  for (int s0 = j0; s0 <= j1; s0 += U) {
-    float2 ml[U];
-    float p[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = min(s0 + u, j1);
-      // (A range behind the first one begins with this sequence.)
-      const int64_t pr = ((unit * a.W + j) * 2 + (j == j0 ? which0 : 0)) * a.rpb + i;
-      const bool none = s0 + u > j1;
-      ml[u] = none ? make_float2(kNegInf, 0.f) : a.ml[pr];
-#pragma unroll
-      for (int e = 0; e < N; ++e) p[u][e] = none ? 0.f : a.opart[pr * DV + lane * N + e];
-    }
-    float mn = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
-    const float f0 = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
-    l *= f0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] *= f0;
-    m = mn;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (ml[u].y == 0.f) continue;  // a piece without a key of this row
-      const float f = __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
-      l += ml[u].y * f;
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = fmaf(p[u][e], f, o[e]);
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  const int mm = row / a.G, h = kvh * a.G + row - mm * a.G;
-  const int64_t off = b * a.o_sb + (int64_t)mm * a.o_sm + (int64_t)h * a.o_sh + lane * N;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float y = o[e] * inv;
-    if (a.out_dtype == 2)
-      reinterpret_cast<float*>(a.out)[off + e] = y;
-    else
-      reinterpret_cast<uint16_t*>(a.out)[off + e] = (uint16_t)(a.out_dtype == 0 ? pack2<BF16>(y, y) : pack2<F16>(y, y));
-  }
-  if (lane == 0 && a.lse != nullptr) a.lse[b * a.l_sb + (int64_t)mm * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m, l);
-}
-
-template <int DV>
-__global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int kt, int64_t n) {
+__global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int sh, uint32_t n) {
+  constexpr int N = DV / 64, U = 8;
+  typedef float Row __attribute__((ext_vector_type(N)));
   __shared__ LatSpan span;
   lat_touch_args();
-  for (int64_t x = blockIdx.x; x < n; x += gridDim.x) {
-    merge_rows<DV>(a, kt, x, span);
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+#pragma unroll 1
+  for (uint32_t x = blockIdx.x; x < n; x += gridDim.x) {
+    const uint32_t parts = a.rpb / 4;
+    uint32_t y = x / parts;
+    const int i = (int)(x - y * parts) * 4 + wid;
+    const uint32_t unit = y % (uint32_t)(a.n_rb * a.Hk), b = y / (uint32_t)(a.n_rb * a.Hk);
+    const int kvh = unit / (uint32_t)a.n_rb, rb = unit % (uint32_t)a.n_rb, row = rb * a.rpb + i;
+    const LatEnd ends(a, rb);
+    const LatCut cut(lat_line<256>(a, ends, sh, 0, (int)b, span), a.W);
+    const int at = span.at;
     __syncthreads();
+    const int j0 = cut.range_of(at), j1 = cut.range_of(at + ends.tiles(len_of(a, (int)b), sh) - 1);
+    if (j0 == j1 || row >= a.R) continue;  // (one piece: written by its workgroup)
+    // A range behind the first one begins with this sequence.
+    const int64_t base = ((int64_t)unit * a.W * 2) * a.rpb + i;
+    const int64_t first = cut.begin(j0) >= at ? 0 : a.rpb;
+    float m = kNegInf, l = 0.f;
+    Row o{};
+#pragma unroll 1
+    for (int s0 = j0; s0 <= j1; s0 += U) {
+      float2 ml[U];
+      Row p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = min(s0 + u, j1);
+        const int64_t pr = base + (int64_t)j * 2 * a.rpb + (j == j0 ? first : 0);
+        ml[u] = a.ml[pr];
+        p[u] = *reinterpret_cast<const Row*>(a.opart + pr * DV + lane * N);
+      }
+      // (All in flight before the first is used: the compiler moves them to their uses.)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float t = p[u][N - 1];
+        asm volatile("" : "+v"(t));
+        p[u][N - 1] = t;
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+      const float f0 = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+      l *= f0;
+      o *= f0;
+      m = mn;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // (Behind the last, and where a piece has no key of this row: nothing.)
+        const bool none = s0 + u > j1 || ml[u].x == kNegInf;
+        const float f = none ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
+        l = fmaf(none ? 0.f : ml[u].y, f, l);
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = fmaf(none ? 0.f : p[u][e], f, o[e]);
+      }
+    }
+    o *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const int pos = row / a.G, h = kvh * a.G + row - pos * a.G;
+    const int64_t off = b_off(a, (int)b, pos, h) + lane * N;
+    if (a.out_vec && a.out_dtype == 2) {
+      *reinterpret_cast<Row*>(reinterpret_cast<float*>(a.out) + off) = o;
+    } else if (a.out_vec && N > 1) {
+      uint32_t w[(N + 1) / 2];
+#pragma unroll
+      for (int e = 0; e + 1 < N; e += 2) w[e / 2] = a.out_dtype == 0 ? pack2<BF16>(o[e], o[e + 1]) : pack2<F16>(o[e], o[e + 1]);
+      uint32_t* p = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + off);
+      typedef uint32_t Out __attribute__((ext_vector_type((N + 1) / 2)));
+      Out v;
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) v[e] = w[e];
+      *reinterpret_cast<Out*>(p) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) store1(a, off + e, o[e]);
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m, l);
   }
 }
 
@@ -674,15 +695,15 @@ hipError_t launch_latent(const LatArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_latent_merge(const LatArgs& a, int kt, hipStream_t s) {
+hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   if (a.W == 1) return hipSuccess;
-  const int64_t n = (int64_t)a.B * a.Hk * a.n_rb * (a.rpb / 4);
+  const uint32_t n = (uint32_t)((int64_t)a.B * a.Hk * a.n_rb * (a.rpb / 4));  // (below 2^31)
   const dim3 grid((unsigned)(n < (1 << 20) ? n : 1 << 20)), block(256);
   switch (a.dv) {
-    case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, kt, n); break;
-    case 128: hipLaunchKernelGGL(latent_merge_kernel<128>, grid, block, 0, s, a, kt, n); break;
-    case 256: hipLaunchKernelGGL(latent_merge_kernel<256>, grid, block, 0, s, a, kt, n); break;
-    default: hipLaunchKernelGGL(latent_merge_kernel<512>, grid, block, 0, s, a, kt, n); break;
+    case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, sh, n); break;
+    case 128: hipLaunchKernelGGL(latent_merge_kernel<128>, grid, block, 0, s, a, sh, n); break;
+    case 256: hipLaunchKernelGGL(latent_merge_kernel<256>, grid, block, 0, s, a, sh, n); break;
+    default: hipLaunchKernelGGL(latent_merge_kernel<512>, grid, block, 0, s, a, sh, n); break;
   }
   return hipGetLastError();
 }

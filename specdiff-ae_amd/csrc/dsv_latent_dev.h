@@ -6,14 +6,13 @@
 
 namespace dsv {
 
+// (Small code throughout: a kernel's instructions come from memory at its first pass
+// over them, 64 bytes a time, which is most of what a short call takes.)
 __device__ __forceinline__ int len_of(const LatArgs& a, int b) {
-  int64_t n = a.n_keys;
-  if (a.seqlens != nullptr) {
-    const int64_t x = a.seqlens_i64 ? reinterpret_cast<const int64_t*>(a.seqlens)[b]
-                                    : (int64_t) reinterpret_cast<const int32_t*>(a.seqlens)[b];
-    n = x < 0 ? 0 : (x < n ? x : n);
-  }
-  return (int)n;
+  if (a.seqlens == nullptr) return (int)a.n_keys;
+  const int32_t* p = reinterpret_cast<const int32_t*>(a.seqlens) + ((int64_t)b << a.seqlens_i64);
+  const int32_t lo = p[0], hi = a.seqlens_i64 ? p[1] : lo >> 31, n = (int)a.n_keys;
+  return hi < 0 ? 0 : (hi > 0 || (uint32_t)lo > (uint32_t)n ? n : lo);
 }
 
 // Physical page of key n, clamped to the pool.
@@ -40,11 +39,12 @@ struct LatSpan {
 // or the place of sequence find_b (`at`).
 // Every thread of the workgroup calls it; ends with a barrier.
 template <int NT>
-__device__ __forceinline__ int lat_line(const LatArgs& a, int rb, int kt, int j, int find_b, LatSpan& s) {
+__device__ __forceinline__ int lat_line(const LatArgs& a, const LatEnd& end, int sh, int j, int find_b, LatSpan& s) {
   const int per = (a.B + NT - 1) / NT;
   const int lo = min((int)threadIdx.x * per, a.B), hi = min(lo + per, a.B);
   int sum = 0;
-  for (int b = lo; b < hi; ++b) sum += lat_tiles(a, len_of(a, b), rb, kt);
+#pragma unroll 1
+  for (int b = lo; b < hi; ++b) sum += end.tiles(len_of(a, b), sh);
   int pre = sum, total = 0;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   if (a.B > 1) {
@@ -62,19 +62,19 @@ __device__ __forceinline__ int lat_line(const LatArgs& a, int rb, int kt, int j,
     total += s.wave[w];
   }
   pre -= sum;  // tiles before this thread's sequences
-  if (find_b >= 0) {
-    if (find_b >= lo && find_b < hi) {
-      for (int b = lo; b < find_b; ++b) pre += lat_tiles(a, len_of(a, b), rb, kt);
-      s.at = pre;
+  // The thread that has it walks to it.
+  const int start = LatCut(total, a.W).begin(j);
+  if (find_b >= 0 ? find_b >= lo && find_b < hi : start >= pre && start < pre + sum) {
+    int b = lo;
+#pragma unroll 1
+    for (;; ++b) {
+      const int t = end.tiles(len_of(a, b), sh);
+      if (find_b >= 0 ? b == find_b : start < pre + t) break;
+      pre += t;
     }
-  } else {
-    const int start = LatCut(total, a.W).begin(j);
-    if (start >= pre && start < pre + sum) {
-      int b = lo;
-      for (int t; start >= pre + (t = lat_tiles(a, len_of(a, b), rb, kt)); ++b) pre += t;
-      s.b = b;
-      s.off = start - pre;
-    }
+    s.b = b;
+    s.at = pre;
+    s.off = start - pre;
   }
   __syncthreads();
   return total;
@@ -149,6 +149,13 @@ __device__ __forceinline__ int64_t b_off(const LatArgs& a, int b, int m, int h) 
   return b * a.o_sb + (int64_t)m * a.o_sm + (int64_t)h * a.o_sh;
 }
 
+__device__ __forceinline__ void store1(const LatArgs& a, int64_t off, float x) {
+  if (a.out_dtype == 2)
+    reinterpret_cast<float*>(a.out)[off] = x;
+  else
+    reinterpret_cast<uint16_t*>(a.out)[off] = (uint16_t)(a.out_dtype == 0 ? pack2<BF16>(x, x) : pack2<F16>(x, x));
+}
+
 // ln sum exp of a row from its maximum (a score) and its sum relative to it.
 __device__ __forceinline__ float lat_lse(const LatArgs& a, float m, float l) {
   return l == 0.f ? kNegInf : (m * a.scale_log2 + __log2f(l)) * kLn2;
@@ -196,7 +203,7 @@ __device__ __noinline__ void lat_exact_rows(const LatArgs* ap, const LatPiece pc
   constexpr int N = DV / 64;
   const LatArgs& a = *ap;
   const int lane = threadIdx.x & 63, b = pc.b;
-  const int end = min(lat_end(a, pc.len, rb), pc.t1 * kt);
+  const int end = min(LatEnd(a, rb)(pc.len), pc.t1 * kt);
   const E* kn = reinterpret_cast<const E*>(a.kn.p) + b * a.kn.sb + kvh * a.kn.sh;
   const E* kr = reinterpret_cast<const E*>(a.kr.p) + b * a.kr.sb + kvh * a.kr.sh;
   const E* vb = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + kvh * a.v.sh;

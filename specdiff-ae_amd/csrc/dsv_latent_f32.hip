@@ -19,7 +19,7 @@ constexpr float kTau = 8.0f;
 
 template <int DN, int DR, int DV>
 __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
-  constexpr int KT = kLatTileF32, ROWS = 16;
+  constexpr int KT = 1 << kLatTileF32, ROWS = 16;
   constexpr int SN = DN / 16, SR = DR / 16, CB = DV / 64;
   constexpr int PST = KT + 4;  // floats per row of probabilities
   __shared__ __attribute__((aligned(16))) float p_lds[ROWS * PST];
@@ -36,7 +36,8 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
   const int rb = w % a.n_rb;
   w /= a.n_rb;
   const int kvh = w % a.Hk, rj = w / a.Hk;
-  const int total = lat_line<256>(a, rb, KT, rj, -1, span);
+  const LatEnd ends(a, rb);
+  const int total = lat_line<256>(a, ends, kLatTileF32, rj, -1, span);
   const LatCut cut(total, a.W);
   const int start = cut.begin(rj), stop = cut.begin(rj + 1);
   if (start >= stop) return;
@@ -49,7 +50,7 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
 
   for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
-    const int tiles = lat_tiles(a, len, rb, KT);
+    const int tiles = ends.tiles(len, kLatTileF32);
     const int t1 = min(tiles, t0 + (stop - at));
     LatPiece pc;
     pc.b = b;
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
     pc.t0 = t0;
     pc.t1 = t1;
     pc.slot = t0 == 0 && t1 == tiles ? -1 : (((int64_t)kvh * a.n_rb + rb) * a.W + rj) * 2 + (at == start ? 0 : 1);
-    const int end = lat_end(a, len, rb);
+    const int end = ends(len);
     if (a.parent != nullptr) lat_tree<256>(a, b, m_lo, m_hi - m_lo + 1, par, vis);
     const float* kn = reinterpret_cast<const float*>(a.kn.p) + b * a.kn.sb + kvh * a.kn.sh;
     const float* kr = reinterpret_cast<const float*>(a.kr.p) + b * a.kr.sb + kvh * a.kr.sh;

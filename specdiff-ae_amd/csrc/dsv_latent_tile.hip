@@ -83,7 +83,7 @@ struct ExpLds {
 template <typename T, int DN, int DR>
 __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
   using L = ExpLds<DN, DR>;
-  constexpr int DV = DN, KT = kLatTileExp;
+  constexpr int DV = DN, KT = 1 << kLatTileExp;
   constexpr int KSN = DN / 16, KSR = DR / 16, DT = DV / 32;
   constexpr int CHN = DN / 8, CHR = DR / 8, CHV = DV / 8;
   constexpr int SHIFT = kProbShift<T, 10>;
@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
   w /= a.W;
   const int rb = a.n_rb - 1 - w % a.n_rb, kvh = w / a.n_rb;
 
-  const int total = lat_line<512>(a, rb, KT, rj, -1, lds.span);
+  const LatEnd ends(a, rb);
+  const int total = lat_line<512>(a, ends, kLatTileExp, rj, -1, lds.span);
   const LatCut cut(total, a.W);
   const int start = cut.begin(rj), stop = cut.begin(rj + 1);
   if (start >= stop) return;
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
 
   for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
-    const int tiles = lat_tiles(a, len, rb, KT);
+    const int tiles = ends.tiles(len, kLatTileExp);
     const int te = min(tiles, tb + (stop - at));
     LatPiece pc;
     pc.b = b;
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     pc.t0 = tb;
     pc.t1 = te;
     pc.slot = tb == 0 && te == tiles ? -1 : (((int64_t)kvh * a.n_rb + rb) * a.W + rj) * 2 + (at == start ? 0 : 1);
-    const int end = lat_end(a, len, rb);
+    const int end = ends(len);
     const int ntiles = end > 0 ? te - tb : 0;
     const int n0 = len - a.M;
 
