@@ -64,16 +64,13 @@ __device__ __forceinline__ void dma_lane(uint32_t lds, const void* vaddr) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(vaddr) : "memory", "m0");
 }
 
-// The same from a uniform address plus a 32-bit byte offset per lane (valid ones).
-// SALU: the address was made by scalar instructions, so that one wait state is enough.
-template <bool NT = true, bool SALU = false>
+// The same from a uniform address plus a 32-bit byte offset per lane (valid ones).  The
+// address is copied by a scalar instruction, which waits for whatever wrote it, and stands
+// between the write of m0 and the load.
 __device__ __forceinline__ void dma_off(uint32_t lds, uint64_t base, uint32_t voff) {
-  static_assert(!NT, "");
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
-  if constexpr (SALU)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff), "s"(base) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff), "s"(base) : "memory", "m0");
+  uint64_t from;
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0" : "=&s"(from) : "s"(m0), "v"(voff), "s"(base) : "memory", "m0");
 }
 
 // Wait until at most N of this wave's vector-memory operations are pending.

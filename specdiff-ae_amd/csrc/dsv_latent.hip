@@ -133,135 +133,155 @@ struct LatLoader {
   uint64_t base;
   int32_t pwin;                                    // lane l: physical page of the sequence's page pw0 + l
   int pw0;
+  int shift, mask;                                 // of the page size (a dense cache is one page, number 0)
+  uint64_t sp2;
+  uint32_t kst2;
 
   __device__ __forceinline__ LatLoader(const LatArgs& args, int w, int l, uint32_t ring) : a(args), wid(w), lane(l) {
     dstn = ring + w * 16 * L::NB;
     dstr = ring + L::KT * L::NB + w * 16 * L::RB;
-    run_ok = (a.pt == nullptr || a.ps_shift >= 4) && a.kn.st <= (1 << 24);
+    shift = a.pt != nullptr ? a.ps_shift : 30;
+    mask = (1 << shift) - 1;
+    sp2 = (uint64_t)(2 * a.kn.sp);
+    kst2 = (uint32_t)(2 * a.kn.st);
+    run_ok = (a.pt == nullptr || a.ps_shift >= 4) && a.kn.st > 0 && a.kn.st <= (1 << 24);
   }
   __device__ __forceinline__ void sequence(int b_, int end_) {
     b = b_;
     end = end_;
     base = (uint64_t)a.kn.p + 2 * (b * a.kn.sb);
-    pw0 = -64;
+    pw0 = a.pt != nullptr ? -64 : 0;
+    pwin = 0;
   }
-  // Rows at even distances from a uniform address.
-  __device__ __forceinline__ void run(uint32_t buf, uint64_t addr) {
-    const uint32_t ln = again(lane), st2 = (uint32_t)(2 * a.kn.st);
-    uint64_t r = addr;
-#pragma unroll
-    for (int x = 0; x < IPN; ++x) {
-      const uint32_t k = ln / (64 / KPI), c = ln % (64 / KPI);
-      dma_off<false, true>(dstn + buf + x * 1024, r, (KPI > 1 ? k * st2 : 0) + ((c ^ swz_n(x * KPI + (KPI > 1 ? k : 0))) << 4));
-      r += (uint64_t)KPI * st2;
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int x = 0; x < IPR; ++x) {
-      const uint32_t k = x * KPR + ln / (64 / KPR), c = ln % (64 / KPR);
-      dma_off<false, true>(dstr + buf + x * 1024, addr + L::NB, k * st2 + ((c ^ swz_r<DR>(k)) << 4));
-      __builtin_amdgcn_sched_barrier(0);
+  // A wave's rows: 16 at even distances st2 from a uniform address, or (st2 = 0) anywhere,
+  // lane l knowing the address of row l % 16.
+  uint64_t from;
+  uint32_t st2;
+  // Instruction x of such rows.
+  __device__ __forceinline__ void one(uint32_t buf, int x, uint32_t ln) const {
+    if (x < IPN) {
+      const uint32_t k = KPI > 1 ? ln / (64 / KPI) : 0, c = ln % (64 / KPI);
+      dma_off(dstn + buf + x * 1024, from, (x * KPI + k) * st2 + ((c ^ swz_n(x * KPI + k)) << 4));
+    } else {
+      const uint32_t k = (x - IPN) * KPR + ln / (64 / KPR), c = ln % (64 / KPR);
+      dma_off(dstr + buf + (x - IPN) * 1024, from + L::NB, k * st2 + ((c ^ swz_r<DR>(k)) << 4));
     }
   }
-  // Rows anywhere: lane l knows the address of row l % 16.
-  __device__ __forceinline__ void rows(uint32_t buf, uint64_t addr) {
+  __device__ __forceinline__ void all(uint32_t buf, uint64_t addr) const {
     const uint32_t ln = again(lane);
-#pragma unroll 1
+    if (st2 != 0) {
+#pragma unroll 2
+      for (int x = 0; x < N; ++x) one(buf, x, ln);
+      return;
+    }
+#pragma unroll 4
     for (int x = 0; x < IPN; ++x) {
       const int k = x * KPI + ln / (64 / KPI);
       const char* r = (const char*)__shfl((long long)addr, k);
       dma_lane<false>(dstn + buf + x * 1024, r + (((ln % (64 / KPI)) ^ swz_n(k)) << 4));
     }
-#pragma unroll 1
+#pragma unroll
     for (int x = 0; x < IPR; ++x) {
       const int k = x * KPR + ln / (64 / KPR);
       const char* r = (const char*)__shfl((long long)addr, k);
       dma_lane<false>(dstr + buf + x * 1024, r + L::NB + (((ln % (64 / KPR)) ^ swz_r<DR>(k)) << 4));
     }
   }
-  // Keys [kb, kb + 64) into a buffer; those at or behind the end are replaced by the last
-  // one (no row sees them).  Page numbers are kept in a window: a load at the use would be
-  // waited for, and the tiles in flight with it.
-  template <bool FIRST>
-  __device__ __forceinline__ void issue(uint32_t buf, int kb) {
-    const int n0 = min(kb + wid * 16, end - 1), n1 = min(kb + wid * 16 + 15, end - 1);
-    if (a.pt != nullptr) {
-      const int p0 = n0 >> a.ps_shift, p1 = n1 >> a.ps_shift;
-      if (FIRST || p0 < pw0 || p1 >= pw0 + 64) {
-        pw0 = p0;
-        pwin = (int32_t)page_of(a, b, (int)min((int64_t)(p0 + lane) << a.ps_shift, (int64_t)end - 1));
-        asm volatile("" : "+v"(pwin));  // (waited for here)
-      }
-    }
-    if (!FIRST && run_ok && n1 == n0 + 15) {
-      const int64_t pg = a.pt != nullptr ? __builtin_amdgcn_readlane(pwin, (n0 >> a.ps_shift) - pw0) : 0;
-      const uint64_t at = base + 2 * key_off(a, a.kn, n0, pg);
-      run(buf, ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32) |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at));
-    } else {
-      const int n = min(n0 + (lane & 15), end - 1);
-      rows(buf, base + 2 * key_off(a, a.kn, n, a.pt != nullptr ? __shfl(pwin, (n >> a.ps_shift) - pw0) : 0));
-    }
+  __device__ __forceinline__ static uint64_t uniform64(uint64_t x) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
   }
-  // The query rows [row0, row0 + n); those behind the last are replaced by it.
-  __device__ __forceinline__ void queries(uint32_t buf, int row0, int n) {
-    if (wid * 16 >= n) return;
+  // The keys [kb, kb + 64); those at or behind the end are replaced by the last one (no row
+  // sees them).  Page numbers are kept in a window: a load at the use would be waited for,
+  // and the tiles in flight with it.  Returns a lane's address where they lie apart.
+  __device__ __forceinline__ uint64_t keys(int kb) {
+    const int n0 = kb + wid * 16;
+    if (!run_ok || n0 + 15 >= end || (uint32_t)((n0 >> shift) - pw0) >= 64u) return keys_slow(kb);
+    run(n0);
+    return 0;
+  }
+  __device__ __forceinline__ void run(int n0) {
+    const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane(pwin, (n0 >> shift) - pw0);
+    from = base + (uint64_t)pg * sp2 + (uint64_t)(uint32_t)(n0 & mask) * kst2;
+    st2 = kst2;
+  }
+  __device__ __forceinline__ uint64_t keys_slow(int kb) {
+    const int n0 = min(kb + wid * 16, end - 1), n1 = min(kb + wid * 16 + 15, end - 1);
+    const int p0 = n0 >> shift;
+    if (a.pt != nullptr && (p0 < pw0 || n1 >> shift >= pw0 + 64)) {
+      pw0 = p0;
+      pwin = (int32_t)page_of(a, b, (int)min((int64_t)(p0 + lane) << shift, (int64_t)end - 1));
+      asm volatile("" : "+v"(pwin));  // (waited for here)
+    }
+    if (run_ok && n1 == n0 + 15) {
+      run(n0);
+      return 0;
+    }
+    st2 = 0;
+    const int n = min(n0 + (lane & 15), end - 1);
+    return base + 2 * key_off(a, a.kn, n, a.pt != nullptr ? __shfl(pwin, (n >> shift) - pw0) : 0);
+  }
+  // The query rows [row0, row0 + 16) of this wave; those behind the last are replaced by it.
+  __device__ __forceinline__ uint64_t queries(int row0) {
     const int r = min(row0 + wid * 16 + (lane & 15), a.R - 1), m = r / a.G;
-    rows(buf, (uint64_t)a.q + 2 * (b * a.q_sb + (int64_t)m * a.q_sm + (int64_t)(r - m * a.G) * a.q_sh));
+    const uint64_t at = (uint64_t)a.q + 2 * (b * a.q_sb + (int64_t)m * a.q_sm + (int64_t)(r - m * a.G) * a.q_sh);
+    st2 = 0;
+    if (row0 + wid * 16 + 15 < a.R && (a.M == 1 || a.q_sm == a.G * a.q_sh) && a.q_sh > 0 && a.q_sh <= (1 << 24)) {
+      from = uniform64(at);
+      st2 = (uint32_t)(2 * a.q_sh);
+    }
+    return at;
   }
 };
 
 // Rows of a block from LDS (fp32, chunk c of row r at c ^ (r & 15)) into the output or a
-// partial: a wave takes a row at a time.  red: [groups][ROWS] sums.
+// partial.  red: [groups][ROWS] sums; off, fac: room for a row's place and factor.  Called
+// by every thread; the caller's next barrier ends it.
 template <int DC, int ROWS, int GROUPS>
 __device__ __forceinline__ void lat_store_rows(const LatArgs& a, const LatPiece& pc, int rb, const uint8_t* acc, const float* m,
-                                               const float (*red)[ROWS], float back) {
-  constexpr int N = DC / 64;
-  const int lane = threadIdx.x & 63;
+                                               const float (*red)[ROWS], float back, int64_t* off, float* fac) {
   const bool part = pc.slot >= 0;
-#pragma unroll 1
-  for (int r = threadIdx.x >> 6; r < ROWS; r += 4) {
-    const int row = rb * ROWS + r;
-    if (row >= a.R) break;
+  const int rows = min(ROWS, a.R - rb * ROWS);
+  if ((int)threadIdx.x < rows) {
+    const int r = threadIdx.x, row = rb * ROWS + r, pos = row / a.G, h = row - pos * a.G;
     float l = 0.f;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) l += red[g][r];
     l *= back;
-    const int pos = row / a.G, h = row - pos * a.G;
     const int64_t pr = pc.slot * ROWS + r;
-    const int64_t off = part ? pr * DC : b_off(a, pc.b, pos, h);
-    const float f = part ? back : l > 0.f ? back / l : (l == 0.f ? 0.f : l);
-    if (lane == 0) {
-      if (part)
-        a.ml[pr] = make_float2(m[r], l);
-      else if (a.lse != nullptr)
-        a.lse[pc.b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m[r], l);
+    off[r] = part ? pr * DC : b_off(a, pc.b, pos, h);
+    fac[r] = part ? back : l > 0.f ? back / l : (l == 0.f ? 0.f : l);
+    if (part)
+      a.ml[pr] = make_float2(m[r], l);
+    else if (a.lse != nullptr)
+      a.lse[pc.b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m[r], l);
+  }
+  __syncthreads();
+  auto chunk = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(acc + r * DC * 4 + ((c ^ (r & 15)) << 4)) * fac[r]; };
+  if (part || (a.out_dtype == 2 && a.out_vec)) {
+    float* o = part ? a.opart : reinterpret_cast<float*>(a.out);
+#pragma unroll 4
+    for (int x = threadIdx.x; x < rows * (DC / 4); x += 256) {
+      const int r = x / (DC / 4), c = x % (DC / 4);
+      *reinterpret_cast<f32x4*>(o + off[r] + c * 4) = chunk(r, c);
     }
-    auto chunk = [&](int c) { return *reinterpret_cast<const f32x4*>(acc + r * DC * 4 + ((c ^ (r & 15)) << 4)) * f; };
-    if (part || (a.out_dtype == 2 && a.out_vec)) {
-      float* o = (part ? a.opart : reinterpret_cast<float*>(a.out)) + off;
-#pragma unroll
-      for (int c = 0; c < N / 4; ++c) *reinterpret_cast<f32x4*>(o + (c * 64 + lane) * 4) = chunk(c * 64 + lane);
-    } else if (a.out_vec) {
-      uint32_t w[N / 2];
-#pragma unroll
-      for (int c = 0; c < N / 4; ++c) {
-        const f32x4 x = chunk(lane * (N / 4) + c);
-        w[2 * c] = a.out_dtype == 0 ? pack2<BF16>(x[0], x[1]) : pack2<F16>(x[0], x[1]);
-        w[2 * c + 1] = a.out_dtype == 0 ? pack2<BF16>(x[2], x[3]) : pack2<F16>(x[2], x[3]);
-      }
-      uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + off + lane * N;
-      if constexpr (N == 8)
-        *reinterpret_cast<u32x4*>(o) = u32x4{w[0], w[1], w[N / 2 - 2], w[N / 2 - 1]};
+  } else if (a.out_vec) {
+#pragma unroll 2
+    for (int x = threadIdx.x; x < rows * (DC / 8); x += 256) {
+      const int r = x / (DC / 8), c = x % (DC / 8);
+      const f32x4 u = chunk(r, 2 * c), v = chunk(r, 2 * c + 1);
+      u32x4 w;
+      if (a.out_dtype == 0)
+        w = u32x4{pack2<BF16>(u[0], u[1]), pack2<BF16>(u[2], u[3]), pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3])};
       else
-        *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
-    } else {
-      // (An output whose rows take no vector stores: element by element.)
+        w = u32x4{pack2<F16>(u[0], u[1]), pack2<F16>(u[2], u[3]), pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])};
+      *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.out) + off[r] + c * 8) = w;
+    }
+  } else {
+    // (An output whose rows take no vector stores: element by element.)
 #pragma unroll 1
-      for (int d = lane; d < DC; d += 64) {
-        const float x = *reinterpret_cast<const float*>(acc + r * DC * 4 + (((d >> 2) ^ (r & 15)) << 4) + (d & 3) * 4) * f;
-        store1(a, off + d, x);
-      }
+    for (int x = threadIdx.x; x < rows * DC; x += 256) {
+      const int r = x / DC, d = x % DC;
+      store1(a, off[r] + d, *reinterpret_cast<const float*>(acc + r * DC * 4 + (((d >> 2) ^ (r & 15)) << 4) + (d & 3) * 4) * fac[r]);
     }
   }
 }
@@ -334,6 +354,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   const uint32_t pr = li * 128 + ((lg ^ psw) << 4);
   const float scale = a.scale_log2;
   Loader ld(a, wid, lane, lds_addr(lds.ring));
+  const bool early = !WIDE || a.n_rb == 1;
+  static_assert(!WIDE || Loader::N <= KS / 3 + KT / DS * CB, "");
 
   for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
@@ -365,9 +387,13 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
     if (end > 0) {
       // The queries come through the other buffer (a load that ends in registers would be
       // waited for at its first use, in the loop, and the tiles in flight with it).
-      ld.template issue<true>((uint32_t)(t0 & 1) * L::TILE, t0 * KT);
       const uint32_t other = (uint32_t)((t0 + 1) & 1) * L::TILE;
-      ld.queries(other, rb * ROWS, ROWS);
+      if (wid * 16 < ROWS) {
+        const uint64_t at = ld.queries(rb * ROWS);
+        ld.all(other, at);
+      }
+      const uint64_t at = ld.keys(t0 * KT);
+      ld.all((uint32_t)(t0 & 1) * L::TILE, at);
       wait_vmcnt<0>();
       barrier_lds();
       const uint8_t* qt = lds.ring + other;
@@ -387,16 +413,27 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
       }
     }
     for (int t = t0; t < t1 && end > 0; ++t) {
-      // The other buffer is free once every wave is done with tile t - 1.
-      barrier_lds();
+      // The next tile's loads go out as soon as its buffer is free (every wave done with
+      // tile t - 1), before this tile's are waited for, so that the memory is never idle;
+      // or, where several row blocks share the keys and the products take longer than the
+      // memory, between the products, whose time covers theirs (72 of them take the vector
+      // memory path of a CU 1700 cycles at once).
+      const uint32_t next = (uint32_t)((t + 1) & 1) * L::TILE, stage = (uint32_t)(t & 1) * L::TILE;
+      bool between = false;
+      if (early || t + 1 == t1) barrier_lds();
       if (t + 1 < t1) {
-        ld.template issue<false>((uint32_t)((t + 1) & 1) * L::TILE, (t + 1) * KT);
-        wait_vmcnt<Loader::N>();
+        if (!early) {
+          wait_vmcnt<0>();
+          barrier_lds();
+        }
+        const uint64_t at = ld.keys((t + 1) * KT);
+        between = !early && ld.st2 != 0;
+        if (!between) ld.all(next, at);
+        if (early) wait_vmcnt<Loader::N>();
       } else {
         wait_vmcnt<0>();
       }
-      const uint32_t stage = (uint32_t)(t & 1) * L::TILE;
-      if constexpr (WIDE) barrier_lds();  // (waves that share keys wait for each other's loads)
+      if (WIDE && (early || t + 1 == t1)) barrier_lds();  // (waves that share keys wait for each other's loads)
       asm volatile("" ::: "memory");
       // ---- scores of this wave's keys and rows ----------------------------------------
       Acc s[QR];
@@ -409,6 +446,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         return ks < KSN ? *reinterpret_cast<const u32x4*>(lds.ring + (ko ^ ((x & 15) << 4)) + (x >> 4) * 256)
                         : *reinterpret_cast<const u32x4*>(lds.ring + (ro ^ (x << 4)));
       };
+      const uint32_t ln = again(lane);
       constexpr int KA = 6;  // operands ahead
       u32x4 kf[KA + 1];
 #pragma unroll
@@ -418,6 +456,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         if (x + KA < KS) kf[(x + KA) % (KA + 1)] = read_k(x + KA);
 #pragma unroll
         for (int i = 0; i < QR; ++i) s[i] = mfma<T>(kf[x % (KA + 1)], qf[i][x], s[i]);
+        if (WIDE && x % 3 == 2 && x / 3 < Loader::N && between) ld.one(next, x / 3, ln);
         __builtin_amdgcn_sched_barrier(0);
       }
       const int kb = t * KT;
@@ -529,6 +568,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         const u32x4 v = vf[x % (VA + 1)];
 #pragma unroll
         for (int i = 0; i < RB; ++i) acc[i][x % CB] = mfma<T>(v, (x / CB) % 2 ? pn[i] : pf[i], acc[i][x % CB]);
+        if (WIDE && KS / 3 + x < Loader::N && between) ld.one(next, KS / 3 + x, ln);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (look) {
@@ -568,7 +608,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
     if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0)
       lat_exact_rows<T, DC>(lat_args(), pc, 0, rb, KT, m_lo, lds.vis, wid, ROWS, 4);
     else
-      lat_store_rows<DC, ROWS, KG>(a, pc, rb, lds.ring, lds.m, lds.red, 1.f / (1 << SHIFT));
+      lat_store_rows<DC, ROWS, KG>(a, pc, rb, lds.ring, lds.m, lds.red, 1.f / (1 << SHIFT), reinterpret_cast<int64_t*>(lds.p),
+                                   reinterpret_cast<float*>(lds.p + ROWS * 8));
     // Stores are done before the next piece counts its loads.
     wait_vmcnt<0>();
     __syncthreads();
