@@ -55,6 +55,13 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// x, computed again at every use: what is derived from it is not held in registers
+// across the loop.
+__device__ __forceinline__ uint32_t again(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Chunk c of key k stands at slot c ^ of these: operand reads without bank conflicts.
 template <int CH>
 __device__ __forceinline__ int kswz(int key) {
@@ -132,6 +139,24 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     vofs = L::KN + L::KR + vkey * (2 * DV) + (((vcol >> 3) ^ vswz<CHV>(vkey)) << 4) + (vcol & 7) * 2;
   }
 
+  // DMA: this wave's instructions of a tile and a lane's offsets in them.
+  constexpr int KPN = 1024 / (2 * DN), KPR = 1024 / (2 * DR), NR = DR / 16;
+  const int wr = w4 % NR;  // (two waves load the same rows where there are fewer instructions than waves)
+  const int64_t nstep = 2 * (v_wave ? a.v.st : a.kn.st), rstep = 2 * a.kr.st;
+  const bool near = nstep < (1 << 25) && rstep < (1 << 25);
+  const uint32_t nst2 = (uint32_t)nstep, rst2 = (uint32_t)rstep;
+  const uint32_t dst0 = lds_addr(ring) + (v_wave ? L::KN + L::KR : 0) + w4 * IPN * 1024, dst1 = lds_addr(ring) + L::KN + wr * 1024;
+  uint32_t noff[IPN], roff;
+#pragma unroll
+  for (int x = 0; x < IPN; ++x) {
+    const int k = (w4 * IPN + x) * KPN + lane / CHN;
+    noff[x] = k * nst2 + (((lane % CHN) ^ (v_wave ? vswz<CHV>(k) : kswz<CHN>(k))) << 4);
+  }
+  {
+    const int k = wr * KPR + lane / CHR;
+    roff = k * rst2 + (((lane % CHR) ^ kswz<CHR>(k)) << 4);
+  }
+
   for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
     const int tiles = ends.tiles(len, kLatTileExp);
@@ -154,28 +179,30 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     }
 
     // ---- DMA of a tile's keys (waves 0-3) or values (waves 4-7) ---------------------
-    const char* nbase = reinterpret_cast<const char*>(v_wave ? a.v.p : a.kn.p) +
-                        2 * (v_wave ? b * a.v.sb + kvh * a.v.sh : b * a.kn.sb + kvh * a.kn.sh);
-    const int64_t nst2 = 2 * (v_wave ? a.v.st : a.kn.st);
-    const char* rbase = reinterpret_cast<const char*>(a.kr.p) + 2 * (b * a.kr.sb);
-    const int64_t rst2 = 2 * a.kr.st;
-    const uint32_t dst0 = lds_addr(ring) + (v_wave ? L::KN + L::KR : 0) + w4 * IPN * 1024;
-    constexpr int KPN = 1024 / (2 * DN), KPR = 1024 / (2 * DR), NR = DR / 16;
-    const int wr = w4 % NR;  // (two waves load the same rows where there are fewer instructions than waves)
-    const uint32_t dst1 = lds_addr(ring) + L::KN + wr * 1024;
+    // Where rows see the whole tile, a uniform address plus the lane's offset; at the end of
+    // the keys, the last one in the place of those behind it.
+    const uint64_t nbase = (uint64_t)(v_wave ? a.v.p : a.kn.p) + 2 * (v_wave ? b * a.v.sb + kvh * a.v.sh : b * a.kn.sb + kvh * a.kn.sh);
+    const uint64_t rbase = (uint64_t)a.kr.p + 2 * (b * a.kr.sb);
     auto issue_tile = [&](int t) {
       const int kb = (tb + t) * KT;
       const uint32_t st = (uint32_t)(t & 3) * L::STAGE;
+      if (kb + KT <= end && near) {
+        const uint64_t at = nbase + (uint64_t)(uint32_t)kb * nst2;
 #pragma unroll
-      for (int x = 0; x < IPN; ++x) {
-        const int k = (w4 * IPN + x) * KPN + lane / CHN;
-        const int slot = lane % CHN;
-        const int c = v_wave ? slot ^ vswz<CHV>(k) : slot ^ kswz<CHN>(k);
-        dma_lane<false>(dst0 + st + x * 1024, nbase + min(kb + k, end - 1) * nst2 + c * 16);
-      }
-      if (!v_wave) {
-        const int k = wr * KPR + lane / CHR;
-        dma_lane<false>(dst1 + st, rbase + min(kb + k, end - 1) * rst2 + ((lane % CHR) ^ kswz<CHR>(k)) * 16);
+        for (int x = 0; x < IPN; ++x) dma_off(dst0 + st + x * 1024, at, noff[x]);
+        if (!v_wave) dma_off(dst1 + st, rbase + (uint64_t)(uint32_t)kb * rst2, roff);
+      } else {
+        const int l = again(lane);
+#pragma unroll 1
+        for (int x = 0; x < IPN; ++x) {
+          const int k = (w4 * IPN + x) * KPN + l / CHN;
+          const int c = (l % CHN) ^ (v_wave ? vswz<CHV>(k) : kswz<CHN>(k));
+          dma_lane<false>(dst0 + st + x * 1024, (const char*)nbase + min(kb + k, end - 1) * nstep + c * 16);
+        }
+        if (!v_wave) {
+          const int k = wr * KPR + l / CHR;
+          dma_lane<false>(dst1 + st, (const char*)rbase + min(kb + k, end - 1) * rstep + ((l % CHR) ^ kswz<CHR>(k)) * 16);
+        }
       }
     };
     auto wait_one = [&]() { v_wave ? wait_vmcnt<IPV>() : wait_vmcnt<IPK>(); };
@@ -196,20 +223,21 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     };
 
     f32x16 s_cur = f32x16{};
+    // (Stages are multiples of 1 KiB: XORs within a row leave them alone.)
     auto read_k = [&](int t, int ks) {
-      const uint8_t* o = ring + (uint32_t)(t & 3) * L::STAGE;
-      return ks < KSN ? *reinterpret_cast<const u32x4*>(o + (kofs ^ (ks << 5)))
-                      : *reinterpret_cast<const u32x4*>(o + (rofs ^ ((ks - KSN) << 5)));
+      const uint32_t o = (uint32_t)(t & 3) * L::STAGE;
+      return ks < KSN ? *reinterpret_cast<const u32x4*>(ring + ((kofs + o) ^ (ks << 5)))
+                      : *reinterpret_cast<const u32x4*>(ring + ((rofs + o) ^ ((ks - KSN) << 5)));
     };
-    auto read_vh = [&](int t, int hh, u32x4 (&vf)[2][DT]) {
-      const uint8_t* o = ring + (uint32_t)(t & 3) * L::STAGE;
+    auto read_vh = [&](int t, int hh, u32x4 (&vf)[DT]) {
+      const uint32_t o = vofs + (uint32_t)(t & 3) * L::STAGE;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const uint8_t* p = o + (vofs ^ (dt << 6)) + hh * 16 * (2 * DV);
+        const uint8_t* p = ring + (o ^ (dt << 6)) + hh * 16 * (2 * DV);
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * (2 * DV)));
         const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-        vf[hh][dt] = u32x4{l2[0], l2[1], h2[0], h2[1]};
+        vf[dt] = u32x4{l2[0], l2[1], h2[0], h2[1]};
       }
     };
 
@@ -221,7 +249,7 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     auto step = [&](auto masked_c, int k) {
       constexpr bool MASKED = decltype(masked_c)::value;
       if (!v_wave && k > 0) sync(k);
-      u32x4 kf[KSN], vf[2][DT];
+      u32x4 kf[KSN], vf[DT];
       u32x4 pk[2];
 #pragma unroll
       for (int ks = 0; ks < KSN; ++ks) kf[ks] = read_k(k + 1, ks);
@@ -249,16 +277,11 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
         }
       };
       if (MASKED && (drops || __ballot(mx == kNegInf) != 0ull)) rescale(kExpTau<T>);
-      auto exps = [&](bool with_v) {
+      auto exps = [&]() {
         const float m0 = mx == kNegInf ? 0.f : mx;
         float ts = 0.f;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          if (with_v) {
-            __builtin_amdgcn_sched_barrier(0);
-            read_vh(k, hh, vf);
-            __builtin_amdgcn_sched_barrier(0);
-          }
           uint32_t w4x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -271,33 +294,44 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
         }
         return ts;
       };
-      float ts = exps(true);
+      float ts = exps();
       if (!drops && __ballot(!(ts <= kExpBound<T>)) != 0ull) {
         rescale(0.f);
-        ts = exps(false);
+        ts = exps();
       }
       lsum += ts;
-      if (MASKED && drops) {
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= nonfinite2<T>(vf[hh][dt][e]);
+      __builtin_amdgcn_sched_barrier(0);
+      read_vh(k, 0, vf);
+      if (v_wave) {
+        // (The second half of the values after the barrier, while the products run: the
+        // stage is overwritten a barrier later.)
+        sync(k);
       }
-      if (v_wave) sync(k);
       {
         f32x16 sn = f32x16{};
 #pragma unroll
         for (int ks = 0; ks < KSN; ++ks) sn = mfma32<T>(kf[ks], qf[ks], sn);
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 vg[DT];
+        read_vh(k, 1, vg);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<T>(vf[dt], pk[0], acc[dt]);
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 kr[KSR];
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<T>(vf[hh][dt], pk[hh], acc[dt]);
+        for (int ks = 0; ks < KSR; ++ks) kr[ks] = read_k(k + 1, KSN + ks);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<T>(vg[dt], pk[1], acc[dt]);
         // (Behind the last tile these products are of an old one and not used.)
 #pragma unroll
-        for (int ks = 0; ks < KSR; ++ks) sn = mfma32<T>(read_k(k + 1, KSN + ks), qf[KSN + ks], sn);
+        for (int ks = 0; ks < KSR; ++ks) sn = mfma32<T>(kr[ks], qf[KSN + ks], sn);
         s_cur = sn;
+        if (MASKED && drops) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= nonfinite2<T>(vf[dt][e]) | nonfinite2<T>(vg[dt][e]);
+        }
       }
     };
 
