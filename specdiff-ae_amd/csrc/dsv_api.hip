@@ -2369,8 +2369,11 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
     p.rpb = 256;
     p.sh = dsv::kLatTileExp;
   } else {
-    p.rpb = R > 32 ? 64 : (R > 16 ? 32 : 16);
     p.sh = dsv::kLatTile;
+    // Blocks of 64 rows where two tiles of them and more fall to a CU; of fewer rows, whose
+    // tiles and partials take less time, where there is less.
+    const int64_t line = B * std::max<int64_t>(1, (n_keys + 63) >> 6), enough = 2 * (int64_t)device_cus();
+    p.rpb = R > 32 && (R + 63) / 64 * line >= enough ? 64 : (R > 16 && (R + 31) / 32 * line >= enough ? 32 : 16);
     // The trees' sets of a block of 64 rows have room for 576 words.
     if (p.rpb == 64 && std::min<int64_t>(64, 63 / p.G + 2) * p.MW > 576) p.rpb = 32;
   }

@@ -5,9 +5,9 @@
 // expanded, kn and v are a head's and kr is shared.  Blocks of 16 rows of a key head,
 // tiles of 64 keys.  Every product is an fp32 matrix product (16x16x4): wave w of four
 // computes the scores of 16 keys and then a quarter of the output's columns.  Operands
-// come straight from the caches (a wave's load takes 16 rows x 64 bytes), because the
-// matrix products at a sixteenth of the 16-bit rate leave time for it: no copy in LDS
-// but the probabilities, held in fp32, and the tile's addresses.
+// come straight from the caches (a wave's load takes 16 rows x 64 bytes, a tile's in flight
+// together), because the matrix products at a sixteenth of the 16-bit rate leave time for
+// it: no copy in LDS but the probabilities, held in fp32, and the tile's addresses.
 
 #include "dsv_latent_dev.h"
 
@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
   __shared__ uint32_t flag[4];
   __shared__ LatSpan span;
 
+  lat_touch_args();
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   int w = (int)blockIdx.x;
@@ -76,20 +77,34 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
     float mx = kNegInf, ls = 0.f;
     bool odd = false;
 
+    auto key_at = [&](int t) { return min(t * KT + wid * 16 + li, end - 1); };
+    int64_t page = a.pt != nullptr && end > 0 ? page_of(a, b, key_at(t0)) : 0;
     for (int t = t0; t < t1 && end > 0; ++t) {
       const int kb = t * KT;
-      // ---- scores of this wave's 16 keys -----------------------------------------------
-      const int n = min(kb + wid * 16 + li, end - 1);
-      const int64_t page = a.pt != nullptr ? page_of(a, b, n) : 0;
+      // ---- loads: the values' places go round through LDS, all of a tile in flight ------
+      const int n = key_at(t);
       const float* k1 = kn + key_off(a, a.kn, n, page) + lg * 4;
       const float* k2 = kr + key_off(a, a.kr, n, page) + lg * 4;
       if (lg == 0) voff[wid * 16 + li] = key_off(a, a.v, n, page);
+      __syncthreads();
+      const float* vc = vb + wid * (DV / 4) + li;
+      float vf[KT / 4][CB];
+#pragma unroll
+      for (int k4 = 0; k4 < KT / 4; ++k4) {
+        const float* vr = vc + voff[k4 * 4 + lg];
+#pragma unroll
+        for (int c = 0; c < CB; ++c) vf[k4][c] = vr[c * 16];
+      }
+      f32x4 kf[SN + SR];
+#pragma unroll
+      for (int x = 0; x < SN + SR; ++x) kf[x] = *reinterpret_cast<const f32x4*>(x < SN ? k1 + x * 16 : k2 + (x - SN) * 16);
+      if (a.pt != nullptr && t + 1 < t1) page = page_of(a, b, key_at(t + 1));
+      // ---- scores of this wave's 16 keys -----------------------------------------------
       f32x4 s{};
 #pragma unroll
       for (int x = 0; x < SN + SR; ++x) {
-        const f32x4 kf = *reinterpret_cast<const f32x4*>(x < SN ? k1 + x * 16 : k2 + (x - SN) * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[x][e], s, 0, 0, 0);
+        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][e], qf[x][e], s, 0, 0, 0);
       }
       const bool whole = lat_whole(a, len, m_lo, kb, KT);
       if (!whole) {
@@ -128,20 +143,17 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
       }
       ls += ps;
       // ---- this wave's columns -----------------------------------------------------------
-      const float* vc = vb + wid * (DV / 4) + li;
-#pragma unroll 4
+#pragma unroll
       for (int k4 = 0; k4 < KT / 4; ++k4) {
         const float pf = p_lds[li * PST + k4 * 4 + lg];
-        const float* vr = vc + voff[k4 * 4 + lg];
-        float vf[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) vf[c] = vr[c * 16];
-        if (!whole && m_hi > m_lo) {
+        for (int c = 0; c < CB; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[k4][c], pf, acc[c], 0, 0, 0);
+      }
+      if (!whole && m_hi > m_lo) {
 #pragma unroll
-          for (int c = 0; c < CB; ++c) odd |= !(fabsf(vf[c]) < __builtin_huge_valf());
-        }
+        for (int k4 = 0; k4 < KT / 4; ++k4)
 #pragma unroll
-        for (int c = 0; c < CB; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[c], pf, acc[c], 0, 0, 0);
+          for (int c = 0; c < CB; ++c) odd |= !(fabsf(vf[k4][c]) < __builtin_huge_valf());
       }
       __syncthreads();
     }

@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
   __shared__ __attribute__((aligned(1024))) L lds;
   uint8_t* const ring = lds.ring;
 
+  lat_touch_args();
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, lj = lane & 31, lg = lane >> 5;
 
