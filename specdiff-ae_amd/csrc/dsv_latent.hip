@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
   const float scale = a.scale_log2;
   Loader ld(a, wid, lane, lds_addr(lds.ring));
   const bool early = !WIDE || a.n_rb == 1;
-  static_assert(!WIDE || Loader::N <= KS / 3 + KT / DS * CB, "");
+  static_assert(!WIDE || Loader::N <= KS / 3 + KT / DS * CB / 2, "the loads are out before the next addresses come");
 
   for (int at = start; at < stop;) {
     const int len = __builtin_amdgcn_readfirstlane(len_of(a, b));
@@ -412,6 +412,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+a"(qf[0][ks]));
       }
     }
+    uint64_t apart = 0;  // a lane's address in the next tile, where they lie apart
+    if (t0 + 1 < t1 && end > 0) apart = ld.keys((t0 + 1) * KT);
     for (int t = t0; t < t1 && end > 0; ++t) {
       // The next tile's loads go out as soon as its buffer is free (every wave done with
       // tile t - 1), before this tile's are waited for, so that the memory is never idle;
@@ -426,9 +428,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
           wait_vmcnt<0>();
           barrier_lds();
         }
-        const uint64_t at = ld.keys((t + 1) * KT);
         between = !early && ld.st2 != 0;
-        if (!between) ld.all(next, at);
+        if (!between) ld.all(next, apart);
         if (early) wait_vmcnt<Loader::N>();
       } else {
         wait_vmcnt<0>();
@@ -569,6 +570,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 #pragma unroll
         for (int i = 0; i < RB; ++i) acc[i][x % CB] = mfma<T>(v, (x / CB) % 2 ? pn[i] : pf[i], acc[i][x % CB]);
         if (WIDE && KS / 3 + x < Loader::N && between) ld.one(next, KS / 3 + x, ln);
+        // (The addresses of the tile after the next, while the products run.)
+        if (x == PK * CB / 2 && t + 2 < t1) apart = ld.keys((t + 2) * KT);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (look) {
