@@ -156,20 +156,33 @@ def desc(t: Optional[torch.Tensor]) -> DsvTensor:
     return d
 
 
+def desc_flat(address: int, dtype: int, *shape: int) -> DsvTensor:
+    """Describe contiguous memory that a call has just allocated."""
+    d = DsvTensor()
+    d.data, d.dtype, d.ndim = address, dtype, len(shape)
+    step = 1
+    for i in range(len(shape) - 1, -1, -1):
+        d.shape[i], d.stride[i] = shape[i], step
+        step *= shape[i]
+    return d
+
+
 def require_gpu(*tensors: Optional[torch.Tensor]) -> torch.device:
     """All tensors must live on one GPU; the kernels have no CPU path."""
-    dev = None
+    # (By number: a device object and a flag per tensor took twice as long.)
+    dev = index = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()
+        if i < 0:
             raise RuntimeError(
                 "diffspec_mi355x kernels run on the GPU only: got a tensor on "
                 f"{t.device}. Move inputs to a ROCm device (there is no CPU fallback)."
             )
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev, index = t.device, i
+        elif i != index:
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
     if dev is None:
         raise RuntimeError("no tensor arguments")
