@@ -16,8 +16,7 @@
 //
 // The running maximum may lag behind the true one: on tiles that all of a wave's rows
 // see whole no maximum is taken, and a tile is redone with it where a lane's 16
-// probabilities sum to more than kSumBound.  Exponents are (s - max) * scale, right for
-// scores of any size.
+// probabilities sum to more than kExpBound.
 
 #include "dsv_dma.h"
 #include "dsv_latent_dev.h"
@@ -210,6 +209,12 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
 
     f32x16 acc[DT];
     float mx = kNegInf, lsum = 0.f;
+    // Probabilities are 2^(s * scale - ms + SHIFT), ms the maximum times the scale, rounded: a
+    // row's sums share a factor 2^err, err = ms - mx * scale, which the end of the piece
+    // takes back.  Where that grows to bits (far), they are 2^((s - mx) * scale + SHIFT), an
+    // instruction more each, and err is 0.
+    float nms = (float)SHIFT, err = 0.f;
+    bool far = false;
     uint32_t odd = 0;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
@@ -269,32 +274,38 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
         for (int v = 1; v < 16; ++v) mt = fmaxf(mt, s_cur[v]);
         mt = halves_max(mt);
         if (__ballot((mt - mx) * scale > tau) != 0ull) {
-          const float mn = fmaxf(mx, mt);
-          const float al = mn == mx ? 1.f : __builtin_amdgcn_exp2f((mx - mn) * scale);
+          const float mn = fmaxf(mx, mt), ms = mn == kNegInf ? 0.f : mn * scale;
+          far = __ballot(fabsf(ms) >= 2097152.f) != 0ull;
+          const float e = far || mn == kNegInf ? 0.f : fmaf(-mn, scale, ms);
+          const float al = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f((mn == mx ? 0.f : (mx - mn) * scale) + (err - e));
           mx = mn;
+          nms = (float)SHIFT - ms;
+          err = e;
           lsum *= al;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
         }
       };
       if (MASKED && (drops || __ballot(mx == kNegInf) != 0ull)) rescale(kExpTau<T>);
-      auto exps = [&]() {
+      auto exps_of = [&](auto far_c) {
+        constexpr bool FAR = decltype(far_c)::value;
         const float m0 = mx == kNegInf ? 0.f : mx;
         float ts = 0.f;
+        auto p1 = [&](float x) { return __builtin_amdgcn_exp2f(FAR ? fmaf(x - m0, scale, (float)SHIFT) : fmaf(x, scale, nms)); };
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           uint32_t w4x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s_cur[hh * 8 + 2 * e] - m0, scale, (float)SHIFT));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s_cur[hh * 8 + 2 * e + 1] - m0, scale, (float)SHIFT));
-            w4x[e] = pack2<T>(p0, p1);
-            ts += p0 + p1;
+            const float a0 = p1(s_cur[hh * 8 + 2 * e]), a1 = p1(s_cur[hh * 8 + 2 * e + 1]);
+            w4x[e] = pack2<T>(a0, a1);
+            ts += a0 + a1;
           }
           pk[hh] = u32x4{w4x[0], w4x[1], w4x[2], w4x[3]};
         }
         return ts;
       };
+      auto exps = [&]() { return far ? exps_of(BoolC<true>{}) : exps_of(BoolC<false>{}); };
       float ts = exps();
       if (!drops && __ballot(!(ts <= kExpBound<T>)) != 0ull) {
         rescale(0.f);
@@ -379,7 +390,7 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
     // ---- the piece's results ---------------------------------------------------------
     __syncthreads();
     if (wave_active) {
-      constexpr float kBack = 1.f / (1 << SHIFT);
+      const float kBack = __builtin_amdgcn_exp2f(err - (float)SHIFT);
       const int row = row0 + lj;
       if (__ballot(odd != 0) != 0ull) {
         lat_exact_rows<T, DV>(lat_args(), pc, kvh, rb, KT, m_lo, nullptr, wid * 32, wid * 32 + 32, 1);
