@@ -623,88 +623,103 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 }
 
 // ---- the partials joined -------------------------------------------------------------
-// A workgroup takes (sequence, unit, 4 rows) at a time, a wave a row of DV / 64 values a
-// lane, eight partials in flight.
+// A workgroup takes (sequence, unit, `per` rows) at a time, a wave a row of DV / 64 values
+// a lane, eight partials in flight.
+template <int N>
+struct Count {
+  static constexpr int value = N;
+};
 template <int DV>
-__global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int sh, uint32_t n) {
-  constexpr int N = DV / 64, U = 8;
+__global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int sh, uint32_t n, int per) {
+  constexpr int N = DV / 64;
   typedef float Row __attribute__((ext_vector_type(N)));
   __shared__ LatSpan span;
   lat_touch_args();
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
 #pragma unroll 1
   for (uint32_t x = blockIdx.x; x < n; x += gridDim.x) {
-    const uint32_t parts = a.rpb / 4;
+    const uint32_t parts = (uint32_t)a.rpb / (uint32_t)per;
     uint32_t y = x / parts;
-    const int i = (int)(x - y * parts) * 4 + wid;
+    const int i0 = (int)(x - y * parts) * per;
     const uint32_t unit = y % (uint32_t)(a.n_rb * a.Hk), b = y / (uint32_t)(a.n_rb * a.Hk);
-    const int kvh = unit / (uint32_t)a.n_rb, rb = unit % (uint32_t)a.n_rb, row = rb * a.rpb + i;
+    const int kvh = unit / (uint32_t)a.n_rb, rb = unit % (uint32_t)a.n_rb;
     const LatEnd ends(a, rb);
     const LatCut cut(lat_line<256>(a, ends, sh, 0, (int)b, span), a.W);
     const int at = span.at;
     __syncthreads();
     const int j0 = cut.range_of(at), j1 = cut.range_of(at + ends.tiles(len_of(a, (int)b), sh) - 1);
-    if (j0 == j1 || row >= a.R) continue;  // (one piece: written by its workgroup)
-    // A range behind the first one begins with this sequence.
-    const int64_t base = ((int64_t)unit * a.W * 2) * a.rpb + i;
-    const int64_t first = cut.begin(j0) >= at ? 0 : a.rpb;
-    float m = kNegInf, l = 0.f;
-    Row o{};
+    if (j0 == j1) continue;  // (one piece: written by its workgroup)
 #pragma unroll 1
-    for (int s0 = j0; s0 <= j1; s0 += U) {
-      float2 ml[U];
-      Row p[U];
+    for (int i = i0 + wid; i < i0 + per && rb * a.rpb + i < a.R; i += 4) {
+      const int row = rb * a.rpb + i;
+      // A range behind the first one begins with this sequence.
+      const int64_t base = ((int64_t)unit * a.W * 2) * a.rpb + i;
+      const int64_t first = cut.begin(j0) >= at ? 0 : a.rpb;
+      float m = kNegInf, l = 0.f;
+      Row o{};
+      auto join = [&](auto count, int s0) {
+        constexpr int U = decltype(count)::value;
+        float2 ml[U];
+        Row p[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = min(s0 + u, j1);
-        const int64_t pr = base + (int64_t)j * 2 * a.rpb + (j == j0 ? first : 0);
-        ml[u] = a.ml[pr];
-        p[u] = *reinterpret_cast<const Row*>(a.opart + pr * DV + lane * N);
+        for (int u = 0; u < U; ++u) {
+          const int j = min(s0 + u, j1);
+          const int64_t pr = base + (int64_t)j * 2 * a.rpb + (j == j0 ? first : 0);
+          ml[u] = a.ml[pr];
+          p[u] = *reinterpret_cast<const Row*>(a.opart + pr * DV + lane * N);
+        }
+        // (All in flight before the first is used: the compiler moves them to their uses.)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float t = p[u][N - 1];
+          asm volatile("" : "+v"(t));
+          p[u][N - 1] = t;
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+        const float f0 = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+        l *= f0;
+        o *= f0;
+        m = mn;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          // (Behind the last, and where a piece has no key of this row: nothing.)
+          const bool none = s0 + u > j1 || ml[u].x == kNegInf;
+          const float f = none ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
+          l = fmaf(none ? 0.f : ml[u].y, f, l);
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] = fmaf(none ? 0.f : p[u][e], f, o[e]);
+        }
+      };
+      // (Two at once where there are no more: loads of nothing cost as much.)
+      if (j1 - j0 < 2) {
+        join(Count<2>{}, j0);
+      } else {
+#pragma unroll 1
+        for (int s0 = j0; s0 <= j1; s0 += 8) join(Count<8>{}, s0);
       }
-      // (All in flight before the first is used: the compiler moves them to their uses.)
+      o *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const int pos = row / a.G, h = kvh * a.G + row - pos * a.G;
+      const int64_t off = b_off(a, (int)b, pos, h) + lane * N;
+      if (a.out_vec && a.out_dtype == 2) {
+        *reinterpret_cast<Row*>(reinterpret_cast<float*>(a.out) + off) = o;
+      } else if (a.out_vec && N > 1) {
+        uint32_t w[(N + 1) / 2];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float t = p[u][N - 1];
-        asm volatile("" : "+v"(t));
-        p[u][N - 1] = t;
+        for (int e = 0; e + 1 < N; e += 2) w[e / 2] = a.out_dtype == 0 ? pack2<BF16>(o[e], o[e + 1]) : pack2<F16>(o[e], o[e + 1]);
+        uint32_t* p = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + off);
+        typedef uint32_t Out __attribute__((ext_vector_type((N + 1) / 2)));
+        Out v;
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) v[e] = w[e];
+        *reinterpret_cast<Out*>(p) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) store1(a, off + e, o[e]);
       }
-      float mn = m;
-#pragma unroll
-      for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
-      const float f0 = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
-      l *= f0;
-      o *= f0;
-      m = mn;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // (Behind the last, and where a piece has no key of this row: nothing.)
-        const bool none = s0 + u > j1 || ml[u].x == kNegInf;
-        const float f = none ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
-        l = fmaf(none ? 0.f : ml[u].y, f, l);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = fmaf(none ? 0.f : p[u][e], f, o[e]);
-      }
+      if (lane == 0 && a.lse != nullptr) a.lse[b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m, l);
     }
-    o *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    const int pos = row / a.G, h = kvh * a.G + row - pos * a.G;
-    const int64_t off = b_off(a, (int)b, pos, h) + lane * N;
-    if (a.out_vec && a.out_dtype == 2) {
-      *reinterpret_cast<Row*>(reinterpret_cast<float*>(a.out) + off) = o;
-    } else if (a.out_vec && N > 1) {
-      uint32_t w[(N + 1) / 2];
-#pragma unroll
-      for (int e = 0; e + 1 < N; e += 2) w[e / 2] = a.out_dtype == 0 ? pack2<BF16>(o[e], o[e + 1]) : pack2<F16>(o[e], o[e + 1]);
-      uint32_t* p = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + off);
-      typedef uint32_t Out __attribute__((ext_vector_type((N + 1) / 2)));
-      Out v;
-#pragma unroll
-      for (int e = 0; e < N / 2; ++e) v[e] = w[e];
-      *reinterpret_cast<Out*>(p) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) store1(a, off + e, o[e]);
-    }
-    if (lane == 0 && a.lse != nullptr) a.lse[b * a.l_sb + (int64_t)pos * a.l_sm + (int64_t)h * a.l_sh] = lat_lse(a, m, l);
   }
 }
 
@@ -741,13 +756,16 @@ hipError_t launch_latent(const LatArgs& a, hipStream_t s) {
 
 hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   if (a.W == 1) return hipSuccess;
-  const uint32_t n = (uint32_t)((int64_t)a.B * a.Hk * a.n_rb * (a.rpb / 4));  // (below 2^31)
+  // Four rows a workgroup where there are few, 16 where the search of their pieces counts.
+  const int64_t blocks = (int64_t)a.B * a.Hk * a.n_rb;
+  const int per = blocks * a.rpb <= 8192 ? 4 : 16;
+  const uint32_t n = (uint32_t)(blocks * (a.rpb / per));  // (below 2^31)
   const dim3 grid((unsigned)(n < (1 << 20) ? n : 1 << 20)), block(256);
   switch (a.dv) {
-    case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, sh, n); break;
-    case 128: hipLaunchKernelGGL(latent_merge_kernel<128>, grid, block, 0, s, a, sh, n); break;
-    case 256: hipLaunchKernelGGL(latent_merge_kernel<256>, grid, block, 0, s, a, sh, n); break;
-    default: hipLaunchKernelGGL(latent_merge_kernel<512>, grid, block, 0, s, a, sh, n); break;
+    case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, sh, n, per); break;
+    case 128: hipLaunchKernelGGL(latent_merge_kernel<128>, grid, block, 0, s, a, sh, n, per); break;
+    case 256: hipLaunchKernelGGL(latent_merge_kernel<256>, grid, block, 0, s, a, sh, n, per); break;
+    default: hipLaunchKernelGGL(latent_merge_kernel<512>, grid, block, 0, s, a, sh, n, per); break;
   }
   return hipGetLastError();
 }
