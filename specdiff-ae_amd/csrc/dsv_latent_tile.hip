@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t again(uint32_t x) {
 // Chunk c of key k stands at slot c ^ of these: operand reads without bank conflicts.
 template <int CH>
 __device__ __forceinline__ int kswz(int key) {
-  return CH >= 8 ? key & (CH - 1) & 15 : (key >> 2) & 3;
+  return CH >= 16 ? key & 15 : CH == 8 ? (key >> 1) & 7 : (key >> 2) & 3;
 }
 template <int CH>
 __device__ __forceinline__ int vswz(int key) {
