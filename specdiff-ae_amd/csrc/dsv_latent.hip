@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < QR; ++i) ls[i] = 0.f;
-    uint32_t odd = 0;
+    bool hides = false;
     if (end > 0) {
       // The queries come through the other buffer (a load that ends in registers would be
       // waited for at its first use, in the loop, and the tiles in flight with it).
@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
       const int kb = t * KT;
       const bool whole = lat_whole(a, len, m_lo, kb, KT);
       // Value v of a result is key 8 (v / 4) + 4 lg + v % 4 of the wave's.
+      hides |= !whole;
       if (!whole) {
         uint32_t keep = 0;
 #pragma unroll 1
@@ -561,7 +562,6 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 #pragma unroll
       for (int i = 0; i < QR; ++i) ls[i] += ps[i];
       // ---- this wave's columns -------------------------------------------------------
-      const bool look = !whole && m_hi > m_lo;
 #pragma unroll
       for (int x = 0; x < PK * CB; ++x) {
         if (x % CB == 0 && x / CB + 1 < PK) read_p(x / CB + 1, (x / CB) % 2 ? pf : pn);
@@ -573,13 +573,6 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         // (The addresses of the tile after the next, while the products run.)
         if (x == PK * CB / 2 && t + 2 < t1) apart = ld.keys((t + 2) * KT);
         __builtin_amdgcn_sched_barrier(0);
-      }
-      if (look) {
-#pragma unroll 1
-        for (int x = 0; x < PK * CB; ++x) {
-          const u32x4 v = read_v(x);
-          odd |= nonfinite2<T>(v[0]) | nonfinite2<T>(v[1]) | nonfinite2<T>(v[2]) | nonfinite2<T>(v[3]);
-        }
       }
     }
 
@@ -594,7 +587,17 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 #pragma unroll
       for (int i = 0; i < RB; ++i) lds.m[i * TR + li] = mx[i];
     }
-    const uint32_t any = __ballot(odd != 0) != 0ull ? 1 : 0;
+    // An infinite or NaN value of a hidden key makes 0 * inf = NaN of rows that do not see it.
+    float bad = 0.f;
+    if (hides) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) bad = fmaf(acc[i][c][v], 0.f, bad);  // (NaN of an infinite sum, too)
+    }
+    const uint32_t any = __ballot(bad != 0.f) != 0ull ? 1 : 0;
     if (lane == 0) lds.flag[wid] = any;
 #pragma unroll
     for (int i = 0; i < RB; ++i)

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
 #pragma unroll
     for (int c = 0; c < CB; ++c) acc[c] = f32x4{};
     float mx = kNegInf, ls = 0.f;
-    bool odd = false;
+    bool hides = false;
 
     auto key_at = [&](int t) { return min(t * KT + wid * 16 + li, end - 1); };
     int64_t page = a.pt != nullptr && end > 0 ? page_of(a, b, key_at(t0)) : 0;
@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
         for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][e], qf[x][e], s, 0, 0, 0);
       }
       const bool whole = lat_whole(a, len, m_lo, kb, KT);
+      hides |= !whole;
       if (!whole) {
 #pragma unroll
         for (int v = 0; v < 4; ++v)
@@ -149,12 +150,6 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
 #pragma unroll
         for (int c = 0; c < CB; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[k4][c], pf, acc[c], 0, 0, 0);
       }
-      if (!whole && m_hi > m_lo) {
-#pragma unroll
-        for (int k4 = 0; k4 < KT / 4; ++k4)
-#pragma unroll
-          for (int c = 0; c < CB; ++c) odd |= !(fabsf(vf[k4][c]) < __builtin_huge_valf());
-      }
       __syncthreads();
     }
 
@@ -162,7 +157,15 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
     float lw = ls + __shfl_xor(ls, 16);
     lw += __shfl_xor(lw, 32);
     if (lg == 0) red[wid][li] = lw;
-    const bool any = __ballot(odd) != 0ull;
+    // An infinite or NaN value of a hidden key makes 0 * inf = NaN of rows that do not see it.
+    float bad = 0.f;
+    if (hides) {
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) bad = fmaf(acc[c][v], 0.f, bad);  // (NaN of an infinite sum, too)
+    }
+    const bool any = __ballot(bad != 0.f) != 0ull;
     if (lane == 0) flag[wid] = any ? 1 : 0;
     __syncthreads();
     if ((flag[0] | flag[1] | flag[2] | flag[3]) != 0) {

@@ -190,6 +190,47 @@ def test_absorbed_hidden_values(gpu, dtype, tree):
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("H,M,n", [(128, 5, 70), (64, 3, 9000), (16, 9, 200), (48, 4, 130)])
+def test_absorbed_hidden_siblings(gpu, dtype, H, M, n):
+    """Blocks of rows that all belong to one node of a tree: its siblings' infinite and NaN rows stay out of them."""
+    q, kv, _, sl, _, rows = make(dtype, 1, M, H, 512, 64, 0, [n], False, seed=H)
+    parent = torch.tensor([-1] + [0] * (M - 1), dtype=torch.int32, device=gpu)  # (a root and its children)
+    kv[0, n - 1, 7] = math.inf      # the last child
+    kv[0, n - M + 1, 3] = math.nan  # the first
+    out, lse = latent_attn_with_kvcache(q, kv, 512, 0.05, cache_seqlens=sl, parent=parent, return_softmax_lse=True)
+    x = f64(kv[0])
+    seen = oracle.visible(M, n, parent.tolist())
+    clean = [m for m in range(M) if m not in (1, M - 1)]
+    x[n - 1] = x[n - M + 1] = 0
+    for h in (0, H // 2, H - 1):
+        ref = oracle.attention(f64(q[0, clean, h]), x, x[:, :512], 0.05, [seen[m] for m in clean])
+        check(out[:, clean], lse[:, :, clean], 0, h, ref, 576, dtype, n, np.abs(x).max())
+    assert not torch.isfinite(out[0, 1].float()).all(-1).any() and not torch.isfinite(out[0, M - 1].float()[:, 7]).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("H", [8, 33, 64])
+def test_absorbed_infinite_last_value(gpu, dtype, H):
+    """An infinite entry of the last token, which stands in for those behind it in its tile: a score of 0 * inf spoils the
+    row, one of -inf (no weight) its own column alone."""
+    n = 90
+    q, kv, _, sl, _, rows = make(dtype, 1, 1, H, 256, 32, 0, [n], False, seed=H)
+    q[..., 9] = 0
+    kv[0, n - 1, 9] = math.inf
+    out, lse = latent_attn_with_kvcache(q, kv, 256, 0.05, cache_seqlens=sl, return_softmax_lse=True)
+    assert torch.isnan(out.float()).all() and torch.isnan(lse).all()
+    q[..., 9] = -2.0 ** -14
+    out, lse = latent_attn_with_kvcache(q, kv, 256, 0.05, cache_seqlens=sl, return_softmax_lse=True)
+    assert torch.isnan(out[..., 9].float()).all()  # (0 * inf, as the formula has it)
+    keep = [c for c in range(256) if c != 9]
+    x = f64(kv[0, :n - 1])
+    for h in range(H):
+        ref = oracle.attention(f64(q[0, :, h]), x, x[:, :256], 0.05, [np.arange(n - 1)])  # (x holds no infinity)
+        ref = {**ref, "out": ref["out"][:, keep], "mass": ref["mass"][:, keep]}
+        check(out[..., keep], lse, 0, h, ref, 288, dtype, n, np.abs(x).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("size", [30.0, 3e3, 1e6])
 def test_absorbed_large_and_growing_scores(gpu, dtype, size):
     """Scores that grow along the cache, so that the maximum moves in every tile, up to far beyond 2^22."""
