@@ -2210,6 +2210,13 @@ int dsv_latent_append(const dsv_tensor* c, const dsv_tensor* k_pe, const dsv_ten
   dsv::LatentAppendArgs a{};
   if ((rc = check_nd(cache, "cache", cache != nullptr && cache->ndim == 2 ? 2 : 3)) != DSV_OK) return rc;
   if ((rc = check_vec16(cache, "cache")) != DSV_OK) return rc;
+  // (No tokens, as a list of capacity 0 has them: their tensors may come without storage.)
+  if (c != nullptr && c->ndim == 2 && c->shape[0] == 0) {
+    if (k_pe == nullptr || k_pe->ndim != 2 || k_pe->shape[0] != 0 || c->shape[1] + k_pe->shape[1] != cache->shape[cache->ndim - 1] ||
+        slots == nullptr || slots->ndim != 1 || slots->shape[0] != 0)
+      return fail(DSV_ERR_INVALID, "c and k_pe must be [T, dc] and [T, dr], dc + dr as wide as cache's rows, and slots [T]");
+    return DSV_OK;
+  }
   auto rows = [&](const dsv_tensor* t, const char* name, int nd) -> int {
     int r;
     if (t == nullptr || t->ndim != nd) return fail(DSV_ERR_INVALID, "%s must be a %d-d tensor", name, nd);

@@ -761,8 +761,9 @@ hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   if (a.W == 1) return hipSuccess;
   // Four rows a workgroup where there are few, 16 where the search of their pieces counts.
   const int64_t blocks = (int64_t)a.B * a.Hk * a.n_rb;
-  const int per = blocks * a.rpb <= 8192 ? 4 : 16;
-  const uint32_t n = (uint32_t)(blocks * (a.rpb / per));  // (below 2^31)
+  int per = blocks * a.rpb <= 8192 ? 4 : 16;
+  while (blocks * (a.rpb / per) > 0x7fffffff) per *= 2;  // (blocks are fewer than 2^30: the plan's range)
+  const uint32_t n = (uint32_t)(blocks * (a.rpb / per));
   const dim3 grid((unsigned)(n < (1 << 20) ? n : 1 << 20)), block(256);
   switch (a.dv) {
     case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, sh, n, per); break;

@@ -199,7 +199,6 @@ void launch_e(const LatentAppendArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_latent_append(const LatentAppendArgs& a, hipStream_t s) {
-  if (a.T == 0) return hipSuccess;
   if (a.dtype == 0)
     launch_e<TagBF16>(a, s);
   else if (a.dtype == 1)

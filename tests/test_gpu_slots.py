@@ -164,6 +164,40 @@ def test_append_in_place_queries_and_flat_cache(gpu):
     assert torch.equal(cache[slots.long(), :dc], c) and (wide[:, dc + dr:] == 0).all()
 
 
+def test_append_of_no_tokens(gpu):
+    cache = torch.ones((4, 8, 96), dtype=BF, device=gpu)
+    m = token_slots(torch.zeros((1, 2), dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu),
+                    torch.zeros(1, dtype=torch.int32, device=gpu), 8, 0)
+    none = lambda *s: torch.empty(s, dtype=BF, device=gpu)  # noqa: E731
+    assert append_latent_kv(none(0, 64), none(0, 32), cache, m["slots"], q_pe=none(0, 4, 32)).shape == (0, 4, 32)
+    assert append_latent_kv(none(0, 64), none(0, 32), cache, m["slots"]) is None
+    assert (cache == 1).all()
+
+
+def test_append_captured(gpu):
+    """A captured append reads its slots and positions anew at every replay."""
+    c, pe = torch.randn((30, 512), device=gpu).to(BF), torch.randn((30, 64), device=gpu).to(BF)
+    cache = torch.zeros((8, 8, 576), dtype=BF, device=gpu)
+    slots, pos = torch.randperm(64, device=gpu)[:30], torch.arange(30, device=gpu)
+    cos, sin = tables(100, 64, False)
+    q = torch.randn((30, 4, 64), device=gpu).to(BF)
+    args = dict(cos=cos, sin=sin, positions=pos, q_pe=q)
+    append_latent_kv(c, pe, cache, slots, **args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = append_latent_kv(c, pe, cache, slots, **args)
+    for i in range(3):
+        cache.fill_(3)
+        slots.copy_(torch.randperm(64, device=gpu)[:30])
+        pos += i
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = cache.clone()
+        cache.fill_(3)
+        want = append_latent_kv(c, pe, cache, slots, **args)
+        assert torch.equal(got, want) and torch.equal(replayed, cache), i
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_decoding_loop(gpu, dtype):
     """Prompts expanded, their rows appended, then steps of extend, slots, append and absorbed attention over a forked

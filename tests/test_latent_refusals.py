@@ -165,10 +165,25 @@ def test_append(dry):
     assert append(dry, dr=24) == UNSUPPORTED
     assert append(dry, page=6) == UNSUPPORTED
     assert append(dry, dc=2056) == UNSUPPORTED
+    none = dict(T=0, slots=i32(0))
+    assert append(dry, **none) == 0 and append(dry, with_q=False, rope=False, **none) == 0
+    assert append(dry, T=0, slots=i32(1)) == INVALID and append(dry, pe=f(0, 24), **none) == INVALID
     cache = f(3, 8, 96)
     assert append(dry, cache=cache, c=cache.view(24, 96)[:6, :64]) == INVALID
     assert append(dry, q=q, qo=q.view(2, 6, 32).transpose(0, 1)) == INVALID
     assert append(dry, cache=cache, qo=cache.view(-1)[:384].view(6, 2, 32)) == INVALID
+
+
+def test_workspace_of_every_plan(dry):
+    """Few enough partials for the largest batches, and none where every workgroup has a unit of its own."""
+    ws = dry.dsv_latent_workspace_bytes
+    assert ws(1 << 20, 1, 512, 128, 0, 64, 0, 1) == 0        # (512 units fill 256 CUs twice)
+    assert ws(1 << 20, 1, 200, 128, 0, 64, 0, 1) > 0         # (rows to be joined of 2^27.6 blocks of 256)
+    assert ws(1, 8192, 128, 128, 0, 8192, 0, 1) == 0
+    assert ws(1 << 20, 1, 1024, 512, 0, 1 << 20, 0, 0) == 0  # (beyond the range: too many tiles)
+    for B, M, H, n in ((1, 1, 16, 1), (1, 1, 128, 1 << 20), (64, 1, 128, 4096), (7, 48, 16, 5000), (3, 1, 1, 200)):
+        for dtype in (0, 1, 2):
+            assert ws(B, M, H, 512, dtype, n, 0, 0) <= 512 * 2 * 2 * 4 * 64 * (512 + 2) * 4
 
 
 def test_no_cpu_path():
