@@ -421,3 +421,140 @@ def test_outputs_beside_the_rows_stay(gpu):
     compare(q, rows, [100, 2], 512, 0.05, out, None, None, range(5), BF)
     big[:, :3, 1:6, 4:516] = 3.0
     assert (big == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("od", [BF, F16, F32])
+def test_expanded_into_strided_outputs(gpu, dtype, od):
+    """Rows at any stride, joined from partials (one head of many keys) and whole; what lies between them stays."""
+    from diffspec_mi355x import _ext
+    lib = _ext.load()
+    for M, N, H in ((5, 4000, 1), (40, 50, 3)):
+        q, k, pe, v, sl = make_exp(dtype, 2, M, N, H, 64, 32, [N, M], seed=M)
+        big = torch.full((2, M + 1, H + 2, 67), 3.0, dtype=od, device=gpu)
+        out = big[:, :M, 1:1 + H, 1:65]
+        lse = torch.full((2, M, H, 2), 5.0, device=gpu)[..., 0].transpose(1, 2)
+        nws = lib.dsv_latent_workspace_bytes(2, M, H, 64, _ext.desc(q).dtype, N, 0, 1)
+        ws, ptr = _ext.scratch(nws, gpu)
+        _ext.check(lib.dsv_latent_expanded(_ext.desc(q), _ext.desc(k), _ext.desc(pe), _ext.desc(v), _ext.desc(sl), N, 1, 0.1,
+                                           _ext.desc(out), _ext.desc(lse), ptr, nws, _ext.stream_of(gpu)), "expanded")
+        compare_exp(q, k, pe, v, [N, M], True, 0.1, out, lse, range(H), dtype)
+        out.fill_(3.0)
+        assert (big == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_expanded_shared_and_strided_inputs(gpu, dtype):
+    """Keys and values shared by the heads or the sequences (stride 0), heads before tokens, one length for all."""
+    B, M, N, H, dn, dr = 2, 33, 290, 3, 128, 32
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rnd = lambda *s: torch.randn(s, generator=g, device=gpu).to(dtype)  # noqa: E731
+    q = rnd(B, H, M, dn + dr).transpose(1, 2)
+    k = rnd(1, H, N, dn).transpose(1, 2).expand(B, N, H, dn)
+    v = rnd(B, N, 1, dn).expand(B, N, H, dn)
+    pe = rnd(1, N, dr + 8)[..., :dr].expand(B, N, dr)
+    for n, causal in ((N, True), (64, False), (torch.tensor(270, device=gpu), True)):
+        out, lse = latent_attn_expanded(q, k, pe, v, cache_seqlens=n, causal=causal, return_softmax_lse=True)
+        compare_exp(q, k, pe, v, [int(n)] * B, causal, (dn + dr) ** -0.5, out, lse, range(H), dtype)
+    one = rnd(B, 1, H, dn).expand(B, N, H, dn)  # (all keys alike: the mean of the values)
+    out, lse = latent_attn_expanded(q, one, pe[:, :1].expand(B, N, dr), v, causal=False, return_softmax_lse=True)
+    compare_exp(q, one, pe[:, :1].expand(B, N, dr), v, [N] * B, False, (dn + dr) ** -0.5, out, lse, range(H), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_expanded_units_of_their_own(gpu, dtype):
+    """So many heads and row blocks that no sequence's keys are shared out."""
+    M, H = 2100, 115
+    q, k, pe, v, sl = make_exp(dtype, 2, M, M, H, 64, 32, [M, 1500], seed=12)
+    out, lse = latent_attn_expanded(q, k, pe, v, cache_seqlens=sl, return_softmax_lse=True)
+    rows = [0, 599, 600, 601, 1023, 1024, 2047, 2099]
+    compare_exp(q, k, pe, v, [M, 1500], True, 96 ** -0.5, out, lse, [0, 57, 114], dtype, rows)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("M,N", [(1, 6000), (300, 700)])
+def test_expanded_very_large_scores(gpu, dtype, M, N):
+    """Scores beyond 2^21, whose product with the scale a fused exponent would round away, growing along the keys
+    (in partials, too).  Scores are single products of short numbers, exact in fp32, so the weights are those of
+    exact differences; the bounds are those of the file's head with delta 0, the product of a difference of up to
+    40 with the scale (2^-23 of it) in its place."""
+    k = torch.zeros((1, N, 1, 64), dtype=dtype, device=gpu)
+    k[0, :, 0, 0] = (1024 + torch.arange(N, device=gpu) // 64).to(dtype)
+    k[0, :, 0, 1] = (torch.arange(N, device=gpu) % 7).to(dtype)
+    q = torch.zeros((1, M, 1, 96), dtype=dtype, device=gpu)
+    q[..., 0] = 4096.0
+    q[..., 1] = 1.0
+    pe = torch.zeros((1, N, 32), dtype=dtype, device=gpu)
+    v = torch.randn((1, N, 1, 64), device=gpu).to(dtype)
+    out, lse = latent_attn_expanded(q, k, pe, v, softmax_scale=1.0, return_softmax_lse=True)
+    x, y = f64(k[0, :, 0]), f64(v[0, :, 0])
+    s = 4096 * x[:, 0] + x[:, 1]
+    assert s.max() > 2 ** 22 and np.array_equal(np.float32(s), s)
+    u = torch.finfo(dtype).eps / 2
+    for m in sorted({0, M // 2, M - 1}):
+        n = N - M + m + 1
+        w = np.exp(s[:n] - s[:n].max())
+        ref, mass = (w @ y[:n]) / w.sum(), (w @ np.abs(y[:n])) / w.sum()
+        tol = mass * (u + 80 * 2.0 ** -24 + (n + 64) * 2.0 ** -24 + 2.0 ** -22) * 1.01 + u * np.abs(ref) + n * 2.0 ** -34 * np.abs(y).max()
+        assert (np.abs(f64(out[0, m, 0]) - ref) <= tol).all(), m
+        want = s[:n].max() + math.log(w.sum())
+        assert abs(float(lse[0, 0, m]) - want) <= 2.0 ** -21 * want
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_absorbed_odd_lengths_and_pages(gpu, dtype):
+    """Lengths below 0 and beyond 32 bits, sequences that share pages, numbers outside the pool (clamped to it)."""
+    q, kv, _, _, _, rows = make(dtype, 1, 2, 4, 256, 32, 16, [96], False, seed=13, spare=0)
+    q = q.expand(4, 2, 4, 288)
+    kv = torch.randn((6, 16, 288), device=gpu).to(dtype)
+    table = torch.tensor([[0, 1, 2, 3], [3, 1, 0, 5], [-7, 2, 99, 5], [1, 1, 1, 1]], device=gpu)
+    lens = torch.tensor([-5, (1 << 40) + 3, 64, 33], device=gpu)
+    out, lse = latent_attn_with_kvcache(q, kv, 256, 0.06, cache_seqlens=lens, page_table=table, return_softmax_lse=True)
+    n = [0, 64, 64, 33]
+    seq = [kv[table[b].clamp(0, 5)].reshape(64, 288)[:n[b]] for b in range(4)]
+    compare(q, seq, n, 256, 0.06, out, lse, None, range(4), dtype)
+    low = lens.clamp(-5, 200).int()
+    again = latent_attn_with_kvcache(q, kv, 256, 0.06, cache_seqlens=low, page_table=table.int())
+    assert torch.equal(out, again)
+
+
+def test_two_graphs_and_new_lengths(gpu):
+    """Two captured graphs replayed in turn while their lengths, tables and caches change."""
+    lens = [4000, 90, 1500]
+    q, kv, table, sl, _, rows = make(BF, 3, 1, 64, 512, 64, 16, lens, False, seed=14)
+    kv.nan_to_num_(0.5)
+    table.clamp_(min=0)
+    calls = [lambda: latent_attn_with_kvcache(q, kv, 512, 0.05, cache_seqlens=sl, page_table=table, return_softmax_lse=True),
+             lambda: latent_attn_with_kvcache(q[:, :, :16], kv, 512, 0.05, cache_seqlens=sl, page_table=table, return_softmax_lse=True)]
+    graphs, outs = [], []
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append(g)
+    for i in range(4):
+        sl.copy_(torch.tensor([[4000, 90, 1500], [1, 4000, 0], [64, 65, 63], [4000, 4000, 4000]][i], device=gpu))
+        table.copy_(table[torch.tensor([1, 2, 0], device=gpu)])
+        kv[i].fill_(0.25)
+        for g in graphs:
+            g.replay()
+        for got, call in zip(outs, calls):
+            want = call()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_absorbed_whole_range_of_batches(gpu, dtype):
+    """Many short sequences of random lengths (each CU's share holds several), and rows left empty."""
+    rng = np.random.default_rng(15)
+    B = 600
+    lens = [int(x) for x in rng.integers(0, 150, B)]
+    q, kv, table, sl, _, rows = make(dtype, B, 2, 3, 256, 64, 16, lens, False, seed=15)
+    out, lse = latent_attn_with_kvcache(q, kv, 256, 0.06, cache_seqlens=sl, page_table=table, return_softmax_lse=True)
+    pick = sorted({0, 599, *(int(x) for x in rng.integers(0, B, 60)), *(i for i, n in enumerate(lens) if n < 3)})
+    for b in pick:
+        compare(q[b:b + 1], rows[b:b + 1], lens[b:b + 1], 256, 0.06, out[b:b + 1], lse[b:b + 1], None, range(3), dtype)
+    assert torch.isfinite(out.float()).all()
