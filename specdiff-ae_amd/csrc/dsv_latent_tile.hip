@@ -16,7 +16,18 @@
 //
 // The running maximum may lag behind the true one: on tiles that all of a wave's rows
 // see whole no maximum is taken, and a tile is redone with it where a lane's 16
-// probabilities sum to more than kExpBound.
+// probabilities sum to more than kExpBound.  An exponent is one product and sum,
+// s * scale - max * scale; where the second rounds to whole bits (2^21 and more), the
+// difference is taken first.
+//
+// Registers: 256 a wave (two on a SIMD).  Tiles' addresses are uniform plus a lane's
+// offset, the values' second half is read behind the barrier: nothing is spilled.
+//
+// Measured (a large bf16 product reaches 1309 TFLOP/s, fp16 1294): a prompt of 8192 tokens,
+// 16 heads of 128 + 64, 344 GFLOP: 331-334 us, 1.03 PFLOP/s, 79 % of that, bound by the
+// matrix units at the clock that the power cap leaves, the softmax beside them.  Chunks of
+// 1001 tokens of two sequences through 5000 to 12007 keys, 8 heads, fp16, 116 GFLOP: 130 us
+// and 16 for joining the partials (33 MB of fp32 written and read).  No bank conflicts.
 
 #include "dsv_dma.h"
 #include "dsv_latent_dev.h"

@@ -10,6 +10,9 @@
 // of L2; a launch of its own for the scan would cost more), finds its tokens'
 // requests by bisection in LDS and writes its share of tokens and table entries.  Beyond, a
 // first launch writes cu and the second bisects in it.
+//
+// Measured: 48 requests with a token each 7.4 us, 512 requests with up to 1000 tokens each
+// (300000 places, 5.2 MB) 8.3 us; the call from Python takes 17.
 
 #include "dsv_internal.h"
 
