@@ -39,7 +39,7 @@
 //
 // Measured at rows of 512 + 64 (a large copy reaches 4.95 TB/s, a large bf16 product
 // 1309 TFLOP/s).  64 sequences of up to 16384 keys, 16 heads, 652 MB: 126 + 6.5 us (the
-// join), 4.9 TB/s, bound by HBM.  One sequence of 2900 keys, 128 heads: 15 + 7 us, bound by
+// join), 4.9 TB/s, bound by HBM.  One sequence of 2900 keys, 128 heads: 15 + 5.5 us, bound by
 // latencies: arguments, lengths, pages, first tile, and the code itself as it is fetched.
 // 32 sequences of 1000 to 8192 keys, 128 heads, fp16: 77 + 11 us; 8 trees of 64 nodes, 32
 // heads: 194 + 16 us, 56 % of the large product's rate: a wave alone on its SIMD does its
@@ -643,7 +643,8 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 
 // ---- the partials joined -------------------------------------------------------------
 // A workgroup takes (sequence, unit, `per` rows) at a time, a wave a row of DV / 64 values
-// a lane, eight partials in flight.
+// a lane, eight partials in flight; of one row (per = 1), the waves take eight partials each
+// in turn and their sums are joined through LDS.
 template <int N>
 struct Count {
   static constexpr int value = N;
@@ -653,8 +654,11 @@ __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int 
   constexpr int N = DV / 64;
   typedef float Row __attribute__((ext_vector_type(N)));
   __shared__ LatSpan span;
+  __shared__ __attribute__((aligned(16))) float part[3 * DV];
+  __shared__ float2 part_ml[3];
   lat_touch_args();
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const bool split = per == 1;
 #pragma unroll 1
   for (uint32_t x = blockIdx.x; x < n; x += gridDim.x) {
     const uint32_t parts = (uint32_t)a.rpb / (uint32_t)per;
@@ -669,7 +673,7 @@ __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int 
     const int j0 = cut.range_of(at), j1 = cut.range_of(at + ends.tiles(len_of(a, (int)b), sh) - 1);
     if (j0 == j1) continue;  // (one piece: written by its workgroup)
 #pragma unroll 1
-    for (int i = i0 + wid; i < i0 + per && rb * a.rpb + i < a.R; i += 4) {
+    for (int i = split ? i0 : i0 + wid; i < i0 + per && rb * a.rpb + i < a.R; i += 4) {
       const int row = rb * a.rpb + i;
       // A range behind the first one begins with this sequence.
       const int64_t base = ((int64_t)unit * a.W * 2) * a.rpb + i;
@@ -712,11 +716,33 @@ __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int 
         }
       };
       // (Two at once where there are no more: loads of nothing cost as much.)
-      if (j1 - j0 < 2) {
+      if (!split && j1 - j0 < 2) {
         join(Count<2>{}, j0);
       } else {
 #pragma unroll 1
-        for (int s0 = j0; s0 <= j1; s0 += 8) join(Count<8>{}, s0);
+        for (int s0 = split ? j0 + 8 * wid : j0; s0 <= j1; s0 += split ? 32 : 8) join(Count<8>{}, s0);
+      }
+      if (split) {
+        if (wid != 0) {
+          *reinterpret_cast<Row*>(part + (wid - 1) * DV + lane * N) = o;
+          if (lane == 0) part_ml[wid - 1] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (wid != 0) break;
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) mn = fmaxf(mn, part_ml[u].x);
+        const float f0 = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+        l *= f0;
+        o *= f0;
+        m = mn;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+          const float2 ml = part_ml[u];
+          const float f = ml.x == mn ? 1.f : __builtin_amdgcn_exp2f((ml.x - mn) * a.scale_log2);
+          l = fmaf(ml.y, f, l);
+          o += *reinterpret_cast<const Row*>(part + u * DV + lane * N) * f;
+        }
       }
       o *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       const int pos = row / a.G, h = kvh * a.G + row - pos * a.G;
@@ -775,10 +801,13 @@ hipError_t launch_latent(const LatArgs& a, hipStream_t s) {
 
 hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   if (a.W == 1) return hipSuccess;
-  // Four rows a workgroup where there are few (128 rows: 7.1 us, with 16 rows 17), 16 where
-  // the search of their pieces counts (16384 rows: 16.4 us, with four 21).
+  // Four rows a workgroup where there are few (128 rows of 23
+  // partials: 7.1 us, with 16 rows 17), 16 where
+  // the search of their pieces counts (16384 rows: 16.4 us, with four 21); one where rows
+  // have many partials (one sequence of 32768 keys, 16 heads, both launches: 46.5 -> 30.7
+  // us; 40 of 2000 keys, six partials a row: 30.8, with one 31.8).
   const int64_t blocks = (int64_t)a.B * a.Hk * a.n_rb;
-  int per = blocks * a.rpb <= 8192 ? 4 : 16;
+  int per = blocks * a.rpb <= 1024 && a.W >= 8 * a.B ? 1 : (blocks * a.rpb <= 8192 ? 4 : 16);
   while (blocks * (a.rpb / per) > 0x7fffffff) per *= 2;  // (blocks are fewer than 2^30: the plan's range)
   const uint32_t n = (uint32_t)(blocks * (a.rpb / per));
   const dim3 grid((unsigned)(n < (1 << 20) ? n : 1 << 20)), block(256);

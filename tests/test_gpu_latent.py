@@ -558,3 +558,29 @@ def test_absorbed_whole_range_of_batches(gpu, dtype):
     for b in pick:
         compare(q[b:b + 1], rows[b:b + 1], lens[b:b + 1], 256, 0.06, out[b:b + 1], lse[b:b + 1], None, range(3), dtype)
     assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("lens", [[20000], [900, 0, 15000]])
+def test_absorbed_many_partials_a_row(gpu, dtype, lens):
+    """Few rows over many keys: more partials a row than a wave joins at once, some without a key of the row."""
+    B = len(lens)
+    q, kv, table, sl, _, rows = make(dtype, B, 2, 3, 256, 64, 64, lens, False, seed=16)
+    out, lse = latent_attn_with_kvcache(q, kv, 256, 0.06, cache_seqlens=sl, page_table=table, return_softmax_lse=True)
+    compare(q, rows, lens, 256, 0.06, out, lse, None, range(3), dtype)
+    # All weight on a token of the first piece, then of the last: the joined maximum is another piece's.
+    for at in (3, lens[-1] - 2):
+        one = rows[-1].clone()
+        one[at] = (q[-1, 0, 0].float() * 3).to(dtype)
+        page = table[-1, at // 64]
+        kv[page, at % 64] = one[at]
+        out, lse = latent_attn_with_kvcache(q, kv, 256, 0.5, cache_seqlens=sl, page_table=table, return_softmax_lse=True)
+        compare(q[-1:], [one], lens[-1:], 256, 0.5, out[-1:], lse[-1:], None, range(3), dtype)
+        kv[page, at % 64] = rows[-1][at]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_expanded_many_partials_a_row(gpu, dtype):
+    q, k, pe, v, sl = make_exp(dtype, 1, 3, 14000, 2, 128, 64, [14000], seed=17)
+    out, lse = latent_attn_expanded(q, k, pe, v, cache_seqlens=sl, return_softmax_lse=True)
+    compare_exp(q, k, pe, v, [14000], True, 192 ** -0.5, out, lse, range(2), dtype)
