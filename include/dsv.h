@@ -667,8 +667,8 @@ int dsv_token_slots(const dsv_tensor* page_table, const dsv_tensor* seqlens,
  *   cache       [P, page, dc + dr] (page a power of two; slot = page number * page +
  *               offset) or [S, dc + dr]
  *   q_pe, q_out optional [T, H, dr]: rotated for every token; q_out may be q_pe itself
- * T <= 2^26 (0: nothing is done), T * (1 + H) * dr / 16 (fp32: 8) <= 2^31.  No other overlap of an input and
- * an output.
+ * T <= 2^24 (0: nothing is done), T * (1 + H) * dr / 16 (fp32: 8) <= 2^31.  No other
+ * overlap of an input and an output.
  */
 int dsv_latent_append(const dsv_tensor* c, const dsv_tensor* k_pe,
                       const dsv_tensor* norm_weight, float eps,

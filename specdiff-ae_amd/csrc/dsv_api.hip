@@ -2329,8 +2329,9 @@ int dsv_latent_append(const dsv_tensor* c, const dsv_tensor* k_pe, const dsv_ten
     // A thread reads what it writes: row for row in place is safe.
     in_place = a.qo == a.q && a.qo_st == a.q_st && a.qo_sh == a.q_sh;
   }
-  if (T > ((int64_t)1 << 26) || T * (1 + a.H) * (dr * es / 32) > ((int64_t)1 << 31))
-    return fail(DSV_ERR_UNSUPPORTED, "more than 2^26 tokens or 2^31 chunk pairs of rotated rows");
+  // (64 threads a token and one a pair: a launch counts fewer than 2^32.)
+  if (T > ((int64_t)1 << 24) || T * (1 + a.H) * (dr * es / 32) > ((int64_t)1 << 31))
+    return fail(DSV_ERR_UNSUPPORTED, "more than 2^24 tokens or 2^31 chunk pairs of rotated rows");
   const Extent outs[2] = {extent_of("cache", cache), extent_of("q_out", q_out)};
   const Extent ins[8] = {extent_of("c", c), extent_of("k_pe", k_pe), extent_of("norm_weight", norm_weight), extent_of("cos", cos),
                          extent_of("sin", sin), extent_of("positions", positions), extent_of("slots", slots),

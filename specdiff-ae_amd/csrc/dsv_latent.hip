@@ -801,11 +801,10 @@ hipError_t launch_latent(const LatArgs& a, hipStream_t s) {
 
 hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   if (a.W == 1) return hipSuccess;
-  // Four rows a workgroup where there are few (128 rows of 23
-  // partials: 7.1 us, with 16 rows 17), 16 where
-  // the search of their pieces counts (16384 rows: 16.4 us, with four 21); one where rows
-  // have many partials (one sequence of 32768 keys, 16 heads, both launches: 46.5 -> 30.7
-  // us; 40 of 2000 keys, six partials a row: 30.8, with one 31.8).
+  // Four rows a workgroup where there are few (128 rows of 23 partials: 7.1 us, with 16 rows
+  // 17), 16 where the search of their pieces counts (16384 rows: 16.4 us, with four 21); one
+  // where rows have many partials (one sequence of 32768 keys, 16 heads, both launches: 46.5
+  // -> 30.7 us; 40 of 2000 keys, six partials a row: 30.8, with one 31.8).
   const int64_t blocks = (int64_t)a.B * a.Hk * a.n_rb;
   int per = blocks * a.rpb <= 1024 && a.W >= 8 * a.B ? 1 : (blocks * a.rpb <= 8192 ? 4 : 16);
   while (blocks * (a.rpb / per) > 0x7fffffff) per *= 2;  // (blocks are fewer than 2^30: the plan's range)

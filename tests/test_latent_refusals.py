@@ -165,6 +165,9 @@ def test_append(dry):
     assert append(dry, dr=24) == UNSUPPORTED
     assert append(dry, page=6) == UNSUPPORTED
     assert append(dry, dc=2056) == UNSUPPORTED
+    for T, want in ((1 << 24, 0), ((1 << 24) + 1, UNSUPPORTED)):
+        assert append(dry, T=1, rope=False, with_q=False, c=f(1, 64).expand(T, 64), pe=f(1, 32).expand(T, 32),
+                      slots=torch.empty(T, dtype=torch.int32)) == want
     none = dict(T=0, slots=i32(0))
     assert append(dry, **none) == 0 and append(dry, with_q=False, rope=False, **none) == 0
     assert append(dry, T=0, slots=i32(1)) == INVALID and append(dry, pe=f(0, 24), **none) == INVALID
