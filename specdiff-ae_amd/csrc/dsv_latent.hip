@@ -707,9 +707,10 @@ __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int 
         m = mn;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          // (Behind the last, and where a piece has no key of this row: nothing.)
-          const bool none = s0 + u > j1 || ml[u].x == kNegInf;
-          const float f = none ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
+          // (Behind the last: nothing.  A piece without a key of this row holds zeros; one whose
+          // maximum is -inf may hold NaN: of NaN scores, or of infinite values of no weight.)
+          const bool none = s0 + u > j1;
+          const float f = ml[u].x == mn ? 1.f : __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
           l = fmaf(none ? 0.f : ml[u].y, f, l);
 #pragma unroll
           for (int e = 0; e < N; ++e) o[e] = fmaf(none ? 0.f : p[u][e], f, o[e]);
