@@ -220,9 +220,9 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
 
     f32x16 acc[DT];
     float mx = kNegInf, lsum = 0.f;
-    // Probabilities are 2^(s * scale - ms + SHIFT), ms the maximum times the scale, rounded: a
-    // row's sums share a factor 2^err, err = ms - mx * scale, which the end of the piece
-    // takes back.  Where that grows to bits (far), they are 2^((s - mx) * scale + SHIFT), an
+    // Probabilities are 2^(s * scale - ms + SHIFT), ms the maximum times the scale, rounded (with
+    // the shift, too: far below zero their sum has a bit less): a row's sums share a factor
+    // 2^-err, err = ms - mx * scale, which the end of the piece takes back.  Where that grows to bits (far), they are 2^((s - mx) * scale + SHIFT), an
     // instruction more each, and err is 0.
     float nms = (float)SHIFT, err = 0.f;
     bool far = false;
@@ -285,12 +285,15 @@ __global__ void __launch_bounds__(512, 2) expanded_kernel(const LatArgs a) {
         for (int v = 1; v < 16; ++v) mt = fmaxf(mt, s_cur[v]);
         mt = halves_max(mt);
         if (__ballot((mt - mx) * scale > tau) != 0ull) {
-          const float mn = fmaxf(mx, mt), ms = mn == kNegInf ? 0.f : mn * scale;
-          far = __ballot(fabsf(ms) >= 2097152.f) != 0ull;
+          const float mn = fmaxf(mx, mt);
+          float top = mn == kNegInf ? 0.f : mn * scale;
+          asm("" : "+v"(top));  // (rounded here, not with the sum below)
+          far = __ballot(fabsf(top) >= 2097152.f) != 0ull;
+          nms = (float)SHIFT - top;
+          const float ms = (float)SHIFT - nms;  // exact: what the shifted sum, rounded again, took off
           const float e = far || mn == kNegInf ? 0.f : fmaf(-mn, scale, ms);
           const float al = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f((mn == mx ? 0.f : (mx - mn) * scale) + (err - e));
           mx = mn;
-          nms = (float)SHIFT - ms;
           err = e;
           lsum *= al;
 #pragma unroll
