@@ -644,13 +644,17 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
 // ---- the partials joined -------------------------------------------------------------
 // A workgroup takes (sequence, unit, `per` rows) at a time, a wave a row of DV / 64 values
 // a lane, eight partials in flight; of one row (per = 1), the waves take eight partials each
-// in turn and their sums are joined through LDS.
+// in turn and their sums are joined through LDS.  The sequences of a unit are all of them
+// (cuts = 0), each sought among the lengths, or those that the starts of the ranges 1 to
+// cuts = W - 1 cut, whichever are fewer: the lengths are read W times a unit at most, not B
+// times (131072 sequences of up to four keys, both launches: 61.5 ms, now 2.0; 600 of up to 400,
+// 128 heads: 170 us, now 156).
 template <int N>
 struct Count {
   static constexpr int value = N;
 };
 template <int DV>
-__global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int sh, uint32_t n, int per) {
+__global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int sh, uint32_t n, int per, int cuts) {
   constexpr int N = DV / 64;
   typedef float Row __attribute__((ext_vector_type(N)));
   __shared__ LatSpan span;
@@ -664,14 +668,18 @@ __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int 
     const uint32_t parts = (uint32_t)a.rpb / (uint32_t)per;
     uint32_t y = x / parts;
     const int i0 = (int)(x - y * parts) * per;
-    const uint32_t unit = y % (uint32_t)(a.n_rb * a.Hk), b = y / (uint32_t)(a.n_rb * a.Hk);
+    const uint32_t unit = y % (uint32_t)(a.n_rb * a.Hk), item = y / (uint32_t)(a.n_rb * a.Hk);
     const int kvh = unit / (uint32_t)a.n_rb, rb = unit % (uint32_t)a.n_rb;
     const LatEnd ends(a, rb);
-    const LatCut cut(lat_line<256>(a, ends, sh, 0, (int)b, span), a.W);
-    const int at = span.at;
+    const int total = lat_line<256>(a, ends, sh, cuts != 0 ? (int)item + 1 : 0, cuts != 0 ? -1 : (int)item, span);
+    const LatCut cut(total, a.W);
+    if (cuts != 0 && cut.begin((int)item + 1) >= total) continue;  // (a range of nothing)
+    const int at = span.at, b = __builtin_amdgcn_readfirstlane(span.b);
     __syncthreads();
-    const int j0 = cut.range_of(at), j1 = cut.range_of(at + ends.tiles(len_of(a, (int)b), sh) - 1);
-    if (j0 == j1) continue;  // (one piece: written by its workgroup)
+    const int j0 = cut.range_of(at), j1 = cut.range_of(at + ends.tiles(len_of(a, b), sh) - 1);
+    // (One piece: written by its workgroup.  Of the ranges that begin within a sequence the first
+    // one's workgroup joins it.)
+    if (j0 == j1 || (cuts != 0 && j0 != (int)item)) continue;
 #pragma unroll 1
     for (int i = split ? i0 : i0 + wid; i < i0 + per && rb * a.rpb + i < a.R; i += 4) {
       const int row = rb * a.rpb + i;
@@ -747,7 +755,7 @@ __global__ void __launch_bounds__(256) latent_merge_kernel(const LatArgs a, int 
       }
       o *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       const int pos = row / a.G, h = kvh * a.G + row - pos * a.G;
-      const int64_t off = b_off(a, (int)b, pos, h) + lane * N;
+      const int64_t off = b_off(a, b, pos, h) + lane * N;
       if (a.out_vec && a.out_dtype == 2) {
         *reinterpret_cast<Row*>(reinterpret_cast<float*>(a.out) + off) = o;
       } else if (a.out_vec && N > 1) {
@@ -806,16 +814,18 @@ hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   // 17), 16 where the search of their pieces counts (16384 rows: 16.4 us, with four 21); one
   // where rows have many partials (one sequence of 32768 keys, 16 heads, both launches: 46.5
   // -> 30.7 us; 40 of 2000 keys, six partials a row: 30.8, with one 31.8).
-  const int64_t blocks = (int64_t)a.B * a.Hk * a.n_rb;
-  int per = blocks * a.rpb <= 1024 && a.W >= 8 * a.B ? 1 : (blocks * a.rpb <= 8192 ? 4 : 16);
+  const int64_t units = (int64_t)a.Hk * a.n_rb, rows = a.B * units * a.rpb;
+  int per = rows <= 1024 && a.W >= 8 * a.B ? 1 : (rows <= 8192 ? 4 : 16);
+  const int cuts = a.W - 1 < a.B ? a.W - 1 : 0;
+  const int64_t blocks = units * (cuts != 0 ? cuts : a.B);
   while (blocks * (a.rpb / per) > 0x7fffffff) per *= 2;  // (blocks are fewer than 2^30: the plan's range)
   const uint32_t n = (uint32_t)(blocks * (a.rpb / per));
   const dim3 grid((unsigned)(n < (1 << 20) ? n : 1 << 20)), block(256);
   switch (a.dv) {
-    case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, sh, n, per); break;
-    case 128: hipLaunchKernelGGL(latent_merge_kernel<128>, grid, block, 0, s, a, sh, n, per); break;
-    case 256: hipLaunchKernelGGL(latent_merge_kernel<256>, grid, block, 0, s, a, sh, n, per); break;
-    default: hipLaunchKernelGGL(latent_merge_kernel<512>, grid, block, 0, s, a, sh, n, per); break;
+    case 64: hipLaunchKernelGGL(latent_merge_kernel<64>, grid, block, 0, s, a, sh, n, per, cuts); break;
+    case 128: hipLaunchKernelGGL(latent_merge_kernel<128>, grid, block, 0, s, a, sh, n, per, cuts); break;
+    case 256: hipLaunchKernelGGL(latent_merge_kernel<256>, grid, block, 0, s, a, sh, n, per, cuts); break;
+    default: hipLaunchKernelGGL(latent_merge_kernel<512>, grid, block, 0, s, a, sh, n, per, cuts); break;
   }
   return hipGetLastError();
 }
