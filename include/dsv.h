@@ -618,9 +618,11 @@ int dsv_pages_compact(const dsv_tensor* kv_pages, const dsv_tensor* page_table,
 /*
  * Models with latent attention keep, of every token, one vector that all heads
  * share and a small rotated key part: a cache row of dc + dr entries, rows [P, page,
- * dc + dr] of a page pool or [B, N, dc + dr] of a dense cache.  (For dsv_pages_fork and
- * dsv_pages_compact a pool [L, P, page, dc + dr] is viewed as [L, 2, P, 1, page,
- * (dc + dr) / 2], the halves of a row in the place of K and V.)
+ * dc + dr] of a page pool or [B, N, dc + dr] of a dense cache.  (For dsv_pages_fork,
+ * dsv_pages_compact and dsv_kv_commit a pool [L, P, page, dc + dr] is viewed as [L, 2, P,
+ * 1, page, (dc + dr) / 2], the halves of a row in the place of K and V; for
+ * dsv_kv_commit of trees whose half rows pass 64 KiB, 113 nodes of 512 + 64 in 16 bits, as
+ * [L, 2, P, h, page, (dc + dr) / 2 / h], parts of whole 16 bytes in the place of heads.)
  */
 
 /*
