@@ -105,12 +105,22 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
       for (int x = 0; x < SN + SR; ++x) kf[x] = *reinterpret_cast<const f32x4*>(x < SN ? k1 + x * 16 : k2 + (x - SN) * 16);
       if (a.pt != nullptr && t + 1 < t1) page = page_of(a, b, key_at(t + 1));
       // ---- scores of this wave's 16 keys -----------------------------------------------
-      f32x4 s{};
+      // (In sums of 64 products, added up with one in between, so that no add waits for a product:
+      // a single chain of all of them rounds its partial sums, up to 8 times as large, as often.)
+      f32x4 s{}, before{};
 #pragma unroll
-      for (int x = 0; x < SN + SR; ++x) {
+      for (int x = 0; x < SN + SR; x += 4) {
+        f32x4 part{};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][e], qf[x][e], s, 0, 0, 0);
+        for (int y = x; y < x + 4 && y < SN + SR; ++y) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[y][e], qf[y][e], part, 0, 0, 0);
+        }
+        s += before;
+        before = part;
+        __builtin_amdgcn_sched_barrier(0);  // (in the order in which the keys arrive)
       }
+      s += before;
       const bool whole = lat_whole(a, len, m_lo, kb, KT);
       hides |= !whole;
       if (!whole) {
