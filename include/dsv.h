@@ -705,8 +705,12 @@ size_t dsv_latent_workspace_bytes(int64_t B, int64_t M, int64_t H, int64_t v_dim
  *   parent       optional [M] or [B, M] int32|int64, M <= 1024 (dsv_tree_verify)
  *   out          [B, M, H, v_dim] bf16|f16|f32;  lse optional [B, H, M] f32
  * A query without a key (len_b < M) gets out = 0 and lse = -inf; with a tree every query
- * of such a sequence does.  Rows that a query does not see never affect it, whatever
- * they hold.  out and lse may not overlap an input.
+ * of such a sequence does.  M is one number: a sequence with fewer new tokens has them in its
+ * last rows, and the rows before them are for the caller to leave out (without a tree).
+ * Rows that a query does not see never affect it, whatever they hold; a NaN score that it
+ * sees makes its row NaN.  Scores, sums and partials are fp32; of 16-bit inputs the weights
+ * are rounded to their type for the product with the values, whatever type out has.  out and
+ * lse may not overlap an input.
  */
 int dsv_latent_attention(const dsv_tensor* q, const dsv_tensor* kv,
                          int64_t v_dim, const dsv_tensor* page_table,
@@ -723,6 +727,7 @@ int dsv_latent_attention(const dsv_tensor* q, const dsv_tensor* kv,
  *   k, v  [B, N, H, dn];  k_pe [B, N, dr]
  *   cache_seqlens, n_keys, softmax_scale, out [B, M, H, dn], lse: as above
  *   causal != 0: query m of sequence b sees keys n <= len_b - M + m, else all n < len_b
+ * Types of sums and weights, NaN: as above.
  */
 int dsv_latent_expanded(const dsv_tensor* q, const dsv_tensor* k,
                         const dsv_tensor* k_pe, const dsv_tensor* v,

@@ -2363,7 +2363,8 @@ struct LatPlan {
 // partial; lines much alike run in turns, others in the load of a CU and what its last
 // range adds; joining 5 and the partials' bytes.  Against the most even use of the last
 // turn alone (heads of 128 + 64): a prompt of 1500 tokens, 32 heads 94 -> 56 us, of 6000, 16
-// heads 232 -> 197, of 3000, 32 heads 158 -> 142.
+// heads 232 -> 197, of 3000, 32 heads 158 -> 142.  The constants are those of 128 + 64; narrower
+// heads, whose tiles take less, were not measured by themselves and follow the same rule.
 int expanded_ranges(const LatPlan& p, int64_t B, int64_t M, int64_t Hk, int64_t n_keys, bool causal) {
   const int64_t cus = device_cus(), units = Hk * p.n_rb;
   constexpr int kSamples = 32;
@@ -2444,8 +2445,9 @@ LatPlan lat_plan(int64_t B, int64_t M, int64_t H, int64_t Hk, int64_t dv, int dt
     // Ranges: as many workgroups as fill the CUs one to four times, whichever leaves
     // fewest idle in the last turn, of two tiles at least.  Against one turn: 2 chunks of 80
     // tokens, 128 heads, 8192 keys (160 blocks) 529 -> 421 us, 2 of 150, 64 heads, 4000 keys
-    // 274 -> 227.  Against one tile at least: 128 heads, 2900 keys 15.0 + 7.1 us, not 14.6 +
-    // 8.4 (four at least: 18.8 + 6.0).
+    // 274 -> 227.  With one tile at least and with four, the join included: 128 heads, 2900
+    // keys 19.8 us, 20.1 and 23.3; 16 heads, 8000 keys 20.9, 21.3 and 23.2; 8 sequences of 2000
+    // 19.7, 20.0 and 22.8 (the other way: 1000 keys 17.0, with one 15.2; 32768 29.3, with four 26.9).
     double best = 0;
     for (int64_t k = 1; k <= 4; ++k) {
       const int64_t w = cus * k / units;

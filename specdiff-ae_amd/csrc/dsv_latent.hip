@@ -103,7 +103,9 @@ __device__ __forceinline__ uint32_t again(uint32_t x) {
 
 // LDS image of a tile: the rows' first dc entries, then their last dr.  Chunk c (16
 // bytes) of key k stands at slot c ^ swz(k): keys read at one chunk (scores) and four
-// keys read at neighbouring chunks (values, transposed) fall on distinct banks.
+// keys read at neighbouring chunks (values, transposed) fall on distinct banks in the
+// reads of 64 rows' products (conflict cycles 5 % of the LDS's).  Those of 16 and 32 rows
+// read eight keys at once, two on a bank (45 %, beside loads that take longer).
 __device__ __forceinline__ int swz_n(int key) { return ((key & 3) << 2) | ((key >> 2) & 3); }
 template <int DR>
 __device__ __forceinline__ int swz_r(int key) {
@@ -810,10 +812,11 @@ hipError_t launch_latent(const LatArgs& a, hipStream_t s) {
 
 hipError_t launch_latent_merge(const LatArgs& a, int sh, hipStream_t s) {
   if (a.W == 1) return hipSuccess;
-  // Four rows a workgroup where there are few (128 rows of 23 partials: 7.1 us, with 16 rows
-  // 17), 16 where the search of their pieces counts (16384 rows: 16.4 us, with four 21); one
-  // where rows have many partials (one sequence of 32768 keys, 16 heads, both launches: 46.5
-  // -> 30.7 us; 40 of 2000 keys, six partials a row: 30.8, with one 31.8).
+  // One row a workgroup where rows are few and have many partials (both launches, in us: one
+  // sequence of 32768 keys, 16 heads 29.3, with four rows 51.9; 2900 keys, 128 heads 19.8, 23.0),
+  // four where there are some (40 of 2000 keys, 16 heads 32.7, with one 33.4, with 16 37.7; 32 of
+  // 4000, 128 heads 72.3, 87.4, 73.3), 16 where the search of their pieces counts (8 trees of 64
+  // nodes, 32 heads 153.5, with four 161.0).
   const int64_t units = (int64_t)a.Hk * a.n_rb, rows = a.B * units * a.rpb;
   int per = rows <= 1024 && a.W >= 8 * a.B ? 1 : (rows <= 8192 ? 4 : 16);
   const int cuts = a.W - 1 < a.B ? a.W - 1 : 0;

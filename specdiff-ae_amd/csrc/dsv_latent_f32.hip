@@ -6,13 +6,17 @@
 // tiles of 64 keys.  Every product is an fp32 matrix product (16x16x4): wave w of four
 // computes the scores of 16 keys and then a quarter of the output's columns.  Operands
 // come straight from the caches (a wave's load takes 16 rows x 64 bytes, a tile's in flight
-// together), because the matrix products at a sixteenth of the 16-bit rate leave time for
-// it: no copy in LDS but the probabilities, held in fp32, and the tile's addresses.
+// together): no copy in LDS but the probabilities, held in fp32, and the tile's addresses.
+// That is the form for few rows: nothing but its neighbours covers a tile's load, and each
+// block of 16 rows reads all keys for itself.
 //
 // Measured (a large fp32 product reaches 153 TFLOP/s): three chunks of 5 tokens through up
-// to 3001 keys, 20 heads, 256 + 32 wide: 24 + 6.5 us for the join, floor 3.7: a workgroup
+// to 3001 keys, 20 heads, 256 + 32 wide: 24 + 5.5 us for the join, floor 3.7: a workgroup
 // has one or two tiles, whose loads take a round trip and its products 4 us.  Four
-// prompts of 77 tokens, 5 heads of 64 + 32: 15 + 5 us, bound by the same latencies.
+// prompts of 77 tokens, 5 heads of 64 + 32: 15 + 5 us, bound by the same latencies.  Of many
+// rows: four chunks of 64 tokens through 2000 keys, 16 heads of 512 + 64, 18 GFLOP: 304 us,
+// 59 TFLOP/s (14 to 31 registers spill at 512); two of 200 tokens through 2000, 16 heads of 128 +
+// 64, 7.8 GFLOP: 198 us, 39 TFLOP/s.
 
 #include "dsv_latent_dev.h"
 

@@ -24,9 +24,10 @@
 // offset, the values' second half is read behind the barrier: nothing is spilled.
 //
 // Measured (a large bf16 product reaches 1309 TFLOP/s, fp16 1294): a prompt of 8192 tokens,
-// 16 heads of 128 + 64, 344 GFLOP: 331-362 us by card, 0.95-1.04 PFLOP/s, bound by the
-// matrix units at the clock that the power cap leaves, the softmax beside them.  Chunks of
-// 1001 tokens of two sequences through 5000 to 12007 keys, 8 heads, fp16, 116 GFLOP: 130 us
+// 16 heads of 128 + 64, 344 GFLOP: 327-362 us by card, 0.95-1.05 PFLOP/s; the matrix units are
+// busy in 48 % of the cycles of the counters' reference clock (the shader clock under this
+// load was not measured, so their share of its own cycles is open).  Chunks of
+// 1001 tokens of two sequences through 5000 to 12007 keys, 8 heads, fp16, 116 GFLOP: 132 us
 // and 16 for joining the partials (33 MB of fp32 written and read).  No bank conflicts.
 
 #include "dsv_dma.h"

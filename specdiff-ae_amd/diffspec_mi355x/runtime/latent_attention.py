@@ -51,7 +51,11 @@ def latent_attn_with_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, v_dim: int
     A cache row is the key of every head and its first ``v_dim`` entries the value of
     every head.  Query m sees the keys up to its own token or, with ``parent``, the
     tokens before the tree, its ancestors and itself.  A query without a key returns
-    zeros and ``-inf``.
+    zeros and ``-inf``.  M is one number for all sequences: one with fewer new tokens has
+    them in its last rows, and the rows before them are for the caller to leave out.
+
+    Scores and sums are float32; of 16-bit inputs the weights are rounded to their type
+    before they meet the values, whatever ``out_dtype``.
 
     Args:
         q: [B, M, H, v_dim + dr] bf16/f16/f32: the queries times the key expansion, then
@@ -110,7 +114,8 @@ def latent_attn_expanded(q: torch.Tensor, k: torch.Tensor, k_pe: torch.Tensor, v
 
     Returns:
         out [B, M, H, dn] (``out_dtype``, default q's) and, if asked, lse [B, H, M] float32.
-        A query without a key gets zeros and ``-inf``.
+        A query without a key gets zeros and ``-inf``.  Scores and sums are float32; of
+        16-bit inputs the weights are rounded to their type before they meet the values.
     """
     lens = cache_seqlens if isinstance(cache_seqlens, torch.Tensor) else None
     dev = _ext.require_gpu(q, k, k_pe, v, lens)
