@@ -41,7 +41,7 @@
 // 1309 TFLOP/s).  64 sequences of up to 16384 keys, 16 heads, 652 MB: 126 + 6.5 us (the
 // join), 4.9 TB/s, bound by HBM.  One sequence of 2900 keys, 128 heads: 15 + 5.5 us, bound by
 // latencies: arguments, lengths, pages, first tile, and the code itself as it is fetched.
-// 32 sequences of 1000 to 8192 keys, 128 heads, fp16: 77 + 11 us; 8 trees of 64 nodes, 32
+// 32 sequences of 1000 to 8192 keys, 128 heads, fp16: 77 + 11 to 14 us; 8 trees of 64 nodes, 32
 // heads: 194 + 16 us, 56 % of the large product's rate: a wave alone on its SIMD does its
 // products, exponents and barriers one after the other (of 4300 cycles a tile the products'
 // own are 2200); a second wave's registers are the output's and the queries'.
