@@ -629,7 +629,10 @@ __global__ void __launch_bounds__(256, 1) latent_kernel(const LatArgs a) {
         }
     __syncthreads();
     const u32x4 fl = *reinterpret_cast<const u32x4*>(lds.flag);
+    bool spreads = false;
     if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0)
+      spreads = __builtin_amdgcn_readfirstlane(lat_spreads<T, DC>(lat_args(), pc, 0, rb, KT, m_lo, lds.span.wave));
+    if (spreads)
       lat_exact_rows<T, DC>(lat_args(), pc, 0, rb, KT, m_lo, lds.vis, wid, ROWS, 4);
     else
       lat_store_rows<DC, ROWS, KG>(a, pc, rb, lds.ring, lds.m, lds.red, 1.f / (1 << SHIFT), reinterpret_cast<int64_t*>(lds.p),

@@ -191,6 +191,36 @@ struct LatPiece {
   int64_t slot;
 };
 
+// Does a piece hold a value that its products spread to rows that do not see it, 0 * inf = NaN?
+// Of the keys that some row of the block (positions from m_lo) does not see, any infinite or
+// NaN one; of the last key, which stands in for those behind the end, an infinite one (what is
+// NaN there is NaN anyway).  So NaN queries and NaN keys that all rows see need no second pass.
+// A wave takes every fourth key; called by all 256 threads, behind a barrier.
+template <typename T, int DV>
+__device__ __noinline__ bool lat_spreads(const LatArgs* ap, const LatPiece pc, int kvh, int rb, int kt, int m_lo, int* flags) {
+  typedef Elem<T> El;
+  typedef typename El::type E;
+  constexpr int N = DV / 64;
+  const LatArgs& a = *ap;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, end = LatEnd(a, rb)(pc.len), n0 = pc.len - a.M;
+  // The first key that not every row sees (of a tree, its first).
+  const int hidden = !a.causal || (a.parent != nullptr && a.M == 1) ? end : a.parent != nullptr ? n0 : n0 + m_lo + 1;
+  const E* vb = reinterpret_cast<const E*>(a.v.p) + pc.b * a.v.sb + kvh * a.v.sh;
+  float odd = 0.f;
+  for (int n = max(min(hidden, end - 1), pc.t0 * kt) + wid; n < min(end, pc.t1 * kt); n += 4) {
+    const E* v = vb + key_off(a, a.v, n, a.pt != nullptr ? page_of(a, pc.b, n) : 0) + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = El::get(v[e]);
+      if (n >= hidden || x == x) odd = fmaf(x, 0.f, odd);
+    }
+  }
+  const bool any = __ballot(odd != 0.f) != 0ull;
+  if (lane == 0) flags[wid] = any ? 1 : 0;
+  __syncthreads();
+  return (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+}
+
 // Rows [i0, i1) by step of a block once more, by one wave, from memory and without
 // matrix products: where a value that some rows see and others do not is infinite or
 // NaN (in the product 0 * inf would reach those others).  A lane takes a key of 64

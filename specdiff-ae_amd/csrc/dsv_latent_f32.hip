@@ -187,7 +187,9 @@ __global__ void __launch_bounds__(256, 1) latent_f32_kernel(const LatArgs a) {
     const bool any = __ballot(bad != 0.f) != 0ull;
     if (lane == 0) flag[wid] = any ? 1 : 0;
     __syncthreads();
-    if ((flag[0] | flag[1] | flag[2] | flag[3]) != 0) {
+    bool spreads = false;
+    if ((flag[0] | flag[1] | flag[2] | flag[3]) != 0) spreads = lat_spreads<float, DV>(lat_args(), pc, kvh, rb, KT, m_lo, span.wave);
+    if (spreads) {
       lat_exact_rows<float, DV>(lat_args(), pc, kvh, rb, KT, m_lo, vis, wid, ROWS, 4);
     } else if (row < a.R) {
       const float l = red[0][li] + red[1][li] + red[2][li] + red[3][li];
